@@ -137,6 +137,11 @@ extern "C" {
                                    kernel): a wait between its wavefronts ran
                                    out of its poll bound and the kernel left
                                    early; the outputs are not valid       */
+#define PKV_STATUS_OUT_OF_BLOCKS 1024 /* build_step: the free list holds fewer blocks
+                                         than the step needs; none was taken */
+#define PKV_STATUS_BAD_PARENT 2048 /* tree_masks: a parent that is neither -1 nor an
+                                      earlier node of the tree; the node counts
+                                      as a root                              */
 
 /* Library version (PKV_VERSION). */
 int pkv_version(void);
@@ -504,6 +509,124 @@ int pkv_sample_rows(int64_t* ids, const void* logits, int64_t rows, int64_t voca
  * key words, one 128-byte line each; 0 when those rows are not split.
  */
 size_t pkv_argmax_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
+
+/*
+ * Metadata of a ragged step from lengths on the device, blocks included (the
+ * host's counterpart is BlockAllocator + make_slot_mapping + the packed
+ * metadata, serving/allocator.py, serving/kv_pool.py:40-55,
+ * serving/fake_paged_attn.py:52-100). Sequence s holds blocks_held[s] blocks
+ * (block_tables row s) and ctx_lens[s] tokens, and gets q_lens[s] more. The
+ * blocks it lacks, ceil((ctx + q) / block_size) - held where that is positive
+ * and q > 0, are handed out in sequence order from free_blocks[free_cursor[0]
+ * ...] (num_free entries in all) and written to its row. Written besides:
+ *   blocks_held_out, ctx_lens_out [n_seq], free_cursor_out [1]: the state after
+ *     the step; other memory than the inputs (PKV_ERR_INVALID otherwise), so a
+ *     step can be taken again from the same state;
+ *   query_start_loc [n_seq + 1]; seq_lens = ctx + q and start_pos = ctx (both 0
+ *     where q = 0) [n_seq]; positions (int32) and slot_mapping (int64)
+ *     [n_tokens]: ctx + i and its slot, behind the last token 0 and INT64_MIN
+ *     (a slot pkv_append skips).
+ * n_tokens bounds the sum of q_lens, max_q_len each of them. All or nothing:
+ * with too few free blocks (PKV_STATUS_OUT_OF_BLOCKS), a row past max_blk
+ * blocks (PKV_STATUS_SHORT_TABLE) or a length outside its bounds
+ * (PKV_STATUS_BAD_QLOC) no block is taken, the state after is the state before,
+ * and positions without a held block have slot INT64_MIN. A block id outside
+ * [1, num_blocks) gives that slot too (PKV_STATUS_BAD_BLOCK). At most 16384
+ * sequences.
+ */
+int pkv_build_step(int32_t* block_tables, int max_blk, const int32_t* blocks_held,
+                   const int32_t* ctx_lens, const int32_t* q_lens, int n_seq,
+                   const int32_t* free_blocks, int num_free, const int32_t* free_cursor,
+                   int block_size, int64_t num_blocks, int64_t n_tokens, int max_q_len,
+                   int32_t* blocks_held_out, int32_t* ctx_lens_out, int32_t* free_cursor_out,
+                   int32_t* query_start_loc, int32_t* seq_lens, int32_t* start_pos,
+                   int32_t* positions, int64_t* slot_mapping, int* status, void* stream);
+
+/*
+ * Ancestor masks and positions of ragged token trees (no counterpart in the
+ * reference). Node i of sequence s is row query_start_loc[s] + i; parents[row]
+ * is its parent's index in the tree (below i) or -1. masks [n_tokens,
+ * mask_words] (int64 words): bit j % 64 of word j / 64 is set where node j is
+ * node i or an ancestor; positions[row] = ctx_lens[s] + depth. Rows behind the
+ * last sequence get empty masks and position 0. A parent that is neither -1 nor
+ * below i makes the node a root (PKV_STATUS_BAD_PARENT); a run of more than
+ * max_nodes or 64 mask_words nodes, or outside [0, n_tokens), is left unwritten
+ * (PKV_STATUS_BAD_QLOC).
+ */
+int pkv_tree_masks(int64_t* masks, int mask_words, int32_t* positions, const int32_t* parents,
+                   const int32_t* query_start_loc, const int32_t* ctx_lens, int n_seq,
+                   int n_tokens, int max_nodes, int* status, void* stream);
+
+/*
+ * Bytes of workspace pkv_paged_tree_attention needs (0 when no context is
+ * split). It needs no initial state; calls in flight together need different
+ * memory.
+ */
+size_t pkv_tree_attention_workspace_bytes(int n_seq, int max_nodes, int hq, int hkv, int d,
+                                          int max_blk, int block_size, int max_ctx_len,
+                                          int part_tokens, int dtype);
+
+/*
+ * Attention of drafted token trees over the paged cache (no counterpart in the
+ * reference). Node i of sequence s is row t = query_start_loc[s] + i of q / out
+ * [n_tokens, hq, d] and of k_new / v_new [n_tokens, hkv, d]. It sees every
+ * context key j < ctx_lens[s] (clamped to [0, max_blk * block_size]) of the
+ * sequence's table, and tree key j (row query_start_loc[s] + j of k_new / v_new)
+ * where bit j % 64 of masks[t][j / 64] is set and j is below the run's length. The
+ * tree's rows are not in the pools; with PKV_KV_FP8 they count as rounded to
+ * fp8, as the pools will hold them. out, lse (nullable, fp32 [n_tokens, hq]) and
+ * scale as in pkv_paged_attention; a row that sees no key gives 0 and +inf.
+ * Values of keys that a row does not see do not reach it, infinities and NaN
+ * included. Table entries outside [0, num_blocks) read as zeros
+ * (PKV_STATUS_BAD_BLOCK); a run outside [0, n_tokens) or of more than max_nodes
+ * nodes is skipped (PKV_STATUS_BAD_QLOC), and rows of no run are left as they
+ * were. max_ctx_len (<= 0: the table's capacity) sizes the context's split, a
+ * longer context is still computed whole; part_tokens forces the split's length
+ * (0: automatic). bf16 / f16 / fp32 (fp8 pools: bf16 / f16), any hq a multiple
+ * of hkv, d a multiple of 8 up to 256, trees of at most 4096 nodes, tensors
+ * 16-byte aligned (fp8 pools 8); PKV_ERR_UNSUPPORTED otherwise.
+ */
+int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k_new,
+                             const void* v_new, const void* k_pool, const void* v_pool,
+                             int64_t num_blocks, int block_size, const int32_t* block_tables,
+                             int max_blk, const int32_t* ctx_lens,
+                             const int32_t* query_start_loc, const int64_t* masks,
+                             int mask_words, int n_seq, int n_tokens, int max_nodes,
+                             int max_ctx_len, int hq, int hkv, int d, float scale,
+                             int part_tokens, int dtype, void* workspace,
+                             size_t workspace_bytes, int* status, void* stream);
+
+/*
+ * The longest path of each drafted tree that the model's picks confirm (no
+ * counterpart in the reference). picks[t] and tokens[t] (int64): the token the
+ * model chose after node t, and the node's own. From node 0 (the root: taken)
+ * down to the lowest-numbered child whose token is the pick at its parent, at
+ * most max_depth nodes. lens[s] = nodes taken (0 for a sequence without nodes),
+ * path[s][k] = their indices in the tree, out_tokens[s][k] = the pick at each:
+ * the sequence's next tokens. Entries from lens[s] on are -1.
+ */
+int pkv_tree_accept(int32_t* lens, int32_t* path, int64_t* out_tokens, const int64_t* picks,
+                    const int64_t* tokens, const int32_t* parents,
+                    const int32_t* query_start_loc, int n_seq, int n_tokens, int max_depth,
+                    int* status, void* stream);
+
+/*
+ * The accepted nodes' K/V rows of every layer into the pools, in one launch (no
+ * counterpart in the reference; the same bytes as pkv_append of those rows per
+ * layer). Row query_start_loc[s] + path[s][k] of k_rows / v_rows (layer l's rows
+ * rows_layer_elems elements after layer l - 1's) goes to position start_pos[s] +
+ * k, k < lens[s], through block_tables; k_pool / v_pool are layer 0's pools, the
+ * next layer's pool_layer_elems elements on. Checks and status bits as
+ * pkv_append_from_table; a path entry outside the run is skipped
+ * (PKV_STATUS_BAD_QLOC).
+ */
+int pkv_write_accepted(void* k_pool, void* v_pool, int64_t pool_layer_elems, int layers,
+                       int64_t num_blocks, int block_size, const void* k_rows,
+                       const void* v_rows, int64_t rows_layer_elems,
+                       const int32_t* block_tables, int max_blk, const int32_t* start_pos,
+                       const int32_t* query_start_loc, const int32_t* path,
+                       const int32_t* lens, int n_seq, int n_tokens, int max_depth,
+                       int64_t row_elems, int dtype, int* status, void* stream);
 
 /*
  * Measurement helper, no counterpart in the reference: reads `bytes` bytes at

@@ -40,6 +40,8 @@ PKV_STATUS_BAD_DISTRIBUTION = 64
 PKV_STATUS_SAMPLE_OVERFLOW = 128
 PKV_STATUS_DIRTY_WORKSPACE = 256
 PKV_STATUS_STALLED = 512
+PKV_STATUS_OUT_OF_BLOCKS = 1024
+PKV_STATUS_BAD_PARENT = 2048
 # part_tokens values selecting a persistent decode kernel (every workgroup an
 # equal share of all sequences' chunks): PART_PERSISTENT and PART_STATIC the
 # register-staged kernel (also the automatic choice for long context
@@ -124,6 +126,18 @@ _SIGNATURES = {
     "pkv_sample_rows": ([_c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_float, _c_int, _c_float,
                          _c_vp, _c_int, _c_vp, _c_vp], _c_int),
     "pkv_stream_read": ([_c_vp, _c_i64, _c_vp, _c_int, _c_vp], _c_int),
+    "pkv_build_step": ([_c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_int,
+                        _c_i64, _c_i64, _c_int] + [_c_vp] * 10, _c_int),
+    "pkv_tree_masks": ([_c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp,
+                        _c_vp], _c_int),
+    "pkv_tree_attention_workspace_bytes": ([_c_int] * 10, _c_size),
+    "pkv_paged_tree_attention": ([_c_vp] * 7 + [_c_i64, _c_int, _c_vp, _c_int, _c_vp, _c_vp,
+                                  _c_vp] + [_c_int] * 8 + [_c_float, _c_int, _c_int, _c_vp,
+                                  _c_size, _c_vp, _c_vp], _c_int),
+    "pkv_tree_accept": ([_c_vp] * 7 + [_c_int, _c_int, _c_int, _c_vp, _c_vp], _c_int),
+    "pkv_write_accepted": ([_c_vp, _c_vp, _c_i64, _c_int, _c_i64, _c_int, _c_vp, _c_vp, _c_i64,
+                            _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int,
+                            _c_i64, _c_int, _c_vp, _c_vp], _c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -229,6 +243,23 @@ def stream_ptr(device: torch.device) -> int:
     if _raw_stream is None or device.index is None:
         return torch.cuda.current_stream(device).cuda_stream
     return _raw_stream(device.index)
+
+
+@contextlib.contextmanager
+def _switched(device):
+    with torch.cuda.device(device):
+        yield
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is the current one: kernels are launched on
+    the current device, whichever device's stream they are given."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return _switched(device)
 
 
 def ptr(t) -> int | None:

@@ -121,6 +121,8 @@ class KVPool:
             raise AssertionError(f"{what}: block table too short for the written positions")
         if bits & _native.PKV_STATUS_BAD_BLOCK:
             raise AssertionError(f"{what}: block table entry is block 0 or outside the pool")
+        if bits & _native.PKV_STATUS_BAD_QLOC and what == "KVPool.write_accepted":
+            raise ValueError(f"{what}: a path entry is no node of its tree")
 
     def write(self, layer: int, slot_mapping: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
         """flat_k[layer][slot_mapping] = k; flat_v[layer][slot_mapping] = v
@@ -188,6 +190,47 @@ class KVPool:
             _native.stream_ptr(self.device))
         _native.check(rc, "pkv_append_from_table")
         self._raise_status(status, "KVPool.write_from_table")
+
+    def write_accepted(self, k_rows: torch.Tensor, v_rows: torch.Tensor, tree, accepted,
+                       meta) -> None:
+        """Every layer's K/V rows of the nodes a verification accepted, in one
+        launch: row accepted.path[s, k] of sequence s's tree goes to position
+        meta.start_pos[s] + k, k < accepted.lens[s]. k_rows, v_rows [num_layers, T,
+        Hkv, D] as the tree's attention used them (serving.tree_decode); tree a
+        TreeMeta, accepted a TreeAccept, meta the accepted tokens' PagedBatchMeta
+        (build_batch_meta with q_lens = accepted.lens). The same bytes as write()
+        of those rows layer by layer."""
+        what = "KVPool.write_accepted"
+        _native.require_device(self.kv, k_rows, v_rows, accepted.path, what=what)
+        shape = (self.num_layers, tree.num_tokens, self.num_kv_heads, self.head_dim)
+        assert k_rows.shape == shape and v_rows.shape == shape, \
+            f"k/v rows {tuple(k_rows.shape)}/{tuple(v_rows.shape)} != expected {shape}"
+        self._check_row_dtype(k_rows, v_rows)
+        n, depth = accepted.path.shape
+        if not (n == tree.num_seqs == meta.num_seqs == accepted.lens.numel()):
+            raise ValueError(f"{what}: {n} paths, {tree.num_seqs} trees, {meta.num_seqs} sequences")
+        if meta.block_size != self.block_size:
+            raise ValueError(f"{what}: blocks of {meta.block_size}, the pool's have {self.block_size}")
+        ts = (k_rows, v_rows, accepted.path, accepted.lens, tree.query_start_loc,
+              meta.block_tables, meta.start_pos)
+        if any(t.device != self.device for t in ts):
+            raise RuntimeError(f"{what}: rows and metadata must be on {self.device}")
+        if any(t.dtype != torch.int32 or not t.is_contiguous() for t in ts[2:]):
+            raise ValueError(f"{what}: paths, lengths and metadata must be contiguous int32")
+        k, v = k_rows.contiguous(), v_rows.contiguous()
+        row = self.num_kv_heads * self.head_dim
+        status = self._status()
+        with _native.on_device(self.device):
+            rc = _native.calls().pkv_write_accepted(
+                self.flat_k[0].data_ptr(), self.flat_v[0].data_ptr(), 2 * self.num_slots * row,
+                self.num_layers, self.num_blocks, self.block_size, k.data_ptr(), v.data_ptr(),
+                tree.num_tokens * row, meta.block_tables.data_ptr(), meta.block_tables.shape[1],
+                meta.start_pos.data_ptr(), tree.query_start_loc.data_ptr(),
+                accepted.path.data_ptr(), accepted.lens.data_ptr(), n, tree.num_tokens, depth,
+                row, _native.kv_code(k.dtype, self.dtype), _native.ptr(status),
+                _native.stream_ptr(self.device))
+        _native.check(rc, "pkv_write_accepted")
+        self._raise_status(status, what)
 
     # ------------------------------------------------------------------
     # gather

@@ -5,6 +5,11 @@ and per sequence with host round trips (serving/paged_mqa.py:87-96,
 serving/fake_paged_attn.py:52-100). Here the ragged host lists are validated
 and packed once per step into a single int32 buffer, copied to the device in
 one transfer, and reused by every layer's append and attention launch.
+
+Where a step's lengths are known on the device only (tokens accepted by a
+verification, serving.tree_decode), build_batch_meta makes the same metadata
+there, from a batch's DeviceTables: blocks taken from a free list, table rows,
+positions and slots in one kernel, without a host round trip.
 """
 from __future__ import annotations
 
@@ -12,6 +17,8 @@ from dataclasses import dataclass
 
 import numpy as np
 import torch
+
+from . import _native
 
 
 @dataclass
@@ -30,6 +37,9 @@ class PagedBatchMeta:
     # seq_lens, start_pos and positions as one contiguous view (pack_batch_meta
     # lays them out back to back), so a decode step advances them with one add
     step_view: torch.Tensor | None = None
+    # int64 [T], build_batch_meta only: each token's pool slot (KVPool.write's
+    # slot_mapping), NO_SLOT behind the last token
+    slot_mapping: torch.Tensor | None = None
 
     @property
     def is_decode(self) -> bool:
@@ -139,3 +149,134 @@ def pack_batch_meta(block_tables, query_start_loc, positions, T: int, device,
         max_kv_len=int(seq_lens.max()) if n else 0,
         block_size=block_size,
     )
+
+
+NO_SLOT = -(1 << 63)  # a slot that an append skips
+
+
+@dataclass
+class DeviceTables:
+    """Block tables of a running batch on the device, and the blocks it may
+    still take: int32 tensors of one device, contiguous."""
+    block_tables: torch.Tensor  # [N, max_blocks]
+    blocks_held: torch.Tensor   # [N] blocks each row holds
+    ctx_lens: torch.Tensor      # [N] tokens whose K/V are in the pool
+    free_blocks: torch.Tensor   # [F] block ids, in the order they are handed out
+    free_cursor: torch.Tensor   # [1] the next of them
+    block_size: int
+    num_blocks: int             # the pool's
+
+    @classmethod
+    def from_host(cls, tables, ctx_lens, free_blocks, max_blocks: int, block_size: int,
+                  num_blocks: int, device) -> "DeviceTables":
+        """From the host's block tables (lists of ids), lengths and the ids set
+        aside for growth (BlockAllocator.allocate_n), rows of max_blocks."""
+        n = len(tables)
+        if len(ctx_lens) != n:
+            raise ValueError(f"{n} block tables but {len(ctx_lens)} context lengths")
+        buf = np.zeros((n, max_blocks), dtype=np.int32)
+        for i, (row, length) in enumerate(zip(tables, ctx_lens)):
+            if len(row) > max_blocks:
+                raise ValueError(f"seq {i}: {len(row)} blocks, rows hold {max_blocks}")
+            if not 0 <= length <= len(row) * block_size:
+                raise ValueError(f"seq {i}: {length} tokens in {len(row)} blocks of {block_size}")
+            buf[i, :len(row)] = row
+        i32 = lambda x: torch.tensor(list(x), dtype=torch.int32, device=device)  # noqa: E731
+        return cls(block_tables=torch.from_numpy(buf).to(device),
+                   blocks_held=i32(len(t) for t in tables), ctx_lens=i32(ctx_lens),
+                   free_blocks=i32(free_blocks), free_cursor=i32([0]), block_size=block_size,
+                   num_blocks=num_blocks)
+
+    def check(self, what: str) -> None:
+        """Types, shapes, device and layout of the tensors (no values)."""
+        bt = self.block_tables
+        _native.require_device(bt, what=what)
+        if bt.dim() != 2:
+            raise ValueError(f"{what}: block_tables must be [N, max_blocks]")
+        n = bt.shape[0]
+        for name, t, numel in (("block_tables", bt, bt.numel()), ("blocks_held", self.blocks_held, n),
+                               ("ctx_lens", self.ctx_lens, n),
+                               ("free_blocks", self.free_blocks, self.free_blocks.numel()),
+                               ("free_cursor", self.free_cursor, 1)):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError(f"{what}: {name} must be a contiguous int32 tensor")
+            if t.device != bt.device:
+                raise RuntimeError(f"{what}: {name} on {t.device}, block_tables on {bt.device}")
+            if t.numel() != numel:
+                raise ValueError(f"{what}: {name} has {t.numel()} elements, expected {numel}")
+
+
+def raise_step_status(status: torch.Tensor, what: str) -> None:
+    """Reads the status word of the calls that make and use a step's metadata
+    (this waits for them) and raises what the host's checks raise."""
+    bits = int(status.item())
+    if bits & _native.PKV_STATUS_OUT_OF_BLOCKS:
+        raise RuntimeError(f"{what}: out of KV blocks")
+    if bits & _native.PKV_STATUS_SHORT_TABLE:
+        raise ValueError(f"{what}: a sequence exceeds its block table row")
+    if bits & _native.PKV_STATUS_BAD_QLOC:
+        raise ValueError(f"{what}: a length or query range is outside its bounds")
+    if bits & _native.PKV_STATUS_BAD_PARENT:
+        raise ValueError(f"{what}: a node's parent is neither -1 nor an earlier node")
+    if bits & _native.PKV_STATUS_BAD_BLOCK:
+        raise AssertionError(f"{what}: a block id is block 0 or outside the pool")
+    if bits:
+        raise RuntimeError(f"{what}: status {bits}")
+
+
+def _status_ptr(status, device, what):
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
+        raise ValueError(f"{what}: status must be one int32 on {device}")
+    return status.data_ptr()
+
+
+def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int, max_q_len: int,
+                     max_kv_len: int = 0, status: torch.Tensor | None = None):
+    """A step's metadata from lengths on the device: sequence i gets q_lens[i]
+    (int32 [N]) more tokens, the blocks it lacks come from the free list in
+    sequence order and are written to tables.block_tables. num_tokens bounds the
+    sum of q_lens and is T of the result, whose rows behind the last token have
+    position 0 and slot NO_SLOT; max_q_len bounds each length, max_kv_len (0: the
+    table's capacity) the contexts after the step.
+
+    Returns (PagedBatchMeta with slot_mapping, DeviceTables after the step).
+    Values as pack_batch_meta gives them; the given tables' other tensors are not
+    changed, so a step whose result is dropped can be taken again. With too few
+    free blocks, a row past max_blocks or a length out of bounds nothing is taken
+    (all or nothing), which `status` (int32 [1], zeroed by the caller, read with
+    raise_step_status) reports. No host synchronisation."""
+    tables.check("build_batch_meta")
+    dev = tables.block_tables.device
+    n, max_blocks = tables.block_tables.shape
+    if q_lens.dtype != torch.int32 or q_lens.numel() != n or q_lens.device != dev:
+        raise ValueError(f"build_batch_meta: q_lens must be int32 [{n}] on {dev}")
+    if num_tokens < 0 or max_q_len < 0:
+        raise ValueError("build_batch_meta: num_tokens and max_q_len must be >= 0")
+    T = int(num_tokens)
+    with _native.on_device(dev):
+        # seq_lens, start_pos and positions back to back, as pack_batch_meta's
+        i32 = torch.empty(5 * n + 2 + T, dtype=torch.int32, device=dev)
+        slots = torch.empty(T, dtype=torch.int64, device=dev)
+        seq_lens, start_pos, positions, qsl, held, ctx, cursor = torch.split(
+            i32, [n, n, T, n + 1, n, n, 1])
+        rc = _native.calls().pkv_build_step(
+            _native.ptr(tables.block_tables), max_blocks, _native.ptr(tables.blocks_held),
+            _native.ptr(tables.ctx_lens), _native.ptr(q_lens.contiguous()), n,
+            _native.ptr(tables.free_blocks), tables.free_blocks.numel(),
+            _native.ptr(tables.free_cursor), tables.block_size, tables.num_blocks, T,
+            int(max_q_len), held.data_ptr(), ctx.data_ptr(), cursor.data_ptr(), qsl.data_ptr(),
+            seq_lens.data_ptr(), start_pos.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+            _status_ptr(status, dev, "build_batch_meta"), _native.stream_ptr(dev))
+    _native.check(rc, "build_batch_meta")
+    meta = PagedBatchMeta(
+        block_tables=tables.block_tables, seq_lens=seq_lens, query_start_loc=qsl,
+        start_pos=start_pos, positions=positions, num_seqs=n, num_tokens=T,
+        max_blocks=max_blocks, max_q_len=int(max_q_len),
+        max_kv_len=int(max_kv_len) if max_kv_len > 0 else max_blocks * tables.block_size,
+        block_size=tables.block_size, step_view=i32[:2 * n + T], slot_mapping=slots)
+    after = DeviceTables(block_tables=tables.block_tables, blocks_held=held, ctx_lens=ctx,
+                         free_blocks=tables.free_blocks, free_cursor=cursor,
+                         block_size=tables.block_size, num_blocks=tables.num_blocks)
+    return meta, after

@@ -1,0 +1,205 @@
+"""Verification of drafted token trees over the paged cache (the target model's
+step of speculative decoding).
+
+A step takes, per sequence, a tree of drafted tokens: node 0 is the last token
+the sequence is sure of (its K/V are not in the pool yet), every other node
+continues an earlier one. The model runs all nodes at once; each attends to its
+sequence's paged context and to itself and its ancestors. The nodes' K/V rows stay
+in dense tensors until it is known which are kept, so rejected drafts cost
+no pool slots.
+
+  build_tree_meta        ancestor masks and RoPE positions from parent indices
+  paged_tree_attention   the attention of one layer
+  tree_accept            each tree's longest path the model's picks confirm
+  paged_meta.build_batch_meta   blocks and slots for the accepted tokens, from
+                         lengths that only the device knows
+  KVPool.write_accepted  the accepted rows of all layers into the pool
+
+None of these synchronises the host. serving.generation.generate_speculative
+runs them with a drafting function. The reference has no counterpart; its greedy loop
+(serving/generation.py:112-148) gives the tokens that a verified run has to give.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _native
+from .paged_meta import DeviceTables, _status_ptr
+
+__all__ = ["TreeMeta", "TreeAccept", "build_tree_meta", "paged_tree_attention", "tree_accept"]
+
+MAX_TREE_NODES = 4096
+
+
+@dataclass
+class TreeMeta:
+    block_tables: torch.Tensor     # int32 [N, max_blocks]
+    ctx_lens: torch.Tensor         # int32 [N] context in the pool
+    query_start_loc: torch.Tensor  # int32 [N + 1] first node of each sequence
+    parents: torch.Tensor          # int32 [T] parent's index in its tree, -1: none
+    masks: torch.Tensor            # int64 [T, W] bit j: tree key j is visible
+    positions: torch.Tensor        # int32 [T] context length + depth
+    num_seqs: int
+    num_tokens: int
+    max_nodes: int
+    max_ctx_len: int
+    block_size: int
+    num_blocks: int
+
+
+@dataclass
+class TreeAccept:
+    lens: torch.Tensor    # int32 [N] nodes accepted, the root among them
+    path: torch.Tensor    # int32 [N, max_depth] their indices in the tree, then -1
+    tokens: torch.Tensor  # int64 [N, max_depth] the pick at each: the next tokens
+
+
+def _int_tensor(t, dtype, numel, device, name, what):
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{what}: {name} must be {dtype} on {device} (got {t.dtype} on {t.device})")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{what}: {name} has {t.numel()} elements, expected {numel}")
+    return t.contiguous()
+
+
+def build_tree_meta(tables: DeviceTables, parents: torch.Tensor, query_start_loc: torch.Tensor,
+                    max_nodes: int, max_ctx_len: int = 0,
+                    status: Optional[torch.Tensor] = None) -> TreeMeta:
+    """Masks and positions of a step's trees: parents int32 [T], sequence s's
+    nodes in rows query_start_loc[s] ... query_start_loc[s + 1] - 1 (int32 [N + 1]).
+    A node's parent is an earlier node of its tree or -1 (a root). max_nodes bounds
+    the trees' sizes, max_ctx_len (0: the table's capacity) the contexts. Rows
+    behind the last sequence get empty masks and position 0. `status` as in
+    build_batch_meta."""
+    tables.check("build_tree_meta")
+    dev = tables.block_tables.device
+    n, max_blocks = tables.block_tables.shape
+    parents = _int_tensor(parents, torch.int32, None, dev, "parents", "build_tree_meta")
+    qsl = _int_tensor(query_start_loc, torch.int32, n + 1, dev, "query_start_loc",
+                      "build_tree_meta")
+    if not 0 <= max_nodes <= MAX_TREE_NODES:
+        raise ValueError(f"build_tree_meta: max_nodes must be in [0, {MAX_TREE_NODES}]")
+    T, words = parents.numel(), max(1, -(-int(max_nodes) // 64))
+    with _native.on_device(dev):
+        masks = torch.empty((T, words), dtype=torch.int64, device=dev)
+        positions = torch.empty(T, dtype=torch.int32, device=dev)
+        rc = _native.calls().pkv_tree_masks(
+            masks.data_ptr(), words, positions.data_ptr(), parents.data_ptr(), qsl.data_ptr(),
+            tables.ctx_lens.data_ptr(), n, T, int(max_nodes),
+            _status_ptr(status, dev, "build_tree_meta"), _native.stream_ptr(dev))
+    _native.check(rc, "build_tree_meta")
+    return TreeMeta(block_tables=tables.block_tables, ctx_lens=tables.ctx_lens,
+                    query_start_loc=qsl, parents=parents, masks=masks, positions=positions,
+                    num_seqs=n, num_tokens=T, max_nodes=int(max_nodes),
+                    max_ctx_len=int(max_ctx_len) if max_ctx_len > 0 else
+                    max_blocks * tables.block_size,
+                    block_size=tables.block_size, num_blocks=tables.num_blocks)
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and 16-byte aligned, as the kernel reads it."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                         k_pool: torch.Tensor, v_pool: torch.Tensor, meta: TreeMeta,
+                         scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                         lse: Optional[torch.Tensor] = None, part_tokens: int = 0,
+                         status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [T, Hq, D] of the trees' nodes attends to each sequence's context in the
+    pools [num_blocks, block_size, Hkv, D] and to the tree keys of k, v [T, Hkv, D]
+    that meta.masks shows each node. fp32, float16 or bfloat16; pools of the same
+    type or float8_e4m3fn (the tree's rows then count as rounded to it). `out` /
+    `lse` (float32 [T, Hq]): where to write; rows of no sequence are left as they
+    were there. A row that sees no key gives 0 and lse +inf. part_tokens (0:
+    automatic) forces the length of the pieces a context is split into."""
+    what = "paged_tree_attention"
+    _native.require_device(q, k, v, k_pool, v_pool, meta.masks, what=what)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, k_pool, v_pool)):
+        raise NotImplementedError(
+            f"{what} is forward-only (inference); run it under torch.no_grad()")
+    dev = q.device
+    if any(t.device != dev for t in (k, v, k_pool, v_pool, meta.masks)):
+        raise RuntimeError(f"{what}: q, k, v, the pools and the metadata must share a device")
+    if q.dim() != 3 or k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
+        raise ValueError(f"{what}: q must be [T, Hq, D], the pools [num_blocks, block_size, Hkv, D]")
+    T, hq, d = q.shape
+    nb, bs, hkv, pd = k_pool.shape
+    if pd != d or k.shape != (T, hkv, d) or v.shape != k.shape:
+        raise ValueError(f"{what}: k and v must be [{T}, {hkv}, {d}] (got {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}), the pools' head dim {d} (got {pd})")
+    if T != meta.num_tokens or bs != meta.block_size:
+        raise ValueError(f"{what}: {T} rows and blocks of {bs}, the metadata has "
+                         f"{meta.num_tokens} and {meta.block_size}")
+    if k.dtype != q.dtype or v.dtype != q.dtype or v_pool.dtype != k_pool.dtype:
+        raise TypeError(f"{what}: q, k and v must share a dtype, and so must the pools")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError(f"{what}: the pools must be contiguous")
+    code = _native.kv_code(q.dtype, k_pool.dtype)
+    masks = meta.masks
+    if masks.dtype != torch.int64 or masks.dim() != 2 or masks.shape[0] != T:
+        raise ValueError(f"{what}: masks must be int64 [{T}, words]")
+    masks = masks.contiguous()
+    with _native.on_device(dev):
+        q, k, v = _dense(q), _dense(k), _dense(v)
+        dst = out
+        if out is None:
+            out = dst = torch.empty_like(q)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+            raise ValueError(f"{what}: out must be {tuple(q.shape)} {q.dtype} on {dev}")
+        elif not out.is_contiguous() or out.data_ptr() % 16:
+            dst = _dense(out)  # holds the rows of no sequence
+        if lse is not None and (lse.shape != (T, hq) or lse.dtype != torch.float32
+                                or lse.device != dev or not lse.is_contiguous()):
+            raise ValueError(f"{what}: lse must be contiguous float32 [{T}, {hq}] on {dev}")
+        n, max_blk = meta.block_tables.shape
+        calls = _native.calls()
+        nbytes = calls.pkv_tree_attention_workspace_bytes(
+            n, meta.max_nodes, hq, hkv, d, max_blk, bs, meta.max_ctx_len, part_tokens, code)
+        # this call's own memory, from the allocator's pool of the current stream
+        # (or of the graph being captured): nothing is shared between calls
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        rc = calls.pkv_paged_tree_attention(
+            dst.data_ptr(), _native.ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            k_pool.data_ptr(), v_pool.data_ptr(), nb, bs,
+            meta.block_tables.data_ptr() if max_blk else None, max_blk,
+            meta.ctx_lens.data_ptr(), meta.query_start_loc.data_ptr(), masks.data_ptr(),
+            masks.shape[1], n, T, meta.max_nodes, meta.max_ctx_len, hq, hkv, d,
+            float(scale if scale is not None and scale > 0 else 0.0), part_tokens, code,
+            _native.ptr(ws), nbytes, _status_ptr(status, dev, what), _native.stream_ptr(dev))
+        _native.check(rc, what)
+        if dst is not out:
+            out.copy_(dst)
+    return out
+
+
+def tree_accept(picks: torch.Tensor, tokens: torch.Tensor, meta: TreeMeta, max_depth: int,
+                status: Optional[torch.Tensor] = None) -> TreeAccept:
+    """The nodes of each tree that the model confirms: from node 0 down to the
+    lowest-numbered child whose token is the pick at its parent, at most max_depth
+    nodes. picks, tokens int64 [T]: the token chosen after each node (argmax, or a
+    draw: accepting exactly the drafts a draw hits leaves the model's
+    distribution as it is), and each node's own."""
+    what = "tree_accept"
+    _native.require_device(picks, tokens, what=what)
+    dev = meta.parents.device
+    picks = _int_tensor(picks, torch.int64, meta.num_tokens, dev, "picks", what)
+    tokens = _int_tensor(tokens, torch.int64, meta.num_tokens, dev, "tokens", what)
+    if max_depth < 1:
+        raise ValueError(f"{what}: max_depth must be at least 1")
+    n = meta.num_seqs
+    with _native.on_device(dev):
+        lens = torch.empty(n, dtype=torch.int32, device=dev)
+        path = torch.empty((n, max_depth), dtype=torch.int32, device=dev)
+        out = torch.empty((n, max_depth), dtype=torch.int64, device=dev)
+        rc = _native.calls().pkv_tree_accept(
+            lens.data_ptr(), path.data_ptr(), out.data_ptr(), picks.data_ptr(),
+            tokens.data_ptr(), meta.parents.data_ptr(), meta.query_start_loc.data_ptr(), n,
+            meta.num_tokens, int(max_depth), _status_ptr(status, dev, what),
+            _native.stream_ptr(dev))
+    _native.check(rc, what)
+    return TreeAccept(lens=lens, path=path, tokens=out)
