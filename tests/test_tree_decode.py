@@ -64,7 +64,8 @@ def test_workspace_sizing():
     size = lambda **kw: f(*{**args, **kw}.values())  # noqa: E731
     assert size() >= 2 * 16 * 32 * 66 * 4       # 16 pieces of 32 rows each
     assert size(part=1024) == 0                 # one piece
-    assert size(max_ctx=64) == 0 and size(max_ctx=0) == size()
+    assert size(max_ctx=64, part=0) == 0        # never split
+    assert size(max_ctx=0) == size() and size(max_ctx=0, part=0) == size(part=0) > 0
     assert size(nodes=0) == size(hkv=0) == size(part=-1) == size(d=0) == 0
 
 

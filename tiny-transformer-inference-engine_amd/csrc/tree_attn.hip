@@ -6,9 +6,14 @@
 //   out = softmax(scale q K^T) V,  lse = m + ln(l);  no key: out 0, lse +inf.
 //
 // Work split. The rows of one (sequence, kv head), node-major (row i G + g),
-// are cut into tiles; the context into partitions of part_len tokens, the last
-// of which takes the tree's keys too. One workgroup of 4 wavefronts per (tile,
-// partition). Every product is a 32 x 32 MFMA with the query rows as columns:
+// are cut into tiles; the context into partitions, the last of which takes the
+// tree's keys too. One workgroup of 4 wavefronts per unit = (tile, partition).
+// Only the device knows the lengths, so every workgroup makes the plan for
+// itself, from all of them (tree_plan_unit): the partitions' length is the work
+// divided by the units wanted, and the units are numbered over the sequences that
+// have them. A batch of ragged contexts so gets pieces of about one size, and no
+// workgroups for what is not there.
+// Every product is a 32 x 32 MFMA with the query rows as columns:
 //   S^T = K Q^T   (32 tokens x 32 rows; a lane holds 16 tokens of one row)
 //   O^T += V^T P^T
 // so softmax statistics stay in a lane (one cross-half exchange), and the
@@ -65,11 +70,13 @@ struct TreeArgs {
   int group;
   int d;
   float scale_log2;
-  int part_tokens;
-  int parts;
-  int tiles;
-  float* ws_o;   // [units][ROWS][d]
-  float* ws_ml;  // [units][ROWS][2]
+  int part_tokens;  // > 0: the partitions' length
+  int min_part;     // else their least length
+  int units;        // and the units wanted
+  int slots;        // partial results the workspace holds; 0: no context is split
+  int4* recs;       // [n_seq] first slot and partitions of a split sequence, else -1
+  float* ws_o;      // [slots][ROWS][d]
+  float* ws_ml;     // [slots][ROWS][2]
   int* status;
 };
 
@@ -119,32 +126,134 @@ struct TreeGeo {
   static_assert(TEAM % CPR == 0 && RPP >= 1 && KT % RPP == 0 && PER >= 1, "chunk split");
 };
 
-struct TreeSeq {
-  int q_begin, n, ctx, part_len, nparts;
-};
-
-// Sequence s's geometry, the same in every kernel. False: nothing to do.
-__device__ __forceinline__ bool tree_seq(const TreeArgs& a, int s, TreeSeq& g, bool flag) {
-  g.q_begin = ld_meta(a.qloc, s);
-  g.n = ld_meta(a.qloc, s + 1) - g.q_begin;
-  if (g.n <= 0) return false;
-  // a run outside [0, T), or longer than the bounds that sized the grid and the
-  // masks: never index by it
-  if (g.q_begin < 0 || g.n > a.max_nodes || g.n > 64 * a.mask_words ||
-      g.q_begin > a.n_tokens - g.n) {
+// Sequence s's run of nodes and context. False: it has no nodes, or its run lies
+// outside [0, T) or exceeds the bounds of the masks (never index by it).
+__device__ __forceinline__ bool tree_seq(const TreeArgs& a, int s, int& q_begin, int& n, int& ctx,
+                                         bool flag) {
+  q_begin = a.qloc[s];
+  const int64_t run = (int64_t)a.qloc[s + 1] - q_begin;
+  n = 0;
+  ctx = 0;
+  if (run <= 0) return false;
+  if (q_begin < 0 || run > a.max_nodes || run > 64 * (int64_t)a.mask_words ||
+      q_begin > a.n_tokens - run) {
     if (flag && a.status) atomicOr(a.status, PKV_STATUS_BAD_QLOC);
     return false;
   }
-  const int64_t cap = (int64_t)a.max_blk << a.bs_shift;
-  const int c = ld_meta(a.ctx_lens, s);
-  g.ctx = c <= 0 ? 0 : (int64_t)c > cap ? (int)cap : c;
-  // a context past the planned bound still gets every key: longer partitions
-  g.part_len = a.part_tokens;
-  if ((int64_t)g.part_len * a.parts < g.ctx) {
-    const int per = (int)(((int64_t)g.ctx + a.parts - 1) / a.parts);
-    g.part_len = per > 0x7fffff00 ? 0x7fffffc0 : (per + 63) & ~63;
+  n = (int)run;
+  const int cap = (int)((int64_t)a.max_blk << a.bs_shift);
+  ctx = min(max(a.ctx_lens[s], 0), cap);
+  return true;
+}
+
+struct TreeUnit {
+  int s, q_begin, n, ctx;
+  int kvh, tile, part, nparts, part_len;
+  int slot;  // of its partial result
+};
+
+struct PlanLds {
+  unsigned long long work[kTreeWaves];
+  int scan[kTreeWaves];
+  int unit[8];
+};
+
+// The partitions of a context: at least part_len long, of equal length.
+__device__ __forceinline__ int tree_parts(const TreeArgs& a, int ctx, int part_len) {
+  return a.slots > 0 && ctx > part_len ? (ctx - 1) / part_len + 1 : 1;
+}
+
+// The unit of this workgroup, or false. Units are numbered by sequence, then
+// partition, kv head and tile; the row tiles of one (sequence, kv head, partition)
+// read the same keys, so each XCD (workgroup b runs on XCD b % 8) takes a
+// contiguous eighth of the numbers, and finds them in its L2.
+template <int ROWS>
+__device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, PlanLds& sh, TreeUnit& u) {
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  // this thread's sequence of each round of 256 (the first stays in registers)
+  int qb0 = 0, n0 = 0, ctx0 = 0;
+  const bool flag = blockIdx.x == 0;
+  if (tid < a.n_seq) tree_seq(a, tid, qb0, n0, ctx0, flag);
+  auto seq = [&](int s, int& qb, int& n, int& ctx, bool f) {
+    if (s < kTreeThreads) {
+      qb = qb0;
+      n = n0;
+      ctx = ctx0;
+    } else {
+      qb = n = ctx = 0;
+      if (s < a.n_seq) tree_seq(a, s, qb, n, ctx, f);
+    }
+  };
+  auto tiles_of = [&](int n) { return (n * a.group + ROWS - 1) / ROWS * a.hkv; };
+  int part_len = a.part_tokens;
+  if (part_len <= 0) {
+    unsigned long long work = 0;
+    for (int s = tid; s < a.n_seq; s += kTreeThreads) {
+      int qb, n, ctx;
+      seq(s, qb, n, ctx, false);
+      work += (unsigned long long)tiles_of(n) * ctx;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
+    if (lane == 0) sh.work[tid >> 6] = work;
+    __syncthreads();
+    work = sh.work[0] + sh.work[1] + sh.work[2] + sh.work[3];
+    const unsigned long long per = (work + a.units - 1) / a.units;
+    part_len = (int)min(max((per + 63) & ~63ull, (unsigned long long)a.min_part), 1ull << 30);
   }
-  g.nparts = g.ctx > 0 ? (int)(((int64_t)g.ctx + g.part_len - 1) / g.part_len) : 1;
+  int total = 0;
+  for (int base = 0; base < a.n_seq; base += kTreeThreads) {
+    int qb, n, ctx, ex;
+    seq(base + tid, qb, n, ctx, flag);
+    total += block_scan<kTreeWaves>(tiles_of(n) * tree_parts(a, ctx, part_len), sh.scan, ex);
+  }
+  // workgroup b: number b / 8 of XCD b % 8's eighth
+  const int x = blockIdx.x & 7;
+  const int from = (int)((int64_t)total * x >> 3);
+  const int mine = from + (int)(blockIdx.x >> 3);
+  const bool have = mine < (int)((int64_t)total * (x + 1) >> 3);
+  if (!have && !flag) return false;
+  int run = 0, split = 0;
+  for (int base = 0; base < a.n_seq; base += kTreeThreads) {
+    const int s = base + tid;
+    int qb, n, ctx, ex, exs;
+    seq(s, qb, n, ctx, false);
+    const int np = tree_parts(a, ctx, part_len);
+    const int cnt = tiles_of(n) * np;
+    const int tot = block_scan<kTreeWaves>(cnt, sh.scan, ex);
+    const int tots = block_scan<kTreeWaves>(np > 1 ? cnt : 0, sh.scan, exs);
+    if (flag && s < a.n_seq && a.slots > 0)
+      a.recs[s] = int4{np > 1 && n > 0 ? split + exs : -1, np, qb, n};
+    const int at = mine - run - ex;
+    if (have && at >= 0 && at < cnt) {
+      sh.unit[0] = s;
+      sh.unit[1] = qb;
+      sh.unit[2] = n;
+      sh.unit[3] = ctx;
+      sh.unit[4] = np;
+      sh.unit[5] = at;
+      sh.unit[6] = np > 1 ? split + exs + at : -1;
+    }
+    run += tot;
+    split += tots;
+  }
+  __syncthreads();
+  if (!have) return false;
+  auto get = [&](int i) { return __builtin_amdgcn_readfirstlane(sh.unit[i]); };
+  u.s = get(0);
+  u.q_begin = get(1);
+  u.n = get(2);
+  u.ctx = get(3);
+  u.nparts = get(4);
+  u.slot = get(6);
+  const int tiles = (u.n * a.group + ROWS - 1) / ROWS;
+  const int at = get(5);
+  u.tile = at % tiles;
+  u.kvh = at / tiles % a.hkv;
+  u.part = at / tiles / a.hkv;
+  // equal lengths, whole chunks
+  u.part_len = u.nparts > 1 ? ((u.ctx - 1) / u.nparts + 64) & ~63 : max(u.ctx, 1);
   return true;
 }
 
@@ -184,45 +293,56 @@ struct RowState {
   unsigned q[QW];
 };
 
-// S^T of the 32 tokens whose K rows start at kl. 16-bit: step ks takes dims
-// 16 ks + 8 (lane / 32) ... + 7 of every token and row; fp32: step (c, j) dim
-// 8 c + 4 (lane / 32) + j.
-template <typename T, int DP, int KPITCH>
-__device__ __forceinline__ floatx16 tree_scores(const char* kl, const RowState<T, DP>& st,
-                                                int lane) {
-  floatx16 s;
+// S^T of a chunk's ST x 32 tokens, whose K rows start at kl. 16-bit: step ks takes
+// dims 16 ks + 8 (lane / 32) ... + 7 of every token and row; fp32: step (c, j) dim
+// 8 c + 4 (lane / 32) + j. The ST sums are independent chains of products.
+template <typename T, int DP, int KPITCH, int ST>
+__device__ __forceinline__ void tree_scores(const char* kl, const RowState<T, DP>& st,
+                                            floatx16 (&s)[ST], int lane) {
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s[r] = 0.f;
+  for (int t = 0; t < ST; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
   const char* row = kl + (lane & 31) * KPITCH + (lane >> 5) * 16;
   if constexpr (sizeof(T) == 2) {
     using v8 = typename Mma32<T>::v8;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
-      const v8 kf = *reinterpret_cast<const v8*>(row + 32 * ks);
       const u32x4 qw = {st.q[4 * ks], st.q[4 * ks + 1], st.q[4 * ks + 2], st.q[4 * ks + 3]};
-      s = Mma32<T>::mma(kf, __builtin_bit_cast(v8, qw), s);
+#pragma unroll
+      for (int t = 0; t < ST; ++t) {
+        const v8 kf = *reinterpret_cast<const v8*>(row + 32 * t * KPITCH + 32 * ks);
+        s[t] = Mma32<T>::mma(kf, __builtin_bit_cast(v8, qw), s[t]);
+      }
     }
   } else {
 #pragma unroll
     for (int c = 0; c < DP / 8; ++c) {
-      const floatx4 kf = *reinterpret_cast<const floatx4*>(row + 32 * c);
+      floatx4 kf[ST];
+#pragma unroll
+      for (int t = 0; t < ST; ++t)
+        kf[t] = *reinterpret_cast<const floatx4*>(row + 32 * t * KPITCH + 32 * c);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        s = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], __uint_as_float(st.q[4 * c + j]), s, 0,
-                                                 0, 0);
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[t][j], __uint_as_float(st.q[4 * c + j]),
+                                                      s[t], 0, 0, 0);
     }
   }
-  return s;
 }
 
-// Online softmax of 32 scores (base 2, lazily moved reference as in
+// Online softmax of the chunk's scores (base 2, lazily moved reference as in
 // chunk_update_sub) and O^T += V^T P^T with the V rows at vl.
-template <typename T, int DP, int VPITCH>
-__device__ __forceinline__ void tree_update(const char* vl, floatx16 s, float sc,
+template <typename T, int DP, int VPITCH, int ST>
+__device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], float sc,
                                             RowState<T, DP>& st, int lane) {
   float mx = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+  for (int t = 0; t < ST; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; r += 2)
+      mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, s[t][r]), s[t][r + 1]);
   if (__builtin_amdgcn_ballot_w64(mx * sc > st.m + kLazy) != 0) {
     const float m_new = fmaxf(st.m, half_max(mx) * sc);
     const float alpha = m_new == -INFINITY ? 1.f : exp2_fast(st.m - m_new);
@@ -232,11 +352,15 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 s, float sc
     st.m = m_new;
   }
   const float nref = st.m == -INFINITY ? 0.f : -st.m;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    s[r] = exp2_fast(__builtin_fmaf(s[r], sc, nref));
-    st.l += s[r];
-  }
+  for (int t = 0; t < ST; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], sc, nref));
+      sum[r & 3] += s[t][r];
+    }
+  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   if constexpr (sizeof(T) == 2) {
     using v8 = typename Mma32<T>::v8;
     // V^T operand by transposing reads (see chunk_update_sub): a 16-lane group
@@ -247,10 +371,10 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 s, float sc
     const char* vt = vl + (4 * (lane >> 5) + (l16 >> 2)) * VPITCH +
                      2 * (16 * ((lane >> 4) & 1) + 4 * (l16 & 3));
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
+    for (int ks = 0; ks < 2 * ST; ++ks) {
       v8 pf;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pf[j] = (T)s[8 * ks + j];
+      for (int j = 0; j < 8; ++j) pf[j] = (T)s[ks >> 1][8 * (ks & 1) + j];
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
         const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -264,18 +388,20 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 s, float sc
   } else {
     const char* vt = vl + 4 * (lane >> 5) * VPITCH + 4 * (lane & 31);
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
+    for (int t = 0; t < ST; ++t)
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
-        const float vf = *reinterpret_cast<const float*>(
-            vt + ((r & 3) + 8 * (r >> 2)) * VPITCH + 128 * dt);
-        st.o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[r], st.o[dt], 0, 0, 0);
-      }
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) {
+          const float vf = *reinterpret_cast<const float*>(
+              vt + (32 * t + (r & 3) + 8 * (r >> 2)) * VPITCH + 128 * dt);
+          st.o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[t][r], st.o[dt], 0, 0, 0);
+        }
   }
 }
 
 template <typename T, int DP, int RW, bool KV8>
-__global__ __launch_bounds__(kTreeThreads) void tree_attn_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_kernel(TreeArgs a) {
   using Geo = TreeGeo<T, DP, RW>;
   constexpr int PER = Geo::PER;
   constexpr int KT = Geo::KT;
@@ -285,22 +411,13 @@ __global__ __launch_bounds__(kTreeThreads) void tree_attn_kernel(TreeArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[Geo::LDS];
   __shared__ unsigned long long odd_rows[kTreeWaves];
 
-  // The row tiles of one (sequence, kv head, partition) read the same keys:
-  // workgroup b runs on XCD b % 8, so they are 8 apart, on one L2.
-  const int b = blockIdx.x;
-  const int tile = (b >> 3) % a.tiles;
-  const int unit = (b >> 3) / a.tiles * 8 + (b & 7);
-  if (unit >= a.n_seq * a.hkv * a.parts) return;
-  const int s = unit % a.n_seq;
-  const int kvh = unit / a.n_seq % a.hkv;
-  const int part = unit / a.n_seq / a.hkv;
-  TreeSeq g;
-  if (!tree_seq(a, s, g, tile == 0 && part == 0 && kvh == 0 && threadIdx.x == 0)) return;
-  if (part >= g.nparts) return;
+  __shared__ PlanLds plan;
+  TreeUnit g;
+  if (!tree_plan_unit<Geo::ROWS>(a, plan, g)) return;
+  const int s = g.s, kvh = g.kvh, tile = g.tile, part = g.part;
   const int G = a.group;
   const int rows_all = g.n * G;
   const int r0 = tile * Geo::ROWS;
-  if (r0 >= rows_all) return;
   const int rows_here = min(Geo::ROWS, rows_all - r0);
   const int d = a.d;
 
@@ -439,21 +556,19 @@ __global__ __launch_bounds__(kTreeThreads) void tree_attn_kernel(TreeArgs a) {
       if constexpr (RW != 1) __syncthreads();
       else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (active) {
+        const int64_t cb = (int64_t)lo + (int64_t)c * KT;
+        floatx16 sc[Geo::ST];
+        tree_scores<T, DP, Geo::KPITCH, Geo::ST>(buf, st, sc, lane);
+        if (cb + KT > hi) {
+          const int left = (int)(hi - cb) - 4 * (lane >> 5);
 #pragma unroll
-        for (int t = 0; t < Geo::ST; ++t) {
-          const int64_t cb = (int64_t)lo + (int64_t)c * KT + 32 * t;
-          if (cb < hi) {
-            floatx16 sc = tree_scores<T, DP, Geo::KPITCH>(buf + 32 * t * Geo::KPITCH, st, lane);
-            if (cb + 32 > hi) {
-              const int left = (int)(hi - cb) - 4 * (lane >> 5);
+          for (int t = 0; t < Geo::ST; ++t)
 #pragma unroll
-              for (int r = 0; r < 16; ++r)
-                if ((r & 3) + 8 * (r >> 2) >= left) sc[r] = -INFINITY;
-            }
-            tree_update<T, DP, Geo::VPITCH>(buf + KT * Geo::KPITCH + 32 * t * Geo::VPITCH, sc,
-                                            a.scale_log2, st, lane);
-          }
+            for (int r = 0; r < 16; ++r)
+              if (32 * t + (r & 3) + 8 * (r >> 2) >= left) sc[t][r] = -INFINITY;
         }
+        tree_update<T, DP, Geo::VPITCH, Geo::ST>(buf + KT * Geo::KPITCH, sc, a.scale_log2, st,
+                                                 lane);
       }
     }
   }
@@ -526,39 +641,39 @@ __global__ __launch_bounds__(kTreeThreads) void tree_attn_kernel(TreeArgs a) {
       if constexpr (RW != 1) __syncthreads();
       else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (c < ntc && active) {
+        const int kb = c * KT;
+        // this row's bits of the chunk's keys, none behind the run's end
+        uint64_t bits = (uint64_t)mrow[kb >> 6] >> (kb & 63);
+        if (g.n - kb < 64) bits &= (1ull << (g.n - kb)) - 1ull;
+        floatx16 sc[Geo::ST];
+        tree_scores<T, DP, Geo::KPITCH, Geo::ST>(buf, st, sc, lane);
 #pragma unroll
         for (int t = 0; t < Geo::ST; ++t) {
-          const int kb = c * KT + 32 * t;
-          if (kb < g.n) {
-            unsigned bits = (unsigned)((uint64_t)mrow[kb >> 6] >> (kb & 63));
-            if (g.n - kb < 32) bits &= (1u << (g.n - kb)) - 1u;
-            floatx16 sc = tree_scores<T, DP, Geo::KPITCH>(buf + 32 * t * Geo::KPITCH, st, lane);
-            const unsigned mine = bits >> (4 * (lane >> 5));
+          const unsigned mine = (unsigned)(bits >> (32 * t)) >> (4 * (lane >> 5));
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (!((mine >> ((r & 3) + 8 * (r >> 2))) & 1u)) sc[r] = -INFINITY;
-            tree_update<T, DP, Geo::VPITCH>(buf + KT * Geo::KPITCH + 32 * t * Geo::VPITCH, sc,
-                                            a.scale_log2, st, lane);
-            unsigned seen_odd = (unsigned)(odd >> (32 * t));
-            while (seen_odd != 0) {  // uniform
-              const int k = __builtin_ctz(seen_odd);
-              seen_odd &= seen_odd - 1;
-              const T* vrow = static_cast<const T*>(a.v_new) +
-                              (int64_t)(g.q_begin + kb + k) * row_stride + (int64_t)kvh * d;
-              if ((bits >> k) & 1u) {
+          for (int r = 0; r < 16; ++r)
+            if (!((mine >> ((r & 3) + 8 * (r >> 2))) & 1u)) sc[t][r] = -INFINITY;
+        }
+        tree_update<T, DP, Geo::VPITCH, Geo::ST>(buf + KT * Geo::KPITCH, sc, a.scale_log2, st,
+                                                 lane);
+        unsigned long long seen_odd = odd;
+        while (seen_odd != 0) {  // uniform
+          const int k = __builtin_ctzll(seen_odd);
+          seen_odd &= seen_odd - 1;
+          const T* vrow = static_cast<const T*>(a.v_new) +
+                          (int64_t)(g.q_begin + kb + k) * row_stride + (int64_t)kvh * d;
+          if ((bits >> k) & 1u) {
 #pragma unroll
-                for (int dt = 0; dt < DP / 32; ++dt)
+            for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
-                  for (int r = 0; r < 16; ++r) {
-                    const int dim = 32 * dt + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                    float x = dim < d ? (float)vrow[dim] : 0.f;
-                    if constexpr (KV8) {  // past the fp8 range: NaN, as the pool will hold
-                      if (!(fabsf(x) <= 464.f)) x = NAN;
-                    }
-                    if (!(fabsf(x) < INFINITY)) st.o[dt][r] += x;
-                  }
+              for (int r = 0; r < 16; ++r) {
+                const int dim = 32 * dt + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                float x = dim < d ? (float)vrow[dim] : 0.f;
+                if constexpr (KV8) {  // past the fp8 range: NaN, as the pool will hold
+                  if (!(fabsf(x) <= 464.f)) x = NAN;
+                }
+                if (!(fabsf(x) < INFINITY)) st.o[dt][r] += x;
               }
-            }
           }
         }
       }
@@ -567,7 +682,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_attn_kernel(TreeArgs a) {
   if (bad_block && a.status) atomicOr(a.status, PKV_STATUS_BAD_BLOCK);
 
   // ---- results
-  const int64_t u = (((int64_t)s * a.hkv + kvh) * a.tiles + tile) * a.parts + part;
+  const int64_t u = g.slot;
   if constexpr (RW != 1) {
     const float L = half_sum(st.l);
     const int row = 32 * w + (lane & 31);
@@ -668,56 +783,87 @@ __global__ __launch_bounds__(kTreeThreads) void tree_attn_kernel(TreeArgs a) {
   }
 }
 
-// One wavefront per row of a split sequence: its partials joined in partition
-// order. Lane l owns dims 4 l ... + 3.
-template <typename T>
+// The rows of split sequences: their partials joined in partition order, DP / 8
+// lanes a row (4 dims and the 4 DP / 2 further on each). What bounds it is the
+// round trip to partials another XCD wrote, so the loads of four partitions are
+// requested at once and no thread takes a second row (64 rows a workgroup in
+// turn took 20.9 us of 128 sequences of 8 x 16 rows and 1.2 K tokens).
+template <typename T, int DP>
 __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, int rows) {
-  const int s = blockIdx.x;
+  constexpr int B = 4;
+  constexpr int LPR = DP / 8;
+  const int4 rec = a.recs[blockIdx.x];
+  const int rows_all = rec.w * a.group;
+  const int rg = blockIdx.z * (kTreeThreads / LPR) + threadIdx.x / LPR;
+  if (rec.x < 0 || rg >= rows_all) return;
+  const int np = rec.y;
   const int kvh = blockIdx.y;
-  TreeSeq g;
-  if (!tree_seq(a, s, g, false) || g.nparts <= 1) return;
-  const int lane = threadIdx.x & 63;
-  const int rows_all = g.n * a.group;
-  for (int rg = blockIdx.z * kTreeWaves + (threadIdx.x >> 6); rg < rows_all;
-       rg += gridDim.z * kTreeWaves) {
-    const int tile = rg / rows;
-    const int64_t u0 = (((int64_t)s * a.hkv + kvh) * a.tiles + tile) * a.parts;
-    const int row = rg - tile * rows;
-    float M = -INFINITY;
-    for (int p = 0; p < g.nparts; ++p) M = fmaxf(M, a.ws_ml[((u0 + p) * rows + row) * 2]);
-    float L = 0.f;
-    floatx4 o = {0.f, 0.f, 0.f, 0.f};
-    const bool mine = 4 * lane < a.d;
-    for (int p = 0; p < g.nparts; ++p) {
-      const int64_t at = (u0 + p) * rows + row;
-      const float mp = a.ws_ml[at * 2];
-      if (mp == -INFINITY) continue;
-      const float wt = exp2f(mp - M);
-      L += wt * a.ws_ml[at * 2 + 1];
-      if (mine) o += wt * *reinterpret_cast<const floatx4*>(a.ws_o + at * a.d + 4 * lane);
-    }
-    const int i = rg / a.group;
-    const int64_t orow = (int64_t)(g.q_begin + i) * a.hq + kvh * a.group + (rg - i * a.group);
-    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-    if (mine) {
-      T v[4];
+  const int tiles = (rows_all + rows - 1) / rows;
+  const int col = 4 * (threadIdx.x % LPR);
+  const bool have[2] = {col < a.d, col + DP / 2 < a.d};
+  const int64_t step = (int64_t)a.hkv * tiles * rows;  // rows from one partition to the next
+  const int tile = rg / rows;
+  const int64_t at0 = ((int64_t)rec.x + kvh * tiles + tile) * rows + (rg - tile * rows);
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + at0;
+  const float* po = a.ws_o + at0 * a.d + (have[0] ? col : 0);
+  const int far = have[1] ? DP / 2 : 0;
+  float M = -INFINITY, L = 0.f;
+  floatx4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int p0 = 0; p0 < np; p0 += B) {
+    float2 x[B];
+    floatx4 v[B][2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (T)(o[e] * inv);
-      __builtin_memcpy(static_cast<T*>(a.out) + orow * a.d + 4 * lane, v, sizeof(v));
+    for (int j = 0; j < B; ++j) {
+      const int p = min(p0 + j, np - 1);
+      x[j] = ml[p * step];
+      v[j][0] = *reinterpret_cast<const floatx4*>(po + p * step * a.d);
+      v[j][1] = *reinterpret_cast<const floatx4*>(po + p * step * a.d + far);
     }
-    if (lane == 0 && a.lse) a.lse[orow] = L == 0.f ? INFINITY : (M + log2f(L)) * kLn2f;
+    float m = M;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      if (p0 + j >= np) x[j].x = -INFINITY;
+      m = fmaxf(m, x[j].x);
+    }
+    const float old = M == -INFINITY ? 0.f : exp2f(M - m);
+    L *= old;
+    o[0] *= old;
+    o[1] *= old;
+#pragma unroll
+    for (int j = 0; j < B; ++j) {
+      // a partition in which the row sees nothing holds zeros
+      const float wt = x[j].x == -INFINITY ? 0.f : exp2f(x[j].x - m);
+      if (p0 + j < np) {
+        L += wt * x[j].y;
+        o[0] += wt * v[j][0];
+        o[1] += wt * v[j][1];
+      }
+    }
+    M = m;
   }
+  const int i = rg / a.group;
+  const int64_t orow = (int64_t)(rec.z + i) * a.hq + kvh * a.group + (rg - i * a.group);
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    T t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = (T)(o[h][e] * inv);
+    if (have[h])
+      __builtin_memcpy(static_cast<T*>(a.out) + orow * a.d + col + h * (DP / 2), t, sizeof(t));
+  }
+  if (col == 0 && a.lse) a.lse[orow] = L == 0.f ? INFINITY : (M + log2f(L)) * kLn2f;
 }
 
 struct TreePlan {
   int dp;    // padded head dim: 32, 64, 128 or 256
   int rw;    // row wavefronts per tile
   int rows;  // rows per tile
-  int tiles;
-  int parts;
-  int part_tokens;
-  size_t units;
-  size_t ws_bytes;
+  int min_part;
+  int units;      // wanted
+  int64_t grid;   // workgroups that hold every unit
+  int64_t slots;  // partial results, 0: no split
+  size_t o_off, ml_off, ws_bytes;
 };
 
 TreePlan tree_plan(int n_seq, int max_nodes, int hq, int hkv, int d, int max_blk, int block_size,
@@ -726,23 +872,38 @@ TreePlan tree_plan(int n_seq, int max_nodes, int hq, int hkv, int d, int max_blk
   p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
   const int64_t rows = (int64_t)max_nodes * (hq / hkv);
   const bool f32 = dtype_base(dtype) == PKV_DTYPE_F32;
-  // one wavefront's rows and registers that hold a chunk: RW = 1
-  p.rw = rows <= 32 && (f32 ? p.dp <= 64 : p.dp <= 128) ? 1 : 4;
-  p.rows = 32 * p.rw;
-  p.tiles = (int)((rows + p.rows - 1) / p.rows);
   const int64_t cap = (int64_t)max_blk * block_size;
   const int64_t bound = max_ctx_len > 0 ? std::min<int64_t>(max_ctx_len, cap) : cap;
-  const int64_t base = (int64_t)n_seq * hkv * p.tiles;
+  // RW = 1 where its registers hold a chunk, and either the rows fit one
+  // wavefront or the whole batch, cut into its 32-row tiles and 128-token rounds,
+  // does not fill the chip: the shortest chain then
+  const int64_t small = n_seq * (int64_t)hkv * ((rows + 31) / 32) * ((bound + 127) / 128);
+  p.rw = (f32 ? p.dp <= 64 : p.dp <= 128) && (rows <= 32 || small <= device_cu_count()) ? 1 : 4;
+  p.rows = 32 * p.rw;
+  const int64_t tiles = (rows + p.rows - 1) / p.rows * hkv;
+  p.min_part = p.rw == 1 ? 128 : 256;
+  p.units = 2 * device_cu_count();
+  const int64_t all = n_seq * tiles;
+  int64_t units = p.units;
   if (part_tokens > 0) {
-    p.part_tokens = (part_tokens + 63) / 64 * 64;
+    const int64_t len = (part_tokens + 63) / 64 * 64;
+    // contexts past the table do not exist, so this holds every partition
+    units = all * ((cap + len - 1) / len);
+    p.slots = cap > len ? units : 0;
+    p.grid = std::max(units, all);
   } else {
-    // about four workgroups per CU, none of fewer than 256 tokens
-    const int64_t want = std::max<int64_t>(1, 4 * device_cu_count() / std::max<int64_t>(base, 1));
-    p.part_tokens = (int)std::max<int64_t>(256, (bound / want + 63) / 64 * 64);
+    // partitions are at least work / units long: at most `units` of them, and one
+    // more a tile; a split context has less than twice its work's share
+    p.slots = bound > p.min_part ? 2 * (int64_t)p.units : 0;
+    p.grid = p.slots ? p.units + all : all;
   }
-  p.parts = (int)std::max<int64_t>(1, (bound + p.part_tokens - 1) / p.part_tokens);
-  p.units = (size_t)base * p.parts;
-  p.ws_bytes = p.parts > 1 ? p.units * p.rows * ((size_t)d + 2) * sizeof(float) : 0;
+  p.grid = (p.grid + 7) / 8 * 8;
+  if (p.slots) {
+    const size_t recs = ((size_t)n_seq * sizeof(int4) + 255) & ~(size_t)255;
+    p.o_off = recs;
+    p.ml_off = p.o_off + (size_t)p.slots * p.rows * d * sizeof(float);
+    p.ws_bytes = p.ml_off + (size_t)p.slots * p.rows * 2 * sizeof(float);
+  }
   return p;
 }
 
@@ -765,11 +926,16 @@ void launch_tree(const TreeArgs& a, const TreePlan& p, unsigned grid, hipStream_
     case 128: launch_tree_dp<T, 128, KV8>(a, p.rw, grid, stream); break;
     default: launch_tree_dp<T, 256, KV8>(a, p.rw, grid, stream); break;
   }
-  if (p.parts > 1) {
+  if (p.slots) {
     const int64_t rows = (int64_t)a.max_nodes * a.group;
-    const dim3 mg((unsigned)a.n_seq, (unsigned)a.hkv,
-                  (unsigned)std::min<int64_t>((rows + kTreeWaves - 1) / kTreeWaves, 1024));
-    tree_merge_kernel<T><<<mg, kTreeThreads, 0, stream>>>(a, p.rows);
+    const int per = kTreeThreads * 8 / p.dp;  // rows per workgroup
+    const dim3 mg((unsigned)a.n_seq, (unsigned)a.hkv, (unsigned)((rows + per - 1) / per));
+    switch (p.dp) {
+      case 32: tree_merge_kernel<T, 32><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
+      case 64: tree_merge_kernel<T, 64><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
+      case 128: tree_merge_kernel<T, 128><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
+      default: tree_merge_kernel<T, 256><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
+    }
   }
 }
 
@@ -846,10 +1012,10 @@ int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k
   const int blk = num_blocks > 0 ? max_blk : 0;
   const TreePlan p = tree_plan(n_seq, max_nodes, hq, hkv, d, blk, block_size, max_ctx_len,
                                part_tokens, dtype);
-  const int64_t groups = (int64_t)n_seq * hkv * p.parts;
-  const int64_t grid = (groups + 7) / 8 * 8 * p.tiles;
-  if (grid > 0x7fffffff || n_seq > 0x7fffffff / 2)
-    return fail(PKV_ERR_UNSUPPORTED, "too many sequences x heads x partitions");
+  const int64_t rows = (int64_t)max_nodes * (hq / hkv);
+  // rows / 8: the join's workgroups at d = 256
+  if (p.grid > 0x7fffffff || rows > 8 * 65535)
+    return fail(PKV_ERR_UNSUPPORTED, "too many sequences x heads x partitions, or rows");
   if (p.ws_bytes > 0 && (!workspace || workspace_bytes < p.ws_bytes))
     return fail(PKV_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", p.ws_bytes,
                 workspace ? workspace_bytes : (size_t)0);
@@ -878,13 +1044,18 @@ int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k
   a.group = hq / hkv;
   a.d = d;
   a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)d)) * 1.4426950408889634f;
-  a.part_tokens = p.part_tokens;
-  a.parts = p.parts;
-  a.tiles = p.tiles;
-  a.ws_o = static_cast<float*>(workspace);
-  a.ws_ml = p.ws_bytes ? a.ws_o + p.units * p.rows * (size_t)d : nullptr;
+  a.part_tokens = (part_tokens + 63) / 64 * 64;
+  a.min_part = p.min_part;
+  a.units = p.units;
+  a.slots = (int)p.slots;
+  if (p.slots) {
+    char* ws = static_cast<char*>(workspace);
+    a.recs = reinterpret_cast<int4*>(ws);
+    a.ws_o = reinterpret_cast<float*>(ws + p.o_off);
+    a.ws_ml = reinterpret_cast<float*>(ws + p.ml_off);
+  }
   a.status = status;
-  const unsigned g32 = (unsigned)grid;
+  const unsigned g32 = (unsigned)p.grid;
   hipStream_t st = (hipStream_t)stream;
   if (qdtype == PKV_DTYPE_F32)
     launch_tree<float, false>(a, p, g32, st);
