@@ -114,8 +114,12 @@ struct TreeGeo {
   static constexpr int TEAM = 64 * RW;               // threads that load a chunk
   static constexpr int RPP = TEAM / CPR;             // rows per pass of the team
   static constexpr int PER = KT / RPP;               // pieces per thread and tensor
+  static constexpr int RPW = 64 / CPR;               // rows one wavefront's load covers
   static constexpr int KPITCH = ES * DP + 16;        // bytes; see the bank notes in ChunkGeo
-  static constexpr int VPITCH = ES * DP + 32;
+  // V: transposing reads take 64 bytes of each of 4 rows a cycle, which 64 bytes
+  // of padding put on distinct banks (32 bytes cost 34% of all LDS cycles in
+  // conflicts); fp32 rows t and t + 4 are read together: 32 bytes
+  static constexpr int VPITCH = ES == 4 ? ES * DP + 32 : DP == 32 ? 64 : ES * DP + 64;
   static constexpr int BUF = KT * (KPITCH + VPITCH);  // one chunk: K rows, then V rows
   static constexpr int NBUF = RW == 1 ? kTreeWaves : 2;
   static constexpr int OPITCH = DP + 4;               // floats, RW = 1's combination
@@ -352,6 +356,8 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
     st.m = m_new;
   }
   const float nref = st.m == -INFINITY ? 0.f : -st.m;
+  // the sum is of the weights before their rounding to T: lse is an fp32 result
+  // (summed two an instruction after it, it was off by the rounding)
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < ST; ++t)
@@ -400,7 +406,10 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
   }
 }
 
-template <typename T, int DP, int RW, bool KV8>
+// WHOLE (block size >= 16): the 2 to 16 rows that one load of a wavefront covers
+// lie in one block, so its table entry and address are scalar work; smaller blocks
+// take both row by row.
+template <typename T, int DP, int RW, bool KV8, bool WHOLE>
 __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_kernel(TreeArgs a) {
   using Geo = TreeGeo<T, DP, RW>;
   constexpr int PER = Geo::PER;
@@ -461,14 +470,23 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
 
   Piece8<T> kr[PER], vr[PER];
   unsigned ok_rows = 0;
-  // registers -> LDS; rows past the range's end, rows of bad blocks and columns
-  // past d as zeros (what the memory there holds never reaches a product)
-  auto stage = [&](char* buf, auto raw) {
+  const bool cols = d == DP;
+  // registers -> LDS. MASKED: rows past the range's end, rows of bad blocks and
+  // columns past d as zeros (what the memory there holds never reaches a product)
+  auto stage = [&](char* buf, bool masked, auto raw) {
     asm volatile("" ::: "memory");
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+#pragma unroll
+        for (int e = 0; e < Piece8<T>::W; ++e) {
+          kr[j].w[e] = (ok_rows >> j) & 1 ? kr[j].w[e] : 0u;
+          vr[j].w[e] = (ok_rows >> j) & 1 ? vr[j].w[e] : 0u;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int row = prow + j * Geo::RPP;
-      const bool ok = (ok_rows >> j) & 1;
       if constexpr (decltype(raw)::value) {  // fp8 bytes as loaded
         const u32x4 k4 = widen8<T>(u32x2{kr[j].w[0], kr[j].w[1]});
         const u32x4 v4 = widen8<T>(u32x2{vr[j].w[0], vr[j].w[1]});
@@ -478,13 +496,31 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
           vr[j].w[e] = v4[e];
         }
       }
-      if (!ok) {
-#pragma unroll
-        for (int e = 0; e < Piece8<T>::W; ++e) kr[j].w[e] = vr[j].w[e] = 0u;
-      }
       *reinterpret_cast<Piece8<T>*>(buf + row * Geo::KPITCH + 8 * ES * pcol) = kr[j];
       *reinterpret_cast<Piece8<T>*>(buf + KT * Geo::KPITCH + row * Geo::VPITCH + 8 * ES * pcol) =
           vr[j];
+    }
+  };
+  auto load = [&](int j, const char* kp, const char* vp) {
+    if constexpr (KV8) {
+      const u32x2 k2 = *reinterpret_cast<const u32x2*>(kp);
+      const u32x2 v2 = *reinterpret_cast<const u32x2*>(vp);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        kr[j].w[e] = k2[e];
+        vr[j].w[e] = v2[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < Piece8<T>::W; e += 4) {
+        const u32x4 k4 = *reinterpret_cast<const u32x4*>(kp + 4 * e);
+        const u32x4 v4 = *reinterpret_cast<const u32x4*>(vp + 4 * e);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          kr[j].w[e + f] = k4[f];
+          vr[j].w[e + f] = v4[f];
+        }
+      }
     }
   };
 
@@ -496,50 +532,47 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
   if (nch > 0) {
     const int32_t* __restrict__ table = a.block_tables + (int64_t)s * a.max_blk;
     const int64_t row_stride = (int64_t)a.hkv * d * PES;
-    const char* kbase = static_cast<const char*>(a.k_pool) + ((int64_t)kvh * d + (col_ok ? 8 * pcol : 0)) * PES;
-    const char* vbase = static_cast<const char*>(a.v_pool) + ((int64_t)kvh * d + (col_ok ? 8 * pcol : 0)) * PES;
+    const int64_t head = ((int64_t)kvh * d) * PES;
+    const char* kbase = static_cast<const char*>(a.k_pool) + head;
+    const char* vbase = static_cast<const char*>(a.v_pool) + head;
+    const unsigned colb = (col_ok ? 8 * pcol : 0) * PES;
     const int bs_mask = (1 << a.bs_shift) - 1;
+    // WHOLE: the first row of this wavefront's load j is wrow + j RPP
+    const int wrow = RW == 1 ? 0 : w * Geo::RPW;
+    const unsigned lane_off = (unsigned)(lane / Geo::CPR) * (unsigned)row_stride + colb;
     int ent[PER];
+    bool some_bad = false;  // WHOLE: a bad block in the chunk requested last
     auto fetch_ent = [&](int c) {
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const int64_t pos = (int64_t)lo + (int64_t)c * KT + prow + j * Geo::RPP;
-        ent[j] = table[(int)(min(pos, (int64_t)hi - 1) >> a.bs_shift)];
+        const int64_t pos = (int64_t)lo + (int64_t)c * KT + (WHOLE ? wrow : prow) + j * Geo::RPP;
+        const int e = (int)(min(pos, (int64_t)hi - 1) >> a.bs_shift);
+        ent[j] = WHOLE ? ld_meta(table, e) : table[e];
       }
     };
     auto issue = [&](int c) {
       ok_rows = 0;
+      some_bad = false;
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const int64_t pos = (int64_t)lo + (int64_t)c * KT + prow + j * Geo::RPP;
-        const bool in = pos < hi;
         const bool good = (uint64_t)(int64_t)ent[j] < (uint64_t)a.num_blocks;
-        bad_block |= in && !good;
-        ok_rows |= (unsigned)(in && good && col_ok) << j;
-        const int64_t slot = in && good ? ((int64_t)ent[j] << a.bs_shift) + ((int)pos & bs_mask) : 0;
-        const char* kp = kbase + slot * row_stride;
-        const char* vp = vbase + slot * row_stride;
-        if constexpr (KV8) {
-          const u32x2 k2 = *reinterpret_cast<const u32x2*>(kp);
-          const u32x2 v2 = *reinterpret_cast<const u32x2*>(vp);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            kr[j].w[e] = k2[e];
-            vr[j].w[e] = v2[e];
-          }
+        const int64_t pos = (int64_t)lo + (int64_t)c * KT + prow + j * Geo::RPP;
+        ok_rows |= (unsigned)(pos < hi && good && col_ok) << j;
+        if constexpr (WHOLE) {
+          // rows past hi are read where their block has them, and zeroed
+          some_bad |= !good;
+          const int first = lo + c * KT + wrow + j * Geo::RPP;
+          const int64_t slot = ((int64_t)(good ? ent[j] : 0) << a.bs_shift) + (first & bs_mask);
+          load(j, kbase + slot * row_stride + lane_off, vbase + slot * row_stride + lane_off);
         } else {
-#pragma unroll
-          for (int e = 0; e < Piece8<T>::W; e += 4) {
-            const u32x4 k4 = *reinterpret_cast<const u32x4*>(kp + 4 * e);
-            const u32x4 v4 = *reinterpret_cast<const u32x4*>(vp + 4 * e);
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              kr[j].w[e + f] = k4[f];
-              vr[j].w[e + f] = v4[f];
-            }
-          }
+          const bool in = pos < hi && good;
+          bad_block |= pos < hi && !good;
+          const int64_t slot =
+              in ? ((int64_t)ent[j] << a.bs_shift) + ((int)pos & bs_mask) : (int64_t)0;
+          load(j, kbase + slot * row_stride + colb, vbase + slot * row_stride + colb);
         }
       }
+      bad_block |= some_bad;
     };
     if (team < nch) {
       fetch_ent(team);
@@ -548,7 +581,8 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
     }
     for (int c = team; c < nch; c += TEAMS) {
       char* buf = RW == 1 ? buf0 : buf0 + ((c & 1) * Geo::BUF);
-      stage(buf, std::integral_constant<bool, KV8>{});
+      stage(buf, !WHOLE || !cols || some_bad || (int64_t)lo + (int64_t)(c + 1) * KT > hi,
+            std::integral_constant<bool, KV8>{});
       if (c + TEAMS < nch) {
         issue(c + TEAMS);
         fetch_ent(min(c + 2 * TEAMS, nch - 1));
@@ -636,7 +670,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
               }
             }
         }
-        stage(buf, std::false_type{});
+        stage(buf, true, std::false_type{});
       }
       if constexpr (RW != 1) __syncthreads();
       else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -909,13 +943,16 @@ TreePlan tree_plan(int n_seq, int max_nodes, int hq, int hkv, int d, int max_blk
 
 template <typename T, int DP, bool KV8>
 void launch_tree_dp(const TreeArgs& a, int rw, unsigned grid, hipStream_t stream) {
+  const bool whole = a.bs_shift >= 4;
   if constexpr (sizeof(T) == 2 ? DP <= 128 : DP <= 64) {
     if (rw == 1) {
-      tree_attn_kernel<T, DP, 1, KV8><<<grid, kTreeThreads, 0, stream>>>(a);
+      whole ? tree_attn_kernel<T, DP, 1, KV8, true><<<grid, kTreeThreads, 0, stream>>>(a)
+            : tree_attn_kernel<T, DP, 1, KV8, false><<<grid, kTreeThreads, 0, stream>>>(a);
       return;
     }
   }
-  tree_attn_kernel<T, DP, 4, KV8><<<grid, kTreeThreads, 0, stream>>>(a);
+  whole ? tree_attn_kernel<T, DP, 4, KV8, true><<<grid, kTreeThreads, 0, stream>>>(a)
+        : tree_attn_kernel<T, DP, 4, KV8, false><<<grid, kTreeThreads, 0, stream>>>(a);
 }
 
 template <typename T, bool KV8>
