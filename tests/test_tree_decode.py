@@ -36,7 +36,8 @@ def attention(**kw):
     (INVALID, b"sizes", dict(part=-1)),
     (INVALID, b"sizes", dict(nodes=-1)),
     (UNSUPPORTED, b"4096", dict(nodes=4097, words=65)),
-    (UNSUPPORTED, b"2\\^31", dict(max_blk=1 << 27)),
+    (UNSUPPORTED, b"2^30", dict(max_blk=(1 << 26) + 1)),
+    (UNSUPPORTED, b"2 GiB", dict(bs=1 << 24, max_blk=1)),
     (INVALID, b"max_nodes", dict(nodes=65)),
     (INVALID, b"max_nodes", dict(words=0)),
     (INVALID, b"null", dict(masks=None)),
@@ -50,7 +51,7 @@ def attention(**kw):
 ])
 def test_attention_refusals(rc, word, kw):
     assert attention(**kw) == rc
-    assert word.replace(b"\\", b"") in _native.lib().pkv_last_error()
+    assert word in _native.lib().pkv_last_error()
 
 
 def test_attention_with_nothing_to_do():

@@ -112,9 +112,12 @@ struct TreeGeo {
   static constexpr int KT = RW == 1 ? 32 : (ES == 2 ? (DP == 256 ? 32 : 64) : (DP <= 64 ? 64 : 32));
   static constexpr int ST = KT / 32;
   static constexpr int TEAM = 64 * RW;               // threads that load a chunk
-  static constexpr int RPP = TEAM / CPR;             // rows per pass of the team
-  static constexpr int PER = KT / RPP;               // pieces per thread and tensor
-  static constexpr int RPW = 64 / CPR;               // rows one wavefront's load covers
+  static constexpr int WROWS = KT / RW;              // consecutive rows a wavefront loads
+  static constexpr int RPL = 64 / CPR;               // of them by one load
+  static constexpr int PER = WROWS / RPL;            // pieces per thread and tensor
+  static constexpr int GR = WROWS < 16 ? WROWS : 16;  // rows that lie in one block of 16
+  static constexpr int NG = WROWS / GR;
+  static constexpr int PG = GR / RPL;                // loads per such group
   static constexpr int KPITCH = ES * DP + 16;        // bytes; see the bank notes in ChunkGeo
   // V: transposing reads take 64 bytes of each of 4 rows a cycle, which 64 bytes
   // of padding put on distinct banks (32 bytes cost 34% of all LDS cycles in
@@ -127,7 +130,7 @@ struct TreeGeo {
   static constexpr int LDS_CHUNKS = NBUF * BUF;
   static constexpr int LDS_COMBINE = RW == 1 ? kTreeWaves * 32 * (OPITCH + 2) * 4 : 0;
   static constexpr int LDS = LDS_CHUNKS > LDS_COMBINE ? LDS_CHUNKS : LDS_COMBINE;
-  static_assert(TEAM % CPR == 0 && RPP >= 1 && KT % RPP == 0 && PER >= 1, "chunk split");
+  static_assert(64 % CPR == 0 && GR % RPL == 0 && NG * PG == PER && PER >= 1, "chunk split");
 };
 
 // Sequence s's run of nodes and context. False: it has no nodes, or its run lies
@@ -309,15 +312,34 @@ __device__ __forceinline__ void tree_scores(const char* kl, const RowState<T, DP
     for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
   const char* row = kl + (lane & 31) * KPITCH + (lane >> 5) * 16;
   if constexpr (sizeof(T) == 2) {
+    // fragments of two groups of steps in registers: a group is requested before
+    // the previous one's products
     using v8 = typename Mma32<T>::v8;
+    constexpr int KS = DP / 16;
+    constexpr int GS = KS < 4 / ST ? KS : 4 / ST;  // steps a group: four products
+    v8 kf[2][GS][ST];
+    auto fetch = [&](int g) {
 #pragma unroll
-    for (int ks = 0; ks < DP / 16; ++ks) {
-      const u32x4 qw = {st.q[4 * ks], st.q[4 * ks + 1], st.q[4 * ks + 2], st.q[4 * ks + 3]};
+      for (int i = 0; i < GS; ++i)
 #pragma unroll
-      for (int t = 0; t < ST; ++t) {
-        const v8 kf = *reinterpret_cast<const v8*>(row + 32 * t * KPITCH + 32 * ks);
-        s[t] = Mma32<T>::mma(kf, __builtin_bit_cast(v8, qw), s[t]);
+        for (int t = 0; t < ST; ++t)
+          kf[g & 1][i][t] =
+              *reinterpret_cast<const v8*>(row + 32 * t * KPITCH + 32 * (g * GS + i));
+    };
+    fetch(0);
+#pragma unroll
+    for (int g = 0; g < KS / GS; ++g) {
+      if (g + 1 < KS / GS) fetch(g + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < GS; ++i) {
+        const int ks = g * GS + i;
+        const u32x4 qw = {st.q[4 * ks], st.q[4 * ks + 1], st.q[4 * ks + 2], st.q[4 * ks + 3]};
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+          s[t] = Mma32<T>::mma(kf[g & 1][i][t], __builtin_bit_cast(v8, qw), s[t]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   } else {
 #pragma unroll
@@ -359,28 +381,25 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
   // the sum is of the weights before their rounding to T: lse is an fp32 result
   // (summed two an instruction after it, it was off by the rounding)
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  auto weights = [&](int t, int r0) {  // 8 of them
 #pragma unroll
-  for (int t = 0; t < ST; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
+    for (int r = r0; r < r0 + 8; ++r) {
       s[t][r] = exp2_fast(__builtin_fmaf(s[t][r], sc, nref));
       sum[r & 3] += s[t][r];
     }
-  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  };
   if constexpr (sizeof(T) == 2) {
     using v8 = typename Mma32<T>::v8;
     // V^T operand by transposing reads (see chunk_update_sub): a 16-lane group
     // reads 4 tokens x 16 dims, so lane l gets dim 32 dt + l % 32 of tokens
     // 16 ks + 4 (l / 32) + 0..3, and of the 4 tokens 8 further on: the tokens
-    // whose probabilities registers 8 ks ... + 7 hold
+    // whose probabilities registers 8 ks ... + 7 hold. A step's operands are
+    // requested, and its weights taken, ahead of the previous step's products
     const int l16 = lane & 15;
     const char* vt = vl + (4 * (lane >> 5) + (l16 >> 2)) * VPITCH +
                      2 * (16 * ((lane >> 4) & 1) + 4 * (l16 & 3));
-#pragma unroll
-    for (int ks = 0; ks < 2 * ST; ++ks) {
-      v8 pf;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pf[j] = (T)s[ks >> 1][8 * (ks & 1) + j];
+    v8 vf[2][DP / 32], pf[2];
+    auto fetch = [&](int ks) {
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) {
         const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -388,11 +407,40 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
         const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) v4s*)(vt + (16 * ks + 8) * VPITCH + 64 * dt));
         const v8s both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        st.o[dt] = Mma32<T>::mma(__builtin_bit_cast(v8, both), pf, st.o[dt]);
+        vf[ks & 1][dt] = __builtin_bit_cast(v8, both);
       }
+    };
+    auto take = [&](int ks) {
+      weights(ks >> 1, 8 * (ks & 1));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pf[ks & 1][j] = (T)s[ks >> 1][8 * (ks & 1) + j];
+    };
+    fetch(0);
+    take(0);
+#pragma unroll
+    for (int ks = 0; ks < 2 * ST; ++ks) {
+      if (ks + 1 < 2 * ST) fetch(ks + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+        st.o[dt] = Mma32<T>::mma(vf[ks & 1][dt], pf[ks & 1], st.o[dt]);
+      if (ks + 1 < 2 * ST) take(ks + 1);
+      if constexpr (DP >= 64) {  // products and vector work side by side
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2 | 0x400, 32 / (DP / 32), 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
   } else {
     const char* vt = vl + 4 * (lane >> 5) * VPITCH + 4 * (lane & 31);
+#pragma unroll
+    for (int t = 0; t < ST; ++t) {
+      weights(t, 0);
+      weights(t, 8);
+    }
 #pragma unroll
     for (int t = 0; t < ST; ++t)
 #pragma unroll
@@ -404,11 +452,16 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
           st.o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[t][r], st.o[dt], 0, 0, 0);
         }
   }
+  st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
-// WHOLE (block size >= 16): the 2 to 16 rows that one load of a wavefront covers
-// lie in one block, so its table entry and address are scalar work; smaller blocks
-// take both row by row.
+// WHOLE (block size >= 16): the rows a wavefront loads are read 16 (or 8) at a time
+// through a buffer resource of their own, whose base is the first of them in
+// their block and whose size ends with the range (or is 0 for a bad block): rows
+// that do not exist read as zeros, the addresses are scalar work, and the table's
+// entries are kept 64 at a time in a register. Smaller blocks take all of it row by
+// row. (Row by row for every block size: 110 us against 104 with scalar addresses
+// in 64 bits, 65533 fp8 tokens, 63 nodes x 32 heads.)
 template <typename T, int DP, int RW, bool KV8, bool WHOLE>
 __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_kernel(TreeArgs a) {
   using Geo = TreeGeo<T, DP, RW>;
@@ -462,15 +515,15 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
     }
   }
 
-  const int prow = tl / Geo::CPR;
-  const int pcol = tl % Geo::CPR;
+  const int wrow = RW == 1 ? 0 : w * Geo::WROWS;  // this wavefront's first row of a chunk
+  const int prow = wrow + lane / Geo::CPR;        // this lane's, of load 0
+  const int pcol = lane % Geo::CPR;
   const bool col_ok = 8 * pcol < d;
   char* const buf0 = lds + (RW == 1 ? w * Geo::BUF : 0);
   const bool active = RW == 1 || 32 * w < rows_here;  // this wavefront has rows
 
   Piece8<T> kr[PER], vr[PER];
   unsigned ok_rows = 0;
-  const bool cols = d == DP;
   // registers -> LDS. MASKED: rows past the range's end, rows of bad blocks and
   // columns past d as zeros (what the memory there holds never reaches a product)
   auto stage = [&](char* buf, bool masked, auto raw) {
@@ -486,7 +539,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int row = prow + j * Geo::RPP;
+      const int row = prow + j * Geo::RPL;
       if constexpr (decltype(raw)::value) {  // fp8 bytes as loaded
         const u32x4 k4 = widen8<T>(u32x2{kr[j].w[0], kr[j].w[1]});
         const u32x4 v4 = widen8<T>(u32x2{vr[j].w[0], vr[j].w[1]});
@@ -524,56 +577,103 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
     }
   };
 
-  // ---- context keys [lo, hi) through the block table
+  // ---- context keys [lo, hi) through the block table (contexts end below 2^30)
   const int lo = part * g.part_len;
-  const int hi = min((int64_t)lo + g.part_len, (int64_t)g.ctx);
+  const int hi = min(lo + g.part_len, g.ctx);
   const int nch = hi > lo ? (hi - lo + KT - 1) / KT : 0;
   bool bad_block = false;
   if (nch > 0) {
     const int32_t* __restrict__ table = a.block_tables + (int64_t)s * a.max_blk;
-    const int64_t row_stride = (int64_t)a.hkv * d * PES;
-    const int64_t head = ((int64_t)kvh * d) * PES;
+    const unsigned row_stride = (unsigned)(a.hkv * d * PES);
+    const int64_t head = (int64_t)kvh * d * PES;
     const char* kbase = static_cast<const char*>(a.k_pool) + head;
     const char* vbase = static_cast<const char*>(a.v_pool) + head;
-    const unsigned colb = (col_ok ? 8 * pcol : 0) * PES;
     const int bs_mask = (1 << a.bs_shift) - 1;
-    // WHOLE: the first row of this wavefront's load j is wrow + j RPP
-    const int wrow = RW == 1 ? 0 : w * Geo::RPW;
-    const unsigned lane_off = (unsigned)(lane / Geo::CPR) * (unsigned)row_stride + colb;
-    int ent[PER];
-    bool some_bad = false;  // WHOLE: a bad block in the chunk requested last
+    const unsigned num_blocks = (unsigned)min(a.num_blocks, (int64_t)0x7fffffff);
+    // WHOLE: this lane's offset in a group of rows; columns past d lie past any end
+    const unsigned lane_off =
+        col_ok ? (unsigned)(lane / Geo::CPR) * row_stride + (unsigned)(8 * pcol * PES) : 0x80000000u;
+    const int blk_last = (hi - 1) >> a.bs_shift;
+    int blk0 = lo >> a.bs_shift;  // WHOLE: first entry in `entries`
+    int entries = 0;
+    auto window = [&](int first) {
+      blk0 = first;
+      entries = table[min(first + lane, blk_last)];
+      asm volatile("" : "+v"(entries));  // waits here, once in 64 blocks
+    };
+    int ent[PER];  // else: the next chunk's entries, row by row
     auto fetch_ent = [&](int c) {
+      if constexpr (!WHOLE) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int64_t pos = (int64_t)lo + (int64_t)c * KT + (WHOLE ? wrow : prow) + j * Geo::RPP;
-        const int e = (int)(min(pos, (int64_t)hi - 1) >> a.bs_shift);
-        ent[j] = WHOLE ? ld_meta(table, e) : table[e];
+        for (int j = 0; j < PER; ++j)
+          ent[j] = table[min(lo + c * KT + prow + j * Geo::RPL, hi - 1) >> a.bs_shift];
       }
     };
     auto issue = [&](int c) {
-      ok_rows = 0;
-      some_bad = false;
+      if constexpr (WHOLE) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const bool good = (uint64_t)(int64_t)ent[j] < (uint64_t)a.num_blocks;
-        const int64_t pos = (int64_t)lo + (int64_t)c * KT + prow + j * Geo::RPP;
-        ok_rows |= (unsigned)(pos < hi && good && col_ok) << j;
-        if constexpr (WHOLE) {
-          // rows past hi are read where their block has them, and zeroed
-          some_bad |= !good;
-          const int first = lo + c * KT + wrow + j * Geo::RPP;
-          const int64_t slot = ((int64_t)(good ? ent[j] : 0) << a.bs_shift) + (first & bs_mask);
-          load(j, kbase + slot * row_stride + lane_off, vbase + slot * row_stride + lane_off);
-        } else {
+        for (int n = 0; n < Geo::NG; ++n) {
+          const int first = lo + c * KT + wrow + n * Geo::GR;
+          const int blk = min(first, hi - 1) >> a.bs_shift;
+          if (blk - blk0 >= 64) window(blk);
+          const unsigned id = (unsigned)__builtin_amdgcn_readlane(entries, blk - blk0);
+          const bool good = id < num_blocks;
+          bad_block |= !good;
+          const int rows = good ? min(hi - first, Geo::GR) : 0;
+          const int extent = rows > 0 ? (rows - 1) * (int)row_stride + d * PES : 0;
+          // a block is less than 2^31 bytes
+          const uint64_t base = (uint64_t)(good ? id : 0u) * (row_stride << a.bs_shift) +
+                                (unsigned)(first & bs_mask) * row_stride;
+          const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
+              const_cast<char*>(kbase + base), (short)0, extent, kRsrcWord3);
+          const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
+              const_cast<char*>(vbase + base), (short)0, extent, kRsrcWord3);
+#pragma unroll
+          for (int i = 0; i < Geo::PG; ++i) {
+            const int j = n * Geo::PG + i;
+            const unsigned off = lane_off + i * Geo::RPL * row_stride;
+            if constexpr (KV8) {
+              const u32x2 k2 =
+                  __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(krs, off, 0, 0));
+              const u32x2 v2 =
+                  __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vrs, off, 0, 0));
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                kr[j].w[e] = k2[e];
+                vr[j].w[e] = v2[e];
+              }
+            } else {
+#pragma unroll
+              for (int e = 0; e < Piece8<T>::W; e += 4) {
+                const u32x4 k4 = __builtin_bit_cast(
+                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, off + 4 * e, 0, 0));
+                const u32x4 v4 = __builtin_bit_cast(
+                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, off + 4 * e, 0, 0));
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                  kr[j].w[e + f] = k4[f];
+                  vr[j].w[e + f] = v4[f];
+                }
+              }
+            }
+          }
+        }
+      } else {
+        ok_rows = 0;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const int pos = lo + c * KT + prow + j * Geo::RPL;
+          const bool good = (unsigned)ent[j] < num_blocks;
           const bool in = pos < hi && good;
           bad_block |= pos < hi && !good;
-          const int64_t slot =
-              in ? ((int64_t)ent[j] << a.bs_shift) + ((int)pos & bs_mask) : (int64_t)0;
-          load(j, kbase + slot * row_stride + colb, vbase + slot * row_stride + colb);
+          ok_rows |= (unsigned)(in && col_ok) << j;
+          const int64_t off = (in ? ((int64_t)ent[j] << a.bs_shift) + (pos & bs_mask) : (int64_t)0) *
+                                  row_stride + (col_ok ? 8 * pcol * PES : 0);
+          load(j, kbase + off, vbase + off);
         }
       }
-      bad_block |= some_bad;
     };
+    if (WHOLE) window(blk0);
     if (team < nch) {
       fetch_ent(team);
       issue(team);
@@ -581,8 +681,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
     }
     for (int c = team; c < nch; c += TEAMS) {
       char* buf = RW == 1 ? buf0 : buf0 + ((c & 1) * Geo::BUF);
-      stage(buf, !WHOLE || !cols || some_bad || (int64_t)lo + (int64_t)(c + 1) * KT > hi,
-            std::integral_constant<bool, KV8>{});
+      stage(buf, !WHOLE, std::integral_constant<bool, KV8>{});
       if (c + TEAMS < nch) {
         issue(c + TEAMS);
         fetch_ent(min(c + 2 * TEAMS, nch - 1));
@@ -590,11 +689,11 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
       if constexpr (RW != 1) __syncthreads();
       else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (active) {
-        const int64_t cb = (int64_t)lo + (int64_t)c * KT;
+        const int cb = lo + c * KT;
         floatx16 sc[Geo::ST];
         tree_scores<T, DP, Geo::KPITCH, Geo::ST>(buf, st, sc, lane);
         if (cb + KT > hi) {
-          const int left = (int)(hi - cb) - 4 * (lane >> 5);
+          const int left = hi - cb - 4 * (lane >> 5);
 #pragma unroll
           for (int t = 0; t < Geo::ST; ++t)
 #pragma unroll
@@ -623,7 +722,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
         ok_rows = 0;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-          const int row = c * KT + prow + j * Geo::RPP;
+          const int row = c * KT + prow + j * Geo::RPL;
           const bool in = row < g.n && col_ok;
           ok_rows |= (unsigned)in << j;
           const int64_t off = ((int64_t)(g.q_begin + (in ? row : 0)) * row_stride +
@@ -656,7 +755,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
         if (odd != 0) {
 #pragma unroll
           for (int j = 0; j < PER; ++j)
-            if ((odd >> (prow + j * Geo::RPP)) & 1) {
+            if ((odd >> (prow + j * Geo::RPL)) & 1) {
 #pragma unroll
               for (int e = 0; e < Piece8<T>::W; ++e) {
                 // element-wise: the row's finite values stay
@@ -1031,8 +1130,10 @@ int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k
   if (max_nodes > kTreeMaxNodes)
     return fail(PKV_ERR_UNSUPPORTED, "trees of at most %d nodes (max_nodes %d)", kTreeMaxNodes,
                 max_nodes);
-  if ((int64_t)max_blk * block_size >= (int64_t)1 << 31)
-    return fail(PKV_ERR_UNSUPPORTED, "block tables of 2^31 tokens or more");
+  if ((int64_t)max_blk * block_size > (int64_t)1 << 30)
+    return fail(PKV_ERR_UNSUPPORTED, "block tables of more than 2^30 tokens");
+  if ((int64_t)block_size * hkv * d * (kv8 ? 1 : elem_bytes(qdtype)) > 0x7fffffff)
+    return fail(PKV_ERR_UNSUPPORTED, "blocks of 2 GiB and more");
   if (n_seq == 0 || max_nodes == 0 || n_tokens == 0) return PKV_OK;
   if ((int64_t)mask_words * 64 < max_nodes)
     return fail(PKV_ERR_INVALID, "masks of %d 64-bit words hold fewer than max_nodes = %d keys",
