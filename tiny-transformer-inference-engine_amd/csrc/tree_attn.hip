@@ -45,6 +45,7 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int kTreeThreads = 256;
 constexpr int kTreeWaves = 4;
+constexpr int kTreeMaxNodes = 4096;
 
 struct TreeArgs {
   void* out;
@@ -111,7 +112,6 @@ struct TreeGeo {
   // tokens per chunk
   static constexpr int KT = RW == 1 ? 32 : (ES == 2 ? (DP == 256 ? 32 : 64) : (DP <= 64 ? 64 : 32));
   static constexpr int ST = KT / 32;
-  static constexpr int TEAM = 64 * RW;               // threads that load a chunk
   static constexpr int WROWS = KT / RW;              // consecutive rows a wavefront loads
   static constexpr int RPL = 64 / CPR;               // of them by one load
   static constexpr int PER = WROWS / RPL;            // pieces per thread and tensor
@@ -125,10 +125,10 @@ struct TreeGeo {
   static constexpr int VPITCH = ES == 4 ? ES * DP + 32 : DP == 32 ? 64 : ES * DP + 64;
   static constexpr int BUF = KT * (KPITCH + VPITCH);  // one chunk: K rows, then V rows
   static constexpr int NBUF = RW == 1 ? kTreeWaves : 2;
-  static constexpr int OPITCH = DP + 4;               // floats, RW = 1's combination
+  static constexpr int OPITCH = DP + 4;               // floats of a result row
   static constexpr int ROWS = 32 * RW;
   static constexpr int LDS_CHUNKS = NBUF * BUF;
-  static constexpr int LDS_COMBINE = RW == 1 ? kTreeWaves * 32 * (OPITCH + 2) * 4 : 0;
+  static constexpr int LDS_COMBINE = kTreeWaves * 32 * (OPITCH + (RW == 1 ? 2 : 0)) * 4;
   static constexpr int LDS = LDS_CHUNKS > LDS_COMBINE ? LDS_CHUNKS : LDS_COMBINE;
   static_assert(64 % CPR == 0 && GR % RPL == 0 && NG * PG == PER && PER >= 1, "chunk split");
 };
@@ -159,106 +159,116 @@ struct TreeUnit {
   int slot;  // of its partial result
 };
 
-struct PlanLds {
-  unsigned long long work[kTreeWaves];
-  int scan[kTreeWaves];
-  int unit[8];
-};
-
 // The partitions of a context: at least part_len long, of equal length.
 __device__ __forceinline__ int tree_parts(const TreeArgs& a, int ctx, int part_len) {
   return a.slots > 0 && ctx > part_len ? (ctx - 1) / part_len + 1 : 1;
 }
 
+// Exclusive prefix sums of x and y over the wavefront; the totals in tx and ty.
+__device__ __forceinline__ void wave_scan2(int& x, int& y, int& tx, int& ty) {
+  const int lane = threadIdx.x & 63;
+  int sx = x, sy = y;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int ux = __shfl_up(sx, o, 64);
+    const int uy = __shfl_up(sy, o, 64);
+    if (lane >= o) {
+      sx += ux;
+      sy += uy;
+    }
+  }
+  tx = __builtin_amdgcn_readlane(sx, 63);
+  ty = __builtin_amdgcn_readlane(sy, 63);
+  x = sx - x;
+  y = sy - y;
+}
+
 // The unit of this workgroup, or false. Units are numbered by sequence, then
 // partition, kv head and tile; the row tiles of one (sequence, kv head, partition)
 // read the same keys, so each XCD (workgroup b runs on XCD b % 8) takes a
-// contiguous eighth of the numbers, and finds them in its L2.
+// contiguous eighth of the numbers, and finds them in its L2. Every wavefront makes
+// the plan for itself, one sequence a lane and round, so there is no barrier in it;
+// the later passes read the lengths from the L1.
 template <int ROWS>
-__device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, PlanLds& sh, TreeUnit& u) {
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  // this thread's sequence of each round of 256 (the first stays in registers)
-  int qb0 = 0, n0 = 0, ctx0 = 0;
-  const bool flag = blockIdx.x == 0;
-  if (tid < a.n_seq) tree_seq(a, tid, qb0, n0, ctx0, flag);
-  auto seq = [&](int s, int& qb, int& n, int& ctx, bool f) {
-    if (s < kTreeThreads) {
-      qb = qb0;
-      n = n0;
-      ctx = ctx0;
-    } else {
-      qb = n = ctx = 0;
-      if (s < a.n_seq) tree_seq(a, s, qb, n, ctx, f);
-    }
-  };
+__device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, TreeUnit& u) {
+  const int lane = threadIdx.x & 63;
+  // workgroup 0's first wavefront also reports bad runs and writes the records
+  const bool flag = blockIdx.x == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x) < 64;
   auto tiles_of = [&](int n) { return (n * a.group + ROWS - 1) / ROWS * a.hkv; };
+  auto load = [&](int r, int& qb, int& n, int& ctx, bool f) {
+    qb = n = ctx = 0;
+    if (64 * r + lane < a.n_seq) tree_seq(a, 64 * r + lane, qb, n, ctx, f);
+  };
+  const int rounds = (a.n_seq + 63) / 64;
   int part_len = a.part_tokens;
   if (part_len <= 0) {
-    unsigned long long work = 0;
-    for (int s = tid; s < a.n_seq; s += kTreeThreads) {
-      int qb, n, ctx;
-      seq(s, qb, n, ctx, false);
-      work += (unsigned long long)tiles_of(n) * ctx;
+    float work = 0.f;
+#pragma unroll 1
+    for (int r = 0; r < rounds; ++r) {
+      int q, m, c;
+      load(r, q, m, c, false);
+      work += (float)tiles_of(m) * (float)c;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
-    if (lane == 0) sh.work[tid >> 6] = work;
-    __syncthreads();
-    work = sh.work[0] + sh.work[1] + sh.work[2] + sh.work[3];
-    const unsigned long long per = (work + a.units - 1) / a.units;
-    part_len = (int)min(max((per + 63) & ~63ull, (unsigned long long)a.min_part), 1ull << 30);
+    work += lane_xor<1>(work);
+    work += lane_xor<2>(work);
+    work += lane_xor<4>(work);
+    work += lane_xor<8>(work);
+    work += lane_xor<16>(work);
+    work += lane_xor<32>(work);
+    // rounded up past the sum's own rounding, so that `slots` holds every partial
+    const float per = work / (float)a.units * 1.0001f;
+    part_len = max(per < 1e9f ? ((int)per + 64) & ~63 : 1 << 30, a.min_part);
+    part_len = __builtin_amdgcn_readfirstlane(part_len);
   }
   int total = 0;
-  for (int base = 0; base < a.n_seq; base += kTreeThreads) {
-    int qb, n, ctx, ex;
-    seq(base + tid, qb, n, ctx, flag);
-    total += block_scan<kTreeWaves>(tiles_of(n) * tree_parts(a, ctx, part_len), sh.scan, ex);
+#pragma unroll 1
+  for (int r = 0; r < rounds; ++r) {
+    int q, m, c;
+    load(r, q, m, c, flag);
+    total += tiles_of(m) * tree_parts(a, c, part_len);
   }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
+  total = __builtin_amdgcn_readfirstlane(total);
   // workgroup b: number b / 8 of XCD b % 8's eighth
-  const int x = blockIdx.x & 7;
-  const int from = (int)((int64_t)total * x >> 3);
-  const int mine = from + (int)(blockIdx.x >> 3);
-  const bool have = mine < (int)((int64_t)total * (x + 1) >> 3);
+  const int xcd = blockIdx.x & 7;
+  const int mine = (int)((int64_t)total * xcd >> 3) + (int)(blockIdx.x >> 3);
+  const bool have = mine < (int)((int64_t)total * (xcd + 1) >> 3);
   if (!have && !flag) return false;
-  int run = 0, split = 0;
-  for (int base = 0; base < a.n_seq; base += kTreeThreads) {
-    const int s = base + tid;
-    int qb, n, ctx, ex, exs;
-    seq(s, qb, n, ctx, false);
-    const int np = tree_parts(a, ctx, part_len);
-    const int cnt = tiles_of(n) * np;
-    const int tot = block_scan<kTreeWaves>(cnt, sh.scan, ex);
-    const int tots = block_scan<kTreeWaves>(np > 1 ? cnt : 0, sh.scan, exs);
-    if (flag && s < a.n_seq && a.slots > 0)
-      a.recs[s] = int4{np > 1 && n > 0 ? split + exs : -1, np, qb, n};
-    const int at = mine - run - ex;
-    if (have && at >= 0 && at < cnt) {
-      sh.unit[0] = s;
-      sh.unit[1] = qb;
-      sh.unit[2] = n;
-      sh.unit[3] = ctx;
-      sh.unit[4] = np;
-      sh.unit[5] = at;
-      sh.unit[6] = np > 1 ? split + exs + at : -1;
+  bool found = false;
+  int run = 0, splits = 0;
+#pragma unroll 1
+  for (int r = 0; r < rounds && (flag || !found); ++r) {
+    int q, m, c, tx, ty;
+    load(r, q, m, c, false);
+    const int parts = tree_parts(a, c, part_len);
+    const int k = tiles_of(m) * parts;
+    int x = k, y = parts > 1 ? k : 0;
+    wave_scan2(x, y, tx, ty);
+    const int first = run + x, slot = splits + y;
+    run += tx;
+    splits += ty;
+    if (flag && a.slots > 0 && 64 * r + lane < a.n_seq)
+      a.recs[64 * r + lane] = int4{parts > 1 && m > 0 ? slot : -1, parts, q, m};
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(have && mine >= first && mine < first + k);
+    if (hit != 0) {
+      const int l = __builtin_ctzll(hit);
+      found = true;
+      u.s = 64 * r + l;
+      u.q_begin = __builtin_amdgcn_readlane(q, l);
+      u.n = __builtin_amdgcn_readlane(m, l);
+      u.ctx = __builtin_amdgcn_readlane(c, l);
+      u.nparts = __builtin_amdgcn_readlane(parts, l);
+      u.tile = mine - __builtin_amdgcn_readlane(first, l);  // of all of the sequence's units
+      u.slot = __builtin_amdgcn_readlane(slot, l) + u.tile;
     }
-    run += tot;
-    split += tots;
   }
-  __syncthreads();
-  if (!have) return false;
-  auto get = [&](int i) { return __builtin_amdgcn_readfirstlane(sh.unit[i]); };
-  u.s = get(0);
-  u.q_begin = get(1);
-  u.n = get(2);
-  u.ctx = get(3);
-  u.nparts = get(4);
-  u.slot = get(6);
+  if (!found) return false;
   const int tiles = (u.n * a.group + ROWS - 1) / ROWS;
-  const int at = get(5);
-  u.tile = at % tiles;
-  u.kvh = at / tiles % a.hkv;
-  u.part = at / tiles / a.hkv;
+  const int i = u.tile;
+  u.tile = i % tiles;
+  u.kvh = i / tiles % a.hkv;
+  u.part = i / tiles / a.hkv;
   // equal lengths, whole chunks
   u.part_len = u.nparts > 1 ? ((u.ctx - 1) / u.nparts + 64) & ~63 : max(u.ctx, 1);
   return true;
@@ -471,11 +481,10 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
   constexpr int PES = KV8 ? 1 : ES;  // pool element bytes
   constexpr int TEAMS = kTreeWaves / RW;
   __shared__ __attribute__((aligned(16))) char lds[Geo::LDS];
-  __shared__ unsigned long long odd_rows[kTreeWaves];
+  __shared__ unsigned long long odd_rows[kTreeMaxNodes / KT];
 
-  __shared__ PlanLds plan;
   TreeUnit g;
-  if (!tree_plan_unit<Geo::ROWS>(a, plan, g)) return;
+  if (!tree_plan_unit<Geo::ROWS>(a, g)) return;
   const int s = g.s, kvh = g.kvh, tile = g.tile, part = g.part;
   const int G = a.group;
   const int rows_all = g.n * G;
@@ -487,13 +496,30 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
   const int lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int team = RW == 1 ? w : 0;
-  const int tl = RW == 1 ? lane : tid;  // thread of the team
+
+  // chunks: the tree's (in the last partition) first, then those of the context
+  // keys [lo, hi) (contexts end below 2^30). A team takes every TEAMS-th
+  const int lo = part * g.part_len;
+  const int hi = min(lo + g.part_len, g.ctx);
+  const int ntc = part == g.nparts - 1 ? (g.n + KT - 1) / KT : 0;
+  const int nch = ntc + (hi > lo ? (hi - lo + KT - 1) / KT : 0);
+
+  const int32_t* __restrict__ table = a.block_tables + (int64_t)s * a.max_blk;
+  const int blk_last = max(hi - 1, 0) >> a.bs_shift;
+  int blk0 = lo >> a.bs_shift;  // WHOLE: first entry in `entries`
+  int entries = 0;
+  if (WHOLE && hi > lo) entries = table[min(blk0 + lane, blk_last)];
 
   // this lane's row
   const int rr = min(r0 + (RW == 1 ? 0 : 32 * w) + (lane & 31), rows_all - 1);
-  const int node = rr / G;
-  const int64_t tok = g.q_begin + node;
-  const int64_t qrow = tok * a.hq + kvh * G + (rr - node * G);
+  // its token, and its row of q and out; taken again where needed (`lane` through an
+  // opaque copy), registers are what the loop is short of
+  auto token_of = [&](int r) { return g.q_begin + r / G; };
+  auto row_of = [&](int r) { return (int64_t)token_of(r) * a.hq + kvh * G + r % G; };
+  auto opaque = [](int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  };
   RowState<T, DP> st;
   st.m = -INFINITY;
   st.l = 0.f;
@@ -504,7 +530,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
   {
     // 16-byte pieces: 8 dims (16-bit) or 4 (fp32), alternating between the halves
     constexpr int E = 16 / ES;
-    const T* qp = static_cast<const T*>(a.q) + qrow * d;
+    const T* qp = static_cast<const T*>(a.q) + row_of(rr) * d;
 #pragma unroll
     for (int c = 0; c < Geo::CPR * ES / 4; ++c) {
       const int dim = 2 * E * c + E * (lane >> 5);
@@ -521,26 +547,179 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
   const bool col_ok = 8 * pcol < d;
   char* const buf0 = lds + (RW == 1 ? w * Geo::BUF : 0);
   const bool active = RW == 1 || 32 * w < rows_here;  // this wavefront has rows
+  for (int i = tid; i < ntc; i += kTreeThreads) odd_rows[i] = 0;
+  if (ntc > 0) __syncthreads();
 
   Piece8<T> kr[PER], vr[PER];
-  unsigned ok_rows = 0;
-  // registers -> LDS. MASKED: rows past the range's end, rows of bad blocks and
-  // columns past d as zeros (what the memory there holds never reaches a product)
-  auto stage = [&](char* buf, bool masked, auto raw) {
-    asm volatile("" ::: "memory");
-    if (masked) {
+  unsigned ok_rows = 0;        // !WHOLE: the context rows that exist
+  uint64_t bits_next = 0;  // tree chunks: this row's mask
+  bool bad_block = false;
+  const unsigned row_elems = (unsigned)(a.hkv * d);
+  const unsigned num_blocks = (unsigned)min(a.num_blocks, (int64_t)0x7fffffff);
+
+  // rows [first, first + GR) of group n through resources of `extent` bytes: what
+  // lies past the end reads as zeros
+  auto load_group = [&](int n, const char* kp, const char* vp, int extent, unsigned stride,
+                        auto raw) {
+    constexpr int B = decltype(raw)::value ? 1 : ES;
+    const __amdgpu_buffer_rsrc_t krs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kp), (short)0, extent, kRsrcWord3);
+    const __amdgpu_buffer_rsrc_t vrs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vp), (short)0, extent, kRsrcWord3);
+    // columns past d lie past any end
+    const unsigned at = col_ok ? (unsigned)(lane / Geo::CPR) * stride + (unsigned)(8 * pcol * B)
+                               : 0x80000000u;
 #pragma unroll
-      for (int j = 0; j < PER; ++j)
+    for (int i = 0; i < Geo::PG; ++i) {
+      const int j = n * Geo::PG + i;
+      const unsigned off = at + i * Geo::RPL * stride;
+      if constexpr (B == 1) {
+        const u32x2 k2 =
+            __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(krs, off, 0, 0));
+        const u32x2 v2 =
+            __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vrs, off, 0, 0));
 #pragma unroll
-        for (int e = 0; e < Piece8<T>::W; ++e) {
-          kr[j].w[e] = (ok_rows >> j) & 1 ? kr[j].w[e] : 0u;
-          vr[j].w[e] = (ok_rows >> j) & 1 ? vr[j].w[e] : 0u;
+        for (int e = 0; e < 2; ++e) {
+          kr[j].w[e] = k2[e];
+          vr[j].w[e] = v2[e];
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < Piece8<T>::W; e += 4) {
+          const u32x4 k4 = __builtin_bit_cast(
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, off + 4 * e, 0, 0));
+          const u32x4 v4 = __builtin_bit_cast(
+              u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, off + 4 * e, 0, 0));
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            kr[j].w[e + f] = k4[f];
+            vr[j].w[e + f] = v4[f];
+          }
+        }
+      }
     }
+  };
+  auto extent_of = [&](int rows, unsigned stride, int bytes) {
+    return rows > 0 ? (min(rows, Geo::GR) - 1) * (int)stride + bytes : 0;
+  };
+
+  auto issue_tree = [&](int c) {
+    const unsigned stride = row_elems * ES;
+#pragma unroll
+    for (int n = 0; n < Geo::NG; ++n) {
+      const int first = c * KT + wrow + n * Geo::GR;
+      const int64_t off = ((int64_t)(g.q_begin + min(first, g.n - 1)) * row_elems +
+                           (int64_t)kvh * d) * ES;
+      load_group(n, static_cast<const char*>(a.k_new) + off,
+                 static_cast<const char*>(a.v_new) + off, extent_of(g.n - first, stride, d * ES),
+                 stride, std::false_type{});
+    }
+    bits_next = (uint64_t)a.masks[(int64_t)token_of(opaque(rr)) * a.mask_words + (c * KT >> 6)] >>
+                (c * KT & 63);
+  };
+  auto issue_ctx = [&](int c) {
+    const unsigned stride = row_elems * PES;
+    const char* kbase = static_cast<const char*>(a.k_pool) + (int64_t)kvh * d * PES;
+    const char* vbase = static_cast<const char*>(a.v_pool) + (int64_t)kvh * d * PES;
+    const int bs_mask = (1 << a.bs_shift) - 1;
+    if constexpr (WHOLE) {
+#pragma unroll
+      for (int n = 0; n < Geo::NG; ++n) {
+        const int first = lo + c * KT + wrow + n * Geo::GR;
+        const int blk = min(first, hi - 1) >> a.bs_shift;
+        if (blk - blk0 >= 64) {
+          blk0 = blk;
+          entries = table[min(blk0 + lane, blk_last)];
+          asm volatile("" : "+v"(entries));  // waits here, once in 64 blocks
+        }
+        const unsigned id = (unsigned)__builtin_amdgcn_readlane(entries, blk - blk0);
+        const bool good = id < num_blocks;
+        bad_block |= !good;
+        // a block is less than 2^31 bytes
+        const uint64_t off = (uint64_t)(good ? id : 0u) * (stride << a.bs_shift) +
+                             (unsigned)(first & bs_mask) * stride;
+        load_group(n, kbase + off, vbase + off, good ? extent_of(hi - first, stride, d * PES) : 0,
+                   stride, std::integral_constant<bool, KV8>{});
+      }
+    } else {
+      ok_rows = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int pos = lo + c * KT + prow + j * Geo::RPL;
+        const int id = table[min(pos, hi - 1) >> a.bs_shift];
+        const bool good = (unsigned)id < num_blocks;
+        const bool in = pos < hi && good;
+        bad_block |= pos < hi && !good;
+        ok_rows |= (unsigned)(in && col_ok) << j;
+        const int64_t off = (in ? ((int64_t)id << a.bs_shift) + (pos & bs_mask) : (int64_t)0) *
+                                stride + (col_ok ? 8 * pcol * PES : 0);
+        if constexpr (KV8) {
+          const u32x2 k2 = *reinterpret_cast<const u32x2*>(kbase + off);
+          const u32x2 v2 = *reinterpret_cast<const u32x2*>(vbase + off);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            kr[j].w[e] = k2[e];
+            vr[j].w[e] = v2[e];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < Piece8<T>::W; e += 4) {
+            const u32x4 k4 = *reinterpret_cast<const u32x4*>(kbase + off + 4 * e);
+            const u32x4 v4 = *reinterpret_cast<const u32x4*>(vbase + off + 4 * e);
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+              kr[j].w[e + f] = k4[f];
+              vr[j].w[e + f] = v4[f];
+            }
+          }
+        }
+      }
+    }
+  };
+  auto issue = [&](int i) {
+    if (i < ntc) issue_tree(i);
+    else issue_ctx(i - ntc);
+  };
+  // the tree's rows before they are staged: as the pool will hold them (fp8), and V
+  // without infinities and NaN, which must not reach the rows that do not see them
+  // (0 x inf): their keys are noted, and they are added to the results of those that do
+  auto prepare_tree = [&](int c) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int row = prow + j * Geo::RPL;
-      if constexpr (decltype(raw)::value) {  // fp8 bytes as loaded
+      if constexpr (KV8) {
+        const u32x4 k4 = widen8<T>(narrow8<T>(u32x4{kr[j].w[0], kr[j].w[1], kr[j].w[2], kr[j].w[3]}));
+        const u32x4 v4 = widen8<T>(narrow8<T>(u32x4{vr[j].w[0], vr[j].w[1], vr[j].w[2], vr[j].w[3]}));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          kr[j].w[e] = k4[e];
+          vr[j].w[e] = v4[e];
+        }
+      }
+      if (!piece_finite<T>(vr[j])) {
+        atomicOr(&odd_rows[c], 1ull << (opaque(prow) + j * Geo::RPL));
+#pragma unroll
+        for (int e = 0; e < Piece8<T>::W; ++e) {
+          if constexpr (ES == 4) {
+            if ((vr[j].w[e] & 0x7f800000u) == 0x7f800000u) vr[j].w[e] = 0u;
+          } else {
+            constexpr unsigned E = std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+            if ((vr[j].w[e] & E) == E) vr[j].w[e] &= 0xffff0000u;
+            if (((vr[j].w[e] >> 16) & E) == E) vr[j].w[e] &= 0x0000ffffu;
+          }
+        }
+      }
+    }
+  };
+  auto prepare_ctx = [&]() {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if constexpr (!WHOLE) {  // what does not exist as zeros
+        if (!((ok_rows >> j) & 1)) {
+#pragma unroll
+          for (int e = 0; e < Piece8<T>::W; ++e) kr[j].w[e] = vr[j].w[e] = 0u;
+        }
+      }
+      if constexpr (KV8) {
         const u32x4 k4 = widen8<T>(u32x2{kr[j].w[0], kr[j].w[1]});
         const u32x4 v4 = widen8<T>(u32x2{vr[j].w[0], vr[j].w[1]});
 #pragma unroll
@@ -549,309 +728,126 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
           vr[j].w[e] = v4[e];
         }
       }
+    }
+  };
+
+  auto step = [&](int i, auto is_tree) {
+    constexpr bool TREE = decltype(is_tree)::value;
+    char* const buf = RW == 1 ? buf0 : buf0 + ((i & 1) * Geo::BUF);
+    asm volatile("" ::: "memory");
+    if constexpr (TREE) prepare_tree(i);
+    else prepare_ctx();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int row = prow + j * Geo::RPL;
       *reinterpret_cast<Piece8<T>*>(buf + row * Geo::KPITCH + 8 * ES * pcol) = kr[j];
       *reinterpret_cast<Piece8<T>*>(buf + KT * Geo::KPITCH + row * Geo::VPITCH + 8 * ES * pcol) =
           vr[j];
     }
-  };
-  auto load = [&](int j, const char* kp, const char* vp) {
-    if constexpr (KV8) {
-      const u32x2 k2 = *reinterpret_cast<const u32x2*>(kp);
-      const u32x2 v2 = *reinterpret_cast<const u32x2*>(vp);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        kr[j].w[e] = k2[e];
-        vr[j].w[e] = v2[e];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < Piece8<T>::W; e += 4) {
-        const u32x4 k4 = *reinterpret_cast<const u32x4*>(kp + 4 * e);
-        const u32x4 v4 = *reinterpret_cast<const u32x4*>(vp + 4 * e);
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          kr[j].w[e + f] = k4[f];
-          vr[j].w[e + f] = v4[f];
-        }
-      }
+    const uint64_t bits = bits_next;
+    if (i + TEAMS < nch) {
+      if constexpr (TREE) issue(i + TEAMS);
+      else issue_ctx(i + TEAMS - ntc);
     }
-  };
-
-  // ---- context keys [lo, hi) through the block table (contexts end below 2^30)
-  const int lo = part * g.part_len;
-  const int hi = min(lo + g.part_len, g.ctx);
-  const int nch = hi > lo ? (hi - lo + KT - 1) / KT : 0;
-  bool bad_block = false;
-  if (nch > 0) {
-    const int32_t* __restrict__ table = a.block_tables + (int64_t)s * a.max_blk;
-    const unsigned row_stride = (unsigned)(a.hkv * d * PES);
-    const int64_t head = (int64_t)kvh * d * PES;
-    const char* kbase = static_cast<const char*>(a.k_pool) + head;
-    const char* vbase = static_cast<const char*>(a.v_pool) + head;
-    const int bs_mask = (1 << a.bs_shift) - 1;
-    const unsigned num_blocks = (unsigned)min(a.num_blocks, (int64_t)0x7fffffff);
-    // WHOLE: this lane's offset in a group of rows; columns past d lie past any end
-    const unsigned lane_off =
-        col_ok ? (unsigned)(lane / Geo::CPR) * row_stride + (unsigned)(8 * pcol * PES) : 0x80000000u;
-    const int blk_last = (hi - 1) >> a.bs_shift;
-    int blk0 = lo >> a.bs_shift;  // WHOLE: first entry in `entries`
-    int entries = 0;
-    auto window = [&](int first) {
-      blk0 = first;
-      entries = table[min(first + lane, blk_last)];
-      asm volatile("" : "+v"(entries));  // waits here, once in 64 blocks
-    };
-    int ent[PER];  // else: the next chunk's entries, row by row
-    auto fetch_ent = [&](int c) {
-      if constexpr (!WHOLE) {
+    if constexpr (RW != 1) __syncthreads();
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (active) {
+      floatx16 sc[Geo::ST];
+      tree_scores<T, DP, Geo::KPITCH, Geo::ST>(buf, st, sc, lane);
+      // keys of the chunk; none behind the end, of the tree only those this row sees
+      const int left = TREE ? g.n - i * KT : hi - lo - (i - ntc) * KT;
+      if (TREE || left < KT) {
+        uint64_t see = left < 64 ? (1ull << left) - 1ull : ~0ull;
+        if constexpr (TREE) see &= bits;
+        see >>= 4 * (lane >> 5);
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-          ent[j] = table[min(lo + c * KT + prow + j * Geo::RPL, hi - 1) >> a.bs_shift];
-      }
-    };
-    auto issue = [&](int c) {
-      if constexpr (WHOLE) {
-#pragma unroll
-        for (int n = 0; n < Geo::NG; ++n) {
-          const int first = lo + c * KT + wrow + n * Geo::GR;
-          const int blk = min(first, hi - 1) >> a.bs_shift;
-          if (blk - blk0 >= 64) window(blk);
-          const unsigned id = (unsigned)__builtin_amdgcn_readlane(entries, blk - blk0);
-          const bool good = id < num_blocks;
-          bad_block |= !good;
-          const int rows = good ? min(hi - first, Geo::GR) : 0;
-          const int extent = rows > 0 ? (rows - 1) * (int)row_stride + d * PES : 0;
-          // a block is less than 2^31 bytes
-          const uint64_t base = (uint64_t)(good ? id : 0u) * (row_stride << a.bs_shift) +
-                                (unsigned)(first & bs_mask) * row_stride;
-          const __amdgpu_buffer_rsrc_t krs = __builtin_amdgcn_make_buffer_rsrc(
-              const_cast<char*>(kbase + base), (short)0, extent, kRsrcWord3);
-          const __amdgpu_buffer_rsrc_t vrs = __builtin_amdgcn_make_buffer_rsrc(
-              const_cast<char*>(vbase + base), (short)0, extent, kRsrcWord3);
-#pragma unroll
-          for (int i = 0; i < Geo::PG; ++i) {
-            const int j = n * Geo::PG + i;
-            const unsigned off = lane_off + i * Geo::RPL * row_stride;
-            if constexpr (KV8) {
-              const u32x2 k2 =
-                  __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(krs, off, 0, 0));
-              const u32x2 v2 =
-                  __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vrs, off, 0, 0));
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                kr[j].w[e] = k2[e];
-                vr[j].w[e] = v2[e];
-              }
-            } else {
-#pragma unroll
-              for (int e = 0; e < Piece8<T>::W; e += 4) {
-                const u32x4 k4 = __builtin_bit_cast(
-                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, off + 4 * e, 0, 0));
-                const u32x4 v4 = __builtin_bit_cast(
-                    u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, off + 4 * e, 0, 0));
-#pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                  kr[j].w[e + f] = k4[f];
-                  vr[j].w[e + f] = v4[f];
-                }
-              }
-            }
-          }
-        }
-      } else {
-        ok_rows = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const int pos = lo + c * KT + prow + j * Geo::RPL;
-          const bool good = (unsigned)ent[j] < num_blocks;
-          const bool in = pos < hi && good;
-          bad_block |= pos < hi && !good;
-          ok_rows |= (unsigned)(in && col_ok) << j;
-          const int64_t off = (in ? ((int64_t)ent[j] << a.bs_shift) + (pos & bs_mask) : (int64_t)0) *
-                                  row_stride + (col_ok ? 8 * pcol * PES : 0);
-          load(j, kbase + off, vbase + off);
-        }
-      }
-    };
-    if (WHOLE) window(blk0);
-    if (team < nch) {
-      fetch_ent(team);
-      issue(team);
-      fetch_ent(min(team + TEAMS, nch - 1));
-    }
-    for (int c = team; c < nch; c += TEAMS) {
-      char* buf = RW == 1 ? buf0 : buf0 + ((c & 1) * Geo::BUF);
-      stage(buf, !WHOLE, std::integral_constant<bool, KV8>{});
-      if (c + TEAMS < nch) {
-        issue(c + TEAMS);
-        fetch_ent(min(c + 2 * TEAMS, nch - 1));
-      }
-      if constexpr (RW != 1) __syncthreads();
-      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (active) {
-        const int cb = lo + c * KT;
-        floatx16 sc[Geo::ST];
-        tree_scores<T, DP, Geo::KPITCH, Geo::ST>(buf, st, sc, lane);
-        if (cb + KT > hi) {
-          const int left = hi - cb - 4 * (lane >> 5);
-#pragma unroll
-          for (int t = 0; t < Geo::ST; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (32 * t + (r & 3) + 8 * (r >> 2) >= left) sc[t][r] = -INFINITY;
-        }
-        tree_update<T, DP, Geo::VPITCH, Geo::ST>(buf + KT * Geo::KPITCH, sc, a.scale_log2, st,
-                                                 lane);
-      }
-    }
-  }
-
-  // ---- the tree's keys, in the last partition
-  if (part == g.nparts - 1) {
-    const int64_t* mrow = a.masks + tok * a.mask_words;
-    const int64_t row_stride = (int64_t)a.hkv * d;
-    const int ntc = (g.n + KT - 1) / KT;
-    for (int c0 = 0; c0 < ntc; c0 += TEAMS) {
-      const int c = c0 + team;
-      char* const buf = buf0;
-      __syncthreads();  // every wavefront is done with the buffers (and odd_rows)
-      if (tl == 0) odd_rows[team] = 0;
-      if constexpr (RW != 1) __syncthreads();
-      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (c < ntc) {
-        ok_rows = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const int row = c * KT + prow + j * Geo::RPL;
-          const bool in = row < g.n && col_ok;
-          ok_rows |= (unsigned)in << j;
-          const int64_t off = ((int64_t)(g.q_begin + (in ? row : 0)) * row_stride +
-                               (int64_t)kvh * d + (col_ok ? 8 * pcol : 0)) * ES;
-#pragma unroll
-          for (int e = 0; e < Piece8<T>::W; e += 4) {
-            u32x4 k4 = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k_new) + off + 4 * e);
-            u32x4 v4 = *reinterpret_cast<const u32x4*>(static_cast<const char*>(a.v_new) + off + 4 * e);
-            if constexpr (KV8) {  // the values the pool will hold
-              k4 = widen8<T>(narrow8<T>(k4));
-              v4 = widen8<T>(narrow8<T>(v4));
-            }
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-              kr[j].w[e + f] = k4[f];
-              vr[j].w[e + f] = v4[f];
-            }
-          }
-          // A V row that is not finite must not reach the rows that do not see
-          // it (0 x inf): it is staged as zeros and added below where it is seen
-          if (in && !piece_finite<T>(vr[j])) {
-            atomicOr(&odd_rows[team], 1ull << (row - c * KT));
-          }
-        }
-      }
-      if constexpr (RW != 1) __syncthreads();
-      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      const unsigned long long odd = odd_rows[team];
-      if (c < ntc) {
-        if (odd != 0) {
-#pragma unroll
-          for (int j = 0; j < PER; ++j)
-            if ((odd >> (prow + j * Geo::RPL)) & 1) {
-#pragma unroll
-              for (int e = 0; e < Piece8<T>::W; ++e) {
-                // element-wise: the row's finite values stay
-                if constexpr (ES == 4) {
-                  if ((vr[j].w[e] & 0x7f800000u) == 0x7f800000u) vr[j].w[e] = 0u;
-                } else {
-                  constexpr unsigned E = std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
-                  if ((vr[j].w[e] & E) == E) vr[j].w[e] &= 0xffff0000u;
-                  if (((vr[j].w[e] >> 16) & E) == E) vr[j].w[e] &= 0x0000ffffu;
-                }
-              }
-            }
-        }
-        stage(buf, true, std::false_type{});
-      }
-      if constexpr (RW != 1) __syncthreads();
-      else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (c < ntc && active) {
-        const int kb = c * KT;
-        // this row's bits of the chunk's keys, none behind the run's end
-        uint64_t bits = (uint64_t)mrow[kb >> 6] >> (kb & 63);
-        if (g.n - kb < 64) bits &= (1ull << (g.n - kb)) - 1ull;
-        floatx16 sc[Geo::ST];
-        tree_scores<T, DP, Geo::KPITCH, Geo::ST>(buf, st, sc, lane);
-#pragma unroll
-        for (int t = 0; t < Geo::ST; ++t) {
-          const unsigned mine = (unsigned)(bits >> (32 * t)) >> (4 * (lane >> 5));
+        for (int t = 0; t < Geo::ST; ++t)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (!((mine >> ((r & 3) + 8 * (r >> 2))) & 1u)) sc[t][r] = -INFINITY;
-        }
-        tree_update<T, DP, Geo::VPITCH, Geo::ST>(buf + KT * Geo::KPITCH, sc, a.scale_log2, st,
-                                                 lane);
-        unsigned long long seen_odd = odd;
-        while (seen_odd != 0) {  // uniform
-          const int k = __builtin_ctzll(seen_odd);
-          seen_odd &= seen_odd - 1;
-          const T* vrow = static_cast<const T*>(a.v_new) +
-                          (int64_t)(g.q_begin + kb + k) * row_stride + (int64_t)kvh * d;
-          if ((bits >> k) & 1u) {
-#pragma unroll
-            for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const int dim = 32 * dt + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                float x = dim < d ? (float)vrow[dim] : 0.f;
-                if constexpr (KV8) {  // past the fp8 range: NaN, as the pool will hold
-                  if (!(fabsf(x) <= 464.f)) x = NAN;
-                }
-                if (!(fabsf(x) < INFINITY)) st.o[dt][r] += x;
-              }
-          }
+            if (!(((unsigned)(see >> (32 * t)) >> ((r & 3) + 8 * (r >> 2))) & 1u))
+              sc[t][r] = -INFINITY;
+      }
+      tree_update<T, DP, Geo::VPITCH, Geo::ST>(buf + KT * Geo::KPITCH, sc, a.scale_log2, st, lane);
+    }
+  };
+  if (WHOLE) asm volatile("" : "+v"(entries));
+  if (team < nch) issue(team);
+  int i = team;
+  for (; i < ntc; i += TEAMS) step(i, std::true_type{});
+  for (; i < nch; i += TEAMS) step(i, std::false_type{});
+  if (bad_block && a.status) atomicOr(a.status, PKV_STATUS_BAD_BLOCK);
+
+  // ---- results, through LDS so that whole rows are stored
+  const int64_t u = g.slot;
+  // 4 dims from col on of row `row` of this tile: what it sees of the tree's values
+  // that are not finite (as the pool will hold them)
+  auto add_odd = [&](floatx4 o, int row, int col) {
+    for (int c = 0; c < ntc; ++c) {
+      unsigned long long seen = odd_rows[c];
+      if (seen == 0) continue;  // uniform
+      const uint64_t vis = (uint64_t)a.masks[(int64_t)token_of(r0 + row) * a.mask_words +
+                                             (c * KT >> 6)] >> (c * KT & 63);
+      for (; seen != 0; seen &= seen - 1) {
+        const int k = __builtin_ctzll(seen);
+        const T* vrow = static_cast<const T*>(a.v_new) +
+                        (int64_t)(g.q_begin + c * KT + k) * row_elems + (int64_t)kvh * d + col;
+        if (!((vis >> k) & 1u)) continue;
+        for (int e = 0; e < 4; ++e) {
+          float x = (float)vrow[e];
+          if (KV8 && !(fabsf(x) <= 464.f)) x = NAN;
+          if (!(fabsf(x) < INFINITY)) o[e] += x;
         }
       }
     }
-  }
-  if (bad_block && a.status) atomicOr(a.status, PKV_STATUS_BAD_BLOCK);
-
-  // ---- results
-  const int64_t u = g.slot;
+    return o;
+  };
   if constexpr (RW != 1) {
     const float L = half_sum(st.l);
+    __syncthreads();  // the chunk buffers are no longer read
+    if (!active) return;
+    float* const ob = reinterpret_cast<float*>(lds) + w * 32 * Geo::OPITCH;
+    float* const mine = ob + (lane & 31) * Geo::OPITCH + 4 * (lane >> 5);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<floatx4*>(mine + 32 * dt + 8 * q4) =
+            floatx4{st.o[dt][4 * q4], st.o[dt][4 * q4 + 1], st.o[dt][4 * q4 + 2],
+                    st.o[dt][4 * q4 + 3]};
+    const bool split = g.nparts > 1;
+    const float inv = split ? 1.f : L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
     const int row = 32 * w + (lane & 31);
-    if (!active || row >= rows_here) return;
-    if (g.nparts > 1) {
-      float* po = a.ws_o + (u * Geo::ROWS + row) * d;
-#pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const int dim = 32 * dt + 8 * q4 + 4 * (lane >> 5);
-          if (dim < d)
-            *reinterpret_cast<floatx4*>(po + dim) =
-                floatx4{st.o[dt][4 * q4], st.o[dt][4 * q4 + 1], st.o[dt][4 * q4 + 2],
-                        st.o[dt][4 * q4 + 3]};
-        }
-      if (lane < 32) {
-        a.ws_ml[(u * Geo::ROWS + row) * 2] = st.m;
-        a.ws_ml[(u * Geo::ROWS + row) * 2 + 1] = L;
+    if (lane < 32 && row < rows_here) {
+      if (split) {
+        *reinterpret_cast<float2*>(a.ws_ml + (u * Geo::ROWS + row) * 2) = float2{st.m, L};
+      } else if (a.lse) {
+        a.lse[row_of(opaque(rr))] = L == 0.f ? INFINITY : (st.m + log2f(L)) * kLn2f;
       }
-    } else {
-      const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-      T* po = static_cast<T*>(a.out) + qrow * d;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wavefront's own rows
+    constexpr int LPR = DP / 4;        // lanes per row
+    constexpr int RPI = 64 / LPR;      // rows per step
+    const int col = 4 * (lane % LPR);
+#pragma unroll 1
+    for (int k = 0; k < 32; k += RPI) {
+      const int rw = k + lane / LPR;
+      const float wt = __shfl(inv, rw, 64);
+      floatx4 o = *reinterpret_cast<const floatx4*>(ob + rw * Geo::OPITCH + col);
+      const int row2 = 32 * w + rw;
+      if (row2 >= rows_here || col >= d) continue;
+      if (ntc > 0) o = add_odd(o, row2, col);
+      if (split) {
+        *reinterpret_cast<floatx4*>(a.ws_o + (u * Geo::ROWS + row2) * d + col) = o;
+      } else {
+        const int rg = r0 + row2;
+        const int nd = rg / G;
+        T v[4];
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const int dim = 32 * dt + 8 * q4 + 4 * (lane >> 5);
-          if (dim < d) {
-            T v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (T)(st.o[dt][4 * q4 + e] * inv);
-            __builtin_memcpy(po + dim, v, sizeof(v));
-          }
-        }
-      if (lane < 32 && a.lse) a.lse[qrow] = L == 0.f ? INFINITY : (st.m + log2f(L)) * kLn2f;
+        for (int e = 0; e < 4; ++e) v[e] = (T)(o[e] * wt);
+        __builtin_memcpy(static_cast<T*>(a.out) +
+                             ((int64_t)(g.q_begin + nd) * a.hq + kvh * G + (rg - nd * G)) * d + col,
+                         v, sizeof(v));
+      }
     }
   } else {
     float* ob = reinterpret_cast<float*>(lds);  // [wave][32][OPITCH]
@@ -896,6 +892,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
       for (int ww = 0; ww < kTreeWaves; ++ww)
         if (wt[ww] != 0.f)
           o += wt[ww] * *reinterpret_cast<const floatx4*>(ob + (ww * 32 + row) * Geo::OPITCH + col);
+      if (ntc > 0) o = add_odd(o, row, col);
       if (g.nparts > 1) {
         *reinterpret_cast<floatx4*>(a.ws_o + (u * Geo::ROWS + row) * d + col) = o;
       } else {
@@ -1079,8 +1076,6 @@ int log2_pow2(int v) {
   if (v <= 0 || (v & (v - 1)) != 0) return -1;
   return __builtin_ctz((unsigned)v);
 }
-
-constexpr int kTreeMaxNodes = 4096;
 
 }  // namespace
 }  // namespace pkv
