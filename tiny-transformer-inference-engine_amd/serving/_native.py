@@ -245,21 +245,23 @@ def stream_ptr(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
-@contextlib.contextmanager
-def _switched(device):
-    with torch.cuda.device(device):
-        yield
+# kernels are launched on the current device, whichever device's stream they are
+# given: make_current(t.device) before, restore() with its result after
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-_HERE = contextlib.nullcontext()
+def make_current(device: torch.device):
+    """The index of the device that was current, None if `device` was already."""
+    here = _get_device()
+    if device.index is None or device.index == here:
+        return None
+    torch.cuda.set_device(device)
+    return here
 
 
-def on_device(device: torch.device):
-    """A context in which `device` is the current one: kernels are launched on
-    the current device, whichever device's stream they are given."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _HERE
-    return _switched(device)
+def restore(previous) -> None:
+    if previous is not None:
+        torch.cuda.set_device(previous)
 
 
 def ptr(t) -> int | None:

@@ -211,24 +211,30 @@ class KVPool:
             raise ValueError(f"{what}: {n} paths, {tree.num_seqs} trees, {meta.num_seqs} sequences")
         if meta.block_size != self.block_size:
             raise ValueError(f"{what}: blocks of {meta.block_size}, the pool's have {self.block_size}")
-        ts = (k_rows, v_rows, accepted.path, accepted.lens, tree.query_start_loc,
-              meta.block_tables, meta.start_pos)
-        if any(t.device != self.device for t in ts):
-            raise RuntimeError(f"{what}: rows and metadata must be on {self.device}")
-        if any(t.dtype != torch.int32 or not t.is_contiguous() for t in ts[2:]):
-            raise ValueError(f"{what}: paths, lengths and metadata must be contiguous int32")
-        k, v = k_rows.contiguous(), v_rows.contiguous()
+        path, lens, qsl = accepted.path, accepted.lens, tree.query_start_loc
+        table, start = meta.block_tables, meta.start_pos
+        dev = self.device
+        if not (k_rows.device == v_rows.device == path.device == lens.device == qsl.device
+                == table.device == start.device == dev):
+            raise RuntimeError(f"{what}: rows and metadata must be on {dev}")
+        for t in (path, lens, qsl, table, start):
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError(f"{what}: paths, lengths and metadata must be contiguous int32")
+        k = k_rows if k_rows.is_contiguous() else k_rows.contiguous()
+        v = v_rows if v_rows.is_contiguous() else v_rows.contiguous()
         row = self.num_kv_heads * self.head_dim
         status = self._status()
-        with _native.on_device(self.device):
+        previous = _native.make_current(dev)
+        try:
             rc = _native.calls().pkv_write_accepted(
                 self.flat_k[0].data_ptr(), self.flat_v[0].data_ptr(), 2 * self.num_slots * row,
                 self.num_layers, self.num_blocks, self.block_size, k.data_ptr(), v.data_ptr(),
-                tree.num_tokens * row, meta.block_tables.data_ptr(), meta.block_tables.shape[1],
-                meta.start_pos.data_ptr(), tree.query_start_loc.data_ptr(),
-                accepted.path.data_ptr(), accepted.lens.data_ptr(), n, tree.num_tokens, depth,
-                row, _native.kv_code(k.dtype, self.dtype), _native.ptr(status),
-                _native.stream_ptr(self.device))
+                tree.num_tokens * row, table.data_ptr(), table.shape[1], start.data_ptr(),
+                qsl.data_ptr(), path.data_ptr(), lens.data_ptr(), n, tree.num_tokens, depth, row,
+                _native.kv_code(k.dtype, self.dtype), _native.ptr(status),
+                _native.stream_ptr(dev))
+        finally:
+            _native.restore(previous)
         _native.check(rc, "pkv_write_accepted")
         self._raise_status(status, what)
 

@@ -34,8 +34,8 @@ class PagedBatchMeta:
     max_q_len: int
     max_kv_len: int
     block_size: int
-    # seq_lens, start_pos and positions as one contiguous view (pack_batch_meta
-    # lays them out back to back), so a decode step advances them with one add
+    # seq_lens, start_pos and positions at the front of one contiguous tensor (both
+    # packers lay them out back to back), so a decode step advances them with one add
     step_view: torch.Tensor | None = None
     # int64 [T], build_batch_meta only: each token's pool slot (KVPool.write's
     # slot_mapping), NO_SLOT behind the last token
@@ -50,11 +50,11 @@ class PagedBatchMeta:
         start_pos and positions + 1 (one kernel when they share step_view)."""
         v = self.step_view
         n, t = self.num_seqs, self.num_tokens
-        if (v is not None and v.numel() == 2 * n + t and v.dtype == torch.int32
+        if (v is not None and v.numel() >= 2 * n + t and v.dtype == torch.int32
                 and self.seq_lens.data_ptr() == v.data_ptr()
                 and self.start_pos.data_ptr() == v.data_ptr() + 4 * n
                 and self.positions.data_ptr() == v.data_ptr() + 8 * n):
-            v.add_(1)
+            (v if v.numel() == 2 * n + t else v[:2 * n + t]).add_(1)
             return
         self.positions.add_(1)
         self.start_pos.add_(1)
@@ -154,10 +154,11 @@ def pack_batch_meta(block_tables, query_start_loc, positions, T: int, device,
 NO_SLOT = -(1 << 63)  # a slot that an append skips
 
 
-@dataclass
+@dataclass(frozen=True)
 class DeviceTables:
     """Block tables of a running batch on the device, and the blocks it may
-    still take: int32 tensors of one device, contiguous."""
+    still take: contiguous int32 tensors of one device, checked when the object
+    is made (its fields are not assigned again)."""
     block_tables: torch.Tensor  # [N, max_blocks]
     blocks_held: torch.Tensor   # [N] blocks each row holds
     ctx_lens: torch.Tensor      # [N] tokens whose K/V are in the pool
@@ -165,6 +166,21 @@ class DeviceTables:
     free_cursor: torch.Tensor   # [1] the next of them
     block_size: int
     num_blocks: int             # the pool's
+
+    def __post_init__(self):
+        bt = self.block_tables
+        if bt.dim() != 2:
+            raise ValueError("DeviceTables: block_tables must be [N, max_blocks]")
+        n = bt.shape[0]
+        for name, numel in (("block_tables", bt.numel()), ("blocks_held", n), ("ctx_lens", n),
+                            ("free_blocks", self.free_blocks.numel()), ("free_cursor", 1)):
+            t = getattr(self, name)
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                raise ValueError(f"DeviceTables: {name} must be a contiguous int32 tensor")
+            if t.device != bt.device:
+                raise RuntimeError(f"DeviceTables: {name} on {t.device}, block_tables on {bt.device}")
+            if t.numel() != numel:
+                raise ValueError(f"DeviceTables: {name} has {t.numel()} elements, expected {numel}")
 
     @classmethod
     def from_host(cls, tables, ctx_lens, free_blocks, max_blocks: int, block_size: int,
@@ -187,23 +203,12 @@ class DeviceTables:
                    free_blocks=i32(free_blocks), free_cursor=i32([0]), block_size=block_size,
                    num_blocks=num_blocks)
 
-    def check(self, what: str) -> None:
-        """Types, shapes, device and layout of the tensors (no values)."""
-        bt = self.block_tables
-        _native.require_device(bt, what=what)
-        if bt.dim() != 2:
-            raise ValueError(f"{what}: block_tables must be [N, max_blocks]")
-        n = bt.shape[0]
-        for name, t, numel in (("block_tables", bt, bt.numel()), ("blocks_held", self.blocks_held, n),
-                               ("ctx_lens", self.ctx_lens, n),
-                               ("free_blocks", self.free_blocks, self.free_blocks.numel()),
-                               ("free_cursor", self.free_cursor, 1)):
-            if t.dtype != torch.int32 or not t.is_contiguous():
-                raise ValueError(f"{what}: {name} must be a contiguous int32 tensor")
-            if t.device != bt.device:
-                raise RuntimeError(f"{what}: {name} on {t.device}, block_tables on {bt.device}")
-            if t.numel() != numel:
-                raise ValueError(f"{what}: {name} has {t.numel()} elements, expected {numel}")
+    def _after(self, blocks_held, ctx_lens, free_cursor) -> "DeviceTables":
+        """The same tables in a later state (tensors of the checked kind)."""
+        new = object.__new__(DeviceTables)
+        new.__dict__.update(self.__dict__, blocks_held=blocks_held, ctx_lens=ctx_lens,
+                            free_cursor=free_cursor)
+        return new
 
 
 def raise_step_status(status: torch.Tensor, what: str) -> None:
@@ -225,8 +230,6 @@ def raise_step_status(status: torch.Tensor, what: str) -> None:
 
 
 def _status_ptr(status, device, what):
-    if status is None:
-        return None
     if status.dtype != torch.int32 or status.numel() != 1 or status.device != device:
         raise ValueError(f"{what}: status must be one int32 on {device}")
     return status.data_ptr()
@@ -247,36 +250,40 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     free blocks, a row past max_blocks or a length out of bounds nothing is taken
     (all or nothing), which `status` (int32 [1], zeroed by the caller, read with
     raise_step_status) reports. No host synchronisation."""
-    tables.check("build_batch_meta")
-    dev = tables.block_tables.device
-    n, max_blocks = tables.block_tables.shape
-    if q_lens.dtype != torch.int32 or q_lens.numel() != n or q_lens.device != dev:
+    bt = tables.block_tables
+    _native.require_device(bt, what="build_batch_meta")
+    dev = bt.device
+    n, max_blocks = bt.shape
+    if q_lens.dtype != torch.int32 or q_lens.device != dev or q_lens.numel() != n:
         raise ValueError(f"build_batch_meta: q_lens must be int32 [{n}] on {dev}")
-    if num_tokens < 0 or max_q_len < 0:
+    T, max_q_len = int(num_tokens), int(max_q_len)
+    if T < 0 or max_q_len < 0:
         raise ValueError("build_batch_meta: num_tokens and max_q_len must be >= 0")
-    T = int(num_tokens)
-    with _native.on_device(dev):
+    q = q_lens if q_lens.is_contiguous() else q_lens.contiguous()
+    bs = tables.block_size
+    free = tables.free_blocks
+    previous = _native.make_current(dev)
+    try:
         # seq_lens, start_pos and positions back to back, as pack_batch_meta's
-        i32 = torch.empty(5 * n + 2 + T, dtype=torch.int32, device=dev)
+        i32 = bt.new_empty(5 * n + 2 + T)
         slots = torch.empty(T, dtype=torch.int64, device=dev)
-        seq_lens, start_pos, positions, qsl, held, ctx, cursor = torch.split(
-            i32, [n, n, T, n + 1, n, n, 1])
+        at = i32.data_ptr()
+        held, ctx = at + 4 * (3 * n + 1 + T), at + 4 * (4 * n + 1 + T)
         rc = _native.calls().pkv_build_step(
-            _native.ptr(tables.block_tables), max_blocks, _native.ptr(tables.blocks_held),
-            _native.ptr(tables.ctx_lens), _native.ptr(q_lens.contiguous()), n,
-            _native.ptr(tables.free_blocks), tables.free_blocks.numel(),
-            _native.ptr(tables.free_cursor), tables.block_size, tables.num_blocks, T,
-            int(max_q_len), held.data_ptr(), ctx.data_ptr(), cursor.data_ptr(), qsl.data_ptr(),
-            seq_lens.data_ptr(), start_pos.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-            _status_ptr(status, dev, "build_batch_meta"), _native.stream_ptr(dev))
-    _native.check(rc, "build_batch_meta")
-    meta = PagedBatchMeta(
-        block_tables=tables.block_tables, seq_lens=seq_lens, query_start_loc=qsl,
-        start_pos=start_pos, positions=positions, num_seqs=n, num_tokens=T,
-        max_blocks=max_blocks, max_q_len=int(max_q_len),
-        max_kv_len=int(max_kv_len) if max_kv_len > 0 else max_blocks * tables.block_size,
-        block_size=tables.block_size, step_view=i32[:2 * n + T], slot_mapping=slots)
-    after = DeviceTables(block_tables=tables.block_tables, blocks_held=held, ctx_lens=ctx,
-                         free_blocks=tables.free_blocks, free_cursor=cursor,
-                         block_size=tables.block_size, num_blocks=tables.num_blocks)
-    return meta, after
+            bt.data_ptr(), max_blocks, tables.blocks_held.data_ptr(), tables.ctx_lens.data_ptr(),
+            q.data_ptr(), n, free.data_ptr(), free.numel(), tables.free_cursor.data_ptr(), bs,
+            tables.num_blocks, T, max_q_len, held, ctx, ctx + 4 * n, at + 4 * (2 * n + T), at,
+            at + 4 * n, at + 8 * n, slots.data_ptr(),
+            None if status is None else _status_ptr(status, dev, "build_batch_meta"),
+            _native.stream_ptr(dev))
+    finally:
+        _native.restore(previous)
+    if rc:
+        _native.check(rc, "build_batch_meta")
+    seq_lens, start_pos, positions, qsl, held, ctx, cursor = i32.split_with_sizes(
+        (n, n, T, n + 1, n, n, 1))
+    if max_kv_len <= 0:
+        max_kv_len = max_blocks * bs
+    meta = PagedBatchMeta(bt, seq_lens, qsl, start_pos, positions, n, T, max_blocks, max_q_len,
+                          int(max_kv_len), bs, i32, slots)
+    return meta, tables._after(held, ctx, cursor)

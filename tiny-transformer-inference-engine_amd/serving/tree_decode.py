@@ -60,9 +60,9 @@ class TreeAccept:
 def _int_tensor(t, dtype, numel, device, name, what):
     if t.dtype != dtype or t.device != device:
         raise ValueError(f"{what}: {name} must be {dtype} on {device} (got {t.dtype} on {t.device})")
-    if numel is not None and t.numel() != numel:
+    if t.numel() != numel:
         raise ValueError(f"{what}: {name} has {t.numel()} elements, expected {numel}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def build_tree_meta(tables: DeviceTables, parents: torch.Tensor, query_start_loc: torch.Tensor,
@@ -74,34 +74,40 @@ def build_tree_meta(tables: DeviceTables, parents: torch.Tensor, query_start_loc
     the trees' sizes, max_ctx_len (0: the table's capacity) the contexts. Rows
     behind the last sequence get empty masks and position 0. `status` as in
     build_batch_meta."""
-    tables.check("build_tree_meta")
-    dev = tables.block_tables.device
-    n, max_blocks = tables.block_tables.shape
-    parents = _int_tensor(parents, torch.int32, None, dev, "parents", "build_tree_meta")
-    qsl = _int_tensor(query_start_loc, torch.int32, n + 1, dev, "query_start_loc",
-                      "build_tree_meta")
+    what = "build_tree_meta"
+    bt = tables.block_tables
+    _native.require_device(bt, what=what)
+    dev = bt.device
+    n, max_blocks = bt.shape
+    T = parents.numel()
+    parents = _int_tensor(parents, torch.int32, T, dev, "parents", what)
+    qsl = _int_tensor(query_start_loc, torch.int32, n + 1, dev, "query_start_loc", what)
+    max_nodes = int(max_nodes)
     if not 0 <= max_nodes <= MAX_TREE_NODES:
-        raise ValueError(f"build_tree_meta: max_nodes must be in [0, {MAX_TREE_NODES}]")
-    T, words = parents.numel(), max(1, -(-int(max_nodes) // 64))
-    with _native.on_device(dev):
+        raise ValueError(f"{what}: max_nodes must be in [0, {MAX_TREE_NODES}]")
+    words = max(1, -(-max_nodes // 64))
+    previous = _native.make_current(dev)
+    try:
         masks = torch.empty((T, words), dtype=torch.int64, device=dev)
-        positions = torch.empty(T, dtype=torch.int32, device=dev)
+        positions = bt.new_empty(T)
         rc = _native.calls().pkv_tree_masks(
             masks.data_ptr(), words, positions.data_ptr(), parents.data_ptr(), qsl.data_ptr(),
-            tables.ctx_lens.data_ptr(), n, T, int(max_nodes),
-            _status_ptr(status, dev, "build_tree_meta"), _native.stream_ptr(dev))
-    _native.check(rc, "build_tree_meta")
-    return TreeMeta(block_tables=tables.block_tables, ctx_lens=tables.ctx_lens,
-                    query_start_loc=qsl, parents=parents, masks=masks, positions=positions,
-                    num_seqs=n, num_tokens=T, max_nodes=int(max_nodes),
-                    max_ctx_len=int(max_ctx_len) if max_ctx_len > 0 else
-                    max_blocks * tables.block_size,
-                    block_size=tables.block_size, num_blocks=tables.num_blocks)
+            tables.ctx_lens.data_ptr(), n, T, max_nodes,
+            None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
+    finally:
+        _native.restore(previous)
+    if rc:
+        _native.check(rc, what)
+    bs = tables.block_size
+    return TreeMeta(bt, tables.ctx_lens, qsl, parents, masks, positions, n, T, max_nodes,
+                    int(max_ctx_len) if max_ctx_len > 0 else max_blocks * bs, bs,
+                    tables.num_blocks)
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
     """t contiguous and 16-byte aligned, as the kernel reads it."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -118,12 +124,14 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     were there. A row that sees no key gives 0 and lse +inf. part_tokens (0:
     automatic) forces the length of the pieces a context is split into."""
     what = "paged_tree_attention"
-    _native.require_device(q, k, v, k_pool, v_pool, meta.masks, what=what)
+    masks = meta.masks
+    _native.require_device(q, k, v, k_pool, v_pool, masks, what=what)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, k_pool, v_pool)):
         raise NotImplementedError(
             f"{what} is forward-only (inference); run it under torch.no_grad()")
     dev = q.device
-    if any(t.device != dev for t in (k, v, k_pool, v_pool, meta.masks)):
+    if not (k.device == v.device == k_pool.device == v_pool.device == masks.device
+            == meta.block_tables.device == dev):
         raise RuntimeError(f"{what}: q, k, v, the pools and the metadata must share a device")
     if q.dim() != 3 or k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
         raise ValueError(f"{what}: q must be [T, Hq, D], the pools [num_blocks, block_size, Hkv, D]")
@@ -135,45 +143,51 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if T != meta.num_tokens or bs != meta.block_size:
         raise ValueError(f"{what}: {T} rows and blocks of {bs}, the metadata has "
                          f"{meta.num_tokens} and {meta.block_size}")
-    if k.dtype != q.dtype or v.dtype != q.dtype or v_pool.dtype != k_pool.dtype:
+    if not (k.dtype == v.dtype == q.dtype) or v_pool.dtype != k_pool.dtype:
         raise TypeError(f"{what}: q, k and v must share a dtype, and so must the pools")
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError(f"{what}: the pools must be contiguous")
     code = _native.kv_code(q.dtype, k_pool.dtype)
-    masks = meta.masks
     if masks.dtype != torch.int64 or masks.dim() != 2 or masks.shape[0] != T:
         raise ValueError(f"{what}: masks must be int64 [{T}, words]")
-    masks = masks.contiguous()
-    with _native.on_device(dev):
+    if lse is not None and (lse.shape != (T, hq) or lse.dtype != torch.float32
+                            or lse.device != dev or not lse.is_contiguous()):
+        raise ValueError(f"{what}: lse must be contiguous float32 [{T}, {hq}] on {dev}")
+    n, max_blk = meta.block_tables.shape
+    max_nodes, max_ctx = meta.max_nodes, meta.max_ctx_len
+    calls = _native.calls()
+    previous = _native.make_current(dev)
+    try:
         q, k, v = _dense(q), _dense(k), _dense(v)
+        if not masks.is_contiguous():
+            masks = masks.contiguous()
         dst = out
         if out is None:
             out = dst = torch.empty_like(q)
         elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
             raise ValueError(f"{what}: out must be {tuple(q.shape)} {q.dtype} on {dev}")
-        elif not out.is_contiguous() or out.data_ptr() % 16:
-            dst = _dense(out)  # holds the rows of no sequence
-        if lse is not None and (lse.shape != (T, hq) or lse.dtype != torch.float32
-                                or lse.device != dev or not lse.is_contiguous()):
-            raise ValueError(f"{what}: lse must be contiguous float32 [{T}, {hq}] on {dev}")
-        n, max_blk = meta.block_tables.shape
-        calls = _native.calls()
+        else:
+            dst = _dense(out)  # a copy holds the rows of no sequence, too
         nbytes = calls.pkv_tree_attention_workspace_bytes(
-            n, meta.max_nodes, hq, hkv, d, max_blk, bs, meta.max_ctx_len, part_tokens, code)
+            n, max_nodes, hq, hkv, d, max_blk, bs, max_ctx, part_tokens, code)
         # this call's own memory, from the allocator's pool of the current stream
         # (or of the graph being captured): nothing is shared between calls
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         rc = calls.pkv_paged_tree_attention(
-            dst.data_ptr(), _native.ptr(lse), q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            k_pool.data_ptr(), v_pool.data_ptr(), nb, bs,
+            dst.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), k.data_ptr(),
+            v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), nb, bs,
             meta.block_tables.data_ptr() if max_blk else None, max_blk,
             meta.ctx_lens.data_ptr(), meta.query_start_loc.data_ptr(), masks.data_ptr(),
-            masks.shape[1], n, T, meta.max_nodes, meta.max_ctx_len, hq, hkv, d,
-            float(scale if scale is not None and scale > 0 else 0.0), part_tokens, code,
-            _native.ptr(ws), nbytes, _status_ptr(status, dev, what), _native.stream_ptr(dev))
-        _native.check(rc, what)
+            masks.shape[1], n, T, max_nodes, max_ctx, hq, hkv, d,
+            float(scale) if scale is not None and scale > 0 else 0.0, part_tokens, code,
+            None if ws is None else ws.data_ptr(), nbytes,
+            None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
+        if rc:
+            _native.check(rc, what)
         if dst is not out:
             out.copy_(dst)
+    finally:
+        _native.restore(previous)
     return out
 
 
@@ -186,20 +200,24 @@ def tree_accept(picks: torch.Tensor, tokens: torch.Tensor, meta: TreeMeta, max_d
     distribution as it is), and each node's own."""
     what = "tree_accept"
     _native.require_device(picks, tokens, what=what)
-    dev = meta.parents.device
-    picks = _int_tensor(picks, torch.int64, meta.num_tokens, dev, "picks", what)
-    tokens = _int_tensor(tokens, torch.int64, meta.num_tokens, dev, "tokens", what)
+    parents, qsl, T, n = meta.parents, meta.query_start_loc, meta.num_tokens, meta.num_seqs
+    dev = parents.device
+    picks = _int_tensor(picks, torch.int64, T, dev, "picks", what)
+    tokens = _int_tensor(tokens, torch.int64, T, dev, "tokens", what)
+    max_depth = int(max_depth)
     if max_depth < 1:
         raise ValueError(f"{what}: max_depth must be at least 1")
-    n = meta.num_seqs
-    with _native.on_device(dev):
-        lens = torch.empty(n, dtype=torch.int32, device=dev)
-        path = torch.empty((n, max_depth), dtype=torch.int32, device=dev)
-        out = torch.empty((n, max_depth), dtype=torch.int64, device=dev)
+    previous = _native.make_current(dev)
+    try:
+        lens = qsl.new_empty(n)
+        path = qsl.new_empty((n, max_depth))
+        out = picks.new_empty((n, max_depth))
         rc = _native.calls().pkv_tree_accept(
             lens.data_ptr(), path.data_ptr(), out.data_ptr(), picks.data_ptr(),
-            tokens.data_ptr(), meta.parents.data_ptr(), meta.query_start_loc.data_ptr(), n,
-            meta.num_tokens, int(max_depth), _status_ptr(status, dev, what),
-            _native.stream_ptr(dev))
-    _native.check(rc, what)
-    return TreeAccept(lens=lens, path=path, tokens=out)
+            tokens.data_ptr(), parents.data_ptr(), qsl.data_ptr(), n, T, max_depth,
+            None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
+    finally:
+        _native.restore(previous)
+    if rc:
+        _native.check(rc, what)
+    return TreeAccept(lens, path, out)
