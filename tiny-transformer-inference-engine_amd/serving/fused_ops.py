@@ -341,21 +341,32 @@ def linear_swiglu(x: torch.Tensor, w_gate_up: torch.Tensor, b_gate_up: torch.Ten
     return out.view(*x.shape[:-1], h)
 
 
+def _check_kv_out(kv_out, shape, x, what):
+    for t in kv_out:
+        if (tuple(t.shape) != shape or t.dtype != x.dtype or t.device != x.device
+                or not t.is_contiguous()):
+            raise ValueError(f"{what}: kv_out must be contiguous {shape} {x.dtype} on {x.device}")
+
+
 def linear_rope_qkv(x: torch.Tensor, w_qkv: torch.Tensor, b_qkv: torch.Tensor | None,
                     positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, hq: int,
-                    hkv: int, d: int):
+                    hkv: int, d: int, kv_out=None):
     """q, k, v projections of x [T, d_model] with W = [Wq; Wk; Wv], q and k
     rotated at positions (fp32 tables cos / sin [max_pos, d/2]): contiguous
-    q [T, hq, d], k [T, hkv, d], v [T, hkv, d] (serving/paged_mqa.py:76-85)."""
+    q [T, hq, d], k [T, hkv, d], v [T, hkv, d] (serving/paged_mqa.py:76-85).
+    kv_out: the tensors to write k and v to (contiguous, of x's dtype)."""
     x2 = _as_rows(x)
     T = x2.shape[0]
     nq, nk = hq * d, hkv * d
+    if kv_out is not None:
+        _check_kv_out(kv_out, (T, hkv, d), x, "linear_rope_qkv")
     few = _linear_ok(x2, w_qkv, b_qkv, nq + 2 * nk)
     if not few and not (_tiles_ok(x2, w_qkv, b_qkv, True) and w_qkv.shape[0] == nq + 2 * nk
                         and d % 2 == 0):
         qkv = F.linear(x2, w_qkv, b_qkv)
-        return rope(qkv[:, :nq], qkv[:, nq:nq + nk], positions, cos, sin, v=qkv[:, nq + nk:],
-                    hq=hq, hkv=hkv, d=d)
+        q, k, v = rope(qkv[:, :nq], qkv[:, nq:nq + nk], positions, cos, sin, v=qkv[:, nq + nk:],
+                       hq=hq, hkv=hkv, d=d)
+        return (q, k, v) if kv_out is None else (q, kv_out[0].copy_(k), kv_out[1].copy_(v))
     _native.require_device(x2, w_qkv, positions, cos, sin, what="linear_rope_qkv")
     cos2, sin2, max_pos = _rope_tables(cos, sin, d, "linear_rope_qkv", not few)
     pos = positions if positions.dtype == torch.int32 else positions.to(torch.int32)
@@ -363,8 +374,7 @@ def linear_rope_qkv(x: torch.Tensor, w_qkv: torch.Tensor, b_qkv: torch.Tensor | 
     if pos.numel() != T:
         raise ValueError("linear_rope_qkv: positions and x disagree on the token count")
     q = x.new_empty((T, hq, d))
-    k = x.new_empty((T, hkv, d))
-    v = x.new_empty((T, hkv, d))
+    k, v = kv_out if kv_out is not None else (x.new_empty((T, hkv, d)), x.new_empty((T, hkv, d)))
     fn = _native.calls().pkv_linear_rope_qkv if few else _native.calls().pkv_linear_tiles_rope_qkv
     rc = fn(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), x2.data_ptr(), w_qkv.data_ptr(),
@@ -452,7 +462,7 @@ def linear_swiglu_rmsnorm(x: torch.Tensor, norm_weight: torch.Tensor, eps: float
 def linear_rope_qkv_rmsnorm(x: torch.Tensor, norm_weight: torch.Tensor, eps: float,
                             w_qkv: torch.Tensor, b_qkv: torch.Tensor | None,
                             positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
-                            hq: int, hkv: int, d: int):
+                            hq: int, hkv: int, d: int, kv_out=None):
     """linear_rope_qkv(rms_norm(x, norm_weight, eps), ...) with the norm
     taken in the projection kernel's prologue (bit-identical to the two
     calls)."""
@@ -461,7 +471,9 @@ def linear_rope_qkv_rmsnorm(x: torch.Tensor, norm_weight: torch.Tensor, eps: flo
     nq, nk = hq * d, hkv * d
     if not (_linear_ok(x2, w_qkv, b_qkv, nq + 2 * nk) and _norm_ok(x2, norm_weight)):
         return linear_rope_qkv(rms_norm(x, norm_weight, eps), w_qkv, b_qkv, positions, cos, sin,
-                               hq, hkv, d)
+                               hq, hkv, d, kv_out)
+    if kv_out is not None:
+        _check_kv_out(kv_out, (T, hkv, d), x, "linear_rope_qkv_rmsnorm")
     _native.require_device(x2, norm_weight, w_qkv, positions, cos, sin,
                            what="linear_rope_qkv_rmsnorm")
     cos2, sin2, max_pos = _rope_tables(cos, sin, d, "linear_rope_qkv_rmsnorm", False)
@@ -470,8 +482,7 @@ def linear_rope_qkv_rmsnorm(x: torch.Tensor, norm_weight: torch.Tensor, eps: flo
     if pos.numel() != T:
         raise ValueError("linear_rope_qkv_rmsnorm: positions and x disagree on the token count")
     q = x.new_empty((T, hq, d))
-    k = x.new_empty((T, hkv, d))
-    v = x.new_empty((T, hkv, d))
+    k, v = kv_out if kv_out is not None else (x.new_empty((T, hkv, d)), x.new_empty((T, hkv, d)))
     rc = _native.calls().pkv_linear_rope_qkv_rmsnorm(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), x2.data_ptr(), norm_weight.data_ptr(),
         float(eps), w_qkv.data_ptr(), _native.ptr(b_qkv), T, x2.shape[1], _x_stride(x2),

@@ -7,6 +7,8 @@ Entry points and their reference counterparts:
   generate_paged        serving/generation.py:91-110   greedy, one sequence
   prefill_seq           serving/generation.py:71-77
   decode_step           serving/generation.py:80-88
+  generate_speculative  no counterpart: generate_batched's tokens, several a
+                        step, by verifying a drafting function's trees
 
 The batched entry points share one driver (_drive): a _Cohort holds the
 calls' sequences, feeds the model one prefill step of whole prompts and then
@@ -23,8 +25,10 @@ from __future__ import annotations
 import torch
 
 from .batch import build_batch_step
+from .paged_meta import DeviceTables, build_batch_meta, raise_step_status
 from .sampling import greedy, sample
-from .sequence import Sequence
+from .sequence import Sequence, blocks_for
+from .tree_decode import MAX_TREE_NODES, build_tree_meta, tree_accept
 
 
 class _Cohort:
@@ -110,6 +114,82 @@ def generate_batched(model, prompts_ids, max_new_tokens, pool, alloc, block_size
         return [[] for _ in prompts_ids]
     with _Cohort(prompts_ids, block_size, alloc, _model_device(model)) as cohort:
         return _drive(model, pool, cohort, max_new_tokens, _greedy_ids)
+
+
+def _draft_tree(draft, history, limit):
+    """draft(history) -> (tokens, parents), checked; the nodes below the root as
+    (tokens, parents of the whole tree), at most `limit` of them."""
+    tokens, parents = draft(history)
+    tokens, parents = [int(t) for t in tokens][:limit], [int(p) for p in parents][:limit]
+    if len(tokens) != len(parents):
+        raise ValueError("a draft needs one parent per token")
+    for i, p in enumerate(parents):
+        if not -1 <= p < i:
+            raise ValueError(f"draft node {i}: parent {p} is neither -1 nor an earlier node")
+    return tokens, [p + 1 for p in parents]
+
+
+@torch.no_grad()
+def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft, block_size=16,
+                         max_drafts=15, max_depth=8):
+    """generate_batched on a ROCm device, several tokens a step. draft(token_ids)
+    is called per row and step with the row's tokens so far and proposes a tree
+    that goes on from the last of them: (tokens, parents), parents[i] the index of
+    the proposed token that token i follows, -1 for those that follow the last
+    token; at most max_drafts of them are used. The model verifies all rows' trees
+    in one pass and keeps, per row, the longest path of its own greedy choices and
+    the token after it, up to max_depth tokens: whatever is drafted, the tokens
+    are greedy ones. Rejected drafts take no pool slots."""
+    if max_new_tokens < 0:
+        raise ValueError("max_new_tokens must be >= 0")
+    if max_depth < 1 or not 0 <= max_drafts < MAX_TREE_NODES:
+        raise ValueError(f"need max_depth >= 1 and 0 <= max_drafts < {MAX_TREE_NODES}")
+    if not prompts_ids:
+        return []
+    if not all(prompts_ids):
+        raise ValueError("every prompt must contain at least one token")
+    if max_new_tokens == 0:
+        return [[] for _ in prompts_ids]
+    device = _model_device(model)
+    stock = []
+    with _Cohort(prompts_ids, block_size, alloc, device) as cohort:
+        first = _greedy_ids(model.forward_batch(cohort.prefill_batch(), pool))
+        rows = [list(ids) + [tok] for ids, tok in zip(prompts_ids, first)]
+        goal = [len(ids) + max_new_tokens for ids in prompts_ids]
+        # a row's last step may accept up to max_depth - 1 tokens past its goal
+        need = [blocks_for(g + max_depth, block_size) for g in goal]
+        held = [len(r.block_table) for r in cohort.rows]
+        try:
+            stock = alloc.allocate_n(sum(need) - sum(held))
+            tables = DeviceTables.from_host([r.block_table for r in cohort.rows],
+                                            [len(ids) for ids in prompts_ids], stock, max(need),
+                                            block_size, pool.num_blocks, device)
+            status = torch.zeros(1, dtype=torch.int32, device=device)
+            while any(len(r) < g for r, g in zip(rows, goal)):
+                tokens, parents, starts = [], [], [0]
+                for row, g in zip(rows, goal):
+                    if len(row) < g:  # a finished row takes no nodes
+                        t, p = _draft_tree(draft, list(row), max_drafts)
+                        tokens += [row[-1]] + t
+                        parents += [-1] + p
+                    starts.append(len(tokens))
+                i32 = torch.tensor(parents + starts, dtype=torch.int32, device=device)
+                ids = torch.tensor(tokens, dtype=torch.long, device=device)
+                tree = build_tree_meta(tables, i32[:len(parents)], i32[len(parents):],
+                                       1 + max_drafts, max(len(r) for r in rows), status=status)
+                logits, k_rows, v_rows = model.forward_tree(ids, pool, tree)
+                accepted = tree_accept(greedy(logits)[:, 0], ids, tree, max_depth, status=status)
+                meta, tables = build_batch_meta(tables, accepted.lens, len(rows) * max_depth,
+                                                max_depth, status=status)
+                pool.write_accepted(k_rows, v_rows, tree, accepted, meta)
+                # one copy to the host: lengths and tokens of the whole batch
+                new = torch.cat([accepted.lens[:, None].long(), accepted.tokens], 1).tolist()
+                for row, (n, *toks) in zip(rows, new):
+                    row += toks[:n]
+            raise_step_status(status, "generate_speculative")
+        finally:
+            alloc.free(stock)
+    return [row[len(ids):g] for row, ids, g in zip(rows, prompts_ids, goal)]
 
 
 def _default_tokenizer():

@@ -92,6 +92,26 @@ class PagedTransformer(nn.Module):
             x = x.index_select(0, meta.query_start_loc[1:].long() - 1)
         return self.lm_head(self.final_norm(x))
 
+    @torch.no_grad()
+    def forward_tree(self, input_ids, pool, tree):
+        """The nodes of drafted trees in one pass on a ROCm device: input_ids [T]
+        their tokens, tree a TreeMeta (serving.tree_decode). Returns the logits of
+        every node [T, vocab] and the nodes' K and V rows of all layers, each
+        [num_layers, T, Hkv, D] in the model's dtype, for KVPool.write_accepted;
+        the pool is read only."""
+        x = self.embedding(input_ids).contiguous()
+        if not x.is_cuda:
+            raise RuntimeError("forward_tree requires the model on a ROCm GPU device")
+        shape = (len(self.layers), x.shape[0], pool.num_kv_heads, pool.head_dim)
+        k_rows, v_rows = x.new_empty(shape), x.new_empty(shape)
+        attr = fused_ops.module_attr
+        for i, layer in enumerate(self.layers):
+            attr(layer, "attn").forward_tree_residual_(x, attr(layer, "attn_norm"), pool,
+                                                       layer.layer_idx, tree, k_rows[i],
+                                                       v_rows[i])
+            attr(layer, "mlp").forward_residual_(x, attr(layer, "mlp_norm"))
+        return self.lm_head(self.final_norm(x)), k_rows, v_rows
+
 
 def load_paged_model(ckpt_path, device):
     """Checkpoint {model, model_config, ...} -> (PagedTransformer, ModelConfig)

@@ -24,6 +24,7 @@ from . import fused_ops
 from .fused_ops import FusedRows
 from .layers import RoPE
 from .paged_meta import PagedBatchMeta, pack_batch_meta
+from .tree_decode import paged_tree_attention
 
 
 def _get_kv_pool(pool, layer_idx):
@@ -115,6 +116,24 @@ class MQA_Paged(nn.Module):
                                                     meta.positions, cos, sin, self.num_heads,
                                                     self.num_kv_heads, self.headdim)
         out = paged_attention_append_meta(q, k, v, pool, layer_idx, meta)
+        proj = attr(self, "out")
+        return fused_ops.linear_residual_(x, out.view(T, d_model), attr(proj, "weight"),
+                                          attr(proj, "bias"))
+
+    def forward_tree_residual_(self, x, norm, pool, layer_idx, tree, k_rows, v_rows):
+        """forward_meta_residual_ for the nodes of drafted trees (a TreeMeta,
+        serving.tree_decode): RoPE at the nodes' positions, each node attending to
+        its context in the pool, its ancestors and itself. The nodes' K/V rows are
+        written to k_rows, v_rows [T, Hkv, D] and not to the pool. Returns x."""
+        T, d_model = x.shape
+        w, b = self._qkv.get()
+        attr = fused_ops.module_attr
+        cos, sin = attr(self, "rope")._tables_fp32()
+        q, k, v = fused_ops.linear_rope_qkv_rmsnorm(
+            x, attr(norm, "weight"), norm.eps, w, b, tree.positions, cos, sin, self.num_heads,
+            self.num_kv_heads, self.headdim, kv_out=(k_rows, v_rows))
+        kp, vp = _get_kv_pool(pool, layer_idx)
+        out = paged_tree_attention(q, k, v, kp, vp, tree)
         proj = attr(self, "out")
         return fused_ops.linear_residual_(x, out.view(T, d_model), attr(proj, "weight"),
                                           attr(proj, "bias"))
