@@ -115,13 +115,13 @@ def check(p, out, lse, scale=None):
             tol = tol + 2.0 ** -25 * V1
     tol = tol + u * np.abs(eo) * (1 + 2.0 ** -6) + 1e-30
     got = np64(out)
-    assert np.isfinite(got).all()
-    assert (np.abs(got - eo) <= tol).all(), (np.abs(got - eo) / tol).max()
+    worst = float((np.abs(got - eo) / tol).max()) if np.isfinite(got).all() else np.nan
+    assert worst <= 1
     gl = np64(lse)
     fin = np.isfinite(el)
-    assert (np.isposinf(gl) == ~fin).all()
+    assert np.array_equal(np.isposinf(gl), ~fin)
     ltol = score + (L + 16) * E + np.abs(np.where(fin, el, 0)) * 2 * E + 1e-6
-    assert (np.abs(gl[fin] - el[fin]) <= ltol[fin]).all()
+    assert float((np.abs(gl[fin] - el[fin]) / ltol[fin]).max(initial=0)) <= 1
 
 
 BF, HF, F32, F8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn

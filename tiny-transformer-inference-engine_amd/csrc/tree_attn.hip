@@ -184,9 +184,12 @@ __device__ __forceinline__ void wave_scan2(int& x, int& y, int& tx, int& ty) {
 }
 
 // The unit of this workgroup, or false. Units are numbered by sequence, then
-// partition, kv head and tile; the row tiles of one (sequence, kv head, partition)
-// read the same keys, so each XCD (workgroup b runs on XCD b % 8) takes a
-// contiguous eighth of the numbers, and finds them in its L2. Every wavefront makes
+// partition, kv head and tile, those of split sequences (the largest) apart and
+// first, so that the last workgroups to start are the small ones (64 long-tailed
+// contexts: 80 us of attention and join in plain order); the row tiles of one
+// (sequence, kv head, partition) read the same keys, so each XCD (workgroup b runs
+// on XCD b % 8) takes a contiguous eighth of the numbers, and finds them in its L2.
+// Every wavefront makes
 // the plan for itself, one sequence a lane and round, so there is no barrier in it;
 // the later passes read the lengths from the L1.
 template <int ROWS>
@@ -202,55 +205,76 @@ __device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, TreeUnit& u) {
   const int rounds = (a.n_seq + 63) / 64;
   int part_len = a.part_tokens;
   if (part_len <= 0) {
-    float work = 0.f;
+    float work = 0.f, tiles = 0.f;
 #pragma unroll 1
     for (int r = 0; r < rounds; ++r) {
       int q, m, c;
       load(r, q, m, c, false);
+      tiles += (float)tiles_of(m);
       work += (float)tiles_of(m) * (float)c;
     }
-    work += lane_xor<1>(work);
-    work += lane_xor<2>(work);
-    work += lane_xor<4>(work);
-    work += lane_xor<8>(work);
-    work += lane_xor<16>(work);
-    work += lane_xor<32>(work);
-    // rounded up past the sum's own rounding, so that `slots` holds every partial
-    const float per = work / (float)a.units * 1.0001f;
+    auto sum = [](float x) {
+      x += lane_xor<1>(x);
+      x += lane_xor<2>(x);
+      x += lane_xor<4>(x);
+      x += lane_xor<8>(x);
+      x += lane_xor<16>(x);
+      return x + lane_xor<32>(x);
+    };
+    work = sum(work);
+    // every tile has one unit more than its share, so that those left of `units` are
+    // what the work is cut into: the batch runs in one round of workgroups where it
+    // can, and ends together. Rounded up past the sums' own rounding, so that `slots`
+    // holds every partial
+    const float want = fmaxf((float)a.units - sum(tiles), 0.5f * (float)a.units);
+    const float per = work / want * 1.0001f;
     part_len = max(per < 1e9f ? ((int)per + 64) & ~63 : 1 << 30, a.min_part);
     part_len = __builtin_amdgcn_readfirstlane(part_len);
   }
-  int total = 0;
+  int split = 0, whole = 0;  // units of split sequences, and of the others
 #pragma unroll 1
   for (int r = 0; r < rounds; ++r) {
     int q, m, c;
     load(r, q, m, c, flag);
-    total += tiles_of(m) * tree_parts(a, c, part_len);
+    const int parts = tree_parts(a, c, part_len);
+    const int k = tiles_of(m) * parts;
+    split += parts > 1 ? k : 0;
+    whole += parts > 1 ? 0 : k;
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) total += __shfl_xor(total, o, 64);
-  total = __builtin_amdgcn_readfirstlane(total);
-  // workgroup b: number b / 8 of XCD b % 8's eighth
-  const int xcd = blockIdx.x & 7;
-  const int mine = (int)((int64_t)total * xcd >> 3) + (int)(blockIdx.x >> 3);
-  const bool have = mine < (int)((int64_t)total * (xcd + 1) >> 3);
+  for (int o = 32; o > 0; o >>= 1) {
+    split += __shfl_xor(split, o, 64);
+    whole += __shfl_xor(whole, o, 64);
+  }
+  split = __builtin_amdgcn_readfirstlane(split);
+  whole = __builtin_amdgcn_readfirstlane(whole);
+  // workgroup b: number b / 8 of XCD b % 8's eighths, the split sequences' first
+  const int64_t xcd = blockIdx.x & 7;
+  const int s0 = (int)(split * xcd >> 3), s1 = (int)(split * (xcd + 1) >> 3);
+  const int w0 = (int)(whole * xcd >> 3), w1 = (int)(whole * (xcd + 1) >> 3);
+  const int nth = (int)(blockIdx.x >> 3);
+  const bool is_split = nth < s1 - s0;
+  const int mine = is_split ? s0 + nth : w0 + nth - (s1 - s0);
+  const bool have = is_split || mine < w1;
   if (!have && !flag) return false;
   bool found = false;
-  int run = 0, splits = 0;
+  int run = 0, slots = 0;
 #pragma unroll 1
   for (int r = 0; r < rounds && (flag || !found); ++r) {
     int q, m, c, tx, ty;
     load(r, q, m, c, false);
     const int parts = tree_parts(a, c, part_len);
     const int k = tiles_of(m) * parts;
-    int x = k, y = parts > 1 ? k : 0;
+    int x = parts > 1 ? 0 : k, y = parts > 1 ? k : 0;
     wave_scan2(x, y, tx, ty);
-    const int first = run + x, slot = splits + y;
+    const int slot = slots + y;
+    const int first = is_split ? slot : run + x;
     run += tx;
-    splits += ty;
+    slots += ty;
     if (flag && a.slots > 0 && 64 * r + lane < a.n_seq)
       a.recs[64 * r + lane] = int4{parts > 1 && m > 0 ? slot : -1, parts, q, m};
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(have && mine >= first && mine < first + k);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(have && (parts > 1) == is_split &&
+                                                     mine >= first && mine < first + k);
     if (hit != 0) {
       const int l = __builtin_ctzll(hit);
       found = true;
@@ -260,7 +284,7 @@ __device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, TreeUnit& u) {
       u.ctx = __builtin_amdgcn_readlane(c, l);
       u.nparts = __builtin_amdgcn_readlane(parts, l);
       u.tile = mine - __builtin_amdgcn_readlane(first, l);  // of all of the sequence's units
-      u.slot = __builtin_amdgcn_readlane(slot, l) + u.tile;
+      u.slot = mine;
     }
   }
   if (!found) return false;
@@ -779,6 +803,11 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
 
   // ---- results, through LDS so that whole rows are stored
   const int64_t u = g.slot;
+  auto some_odd = [&]() {
+    bool any = false;
+    for (int c = 0; c < ntc; ++c) any |= odd_rows[c] != 0;
+    return any;
+  };
   // 4 dims from col on of row `row` of this tile: what it sees of the tree's values
   // that are not finite (as the pool will hold them)
   auto add_odd = [&](floatx4 o, int row, int col) {
@@ -828,14 +857,15 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
     constexpr int LPR = DP / 4;        // lanes per row
     constexpr int RPI = 64 / LPR;      // rows per step
     const int col = 4 * (lane % LPR);
-#pragma unroll 1
+    const bool odd = some_odd();
+#pragma unroll 4
     for (int k = 0; k < 32; k += RPI) {
       const int rw = k + lane / LPR;
       const float wt = __shfl(inv, rw, 64);
       floatx4 o = *reinterpret_cast<const floatx4*>(ob + rw * Geo::OPITCH + col);
       const int row2 = 32 * w + rw;
       if (row2 >= rows_here || col >= d) continue;
-      if (ntc > 0) o = add_odd(o, row2, col);
+      if (odd) o = add_odd(o, row2, col);
       if (split) {
         *reinterpret_cast<floatx4*>(a.ws_o + (u * Geo::ROWS + row2) * d + col) = o;
       } else {
@@ -867,6 +897,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
       ml[(w * 32 + lane) * 2 + 1] = L1;
     }
     __syncthreads();
+    const bool odd = some_odd();
     const int row = tid >> 3;  // 8 threads a row
     if (row >= rows_here) return;
     float M = -INFINITY;
@@ -892,7 +923,7 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
       for (int ww = 0; ww < kTreeWaves; ++ww)
         if (wt[ww] != 0.f)
           o += wt[ww] * *reinterpret_cast<const floatx4*>(ob + (ww * 32 + row) * Geo::OPITCH + col);
-      if (ntc > 0) o = add_odd(o, row, col);
+      if (odd) o = add_odd(o, row, col);
       if (g.nparts > 1) {
         *reinterpret_cast<floatx4*>(a.ws_o + (u * Geo::ROWS + row) * d + col) = o;
       } else {
@@ -1027,7 +1058,8 @@ TreePlan tree_plan(int n_seq, int max_nodes, int hq, int hkv, int d, int max_blk
     p.slots = bound > p.min_part ? 2 * (int64_t)p.units : 0;
     p.grid = p.slots ? p.units + all : all;
   }
-  p.grid = (p.grid + 7) / 8 * 8;
+  // an XCD's two shares are each rounded up
+  p.grid = (p.grid + 7) / 8 * 8 + 8;
   if (p.slots) {
     const size_t recs = ((size_t)n_seq * sizeof(int4) + 255) & ~(size_t)255;
     p.o_off = recs;
