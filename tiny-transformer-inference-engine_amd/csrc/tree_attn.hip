@@ -73,6 +73,7 @@ struct TreeArgs {
   float scale_log2;
   int part_tokens;  // > 0: the partitions' length
   int min_part;     // else their least length
+  int max_parts;    // of one context, at most (longer ones then)
   int units;        // and the units wanted
   int slots;        // partial results the workspace holds; 0: no context is split
   int4* recs;       // [n_seq] first slot and partitions of a split sequence, else -1
@@ -133,24 +134,18 @@ struct TreeGeo {
   static_assert(64 % CPR == 0 && GR % RPL == 0 && NG * PG == PER && PER >= 1, "chunk split");
 };
 
-// Sequence s's run of nodes and context. False: it has no nodes, or its run lies
-// outside [0, T) or exceeds the bounds of the masks (never index by it).
-__device__ __forceinline__ bool tree_seq(const TreeArgs& a, int s, int& q_begin, int& n, int& ctx,
-                                         bool flag) {
-  q_begin = a.qloc[s];
-  const int64_t run = (int64_t)a.qloc[s + 1] - q_begin;
-  n = 0;
-  ctx = 0;
-  if (run <= 0) return false;
-  if (q_begin < 0 || run > a.max_nodes || run > 64 * (int64_t)a.mask_words ||
-      q_begin > a.n_tokens - run) {
-    if (flag && a.status) atomicOr(a.status, PKV_STATUS_BAD_QLOC);
-    return false;
-  }
-  n = (int)run;
-  const int cap = (int)((int64_t)a.max_blk << a.bs_shift);
-  ctx = min(max(a.ctx_lens[s], 0), cap);
-  return true;
+// Sequence s's run of nodes and its context, 0 and 0 where it has no nodes, or where
+// its run [q_begin, q_end) lies outside [0, T) or exceeds the bounds of the masks
+// (never index by it).
+__device__ __forceinline__ void tree_seq(const TreeArgs& a, int q_begin, int q_end, int len, int& n,
+                                         int& ctx, bool flag) {
+  const int64_t run = (int64_t)q_end - q_begin;
+  const bool bad = run > 0 && (q_begin < 0 || run > a.max_nodes ||
+                               run > 64 * (int64_t)a.mask_words || q_begin > a.n_tokens - run);
+  if (bad && flag && a.status) atomicOr(a.status, PKV_STATUS_BAD_QLOC);
+  const bool ok = run > 0 && !bad;
+  n = ok ? (int)run : 0;
+  ctx = ok ? min(max(len, 0), (int)((int64_t)a.max_blk << a.bs_shift)) : 0;
 }
 
 struct TreeUnit {
@@ -161,7 +156,7 @@ struct TreeUnit {
 
 // The partitions of a context: at least part_len long, of equal length.
 __device__ __forceinline__ int tree_parts(const TreeArgs& a, int ctx, int part_len) {
-  return a.slots > 0 && ctx > part_len ? (ctx - 1) / part_len + 1 : 1;
+  return a.slots > 0 && ctx > part_len ? min((ctx - 1) / part_len + 1, a.max_parts) : 1;
 }
 
 // Exclusive prefix sums of x and y over the wavefront; the totals in tx and ty.
@@ -199,19 +194,27 @@ __device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, TreeUnit& u) {
   const bool flag = blockIdx.x == 0 && __builtin_amdgcn_readfirstlane(threadIdx.x) < 64;
   auto tiles_of = [&](int n) { return (n * a.group + ROWS - 1) / ROWS * a.hkv; };
   auto load = [&](int r, int& qb, int& n, int& ctx, bool f) {
-    qb = n = ctx = 0;
-    if (64 * r + lane < a.n_seq) tree_seq(a, 64 * r + lane, qb, n, ctx, f);
+    const int s = min(64 * r + lane, a.n_seq - 1);
+    qb = a.qloc[s];
+    const int qe = a.qloc[s + 1];
+    const int len = a.ctx_lens[s];
+    tree_seq(a, qb, 64 * r + lane < a.n_seq ? qe : qb, len, n, ctx, f);
   };
   const int rounds = (a.n_seq + 63) / 64;
   int part_len = a.part_tokens;
   if (part_len <= 0) {
     float work = 0.f, tiles = 0.f;
+    // the first read of the lengths: four rounds' loads together
 #pragma unroll 1
-    for (int r = 0; r < rounds; ++r) {
-      int q, m, c;
-      load(r, q, m, c, false);
-      tiles += (float)tiles_of(m);
-      work += (float)tiles_of(m) * (float)c;
+    for (int r0 = 0; r0 < rounds; r0 += 4) {
+      int q[4], m[4], c[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load(r0 + i, q[i], m[i], c[i], false);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        tiles += (float)tiles_of(m[i]);
+        work += (float)tiles_of(m[i]) * (float)c[i];
+      }
     }
     auto sum = [](float x) {
       x += lane_xor<1>(x);
@@ -1021,6 +1024,7 @@ struct TreePlan {
   int rw;    // row wavefronts per tile
   int rows;  // rows per tile
   int min_part;
+  int64_t max_parts;  // of one context, by its bound
   int units;      // wanted
   int64_t grid;   // workgroups that hold every unit
   int64_t slots;  // partial results, 0: no split
@@ -1045,18 +1049,18 @@ TreePlan tree_plan(int n_seq, int max_nodes, int hq, int hkv, int d, int max_blk
   p.min_part = p.rw == 1 ? 128 : 256;
   p.units = 2 * device_cu_count();
   const int64_t all = n_seq * tiles;
-  int64_t units = p.units;
   if (part_tokens > 0) {
     const int64_t len = (part_tokens + 63) / 64 * 64;
-    // contexts past the table do not exist, so this holds every partition
-    units = all * ((cap + len - 1) / len);
-    p.slots = cap > len ? units : 0;
-    p.grid = std::max(units, all);
+    // contexts past the table do not exist
+    p.max_parts = std::max<int64_t>((cap + len - 1) / len, 1);
+    p.grid = all * p.max_parts;
+    p.slots = p.max_parts > 1 ? p.grid : 0;
   } else {
-    // partitions are at least work / units long: at most `units` of them, and one
-    // more a tile; a split context has less than twice its work's share
-    p.slots = bound > p.min_part ? 2 * (int64_t)p.units : 0;
-    p.grid = p.slots ? p.units + all : all;
+    // the work is cut into max(units - tiles, units / 2) shares, one unit more a
+    // tile; a split context has less than twice its work's share
+    p.max_parts = std::max<int64_t>((bound + p.min_part - 1) / p.min_part, 1);
+    p.grid = std::min(std::max<int64_t>(p.units, p.units / 2 + all), all * p.max_parts);
+    p.slots = p.max_parts > 1 ? std::min(2 * (int64_t)p.units, all * p.max_parts) : 0;
   }
   // an XCD's two shares are each rounded up
   p.grid = (p.grid + 7) / 8 * 8 + 8;
@@ -1211,6 +1215,7 @@ int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k
   a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)d)) * 1.4426950408889634f;
   a.part_tokens = (part_tokens + 63) / 64 * 64;
   a.min_part = p.min_part;
+  a.max_parts = (int)p.max_parts;
   a.units = p.units;
   a.slots = (int)p.slots;
   if (p.slots) {
