@@ -452,6 +452,7 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
 #pragma unroll
       for (int j = 0; j < 8; ++j) pf[ks & 1][j] = (T)s[ks >> 1][8 * (ks & 1) + j];
     };
+    __builtin_amdgcn_s_setprio(1);
     fetch(0);
     take(0);
 #pragma unroll
@@ -462,13 +463,6 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
       for (int dt = 0; dt < DP / 32; ++dt)
         st.o[dt] = Mma32<T>::mma(vf[ks & 1][dt], pf[ks & 1], st.o[dt]);
       if (ks + 1 < 2 * ST) take(ks + 1);
-      if constexpr (DP >= 64) {  // products and vector work side by side
-#pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) {
-          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x2 | 0x400, 32 / (DP / 32), 0);
-        }
-      }
       __builtin_amdgcn_sched_barrier(0);
     }
   } else {
@@ -489,6 +483,7 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
           st.o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf, s[t][r], st.o[dt], 0, 0, 0);
         }
   }
+  __builtin_amdgcn_s_setprio(0);
   st.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 
@@ -780,7 +775,11 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
     else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     if (active) {
       floatx16 sc[Geo::ST];
+      // wavefronts that feed the matrix unit go first: the other one of the SIMD has
+      // vector work or waits (111 -> 107 us over 65533 fp8 tokens, join included)
+      __builtin_amdgcn_s_setprio(1);
       tree_scores<T, DP, Geo::KPITCH, Geo::ST>(buf, st, sc, lane);
+      __builtin_amdgcn_s_setprio(0);
       // keys of the chunk; none behind the end, of the tree only those this row sees
       const int left = TREE ? g.n - i * KT : hi - lo - (i - ntc) * KT;
       if (TREE || left < KT) {
