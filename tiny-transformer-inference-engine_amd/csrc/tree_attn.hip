@@ -950,14 +950,18 @@ __global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_ker
 // lanes a row (4 dims and the 4 DP / 2 further on each). What bounds it is the
 // round trip to partials another XCD wrote, so the loads of four partitions are
 // requested at once and no thread takes a second row (64 rows a workgroup in
-// turn took 20.9 us of 128 sequences of 8 x 16 rows and 1.2 K tokens).
-template <typename T, int DP>
+// turn took 20.9 us of 128 sequences of 8 x 16 rows and 1.2 K tokens). WIDE, where
+// rows are few: a wavefront a row, its groups of lanes take every PS-th partition
+// (2016 rows of 32 partitions: 7.6 us, 10.7 with the rows packed).
+template <typename T, int DP, bool WIDE>
 __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, int rows) {
   constexpr int B = 4;
   constexpr int LPR = DP / 8;
+  constexpr int PS = WIDE ? 64 / LPR : 1;
   const int4 rec = a.recs[blockIdx.x];
   const int rows_all = rec.w * a.group;
-  const int rg = blockIdx.z * (kTreeThreads / LPR) + threadIdx.x / LPR;
+  const int rg = blockIdx.z * (kTreeThreads / LPR / PS) + threadIdx.x / (LPR * PS);
+  const int pg = WIDE ? (int)(threadIdx.x % 64) / LPR : 0;
   if (rec.x < 0 || rg >= rows_all) return;
   const int np = rec.y;
   const int kvh = blockIdx.y;
@@ -972,12 +976,12 @@ __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, in
   const int far = have[1] ? DP / 2 : 0;
   float M = -INFINITY, L = 0.f;
   floatx4 o[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  for (int p0 = 0; p0 < np; p0 += B) {
+  for (int p0 = pg; p0 < np; p0 += PS * B) {
     float2 x[B];
     floatx4 v[B][2];
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-      const int p = min(p0 + j, np - 1);
+      const int p = min(p0 + PS * j, np - 1);
       x[j] = ml[p * step];
       v[j][0] = *reinterpret_cast<const floatx4*>(po + p * step * a.d);
       v[j][1] = *reinterpret_cast<const floatx4*>(po + p * step * a.d + far);
@@ -985,7 +989,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, in
     float m = M;
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-      if (p0 + j >= np) x[j].x = -INFINITY;
+      if (p0 + PS * j >= np) x[j].x = -INFINITY;
       m = fmaxf(m, x[j].x);
     }
     const float old = M == -INFINITY ? 0.f : exp2f(M - m);
@@ -996,13 +1000,29 @@ __global__ __launch_bounds__(kTreeThreads) void tree_merge_kernel(TreeArgs a, in
     for (int j = 0; j < B; ++j) {
       // a partition in which the row sees nothing holds zeros
       const float wt = x[j].x == -INFINITY ? 0.f : exp2f(x[j].x - m);
-      if (p0 + j < np) {
+      if (p0 + PS * j < np) {
         L += wt * x[j].y;
         o[0] += wt * v[j][0];
         o[1] += wt * v[j][1];
       }
     }
     M = m;
+  }
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int k = LPR; k < 64; k <<= 1) {
+      const float m2 = __shfl_xor(M, k, 64), l2 = __shfl_xor(L, k, 64);
+      const float m = fmaxf(M, m2);
+      const float w1 = M == -INFINITY ? 0.f : exp2f(M - m);
+      const float w2 = m2 == -INFINITY ? 0.f : exp2f(m2 - m);
+      L = w1 * L + w2 * l2;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[h][e] = w1 * o[h][e] + w2 * __shfl_xor(o[h][e], k, 64);
+      M = m;
+    }
+    if (pg != 0) return;
   }
   const int i = rg / a.group;
   const int64_t orow = (int64_t)(rec.z + i) * a.hq + kvh * a.group + (rg - i * a.group);
@@ -1086,6 +1106,14 @@ void launch_tree_dp(const TreeArgs& a, int rw, unsigned grid, hipStream_t stream
         : tree_attn_kernel<T, DP, 4, KV8, false><<<grid, kTreeThreads, 0, stream>>>(a);
 }
 
+template <typename T, int DP>
+void launch_merge(const TreeArgs& a, int tile, int64_t rows, bool wide, hipStream_t stream) {
+  const int per = wide ? kTreeThreads / 64 : kTreeThreads * 8 / DP;
+  const dim3 grid((unsigned)a.n_seq, (unsigned)a.hkv, (unsigned)((rows + per - 1) / per));
+  wide ? tree_merge_kernel<T, DP, true><<<grid, kTreeThreads, 0, stream>>>(a, tile)
+       : tree_merge_kernel<T, DP, false><<<grid, kTreeThreads, 0, stream>>>(a, tile);
+}
+
 template <typename T, bool KV8>
 void launch_tree(const TreeArgs& a, const TreePlan& p, unsigned grid, hipStream_t stream) {
   switch (p.dp) {
@@ -1096,13 +1124,16 @@ void launch_tree(const TreeArgs& a, const TreePlan& p, unsigned grid, hipStream_
   }
   if (p.slots) {
     const int64_t rows = (int64_t)a.max_nodes * a.group;
-    const int per = kTreeThreads * 8 / p.dp;  // rows per workgroup
-    const dim3 mg((unsigned)a.n_seq, (unsigned)a.hkv, (unsigned)((rows + per - 1) / per));
+    const int per = kTreeThreads * 8 / p.dp;  // rows per workgroup, packed
+    const int64_t packed = (rows + per - 1) / per * a.n_seq * a.hkv;
+    // fewer workgroups than CUs, and more partitions than two rounds of loads: a
+    // wavefront a row (four requests' 64 rows of up to 4 partitions: 4.2 us so, 3.5 packed)
+    const bool wide = packed < device_cu_count() && a.max_parts > 8;
     switch (p.dp) {
-      case 32: tree_merge_kernel<T, 32><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
-      case 64: tree_merge_kernel<T, 64><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
-      case 128: tree_merge_kernel<T, 128><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
-      default: tree_merge_kernel<T, 256><<<mg, kTreeThreads, 0, stream>>>(a, p.rows); break;
+      case 32: launch_merge<T, 32>(a, p.rows, rows, wide, stream); break;
+      case 64: launch_merge<T, 64>(a, p.rows, rows, wide, stream); break;
+      case 128: launch_merge<T, 128>(a, p.rows, rows, wide, stream); break;
+      default: launch_merge<T, 256>(a, p.rows, rows, wide, stream); break;
     }
   }
 }
@@ -1181,8 +1212,8 @@ int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k
   const TreePlan p = tree_plan(n_seq, max_nodes, hq, hkv, d, blk, block_size, max_ctx_len,
                                part_tokens, dtype);
   const int64_t rows = (int64_t)max_nodes * (hq / hkv);
-  // rows / 8: the join's workgroups at d = 256
-  if (p.grid > 0x7fffffff || rows > 8 * 65535)
+  // rows / 4: the join's workgroups, at most
+  if (p.grid > 0x7fffffff || rows > 4 * 65535)
     return fail(PKV_ERR_UNSUPPORTED, "too many sequences x heads x partitions, or rows");
   if (p.ws_bytes > 0 && (!workspace || workspace_bytes < p.ws_bytes))
     return fail(PKV_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", p.ws_bytes,
