@@ -228,6 +228,28 @@ def test_arbitrary_masks_and_empty_rows(dt, d):
         assert (out[-3:] == 0).all() and torch.isposinf(lse[-3:]).all()
 
 
+@pytest.mark.parametrize("dt,d", [(BF, 64), (F32, 64), (BF, 128), (BF, 256)])
+def test_nan_that_is_seen_stays(dt, d):
+    """A query of NaN, and a context key of NaN: every row that they meet is NaN, whole or
+    split (in whichever piece the key lies), the other rows as they were."""
+    for at in (3, 120, 190):
+        p = Problem([200, 60], [6, 4], 8, 1, d, 16, dt, seed=16)
+        slot = p.tables[0][at // 16] * 16 + at % 16
+        p.q[7, 2, 5] = float("nan")
+        clean = [np64(x) for x in p.run()]
+        p.kp.view(-1, 1, d)[slot, 0, 1] = float("nan")
+        for part in (0, 64):
+            out, lse = (np64(x) for x in p.run(part_tokens=part))
+            assert np.isnan(out[:6]).all() and np.isnan(lse[:6]).all()
+            assert np.isnan(out[7, 2]).all() and np.isnan(lse[7, 2])
+            rest = np.ones((10, 8), dtype=bool)
+            rest[:6] = False
+            rest[7, 2] = False
+            u = torch.finfo(dt).eps
+            assert np.isfinite(out[rest]).all()
+            assert (np.abs(out - clean[0])[rest] <= 2 * u * 4 + 1e-4).all()
+
+
 def test_large_scores_and_scale():
     p = Problem([300], [12], 8, 1, 64, 16, BF, seed=7, amp=40.0)
     check(p, *p.run())

@@ -184,9 +184,8 @@ __device__ __forceinline__ void wave_scan2(int& x, int& y, int& tx, int& ty) {
 // contexts: 80 us of attention and join in plain order); the row tiles of one
 // (sequence, kv head, partition) read the same keys, so each XCD (workgroup b runs
 // on XCD b % 8) takes a contiguous eighth of the numbers, and finds them in its L2.
-// Every wavefront makes
-// the plan for itself, one sequence a lane and round, so there is no barrier in it;
-// the later passes read the lengths from the L1.
+// Every wavefront makes the plan for itself, one sequence a lane and round, so there
+// is no barrier in it; the later passes read the lengths from the L1.
 template <int ROWS>
 __device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, TreeUnit& u) {
   const int lane = threadIdx.x & 63;
@@ -1193,8 +1192,9 @@ int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k
                 max_nodes);
   if ((int64_t)max_blk * block_size > (int64_t)1 << 30)
     return fail(PKV_ERR_UNSUPPORTED, "block tables of more than 2^30 tokens");
-  if ((int64_t)block_size * hkv * d * (kv8 ? 1 : elem_bytes(qdtype)) > 0x7fffffff)
-    return fail(PKV_ERR_UNSUPPORTED, "blocks of 2 GiB and more");
+  // what one resource spans: a block, or 16 of the tree's rows
+  if (std::max<int64_t>(block_size, 16) * hkv * d * elem_bytes(qdtype) > 0x7fffffff)
+    return fail(PKV_ERR_UNSUPPORTED, "blocks or 16 rows of 2 GiB and more");
   if (n_seq == 0 || max_nodes == 0 || n_tokens == 0) return PKV_OK;
   if ((int64_t)mask_words * 64 < max_nodes)
     return fail(PKV_ERR_INVALID, "masks of %d 64-bit words hold fewer than max_nodes = %d keys",
