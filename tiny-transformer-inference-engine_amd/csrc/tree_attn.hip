@@ -131,6 +131,9 @@ struct TreeGeo {
   static constexpr int LDS_CHUNKS = NBUF * BUF;
   static constexpr int LDS_COMBINE = kTreeWaves * 32 * (OPITCH + (RW == 1 ? 2 : 0)) * 4;
   static constexpr int LDS = LDS_CHUNKS > LDS_COMBINE ? LDS_CHUNKS : LDS_COMBINE;
+  // wavefronts a SIMD holds: of the wide rows (their accumulators and queries take
+  // 192 registers and more) one
+  static constexpr int OCC = DP == 256 || (ES == 4 && DP == 128 && RW == 1) ? 1 : 2;
   static_assert(64 % CPR == 0 && GR % RPL == 0 && NG * PG == PER && PER >= 1, "chunk split");
 };
 
@@ -494,7 +497,8 @@ __device__ __forceinline__ void tree_update(const char* vl, floatx16 (&s)[ST], f
 // row. (Row by row for every block size: 110 us against 104 with scalar addresses
 // in 64 bits, 65533 fp8 tokens, 63 nodes x 32 heads.)
 template <typename T, int DP, int RW, bool KV8, bool WHOLE>
-__global__ __launch_bounds__(kTreeThreads, DP == 256 ? 1 : 2) void tree_attn_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTreeThreads, (TreeGeo<T, DP, RW>::OCC)) void tree_attn_kernel(
+    TreeArgs a) {
   using Geo = TreeGeo<T, DP, RW>;
   constexpr int PER = Geo::PER;
   constexpr int KT = Geo::KT;
@@ -1057,15 +1061,18 @@ TreePlan tree_plan(int n_seq, int max_nodes, int hq, int hkv, int d, int max_blk
   const bool f32 = dtype_base(dtype) == PKV_DTYPE_F32;
   const int64_t cap = (int64_t)max_blk * block_size;
   const int64_t bound = max_ctx_len > 0 ? std::min<int64_t>(max_ctx_len, cap) : cap;
-  // RW = 1 where its registers hold a chunk, and either the rows fit one
+  // RW = 1 where its registers hold a chunk (at 256 dims it spills: 96 requests of
+  // 3 x 8 rows and 1.2 K tokens 62 -> 249 us; 2 requests of 2 x 8 fp32 rows of 128
+  // and 11 K tokens 49 -> 25 us), and either the rows fit one
   // wavefront or the whole batch, cut into its 32-row tiles and 128-token rounds,
   // does not fill the chip: the shortest chain then
   const int64_t small = n_seq * (int64_t)hkv * ((rows + 31) / 32) * ((bound + 127) / 128);
-  p.rw = (f32 ? p.dp <= 64 : p.dp <= 128) && (rows <= 32 || small <= device_cu_count()) ? 1 : 4;
+  p.rw = p.dp <= 128 && (rows <= 32 || small <= device_cu_count()) ? 1 : 4;
   p.rows = 32 * p.rw;
   const int64_t tiles = (rows + p.rows - 1) / p.rows * hkv;
   p.min_part = p.rw == 1 ? 128 : 256;
-  p.units = 2 * device_cu_count();
+  // workgroups that run at once (TreeGeo::OCC)
+  p.units = (p.dp == 256 || (f32 && p.dp == 128 && p.rw == 1) ? 1 : 2) * device_cu_count();
   const int64_t all = n_seq * tiles;
   if (part_tokens > 0) {
     const int64_t len = (part_tokens + 63) / 64 * 64;
@@ -1094,7 +1101,7 @@ TreePlan tree_plan(int n_seq, int max_nodes, int hq, int hkv, int d, int max_blk
 template <typename T, int DP, bool KV8>
 void launch_tree_dp(const TreeArgs& a, int rw, unsigned grid, hipStream_t stream) {
   const bool whole = a.bs_shift >= 4;
-  if constexpr (sizeof(T) == 2 ? DP <= 128 : DP <= 64) {
+  if constexpr (DP <= 128) {
     if (rw == 1) {
       whole ? tree_attn_kernel<T, DP, 1, KV8, true><<<grid, kTreeThreads, 0, stream>>>(a)
             : tree_attn_kernel<T, DP, 1, KV8, false><<<grid, kTreeThreads, 0, stream>>>(a);
