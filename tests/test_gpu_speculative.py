@@ -184,7 +184,7 @@ def test_generate_speculative_edges():
     assert one == generate_batched(model, [[1, 2]], 1, pool, alloc)
     assert generate_speculative(model, [[1, 2]], 9, pool, alloc, none, max_drafts=0,
                                 max_depth=1) == generate_batched(model, [[1, 2]], 9, pool, alloc)
-    for bad in ([], [0]), ([1], [0]), ([1, 2], [-1, 1]), ([1], [-2]):
+    for bad in ([], [0]), ([1], [0]), ([1, 2], [-1, 1]), ([1], [-2]), ([97], [-1]), ([-1], [-1]):
         with pytest.raises(ValueError):
             generate_speculative(model, [[1, 2]], 5, pool, alloc, lambda h, b=bad: b)
     with pytest.raises(ValueError):

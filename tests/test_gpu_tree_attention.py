@@ -157,6 +157,30 @@ def test_matches_definition(case, part):
     check(p, *p.run(part_tokens=part))
 
 
+@pytest.mark.parametrize("n", [64, 65, 257, 321])
+@pytest.mark.parametrize("dt,hq,part", [(BF, 4, 64), (BF, 40, 0), (F32, 4, 0)])
+def test_many_sequences(n, dt, hq, part):
+    """Plans of several rounds of 64 sequences, some of them without nodes."""
+    print(f"[tree] n={n} {dt} hq={hq} part={part}", flush=True)
+    rng = np.random.default_rng(n)
+    ctx = rng.integers(0, 40, size=n)
+    ctx[::50] = 300
+    nodes = rng.integers(0, 4, size=n)
+    nodes[-1] = 2
+    p = Problem(ctx.tolist(), nodes.tolist(), hq, 1, 64, 16, dt, seed=n)
+    check(p, *p.run(part_tokens=part))
+
+
+@pytest.mark.parametrize("dt,kv,d,bs,nodes", [(BF, None, 128, 16, [3, 2]), (BF, F8, 64, 16, [9, 40]),
+                                              (F32, None, 64, 32, [5, 1]), (HF, None, 64, 8, [3, 20])])
+@pytest.mark.parametrize("part", [8192, 2048])
+def test_long_partitions(dt, kv, d, bs, nodes, part):
+    """Partitions of more blocks than the table entries held in a register (64)."""
+    print(f"[tree] {dt} {kv} d={d} bs={bs} {nodes} part={part}", flush=True)
+    p = Problem([5003, 2100], nodes, 8, 1, d, bs, dt, kv, seed=21)
+    check(p, *p.run(part_tokens=part))
+
+
 @pytest.mark.parametrize("dt,kv,d", [(BF, None, 128), (F32, None, 64), (HF, F8, 64),
                                      (F32, None, 128)])
 @pytest.mark.parametrize("fill", [float("nan"), 3e38])

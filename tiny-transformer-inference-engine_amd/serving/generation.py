@@ -116,16 +116,18 @@ def generate_batched(model, prompts_ids, max_new_tokens, pool, alloc, block_size
         return _drive(model, pool, cohort, max_new_tokens, _greedy_ids)
 
 
-def _draft_tree(draft, history, limit):
+def _draft_tree(draft, history, limit, vocab):
     """draft(history) -> (tokens, parents), checked; the nodes below the root as
     (tokens, parents of the whole tree), at most `limit` of them."""
     tokens, parents = draft(history)
     tokens, parents = [int(t) for t in tokens][:limit], [int(p) for p in parents][:limit]
     if len(tokens) != len(parents):
         raise ValueError("a draft needs one parent per token")
-    for i, p in enumerate(parents):
+    for i, (t, p) in enumerate(zip(tokens, parents)):
         if not -1 <= p < i:
             raise ValueError(f"draft node {i}: parent {p} is neither -1 nor an earlier node")
+        if not 0 <= t < vocab:
+            raise ValueError(f"draft node {i}: token {t} is outside the vocabulary ({vocab})")
     return tokens, [p + 1 for p in parents]
 
 
@@ -151,6 +153,7 @@ def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft,
     if max_new_tokens == 0:
         return [[] for _ in prompts_ids]
     device = _model_device(model)
+    vocab = model.lm_head.out_features
     stock = []
     with _Cohort(prompts_ids, block_size, alloc, device) as cohort:
         first = _greedy_ids(model.forward_batch(cohort.prefill_batch(), pool))
@@ -169,7 +172,7 @@ def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft,
                 tokens, parents, starts = [], [], [0]
                 for row, g in zip(rows, goal):
                     if len(row) < g:  # a finished row takes no nodes
-                        t, p = _draft_tree(draft, list(row), max_drafts)
+                        t, p = _draft_tree(draft, list(row), max_drafts, vocab)
                         tokens += [row[-1]] + t
                         parents += [-1] + p
                     starts.append(len(tokens))

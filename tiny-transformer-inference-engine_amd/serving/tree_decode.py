@@ -120,8 +120,8 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     pools [num_blocks, block_size, Hkv, D] and to the tree keys of k, v [T, Hkv, D]
     that meta.masks shows each node. fp32, float16 or bfloat16; pools of the same
     type or float8_e4m3fn (the tree's rows then count as rounded to it). `out` /
-    `lse` (float32 [T, Hq]): where to write; rows of no sequence are left as they
-    were there. A row that sees no key gives 0 and lse +inf. part_tokens (0:
+    `lse` (float32 [T, Hq]): where to write, memory of no other operand; rows of no
+    sequence are left as they were there. A row that sees no key gives 0 and lse +inf. part_tokens (0:
     automatic) forces the length of the pieces a context is split into."""
     what = "paged_tree_attention"
     masks = meta.masks
