@@ -162,19 +162,26 @@ __device__ __forceinline__ int tree_parts(const TreeArgs& a, int ctx, int part_l
   return a.slots > 0 && ctx > part_len ? min((ctx - 1) / part_len + 1, a.max_parts) : 1;
 }
 
+// Inclusive prefix sum over the wavefront by VALU data movement: shifts within the
+// rows of 16 lanes, then the sums of lanes 15 and 47 to the rows behind them and
+// lane 31's to the upper half (by LDS permutes each step waits some 100 cycles).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_0(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_or_0<0x111, 0xF>(x);
+  x += dpp_or_0<0x112, 0xF>(x);
+  x += dpp_or_0<0x114, 0xF>(x);
+  x += dpp_or_0<0x118, 0xF>(x);
+  x += dpp_or_0<0x142, 0xA>(x);
+  x += dpp_or_0<0x143, 0xC>(x);
+  return x;
+}
+
 // Exclusive prefix sums of x and y over the wavefront; the totals in tx and ty.
 __device__ __forceinline__ void wave_scan2(int& x, int& y, int& tx, int& ty) {
-  const int lane = threadIdx.x & 63;
-  int sx = x, sy = y;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int ux = __shfl_up(sx, o, 64);
-    const int uy = __shfl_up(sy, o, 64);
-    if (lane >= o) {
-      sx += ux;
-      sy += uy;
-    }
-  }
+  const int sx = wave_scan(x), sy = wave_scan(y);
   tx = __builtin_amdgcn_readlane(sx, 63);
   ty = __builtin_amdgcn_readlane(sy, 63);
   x = sx - x;
@@ -246,13 +253,8 @@ __device__ __forceinline__ bool tree_plan_unit(const TreeArgs& a, TreeUnit& u) {
     split += parts > 1 ? k : 0;
     whole += parts > 1 ? 0 : k;
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    split += __shfl_xor(split, o, 64);
-    whole += __shfl_xor(whole, o, 64);
-  }
-  split = __builtin_amdgcn_readfirstlane(split);
-  whole = __builtin_amdgcn_readfirstlane(whole);
+  split = __builtin_amdgcn_readlane(wave_scan(split), 63);
+  whole = __builtin_amdgcn_readlane(wave_scan(whole), 63);
   // workgroup b: number b / 8 of XCD b % 8's eighths, the split sequences' first
   const int64_t xcd = blockIdx.x & 7;
   const int s0 = (int)(split * xcd >> 3), s1 = (int)(split * (xcd + 1) >> 3);
