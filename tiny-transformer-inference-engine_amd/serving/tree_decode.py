@@ -124,36 +124,39 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     sequence are left as they were there. A row that sees no key gives 0 and lse +inf. part_tokens (0:
     automatic) forces the length of the pieces a context is split into."""
     what = "paged_tree_attention"
-    masks = meta.masks
-    _native.require_device(q, k, v, k_pool, v_pool, masks, what=what)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, k_pool, v_pool)):
+    masks, table = meta.masks, meta.block_tables
+    dev = q.device
+    if not (q.is_cuda and k.device == dev and v.device == dev and k_pool.device == dev
+            and v_pool.device == dev and masks.device == dev and table.device == dev):
+        _native.require_device(q, k, v, k_pool, v_pool, masks, what=what)
+        raise RuntimeError(f"{what}: q, k, v, the pools and the metadata must share a device")
+    if ((q.requires_grad or k.requires_grad or v.requires_grad or k_pool.requires_grad
+         or v_pool.requires_grad) and torch.is_grad_enabled()):
         raise NotImplementedError(
             f"{what} is forward-only (inference); run it under torch.no_grad()")
-    dev = q.device
-    if not (k.device == v.device == k_pool.device == v_pool.device == masks.device
-            == meta.block_tables.device == dev):
-        raise RuntimeError(f"{what}: q, k, v, the pools and the metadata must share a device")
-    if q.dim() != 3 or k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
+    shape, pool_shape = q.shape, k_pool.shape
+    if len(shape) != 3 or len(pool_shape) != 4 or pool_shape != v_pool.shape:
         raise ValueError(f"{what}: q must be [T, Hq, D], the pools [num_blocks, block_size, Hkv, D]")
-    T, hq, d = q.shape
-    nb, bs, hkv, pd = k_pool.shape
+    T, hq, d = shape
+    nb, bs, hkv, pd = pool_shape
     if pd != d or k.shape != (T, hkv, d) or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must be [{T}, {hkv}, {d}] (got {tuple(k.shape)}, "
                          f"{tuple(v.shape)}), the pools' head dim {d} (got {pd})")
     if T != meta.num_tokens or bs != meta.block_size:
         raise ValueError(f"{what}: {T} rows and blocks of {bs}, the metadata has "
                          f"{meta.num_tokens} and {meta.block_size}")
-    if not (k.dtype == v.dtype == q.dtype) or v_pool.dtype != k_pool.dtype:
+    dtype = q.dtype
+    if k.dtype != dtype or v.dtype != dtype or v_pool.dtype != k_pool.dtype:
         raise TypeError(f"{what}: q, k and v must share a dtype, and so must the pools")
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError(f"{what}: the pools must be contiguous")
-    code = _native.kv_code(q.dtype, k_pool.dtype)
+    code = _native.kv_code(dtype, k_pool.dtype)
     if masks.dtype != torch.int64 or masks.dim() != 2 or masks.shape[0] != T:
         raise ValueError(f"{what}: masks must be int64 [{T}, words]")
     if lse is not None and (lse.shape != (T, hq) or lse.dtype != torch.float32
                             or lse.device != dev or not lse.is_contiguous()):
         raise ValueError(f"{what}: lse must be contiguous float32 [{T}, {hq}] on {dev}")
-    n, max_blk = meta.block_tables.shape
+    n, max_blk = table.shape
     max_nodes, max_ctx = meta.max_nodes, meta.max_ctx_len
     calls = _native.calls()
     previous = _native.make_current(dev)
@@ -161,11 +164,10 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         q, k, v = _dense(q), _dense(k), _dense(v)
         if not masks.is_contiguous():
             masks = masks.contiguous()
-        dst = out
         if out is None:
-            out = dst = torch.empty_like(q)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
-            raise ValueError(f"{what}: out must be {tuple(q.shape)} {q.dtype} on {dev}")
+            out = dst = q.new_empty(shape)
+        elif out.shape != shape or out.dtype != dtype or out.device != dev:
+            raise ValueError(f"{what}: out must be {tuple(shape)} {dtype} on {dev}")
         else:
             dst = _dense(out)  # a copy holds the rows of no sequence, too
         nbytes = calls.pkv_tree_attention_workspace_bytes(
@@ -176,11 +178,10 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         rc = calls.pkv_paged_tree_attention(
             dst.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), k.data_ptr(),
             v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), nb, bs,
-            meta.block_tables.data_ptr() if max_blk else None, max_blk,
-            meta.ctx_lens.data_ptr(), meta.query_start_loc.data_ptr(), masks.data_ptr(),
-            masks.shape[1], n, T, max_nodes, max_ctx, hq, hkv, d,
-            float(scale) if scale is not None and scale > 0 else 0.0, part_tokens, code,
-            None if ws is None else ws.data_ptr(), nbytes,
+            table.data_ptr() if max_blk else None, max_blk, meta.ctx_lens.data_ptr(),
+            meta.query_start_loc.data_ptr(), masks.data_ptr(), masks.shape[1], n, T, max_nodes,
+            max_ctx, hq, hkv, d, float(scale) if scale is not None and scale > 0 else 0.0,
+            part_tokens, code, None if ws is None else ws.data_ptr(), nbytes,
             None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
         if rc:
             _native.check(rc, what)
