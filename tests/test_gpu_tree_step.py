@@ -131,6 +131,38 @@ def test_build_batch_meta_all_or_nothing(what, kw):
     assert np.isin(real // 16, [1, 2]).all()
 
 
+@pytest.mark.parametrize("what,held,ctx,q", [("qloc", 1, 16, -1), ("qloc", -1, 16, 3),
+                                             ("short", 1, 16, 40), ("short", 5, 16, 1)])
+@pytest.mark.parametrize("n,at", [(1, 0), (64, 63), (256, 64), (256, 255), (301, 256), (301, 300),
+                                  (2000, 1999)])
+def test_build_batch_meta_one_bad_length_stops_every_sequence(n, at, what, held, ctx, q):
+    """Whichever wavefront and turn of the scan meets it, and beside a fault of the
+    whole step (a free list too short), which must not hide it."""
+    print(f"[step] {what} sequence {at} of {n}", flush=True)
+    for free in (n + 8, 0):
+        helds, ctxs, qs = [1] * n, [16] * n, [2] * n
+        helds[at], ctxs[at], qs[at] = held, ctx, q
+        tables = [[1, 0, 0] for _ in range(n)]
+        dt = raw_tables(tables, helds, ctxs, [2] * free, 0, 16, 9)
+        st = status()
+        meta, after = build_batch_meta(dt, i32(qs), 2 * n + 50, 50, status=st)
+        short = free == 0 and n > 1  # the others lack a block each
+        assert int(st) == BITS[what] | (BITS["blocks"] if short else 0)
+        assert after.block_tables.tolist() == tables and after.free_cursor.tolist() == [0]
+        assert after.blocks_held.tolist() == helds and after.ctx_lens.tolist() == ctxs
+        slots = meta.slot_mapping  # only a table row said to be longer than it is has slots
+        assert bool(((slots == tree_ref.NO_SLOT) | (slots // 16 == 1)).all())
+
+
+def test_build_batch_meta_failed_steps_stay_within_the_rows():
+    """More tokens than T: a sequence's rows end at T for whatever runs on."""
+    st = status()
+    meta, _ = build_batch_meta(raw_tables([[1, 0]] * 3, [1] * 3, [3] * 3, [5], 0, 16, 9),
+                               i32([4, 4, 4]), 6, 4, status=st)
+    assert int(st) & BITS["qloc"]
+    assert meta.query_start_loc.tolist() == [0, 4, 6, 6]
+
+
 def test_build_batch_meta_bad_block_ids():
     compare_step([[1, 0], [9, 0]], [1, 1], [10, 10], [10, 3], [77, 4], 0, 16, 9, 20, 10)
     with pytest.raises(AssertionError):

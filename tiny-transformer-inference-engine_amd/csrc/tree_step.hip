@@ -104,10 +104,11 @@ __global__ __launch_bounds__(kStepThreads) void build_step_kernel(StepArgs a) {
   if (tid == 0) {
     tok0[n] = run_t;
     blk0[n] = run_b;
-    int bad = bad_sh;
+    int bad = 0;
     if (cur < 0 || cur > a.num_free || run_b > a.num_free - cur) bad |= PKV_STATUS_OUT_OF_BLOCKS;
     if (run_t > a.n_tokens) bad |= PKV_STATUS_BAD_QLOC;
-    bad_sh = bad;
+    // other wavefronts may still add the last lengths' bits: no plain store
+    if (bad) atomicOr(&bad_sh, bad);
   }
   __syncthreads();
   const bool fails = bad_sh != 0;
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(kStepThreads) void build_step_kernel(StepArgs a) {
     if (fails && a.status) atomicOr(a.status, bad_sh);
   }
   for (int64_t s = first; s <= n; s += stride) {
-    a.qsl[s] = tok0[s];
+    a.qsl[s] = (int)min((int64_t)tok0[s], a.n_tokens);  // failed steps: within the rows, too
     if (s == n) break;
     const int q = tok0[s + 1] - tok0[s];
     const int c = a.ctx[s];
