@@ -583,7 +583,7 @@ size_t pkv_tree_attention_workspace_bytes(int n_seq, int max_nodes, int hq, int 
  * were. max_ctx_len (<= 0: the table's capacity) sizes the context's split, a
  * longer context is still computed whole; part_tokens forces the split's length
  * (0: automatic). bf16 / f16 / fp32 (fp8 pools: bf16 / f16), any hq a multiple
- * of hkv, d a multiple of 8 up to 256, trees of at most 4096 nodes, tensors
+ * of hkv, d a multiple of 8 up to 256, at most 65536 trees of at most 4096 nodes, tensors
  * 16-byte aligned (fp8 pools 8); PKV_ERR_UNSUPPORTED otherwise.
  */
 int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k_new,

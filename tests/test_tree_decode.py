@@ -37,6 +37,7 @@ def attention(**kw):
     (INVALID, b"sizes", dict(nodes=-1)),
     (UNSUPPORTED, b"4096", dict(nodes=4097, words=65)),
     (UNSUPPORTED, b"2^30", dict(max_blk=(1 << 26) + 1)),
+    (UNSUPPORTED, b"65536", dict(n=65537)),
     (UNSUPPORTED, b"2 GiB", dict(bs=1 << 24, max_blk=1)),
     (INVALID, b"max_nodes", dict(nodes=65)),
     (INVALID, b"max_nodes", dict(words=0)),

@@ -46,6 +46,9 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 constexpr int kTreeThreads = 256;
 constexpr int kTreeWaves = 4;
 constexpr int kTreeMaxNodes = 4096;
+// a lane sums the work of every 64th: 1024 additions in fp32 are off by 6.1e-5 at
+// most, below the 1e-4 by which tree_plan_unit rounds a share up
+constexpr int kTreeMaxSeq = 65536;
 
 struct TreeArgs {
   void* out;
@@ -1202,6 +1205,8 @@ int pkv_paged_tree_attention(void* out, float* lse, const void* q, const void* k
   if (max_nodes > kTreeMaxNodes)
     return fail(PKV_ERR_UNSUPPORTED, "trees of at most %d nodes (max_nodes %d)", kTreeMaxNodes,
                 max_nodes);
+  if (n_seq > kTreeMaxSeq)
+    return fail(PKV_ERR_UNSUPPORTED, "at most %d sequences (%d given)", kTreeMaxSeq, n_seq);
   if ((int64_t)max_blk * block_size > (int64_t)1 << 30)
     return fail(PKV_ERR_UNSUPPORTED, "block tables of more than 2^30 tokens");
   // what one resource spans: a block, or 16 of the tree's rows
