@@ -198,6 +198,22 @@ def test_generate_speculative_edges():
     assert alloc.num_free == 9
 
 
+@pytest.mark.parametrize("new", [1, 2, 17, 33])
+def test_generate_speculative_needs_what_generate_batched_needs(new):
+    """A pool that holds exactly the tokens, prompts that end with the model's last
+    position, and drafts that are right and go on past the goal."""
+    cfg, model = small_model()
+    n = cfg.max_seq_len + 1 - new  # the last token takes no position
+    rng = np.random.default_rng(5)
+    prompts = [rng.integers(0, 97, size=n).tolist(), rng.integers(0, 97, size=3).tolist()]
+    blocks = 1 + cfg.max_seq_len // 16 + -(-(3 + new - 1) // 16)
+    pool, alloc = make_pool(cfg, torch.float32, blocks=blocks), BlockAllocator(blocks)
+    truth = generate_batched(model, prompts, new, pool, alloc)
+    fn = drafts("chain", [t + [1] * 20 for t in truth], prompts)
+    assert generate_speculative(model, prompts, new, pool, alloc, fn) == truth
+    assert alloc.num_free == blocks - 1
+
+
 def test_step_captured_with_the_model():
     """A whole verification step (masks, model, picks, acceptance, blocks, commit) as one
     graph, replayed on other trees' tokens: the eager step's results."""

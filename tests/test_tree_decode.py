@@ -6,6 +6,7 @@ import torch
 
 from oracle import tree_ref
 from serving import _native
+from serving.generation import _draft_tree
 from serving.kv_pool import KVPool
 from serving.paged_meta import DeviceTables, build_batch_meta, raise_step_status
 from serving.tree_decode import (TreeAccept, TreeMeta, build_tree_meta, paged_tree_attention,
@@ -194,3 +195,18 @@ def test_oracle_against_hand_counts():
     t = [[3, 0], [0, 0]]
     r = tree_ref.build_step(t, [1, 0], [15, 0], [2, 1], [6, 7, 8], 1, 16, 9, 4, 2)
     assert t == [[3, 7], [8, 0]] and r["slots"][:3] == [63, 112, 128] and r["cursor"] == 3
+
+
+@pytest.mark.parametrize("limit,depth,want", [
+    (9, 9, ([5, 6, 7, 8, 9, 10], [0, 1, 0, 2, 3, 4])),
+    (4, 9, ([5, 6, 7, 8], [0, 1, 0, 2])),
+    (9, 3, ([5, 6, 7, 9], [0, 1, 0, 3])),
+    (3, 3, ([5, 6, 7], [0, 1, 0])),
+    (9, 2, ([5, 7], [0, 0])),
+    (9, 1, ([], [])),
+    (0, 9, ([], [])),
+])
+def test_draft_trees_are_cut_to_what_a_step_can_keep(limit, depth, want):
+    """Nodes too deep, and those below them, leave their places to others."""
+    draft = lambda h: ([5, 6, 7, 8, 9, 10], [-1, 0, -1, 1, 2, 3])  # noqa: E731
+    assert _draft_tree(draft, [1], limit, depth, 97) == want

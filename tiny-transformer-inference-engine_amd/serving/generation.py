@@ -116,19 +116,29 @@ def generate_batched(model, prompts_ids, max_new_tokens, pool, alloc, block_size
         return _drive(model, pool, cohort, max_new_tokens, _greedy_ids)
 
 
-def _draft_tree(draft, history, limit, vocab):
+def _draft_tree(draft, history, limit, depth, vocab):
     """draft(history) -> (tokens, parents), checked; the nodes below the root as
-    (tokens, parents of the whole tree), at most `limit` of them."""
+    (tokens, parents of the whole tree): the first `limit` of those fewer than
+    `depth` levels below the root, deeper ones can add nothing."""
     tokens, parents = draft(history)
-    tokens, parents = [int(t) for t in tokens][:limit], [int(p) for p in parents][:limit]
+    tokens, parents = [int(t) for t in tokens], [int(p) for p in parents]
     if len(tokens) != len(parents):
         raise ValueError("a draft needs one parent per token")
+    kept, above, node, level = [], [], [], [0]  # node: the place in the tree, None: left out
     for i, (t, p) in enumerate(zip(tokens, parents)):
         if not -1 <= p < i:
             raise ValueError(f"draft node {i}: parent {p} is neither -1 nor an earlier node")
         if not 0 <= t < vocab:
             raise ValueError(f"draft node {i}: token {t} is outside the vocabulary ({vocab})")
-    return tokens, [p + 1 for p in parents]
+        up = 0 if p == -1 else node[p]
+        if up is None or len(kept) == limit or level[up] + 1 >= depth:
+            node.append(None)
+            continue
+        kept.append(t)
+        above.append(up)
+        level.append(level[up] + 1)
+        node.append(len(kept))
+    return kept, above
 
 
 @torch.no_grad()
@@ -138,10 +148,11 @@ def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft,
     is called per row and step with the row's tokens so far and proposes a tree
     that goes on from the last of them: (tokens, parents), parents[i] the index of
     the proposed token that token i follows, -1 for those that follow the last
-    token; at most max_drafts of them are used. The model verifies all rows' trees
+    token; at most max_drafts of them are used, and none too deep to be kept. The model verifies all rows' trees
     in one pass and keeps, per row, the longest path of its own greedy choices and
     the token after it, up to max_depth tokens: whatever is drafted, the tokens
-    are greedy ones. Rejected drafts take no pool slots."""
+    are greedy ones. Rejected drafts take no pool slots, so the pool and the positions
+    needed are generate_batched's."""
     if max_new_tokens < 0:
         raise ValueError("max_new_tokens must be >= 0")
     if max_depth < 1 or not 0 <= max_drafts < MAX_TREE_NODES:
@@ -159,8 +170,8 @@ def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft,
         first = _greedy_ids(model.forward_batch(cohort.prefill_batch(), pool))
         rows = [list(ids) + [tok] for ids, tok in zip(prompts_ids, first)]
         goal = [len(ids) + max_new_tokens for ids in prompts_ids]
-        # a row's last step may accept up to max_depth - 1 tokens past its goal
-        need = [blocks_for(g + max_depth, block_size) for g in goal]
+        # no tree goes past its row's goal, and the last token takes no slot
+        need = [blocks_for(g - 1, block_size) for g in goal]
         held = [len(r.block_table) for r in cohort.rows]
         try:
             stock = alloc.allocate_n(sum(need) - sum(held))
@@ -172,7 +183,8 @@ def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft,
                 tokens, parents, starts = [], [], [0]
                 for row, g in zip(rows, goal):
                     if len(row) < g:  # a finished row takes no nodes
-                        t, p = _draft_tree(draft, list(row), max_drafts, vocab)
+                        t, p = _draft_tree(draft, list(row), max_drafts,
+                                           min(max_depth, g - len(row)), vocab)
                         tokens += [row[-1]] + t
                         parents += [-1] + p
                     starts.append(len(tokens))
