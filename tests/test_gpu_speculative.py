@@ -7,6 +7,8 @@ projections of at most 128 terms and attention over at most 60 keys; a sum of n
 terms is off by at most n 2^-24 of the terms' absolute sum, and the bound used,
 1e-4 of the logits' scale, leaves a factor of 1700 over 2^-24 for the absolute sums
 and their passage through 9 projections of up to 128 terms (9 * 128 = 1152)."""
+from dataclasses import replace
+
 import numpy as np
 import pytest
 import torch
@@ -19,7 +21,7 @@ from serving.layers import ModelConfig
 from serving.paged_meta import DeviceTables, build_batch_meta, raise_step_status
 from serving.paged_model import PagedTransformer
 from serving.sequence import Sequence
-from serving.tree_decode import build_tree_meta, tree_accept
+from serving.tree_decode import build_tree_meta, paged_tree_attention, tree_accept
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -263,3 +265,33 @@ def test_step_captured_with_the_model():
         want = [t.clone() for t in step()]
         assert all(torch.equal(a, b) for a, b in zip(got, want)), it
     raise_step_status(status, "step")
+
+
+def test_metadata_of_another_batch_is_refused():
+    cfg, model = small_model()
+    pool = make_pool(cfg, torch.float32, blocks=4)
+    tables = DeviceTables.from_host([[1], [2]], [5, 9], [3], 2, 16, 4, DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    tree = build_tree_meta(tables, i32([-1, 0, -1]), i32([0, 2, 3]), 2)
+    x = torch.zeros(3, cfg.num_heads, cfg.head_dim, device=DEV)
+    kv = torch.zeros(3, 1, cfg.head_dim, device=DEV)
+    ids = torch.zeros(3, dtype=torch.long, device=DEV)
+    for name in ("ctx_lens", "query_start_loc"):
+        bad = replace(tree, **{name: getattr(tree, name)[:-1]})
+        with pytest.raises(ValueError):
+            paged_tree_attention(x, kv, kv, pool.flat_k[0].view(4, 16, 1, -1),
+                                 pool.flat_v[0].view(4, 16, 1, -1), bad)
+    for name in ("parents", "query_start_loc"):
+        with pytest.raises(ValueError):
+            tree_accept(ids, ids, replace(tree, **{name: getattr(tree, name)[:-1]}), 2)
+    accepted = tree_accept(ids, ids, tree, 2)
+    meta, _ = build_batch_meta(tables, accepted.lens, 4, 2)
+    rows = torch.zeros(cfg.num_layers, 3, 1, cfg.head_dim, device=DEV)
+    for name in ("block_tables", "start_pos"):
+        with pytest.raises(ValueError):
+            pool.write_accepted(rows, rows, tree, accepted,
+                                replace(meta, **{name: getattr(meta, name)[:-1]}))
+    with pytest.raises(ValueError):
+        pool.write_accepted(rows, rows, replace(tree, query_start_loc=tree.query_start_loc[:-1]),
+                            accepted, meta)
+    pool.write_accepted(rows, rows, tree, accepted, meta)

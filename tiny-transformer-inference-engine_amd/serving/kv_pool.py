@@ -220,6 +220,8 @@ class KVPool:
         for t in (path, lens, qsl, table, start):
             if t.dtype != torch.int32 or not t.is_contiguous():
                 raise ValueError(f"{what}: paths, lengths and metadata must be contiguous int32")
+        if table.shape[0] != n or start.numel() != n or qsl.numel() != n + 1:
+            raise ValueError(f"{what}: the metadata's tensors are not those of {n} sequences")
         k = k_rows if k_rows.is_contiguous() else k_rows.contiguous()
         v = v_rows if v_rows.is_contiguous() else v_rows.contiguous()
         row = self.num_kv_heads * self.head_dim

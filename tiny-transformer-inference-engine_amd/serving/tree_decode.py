@@ -157,6 +157,9 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                             or lse.device != dev or not lse.is_contiguous()):
         raise ValueError(f"{what}: lse must be contiguous float32 [{T}, {hq}] on {dev}")
     n, max_blk = table.shape
+    ctx, qsl = meta.ctx_lens, meta.query_start_loc
+    if ctx.numel() != n or qsl.numel() != n + 1:
+        raise ValueError(f"{what}: the metadata's tensors are not those of {n} sequences")
     max_nodes, max_ctx = meta.max_nodes, meta.max_ctx_len
     calls = _native.calls()
     previous = _native.make_current(dev)
@@ -178,8 +181,8 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         rc = calls.pkv_paged_tree_attention(
             dst.data_ptr(), None if lse is None else lse.data_ptr(), q.data_ptr(), k.data_ptr(),
             v.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), nb, bs,
-            table.data_ptr() if max_blk else None, max_blk, meta.ctx_lens.data_ptr(),
-            meta.query_start_loc.data_ptr(), masks.data_ptr(), masks.shape[1], n, T, max_nodes,
+            table.data_ptr() if max_blk else None, max_blk, ctx.data_ptr(),
+            qsl.data_ptr(), masks.data_ptr(), masks.shape[1], n, T, max_nodes,
             max_ctx, hq, hkv, d, float(scale) if scale is not None and scale > 0 else 0.0,
             part_tokens, code, None if ws is None else ws.data_ptr(), nbytes,
             None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
@@ -203,6 +206,8 @@ def tree_accept(picks: torch.Tensor, tokens: torch.Tensor, meta: TreeMeta, max_d
     _native.require_device(picks, tokens, what=what)
     parents, qsl, T, n = meta.parents, meta.query_start_loc, meta.num_tokens, meta.num_seqs
     dev = parents.device
+    qsl = _int_tensor(qsl, torch.int32, n + 1, dev, "query_start_loc", what)
+    parents = _int_tensor(parents, torch.int32, T, dev, "parents", what)
     picks = _int_tensor(picks, torch.int64, T, dev, "picks", what)
     tokens = _int_tensor(tokens, torch.int64, T, dev, "tokens", what)
     max_depth = int(max_depth)
