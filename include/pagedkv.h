@@ -171,7 +171,9 @@ int pkv_append(void* k_pool, void* v_pool, int64_t pool_slots,
  *   block_tables[s * max_blk + p / block_size] * block_size + p % block_size.
  * A position beyond max_blk blocks (PKV_STATUS_SHORT_TABLE) or a physical
  * block outside [1, num_blocks) (PKV_STATUS_BAD_BLOCK; block 0 is reserved)
- * is skipped. Same result as make_slot_mapping + write per sequence.
+ * is skipped. Rows outside [query_start_loc[0], query_start_loc[n_seq]) belong
+ * to no sequence and are not written. Same result as make_slot_mapping + write
+ * per sequence.
  * Replaces serving/kv_pool.py:40-70 as looped in serving/paged_mqa.py:87-99.
  */
 int pkv_append_from_table(void* k_pool, void* v_pool, int64_t num_blocks,

@@ -1,0 +1,142 @@
+"""Metadata that build_batch_meta makes on the device, handed on to what takes a
+step's metadata: appends, attention, the model's step, the accepted rows' way into
+the pool. num_tokens and max_q_len are bounds there, sequences may have no token, and
+a step may fail or be dropped and taken again. Copied rows are compared byte by byte;
+a token of one batch runs through the same kernels with the same partitions as the
+host-packed batch it is compared with, except where a tolerance says otherwise."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_ref, tree_ref
+from serving.kv_pool import KVPool
+from serving.paged_meta import DeviceTables, build_batch_meta, pack_batch_meta
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F8, BF, F32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32
+
+
+def i32(x):
+    return torch.tensor(list(x), dtype=torch.int32, device=DEV)
+
+
+def bits(t):
+    return t.view(torch.uint8) if t.dtype == F8 else t
+
+
+class Batch:
+    """Sequences of ctx tokens over shuffled blocks of bs, blocks behind them for q more."""
+
+    def __init__(self, ctx, q, bs=16, seed=0):
+        rng = np.random.default_rng(seed)
+        self.ctx, self.q, self.bs = list(ctx), list(q), bs
+        held = [-(-c // bs) for c in ctx]
+        need = [max(0, -(-(c + n) // bs) - h) if n else 0 for c, n, h in zip(ctx, q, held)]
+        self.nb = sum(held) + sum(need) + 3
+        ids = rng.permutation(np.arange(1, self.nb)).tolist()
+        self.rows, self.free = [], ids[sum(held):]
+        self.after = []  # the rows with the blocks the step adds
+        for h in held:
+            self.rows.append(ids[:h])
+            ids = ids[h:]
+        spare = list(self.free)
+        for row, n in zip(self.rows, need):
+            self.after.append(row + spare[:n])
+            spare = spare[n:]
+        self.width = max([len(r) for r in self.after] + [1]) + 1
+
+    def tables(self):
+        return DeviceTables.from_host(self.rows, self.ctx, self.free, self.width, self.bs,
+                                      self.nb, DEV)
+
+    def meta(self, pad=0, bound=0, max_kv=0):
+        return build_batch_meta(self.tables(), i32(self.q), sum(self.q) + pad,
+                                bound or max(self.q), max_kv)[0]
+
+    def host_meta(self):
+        """pack_batch_meta of the sequences that have tokens."""
+        some = [s for s, n in enumerate(self.q) if n]
+        pos = [self.ctx[s] + i for s in some for i in range(self.q[s])]
+        return pack_batch_meta([self.after[s] for s in some],
+                               np.cumsum([0] + [self.q[s] for s in some]).tolist(), pos,
+                               len(pos), torch.device(DEV), self.bs)
+
+    def slots(self):
+        return np.concatenate([np.asarray(paged_ref.make_slot_mapping(c, n, t, self.bs),
+                                          dtype=np.int64)
+                               for c, n, t in zip(self.ctx, self.q, self.after)])
+
+    def pool(self, hkv, d, dtype, layers=1, seed=1):
+        pool = KVPool(layers, self.bs, self.nb, hkv, d, dtype, DEV)
+        g = torch.Generator().manual_seed(seed)
+        pool.kv.copy_(torch.randn(pool.kv.shape, generator=g).to(dtype))
+        return pool
+
+
+# ---- rows behind the last token
+
+PADDED = [([20, 3, 37], [4, 1, 0]), ([20, 3, 37], [0, 5, 2]), ([5], [3]), ([33, 16], [0, 0]),
+          ([16, 31, 0, 8], [1, 0, 1, 0])]
+
+
+@pytest.mark.parametrize("ctx,q", PADDED)
+@pytest.mark.parametrize("dtype,kv,d", [(F32, F32, 8), (BF, BF, 64), (BF, BF, 5), (BF, F8, 64),
+                                        (F32, F8, 8)])
+def test_padding_is_not_appended(ctx, q, dtype, kv, d):
+    """KVPool.write_from_table with more rows than tokens: the others' slots keep what
+    they held, the last sequence's context among them."""
+    print(f"[append] {ctx} {q} {dtype} {kv} d={d}", flush=True)
+    b = Batch(ctx, q)
+    for pad in (1, 40):
+        T = sum(q) + pad
+        pool, want = b.pool(2, d, kv, 2), b.pool(2, d, kv, 2)
+        g = torch.Generator().manual_seed(2)
+        k, v = (torch.randn(T, 2, d, generator=g).to(dtype).to(DEV) for _ in range(2))
+        pool.write_from_table(1, k, v, b.meta(pad, 8))
+        real = torch.from_numpy(b.slots()).to(DEV)
+        for flat, rows in ((want.flat_k[1], k), (want.flat_v[1], v)):
+            bits(flat)[real] = bits(rows[:sum(q)].to(kv))
+        assert torch.equal(bits(pool.kv), bits(want.kv))
+
+
+def test_padding_is_not_appended_many_sequences():
+    """More sequences than query_start_loc entries fit the append's LDS."""
+    n = 4200
+    rng = np.random.default_rng(3)
+    b = Batch(rng.integers(0, 5, size=n).tolist(), (rng.integers(0, 3, size=n - 1)).tolist() + [0],
+              bs=4)
+    pool, want = b.pool(1, 8, F32), b.pool(1, 8, F32)
+    k = torch.randn(sum(b.q) + 50, 1, 8, device=DEV)
+    pool.write_from_table(0, k, -k, b.meta(50))
+    real = torch.from_numpy(b.slots()).to(DEV)
+    want.flat_k[0][real], want.flat_v[0][real] = k[:sum(b.q)], -k[:sum(b.q)]
+    assert torch.equal(pool.kv, want.kv)
+
+
+@pytest.mark.parametrize("dtype,kv,hq,hkv,d", [(F32, F32, 8, 1, 64), (F32, F32, 4, 4, 80),
+                                               (BF, BF, 8, 1, 64), (BF, BF, 16, 1, 64),
+                                               (BF, BF, 32, 1, 128), (BF, F8, 16, 1, 64)])
+@pytest.mark.parametrize("ctx,q", [([20, 300, 37], [1, 0, 1]), ([20, 300, 37], [1, 1, 0]),
+                                   ([20, 70, 37], [0, 1, 7]), ([20, 5, 37], [40, 1, 0]),
+                                   ([5000, 17, 90], [1, 1, 0]), ([5000, 17, 90], [1, 9, 0])])
+def test_padded_steps_append_and_attend(ctx, q, dtype, kv, hq, hkv, d):
+    """paged_attention_append_meta (fused or not) of a padded step: pool and rows as the
+    host-packed batch of the sequences with tokens gives them, rows behind untouched."""
+    from serving.fake_paged_attn import paged_attention_append_meta
+    print(f"[fused] {ctx} {q} {dtype} {kv} {hq}x{hkv}x{d}", flush=True)
+    b = Batch(ctx, q)
+    T, pad = sum(q), 4
+    g = torch.Generator().manual_seed(4)
+    rows = [torch.randn(T + pad, h, d, generator=g).to(dtype).to(DEV) for h in (hq, hkv, hkv)]
+    got, want = b.pool(hkv, d, kv), b.pool(hkv, d, kv)
+    out = torch.full_like(rows[0], 9.0)
+    paged_attention_append_meta(*rows, got, 0, b.meta(pad), out=out)
+    ref = paged_attention_append_meta(*[x[:T].contiguous() for x in rows], want, 0, b.host_meta())
+    assert torch.equal(bits(got.kv), bits(want.kv))
+    # other partitions of the contexts: sums of at most 5001 weights in another order, and
+    # 16-bit probabilities against another maximum; values of at most 6
+    u = torch.finfo(dtype).eps / 2
+    tol = 6 * (2 * 5001 * 2.0 ** -24 + (2 * u if dtype != F32 else 0)) + 2 * u
+    assert float((out[:T].float() - ref.float()).abs().max()) <= tol
+    assert (out[T:] == 9).all()

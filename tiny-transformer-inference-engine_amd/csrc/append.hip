@@ -65,8 +65,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(
   }
 }
 
-// Sequence owning token `t`: the largest s with qloc[s] <= t (qloc is the
-// non-decreasing cumulative query count, n_seq + 1 entries).
+// Sequence owning token `t`, qloc[0] <= t < qloc[n_seq]: the largest s with
+// qloc[s] <= t (qloc is the non-decreasing cumulative query count, n_seq + 1
+// entries). Rows outside that range are padding (a batch whose lengths only the
+// device knows has more rows than tokens) and are nobody's.
 __device__ __forceinline__ int seq_of_token(const int32_t* __restrict__ qloc,
                                             int n_seq, int64_t t) {
   int lo = 0, hi = n_seq - 1;
@@ -107,6 +109,7 @@ __global__ __launch_bounds__(kThreads) void append_table_kernel(
        i += stride) {
     const int64_t tok = i / ppr;
     const int64_t pc = i - tok * ppr;
+    if (tok < ql[0] || tok >= ql[n_seq]) continue;  // no sequence's row
     const int s = seq_of_token(ql, n_seq, tok);
     // rows of sequences with fewer than min_qlen tokens are another
     // launch's (the fused decode append of a mixed batch)
@@ -225,6 +228,7 @@ __global__ __launch_bounds__(kThreads) void append_table_fp8_kernel(
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += stride) {
     const int64_t tok = i / ppr;
     const int64_t pc = i - tok * ppr;
+    if (tok < ql[0] || tok >= ql[n_seq]) continue;  // no sequence's row
     const int s = seq_of_token(ql, n_seq, tok);
     if (min_qlen > 1 && ql[s + 1] - ql[s] < min_qlen) continue;
     const int64_t pos = (int64_t)start_pos[s] + (tok - ql[s]);

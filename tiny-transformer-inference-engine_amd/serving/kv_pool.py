@@ -175,7 +175,8 @@ class KVPool:
     def write_from_table(self, layer: int, k: torch.Tensor, v: torch.Tensor, meta) -> None:
         """Append the step's new K/V rows of every sequence with slots computed
         in-kernel from `meta` (a PagedBatchMeta): equivalent to
-        make_slot_mapping per sequence + one write (serving/paged_mqa.py:87-99)."""
+        make_slot_mapping per sequence + one write (serving/paged_mqa.py:87-99).
+        Rows behind the last sequence's are not written."""
         self.check_rows(k, v, meta)
         _native.require_device(self.kv, k, v, what="KVPool.write_from_table")
         k = k.contiguous()
