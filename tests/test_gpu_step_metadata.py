@@ -140,3 +140,59 @@ def test_padded_steps_append_and_attend(ctx, q, dtype, kv, hq, hkv, d):
     tol = 6 * (2 * 5001 * 2.0 ** -24 + (2 * u if dtype != F32 else 0)) + 2 * u
     assert float((out[:T].float() - ref.float()).abs().max()) <= tol
     assert (out[T:] == 9).all()
+
+
+# ---- sequences without a token in the model's step
+
+def small_model(dtype=F32):
+    from serving.layers import ModelConfig
+    from serving.paged_model import PagedTransformer
+    cfg = ModelConfig(vocab_size=97, d_model=128, num_layers=2, num_heads=4, num_kv_heads=1,
+                      max_seq_len=160)
+    torch.manual_seed(0)
+    return cfg, PagedTransformer(cfg).to(DEV, dtype).eval()
+
+
+def test_bounds_are_no_decode_batch():
+    b = Batch([20, 5], [1, 1])
+    assert b.host_meta().is_decode
+    assert not b.meta().is_decode  # one token a sequence at most, as far as the host knows
+
+
+@pytest.mark.parametrize("ctx,q,pad", [([20, 3, 37], [1, 0, 1], 1), ([20, 3, 37], [1, 1, 0], 1),
+                                       ([20, 3, 37], [0, 1, 1], 1), ([20, 3, 37], [0, 3, 0], 0),
+                                       ([20, 3, 37], [5, 0, 2], 9), ([20, 3], [0, 0], 2),
+                                       ([20, 3], [0, 0], 0), ([20, 3, 37], [1, 1, 1], 0)])
+def test_forward_step_with_empty_sequences(ctx, q, pad):
+    """Logits row s is sequence s's: its last token's, zeros where it has none. The pass
+    is the host-packed batch's of the other sequences, its projections over another
+    number of rows: sums of at most 128 terms in another order, 9 of them (see
+    test_gpu_speculative.py)."""
+    print(f"[step] {ctx} {q} pad={pad}", flush=True)
+    cfg, model = small_model()
+    b = Batch(ctx, q)
+    T = sum(q)
+    got, want = (b.pool(1, cfg.head_dim, F32, cfg.num_layers) for _ in range(2))
+    ids = torch.arange(T + pad, device=DEV) % 97
+    logits = model.forward_step(ids, got, b.meta(pad, max(max(q), 1)))
+    assert logits.shape == (len(q), 97)
+    some = [s for s, n in enumerate(q) if n]
+    if some:
+        ref = model.forward_step(ids[:T], want, b.host_meta())
+        scale = float(ref.abs().max())
+        assert float((logits[some] - ref).abs().max()) <= 1e-4 * scale
+        assert float((got.kv - want.kv).abs().max()) <= 1e-4 * float(want.kv.abs().max())
+    else:
+        assert torch.equal(got.kv, want.kv)
+    none = [s for s, n in enumerate(q) if not n]
+    assert (logits[none] == 0).all()
+
+
+def test_decode_graph_refuses_bounds():
+    from serving.graph_step import DecodeStepGraph
+    cfg, model = small_model()
+    b = Batch([20, 3], [1, 0])
+    pool = b.pool(1, cfg.head_dim, F32, cfg.num_layers)
+    ids = torch.zeros(2, dtype=torch.long, device=DEV)
+    with pytest.raises(ValueError, match="decode batch"):
+        DecodeStepGraph(model, pool, b.meta(1), ids)

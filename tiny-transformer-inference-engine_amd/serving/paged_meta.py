@@ -40,10 +40,14 @@ class PagedBatchMeta:
     # int64 [T], build_batch_meta only: each token's pool slot (KVPool.write's
     # slot_mapping), NO_SLOT behind the last token
     slot_mapping: torch.Tensor | None = None
+    # False (build_batch_meta): num_tokens and max_q_len are bounds on lengths that
+    # only the device knows; there may be rows of no sequence and sequences of no token
+    exact: bool = True
 
     @property
     def is_decode(self) -> bool:
-        return self.max_q_len == 1 and self.num_tokens == self.num_seqs
+        """One token a sequence: token row s is sequence s's."""
+        return self.exact and self.max_q_len == 1 and self.num_tokens == self.num_seqs
 
     def advance_(self) -> None:
         """Every sequence one token further, on the device: seq_lens,
@@ -245,7 +249,10 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     table's capacity) the contexts after the step.
 
     Returns (PagedBatchMeta with slot_mapping, DeviceTables after the step).
-    Values as pack_batch_meta gives them; the given tables' other tensors are not
+    Values as pack_batch_meta gives them, and like its result the step can go to
+    KVPool.write_from_table, paged_attention_append_meta and
+    PagedTransformer.forward_step, though never as a decode batch (is_decode): its
+    lengths are not the host's to know; the given tables' other tensors are not
     changed, so a step whose result is dropped can be taken again. With too few
     free blocks, a row past max_blocks or a length out of bounds nothing is taken
     (all or nothing), which `status` (int32 [1], zeroed by the caller, read with
@@ -285,5 +292,5 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     if max_kv_len <= 0:
         max_kv_len = max_blocks * bs
     meta = PagedBatchMeta(bt, seq_lens, qsl, start_pos, positions, n, T, max_blocks, max_q_len,
-                          int(max_kv_len), bs, i32, slots)
+                          int(max_kv_len), bs, i32, slots, False)
     return meta, tables._after(held, ctx, cursor)

@@ -67,7 +67,10 @@ class PagedTransformer(nn.Module):
 
     @torch.no_grad()
     def forward_step(self, input_ids, pool, meta):
-        """forward_batch with pre-packed metadata (PagedBatchMeta).
+        """forward_batch with pre-packed metadata (PagedBatchMeta). With lengths
+        from the device (build_batch_meta) input_ids has num_tokens rows, those
+        behind the last token of any value, and a sequence without a token gets
+        logits of zeros.
 
         On a ROCm device every norm runs in the prologue of the projection
         that consumes it and every residual add in the epilogue of the
@@ -82,15 +85,25 @@ class PagedTransformer(nn.Module):
                 x = layer.forward_meta(x, pool, meta)
             last = meta.query_start_loc[1:].long() - 1
             return self.lm_head(self.final_norm(x.index_select(0, last)))
+        if not meta.exact and x.shape[0] == 0:
+            return x.new_zeros((meta.num_seqs, self.lm_head.out_features))
         x = x.contiguous()
         attr = fused_ops.module_attr
         for layer in self.layers:
             attr(layer, "attn").forward_meta_residual_(x, attr(layer, "attn_norm"), pool,
                                                        layer.layer_idx, meta)
             attr(layer, "mlp").forward_residual_(x, attr(layer, "mlp_norm"))
+        if not meta.exact:
+            return self._logits_of_last(x, meta.query_start_loc)
         if not meta.is_decode:
             x = x.index_select(0, meta.query_start_loc[1:].long() - 1)
         return self.lm_head(self.final_norm(x))
+
+    def _logits_of_last(self, x, qsl):
+        """Logits of each sequence's last row of x, zeros where it has none."""
+        rows = x.index_select(0, (qsl[1:].long() - 1).clamp_(min=0))
+        return self.lm_head(self.final_norm(rows)).masked_fill_(
+            (qsl[1:] == qsl[:-1])[:, None], 0)
 
     @torch.no_grad()
     def forward_tree(self, input_ids, pool, tree):
