@@ -196,3 +196,46 @@ def test_decode_graph_refuses_bounds():
     ids = torch.zeros(2, dtype=torch.long, device=DEV)
     with pytest.raises(ValueError, match="decode batch"):
         DecodeStepGraph(model, pool, b.meta(1), ids)
+
+
+# ---- advance_
+
+@pytest.mark.parametrize("ctx,q,pad", [([20, 3, 31], [1, 0, 1], 2), ([16, 15], [1, 1], 0),
+                                       ([4, 9], [0, 3], 1)])
+def test_advance_leaves_padding_and_slots_of_nobody(ctx, q, pad):
+    b = Batch(ctx, q)
+    meta, T = b.meta(pad), sum(q)
+    was = {n: getattr(meta, n).tolist() for n in ("seq_lens", "start_pos", "positions")}
+    for step in (1, 2):
+        meta.advance_()
+        assert meta.seq_lens.tolist() == [x + step if n else 0 for x, n in zip(was["seq_lens"], q)]
+        assert meta.start_pos.tolist() == [x + step if n else 0
+                                           for x, n in zip(was["start_pos"], q)]
+        assert meta.positions.tolist() == [x + step for x in was["positions"][:T]] + [0] * pad
+    # the next tokens' slots are another step's to give: an append skips these
+    assert meta.slot_mapping.tolist() == [tree_ref.NO_SLOT] * (T + pad)
+    pool, want = b.pool(1, 8, F32), b.pool(1, 8, F32)
+    k = torch.ones(T + pad, 1, 8, device=DEV)
+    pool.write(0, meta.slot_mapping, k, k)
+    assert torch.equal(pool.kv, want.kv)
+
+
+def test_advance_in_a_graph():
+    b = Batch([20, 3, 31], [1, 0, 1])
+    meta, twin = b.meta(2), b.meta(2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        meta.advance_()
+        twin.advance_()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        meta.advance_()
+    for it in range(4):
+        graph.replay()
+        twin.advance_()
+        torch.cuda.synchronize()
+        for name in ("seq_lens", "start_pos", "positions", "slot_mapping"):
+            assert torch.equal(getattr(meta, name), getattr(twin, name)), (it, name)

@@ -34,8 +34,8 @@ class PagedBatchMeta:
     max_q_len: int
     max_kv_len: int
     block_size: int
-    # seq_lens, start_pos and positions at the front of one contiguous tensor (both
-    # packers lay them out back to back), so a decode step advances them with one add
+    # seq_lens, start_pos and positions as one contiguous view (pack_batch_meta
+    # lays them out back to back), so a decode step advances them with one add
     step_view: torch.Tensor | None = None
     # int64 [T], build_batch_meta only: each token's pool slot (KVPool.write's
     # slot_mapping), NO_SLOT behind the last token
@@ -51,14 +51,27 @@ class PagedBatchMeta:
 
     def advance_(self) -> None:
         """Every sequence one token further, on the device: seq_lens,
-        start_pos and positions + 1 (one kernel when they share step_view)."""
+        start_pos and positions + 1 (one kernel when they share step_view).
+        With lengths from the device only sequences that have tokens, and their
+        rows; slot_mapping becomes NO_SLOT throughout, as the slots of later tokens
+        are another build_batch_meta's to give."""
+        if not self.exact:
+            some = (self.query_start_loc[1:] > self.query_start_loc[:-1]).int()
+            self.seq_lens.add_(some)
+            self.start_pos.add_(some)
+            rows = torch.arange(self.num_tokens, dtype=torch.int32,
+                                device=self.positions.device)
+            self.positions.add_((rows < self.query_start_loc[-1]).int())
+            if self.slot_mapping is not None:
+                self.slot_mapping.fill_(NO_SLOT)
+            return
         v = self.step_view
         n, t = self.num_seqs, self.num_tokens
-        if (v is not None and v.numel() >= 2 * n + t and v.dtype == torch.int32
+        if (v is not None and v.numel() == 2 * n + t and v.dtype == torch.int32
                 and self.seq_lens.data_ptr() == v.data_ptr()
                 and self.start_pos.data_ptr() == v.data_ptr() + 4 * n
                 and self.positions.data_ptr() == v.data_ptr() + 8 * n):
-            (v if v.numel() == 2 * n + t else v[:2 * n + t]).add_(1)
+            v.add_(1)
             return
         self.positions.add_(1)
         self.start_pos.add_(1)
@@ -271,7 +284,6 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     free = tables.free_blocks
     previous = _native.make_current(dev)
     try:
-        # seq_lens, start_pos and positions back to back, as pack_batch_meta's
         i32 = bt.new_empty(5 * n + 2 + T)
         slots = torch.empty(T, dtype=torch.int64, device=dev)
         at = i32.data_ptr()
@@ -292,5 +304,5 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     if max_kv_len <= 0:
         max_kv_len = max_blocks * bs
     meta = PagedBatchMeta(bt, seq_lens, qsl, start_pos, positions, n, T, max_blocks, max_q_len,
-                          int(max_kv_len), bs, i32, slots, False)
+                          int(max_kv_len), bs, None, slots, False)
     return meta, tables._after(held, ctx, cursor)
