@@ -532,8 +532,10 @@ size_t pkv_argmax_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
  * with too few free blocks (PKV_STATUS_OUT_OF_BLOCKS), a row past max_blk
  * blocks (PKV_STATUS_SHORT_TABLE) or a length outside its bounds
  * (PKV_STATUS_BAD_QLOC) no block is taken, the state after is the state before,
- * and positions without a held block have slot INT64_MIN. A block id outside
- * [1, num_blocks) gives that slot too (PKV_STATUS_BAD_BLOCK). At most 16384
+ * and no append writes a row of the step: seq_lens is 0, start_pos -2^30 and
+ * slot_mapping INT64_MIN throughout (appends by position raise
+ * PKV_STATUS_SHORT_TABLE). A block id outside [1, num_blocks) gives its tokens slot
+ * INT64_MIN (PKV_STATUS_BAD_BLOCK). At most 16384
  * sequences.
  */
 int pkv_build_step(int32_t* block_tables, int max_blk, const int32_t* blocks_held,

@@ -239,3 +239,74 @@ def test_advance_in_a_graph():
         torch.cuda.synchronize()
         for name in ("seq_lens", "start_pos", "positions", "slot_mapping"):
             assert torch.equal(getattr(meta, name), getattr(twin, name)), (it, name)
+
+
+# ---- a step that fails is no step for anybody
+
+FAILS = {  # sequence 0 lacks a block, sequence 1 has one to spare
+    "blocks": dict(free=[]),
+    "cursor": dict(cursor=7),
+    "short": dict(q=[40, 3]),
+    "far": dict(ctx=[16, 2147483000]),
+    "long": dict(q=[3, 9]),          # past max_q_len
+    "negative": dict(q=[3, -1]),
+    "tokens": dict(T=5),             # more tokens than rows
+    "held": dict(held=[1, -1]),
+}
+
+
+@pytest.mark.parametrize("what", FAILS)
+@pytest.mark.parametrize("stale", [0, 5])
+def test_failed_steps_write_nothing(what, stale):
+    """Every way of a step's rows into the pool: accepted rows, the append through the
+    table, the append through slots, attention's own append. Row 0 of the table may
+    name a block behind those it holds that is another sequence's by now."""
+    from serving.fake_paged_attn import paged_attention_append_meta
+    from serving.tree_decode import TreeAccept, build_tree_meta
+    print(f"[failed] {what} stale={stale}", flush=True)
+    a = dict(ctx=[16, 10], q=[3, 3], held=[1, 1], free=[6, 7], cursor=0, T=12)
+    a.update(FAILS[what])
+    dt = DeviceTables(block_tables=i32([1, stale, stale, 2, 0, 0]).view(2, 3),
+                      blocks_held=i32(a["held"]), ctx_lens=i32(a["ctx"]),
+                      free_blocks=i32(a["free"]), free_cursor=i32([a["cursor"]]), block_size=16,
+                      num_blocks=9)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    tree = build_tree_meta(dt, i32([-1, 0, 1] * 2), i32([0, 3, 6]), 3)
+    meta, after = build_batch_meta(dt, i32(a["q"]), a["T"], 8 if what != "short" else 50,
+                                   status=st)
+    assert int(st) != 0
+    assert after.blocks_held.tolist() == a["held"] and after.ctx_lens.tolist() == a["ctx"]
+    for dtype, kv, hq in ((F32, F32, 8), (BF, BF, 16), (BF, F8, 16)):
+        b = Batch([16, 10], [3, 3])
+        b.nb = 9
+        pool, want = b.pool(1, 64, kv, 2), b.pool(1, 64, kv, 2)
+        rows = torch.ones(2, 6, 1, 64, dtype=dtype, device=DEV)
+        acc = TreeAccept(lens=i32([3, 3]), path=i32([0, 1, 2] * 2).view(2, 3), tokens=None)
+        pool.write_accepted(rows, rows, tree, acc, meta)
+        assert torch.equal(bits(pool.kv), bits(want.kv)), "write_accepted"
+        k = torch.ones(a["T"], 1, 64, dtype=dtype, device=DEV)
+        pool.write_from_table(1, k, k, meta)
+        assert torch.equal(bits(pool.kv), bits(want.kv)), "write_from_table"
+        pool.write(0, meta.slot_mapping, k, k)
+        assert torch.equal(bits(pool.kv), bits(want.kv)), "write"
+        q = torch.ones(a["T"], hq, 64, dtype=dtype, device=DEV)
+        paged_attention_append_meta(q, k, k, pool, 0, meta)
+        assert torch.equal(bits(pool.kv), bits(want.kv)), "paged_attention_append_meta"
+
+
+def test_a_failed_step_after_a_dropped_one():
+    """A dropped step's block goes to another sequence, and a step that then fails
+    leaves that sequence's rows alone."""
+    from serving.tree_decode import TreeAccept, build_tree_meta
+    dt = DeviceTables.from_host([[1], [2]], [16, 16], [5, 6], 3, 16, 9, DEV)
+    build_batch_meta(dt, i32([1, 0]), 2, 1)                      # block 5 to row 0: dropped
+    _, dt = build_batch_meta(dt, i32([0, 1]), 2, 1)              # sequence 1's by now
+    pool = KVPool(1, 16, 9, 1, 8, F32, DEV)
+    pool.kv.normal_()
+    before = pool.kv.clone()
+    tree = build_tree_meta(dt, i32([-1, -1]), i32([0, 1, 2]), 1)
+    meta, _ = build_batch_meta(dt, i32([1, 17]), 18, 17)         # two blocks of the one left
+    rows = torch.ones(1, 2, 1, 8, device=DEV)
+    pool.write_accepted(rows, rows, tree, TreeAccept(i32([1, 1]), i32([0, 0]).view(2, 1), None),
+                        meta)
+    assert torch.equal(pool.kv, before)

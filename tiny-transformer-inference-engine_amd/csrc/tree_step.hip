@@ -18,6 +18,9 @@ constexpr int kStepThreads = 256;
 constexpr int kStepWaves = kStepThreads / 64;
 constexpr int kStepMaxSeq = 16384;  // two ints a sequence in LDS
 constexpr int64_t kNoSlot = INT64_MIN;
+// start_pos in a failed step: no append takes a position below 0, and adding a
+// run's index to it, or taking it from a position, stays an int
+constexpr int kNoPos = -(1 << 30);
 
 // ---------------------------------------------------------------------------
 // Step metadata. need_s = blocks sequence s lacks for its ctx + q tokens; the
@@ -26,7 +29,9 @@ constexpr int64_t kNoSlot = INT64_MIN;
 // table entries only past held_s, where no slot is looked up), so every
 // workgroup scans all lengths for itself and no order between workgroups is
 // needed. All or nothing: where the free list or a row of the table is too
-// short, or a length is bad, no block is taken.
+// short, or a length is bad, no block is taken, and the metadata names no
+// position or slot that whoever is handed it could write to: the host, which only
+// learns of the failure later, has launched them already.
 // ---------------------------------------------------------------------------
 struct StepArgs {
   int32_t* table;
@@ -125,8 +130,8 @@ __global__ __launch_bounds__(kStepThreads) void build_step_kernel(StepArgs a) {
     const int c = a.ctx[s];
     a.held_out[s] = a.held[s] + (fails ? 0 : blk0[s + 1] - blk0[s]);
     a.ctx_out[s] = fails ? c : c + q;
-    a.seq_lens[s] = q > 0 ? c + q : 0;
-    a.start_pos[s] = q > 0 ? c : 0;
+    a.seq_lens[s] = fails || q == 0 ? 0 : c + q;
+    a.start_pos[s] = fails ? kNoPos : q > 0 ? c : 0;
   }
   bool bad_block = false;
   if (!fails) {
@@ -143,16 +148,14 @@ __global__ __launch_bounds__(kStepThreads) void build_step_kernel(StepArgs a) {
     if (t < run_t) {
       const int s = upper_seq(tok0, n, (int)t);
       pos = (int64_t)a.ctx[s] + ((int)t - tok0[s]);
-      const int64_t page = pos >> a.bs_shift;
-      const int64_t fresh = page - a.held[s];
-      int id = 0;
-      if (fresh < 0) {
-        if (page < a.max_blk) id = a.table[(int64_t)s * a.max_blk + page];
-      } else if (!fails) {
-        id = a.free_blocks[cur + blk0[s] + fresh];
+      if (!fails) {
+        const int64_t page = pos >> a.bs_shift;
+        const int64_t fresh = page - a.held[s];
+        const int id = fresh < 0 ? a.table[(int64_t)s * a.max_blk + page]
+                                 : a.free_blocks[cur + blk0[s] + fresh];
+        if (id > 0 && id < a.num_blocks) slot = ((int64_t)id << a.bs_shift) + (pos & bs_mask);
+        else bad_block = true;
       }
-      if (id > 0 && id < a.num_blocks) slot = ((int64_t)id << a.bs_shift) + (pos & bs_mask);
-      else bad_block |= !fails;
     }
     a.positions[t] = (int)pos;
     a.slots[t] = slot;

@@ -268,8 +268,10 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     lengths are not the host's to know; the given tables' other tensors are not
     changed, so a step whose result is dropped can be taken again. With too few
     free blocks, a row past max_blocks or a length out of bounds nothing is taken
-    (all or nothing), which `status` (int32 [1], zeroed by the caller, read with
-    raise_step_status) reports. No host synchronisation."""
+    (all or nothing) and the metadata names no slot or position that an append
+    writes to, so the calls launched with it leave the pool as it is; `status` (int32
+    [1], zeroed by the caller, read with raise_step_status) reports it. No host
+    synchronisation."""
     bt = tables.block_tables
     _native.require_device(bt, what="build_batch_meta")
     dev = bt.device
