@@ -520,7 +520,9 @@ size_t pkv_argmax_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
  * (block_tables row s) and ctx_lens[s] tokens, and gets q_lens[s] more. The
  * blocks it lacks, ceil((ctx + q) / block_size) - held where that is positive
  * and q > 0, are handed out in sequence order from free_blocks[free_cursor[0]
- * ...] (num_free entries in all) and written to its row. Written besides:
+ * ...] (num_free entries in all) and written to its row; entries behind its
+ * blocks, up to the first 0, become 0 (a step that was dropped may have left ids
+ * there). Written besides:
  *   blocks_held_out, ctx_lens_out [n_seq], free_cursor_out [1]: the state after
  *     the step; other memory than the inputs (PKV_ERR_INVALID otherwise), so a
  *     step can be taken again from the same state;

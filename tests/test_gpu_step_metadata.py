@@ -310,3 +310,32 @@ def test_a_failed_step_after_a_dropped_one():
     pool.write_accepted(rows, rows, tree, TreeAccept(i32([1, 1]), i32([0, 0]).view(2, 1), None),
                         meta)
     assert torch.equal(pool.kv, before)
+
+
+def test_rows_hold_their_blocks_and_zeros_behind_them():
+    """After a step the table names no block that a dropped step had put there, whether
+    the step succeeds or fails; the same sequence may take the same block again."""
+    dt = DeviceTables.from_host([[1], [2], [3]], [16, 16, 9], [5, 6, 7, 8], 4, 16, 9, DEV)
+    build_batch_meta(dt, i32([33, 0, 7]), 64, 40)
+    assert dt.block_tables.tolist() == [[1, 5, 6, 7], [2, 0, 0, 0], [3, 0, 0, 0]]
+    build_batch_meta(dt, i32([0, 0, 60]), 64, 60)               # fails: row 2 is too short
+    assert dt.block_tables.tolist() == [[1, 0, 0, 0], [2, 0, 0, 0], [3, 0, 0, 0]]
+    build_batch_meta(dt, i32([33, 0, 7]), 64, 40)
+    _, after = build_batch_meta(dt, i32([1, 20, 0]), 64, 40)
+    assert after.block_tables.tolist() == [[1, 5, 0, 0], [2, 6, 7, 0], [3, 0, 0, 0]]
+    _, last = build_batch_meta(after, i32([0, 0, 0]), 64, 40)   # nothing to add
+    assert last.block_tables.tolist() == [[1, 5, 0, 0], [2, 6, 7, 0], [3, 0, 0, 0]]
+
+
+def test_stale_entries_of_many_sequences():
+    n = 700
+    dt = DeviceTables.from_host([[1 + s] for s in range(n)], [16] * n, range(n + 1, 4 * n + 1), 5,
+                                16, 4 * n + 1, DEV)
+    build_batch_meta(dt, i32([33] * n), 33 * n, 33)
+    rng = np.random.default_rng(5)
+    q = rng.integers(0, 34, size=n).tolist()
+    _, after = build_batch_meta(dt, i32(q), 33 * n, 33)
+    host = [[1 + s, 0, 0, 0, 0] for s in range(n)]
+    tree_ref.build_step(host, [1] * n, [16] * n, q, list(range(n + 1, 4 * n + 1)), 0, 16, 4 * n + 1,
+                        33 * n, 33)
+    assert after.block_tables.tolist() == host

@@ -26,7 +26,8 @@ constexpr int kNoPos = -(1 << 30);
 // Step metadata. need_s = blocks sequence s lacks for its ctx + q tokens; the
 // new blocks are handed out in sequence order from free[cursor ...]. Nothing
 // read here is written (held_out, ctx_out and cursor_out are other memory, and
-// table entries only past held_s, where no slot is looked up), so every
+// table entries only past held_s, where no slot is looked up and each entry has
+// one thread that writes it), so every
 // workgroup scans all lengths for itself and no order between workgroups is
 // needed. All or nothing: where the free list or a row of the table is too
 // short, or a length is bad, no block is taken, and the metadata names no
@@ -161,6 +162,15 @@ __global__ __launch_bounds__(kStepThreads) void build_step_kernel(StepArgs a) {
     a.slots[t] = slot;
   }
   if (bad_block && a.status) atomicOr(a.status, PKV_STATUS_BAD_BLOCK);
+  // Ids behind a row's blocks are left from a step that was dropped and may be another
+  // sequence's by now: zeros again, up to the first zero (one entry, usually).
+  for (int64_t s = first; s < n; s += stride) {
+    const int held = a.held[s];
+    int32_t* const row = a.table + s * a.max_blk;
+    if (held < 0) continue;
+    for (int64_t p = held + (fails ? 0 : blk0[s + 1] - blk0[s]); p < a.max_blk && row[p] != 0; ++p)
+      row[p] = 0;
+  }
 }
 
 // ---------------------------------------------------------------------------

@@ -266,7 +266,9 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     KVPool.write_from_table, paged_attention_append_meta and
     PagedTransformer.forward_step, though never as a decode batch (is_decode): its
     lengths are not the host's to know; the given tables' other tensors are not
-    changed, so a step whose result is dropped can be taken again. With too few
+    changed, so a step whose result is dropped can be taken again (the table itself
+    is one for all states: its rows are those of the last step taken, zeros behind
+    the blocks they hold). With too few
     free blocks, a row past max_blocks or a length out of bounds nothing is taken
     (all or nothing) and the metadata names no slot or position that an append
     writes to, so the calls launched with it leave the pool as it is; `status` (int32
