@@ -635,6 +635,21 @@ int pkv_write_accepted(void* k_pool, void* v_pool, int64_t pool_layer_elems, int
                        int64_t row_elems, int dtype, int* status, void* stream);
 
 /*
+ * pkv_write_accepted for the tokens of a step: of each path at most
+ * step_start_loc[s + 1] - step_start_loc[s] rows are written (the query_start_loc
+ * of the metadata that start_pos is from; a step may take fewer tokens of a
+ * sequence than were accepted, or none, and its start_pos then names no position).
+ */
+int pkv_write_accepted_step(void* k_pool, void* v_pool, int64_t pool_layer_elems, int layers,
+                            int64_t num_blocks, int block_size, const void* k_rows,
+                            const void* v_rows, int64_t rows_layer_elems,
+                            const int32_t* block_tables, int max_blk, const int32_t* start_pos,
+                            const int32_t* step_start_loc, const int32_t* query_start_loc,
+                            const int32_t* path, const int32_t* lens, int n_seq, int n_tokens,
+                            int max_depth, int64_t row_elems, int dtype, int* status,
+                            void* stream);
+
+/*
  * Measurement helper, no counterpart in the reference: reads `bytes` bytes at
  * p (16-byte aligned, a multiple of 16) once with 16-byte non-temporal loads
  * from `grid` workgroups of 256 threads and writes nothing (sink, nullable,

@@ -339,3 +339,29 @@ def test_stale_entries_of_many_sequences():
     tree_ref.build_step(host, [1] * n, [16] * n, q, list(range(n + 1, 4 * n + 1)), 0, 16, 4 * n + 1,
                         33 * n, 33)
     assert after.block_tables.tolist() == host
+
+
+@pytest.mark.parametrize("kv", [F32, F8])
+@pytest.mark.parametrize("packed", [False, True])
+def test_write_accepted_writes_the_steps_tokens_only(kv, packed):
+    """Paths longer than the tokens the step has for a sequence (a finished one's 0, a
+    goal's rest): the rows behind them are not written, neither into the context's
+    first positions nor past the sequence's blocks."""
+    from serving.tree_decode import TreeAccept, build_tree_meta
+    b = Batch([20, 14, 3, 40], [0, 2, 4, 0])
+    dt = b.tables()
+    tree = build_tree_meta(dt, i32([-1, 0, 1, 2] * 4), i32([0, 4, 8, 12, 16]), 4)
+    if packed:
+        meta = pack_batch_meta(b.after, [0, 0, 2, 6, 6], [14, 15, 3, 4, 5, 6], 6,
+                               torch.device(DEV), 16)
+    else:
+        meta, _ = build_batch_meta(dt, i32(b.q), 16, 4)
+    acc = TreeAccept(i32([4, 4, 4, 3]), i32([0, 1, 2, 3] * 3 + [0, 1, 2, -1]).view(4, 4), None)
+    pool, want = b.pool(2, 8, kv, 3), b.pool(2, 8, kv, 3)
+    k, v = torch.randn(2, 3, 16, 2, 8, device=DEV).unbind(0)
+    pool.write_accepted(k, v, tree, acc, meta)
+    slots = torch.from_numpy(b.slots()).to(DEV)
+    for layer in range(3):
+        for flat, rows in ((want.flat_k[layer], k), (want.flat_v[layer], v)):
+            bits(flat)[slots] = bits(rows[layer, [4, 5, 8, 9, 10, 11]].to(kv))
+    assert torch.equal(bits(pool.kv), bits(want.kv))

@@ -75,7 +75,7 @@ PyObject* checked(const char* name, R (*fn)(A...), PyObject* const* args, Py_ssi
   X(pkv_linear_tiles_rope_qkv) X(pkv_argmax_rows) X(pkv_sample_rows)                         \
   X(pkv_argmax_workspace_bytes) X(pkv_stream_read) X(pkv_build_step) X(pkv_tree_masks)        \
   X(pkv_tree_attention_workspace_bytes) X(pkv_paged_tree_attention) X(pkv_tree_accept)       \
-  X(pkv_write_accepted)
+  X(pkv_write_accepted) X(pkv_write_accepted_step)
 
 #define DEFINE(name)                                                                         \
   decltype(&::name) ptr_##name = nullptr;                                                    \

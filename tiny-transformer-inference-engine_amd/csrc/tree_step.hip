@@ -311,8 +311,9 @@ __global__ __launch_bounds__(kStepThreads) void tree_accept_kernel(AcceptArgs a)
 
 // ---------------------------------------------------------------------------
 // Accepted rows: row path[s][k] of sequence s's nodes, every layer's K and V,
-// to position start_pos[s] + k. blockIdx.y is (layer, K or V); a thread moves
-// one piece of E elements.
+// to position start_pos[s] + k, as far as the step has tokens for the sequence
+// (step_loc): its blocks hold no more, and without a token its start_pos names no
+// position. blockIdx.y is (layer, K or V); a thread moves one piece of E elements.
 // ---------------------------------------------------------------------------
 struct CommitArgs {
   char* k_pool;
@@ -326,6 +327,7 @@ struct CommitArgs {
   const int32_t* table;
   int max_blk;
   const int32_t* start_pos;
+  const int32_t* step_loc;  // nullable: no bound but lens
   const int32_t* qsl;
   const int32_t* path;
   const int32_t* lens;
@@ -362,7 +364,9 @@ __global__ __launch_bounds__(kStepThreads) void commit_kernel(CommitArgs a) {
     const int64_t pc = i - e * ppr;
     const int s = (int)(e / a.max_depth);
     const int k = (int)(e - (int64_t)s * a.max_depth);
-    if (k >= a.lens[s]) continue;
+    const int len = a.lens[s];  // with the step's bounds one round trip
+    const int most = a.step_loc ? a.step_loc[s + 1] - a.step_loc[s] : len;
+    if (k >= min(len, most)) continue;
     const bool flag = a.status && pc == 0 && first_plane;
     const int qb = a.qsl[s];
     const int n = a.qsl[s + 1] - qb;
@@ -517,13 +521,14 @@ int pkv_tree_accept(int32_t* lens, int32_t* path, int64_t* out_tokens, const int
   return check_launch("tree_accept");
 }
 
-int pkv_write_accepted(void* k_pool, void* v_pool, int64_t pool_layer_elems, int layers,
-                       int64_t num_blocks, int block_size, const void* k_rows,
-                       const void* v_rows, int64_t rows_layer_elems,
-                       const int32_t* block_tables, int max_blk, const int32_t* start_pos,
-                       const int32_t* query_start_loc, const int32_t* path,
-                       const int32_t* lens, int n_seq, int n_tokens, int max_depth,
-                       int64_t row_elems, int dtype, int* status, void* stream) {
+int pkv_write_accepted_step(void* k_pool, void* v_pool, int64_t pool_layer_elems, int layers,
+                            int64_t num_blocks, int block_size, const void* k_rows,
+                            const void* v_rows, int64_t rows_layer_elems,
+                            const int32_t* block_tables, int max_blk, const int32_t* start_pos,
+                            const int32_t* step_start_loc, const int32_t* query_start_loc,
+                            const int32_t* path, const int32_t* lens, int n_seq, int n_tokens,
+                            int max_depth, int64_t row_elems, int dtype, int* status,
+                            void* stream) {
   fail(PKV_OK, "%s", "");
   const bool kv8 = dtype_kv8(dtype);
   const int base = dtype_base(dtype);
@@ -553,6 +558,7 @@ int pkv_write_accepted(void* k_pool, void* v_pool, int64_t pool_layer_elems, int
   a.table = block_tables;
   a.max_blk = max_blk;
   a.start_pos = start_pos;
+  a.step_loc = step_start_loc;
   a.qsl = query_start_loc;
   a.path = path;
   a.lens = lens;
@@ -585,6 +591,19 @@ int pkv_write_accepted(void* k_pool, void* v_pool, int64_t pool_layer_elems, int
       wide ? launch_commit<f16, false, 8>(a, st) : launch_commit<f16, false, 1>(a, st);
   }
   return check_launch("write_accepted");
+}
+
+int pkv_write_accepted(void* k_pool, void* v_pool, int64_t pool_layer_elems, int layers,
+                       int64_t num_blocks, int block_size, const void* k_rows,
+                       const void* v_rows, int64_t rows_layer_elems,
+                       const int32_t* block_tables, int max_blk, const int32_t* start_pos,
+                       const int32_t* query_start_loc, const int32_t* path,
+                       const int32_t* lens, int n_seq, int n_tokens, int max_depth,
+                       int64_t row_elems, int dtype, int* status, void* stream) {
+  return pkv_write_accepted_step(k_pool, v_pool, pool_layer_elems, layers, num_blocks, block_size,
+                                 k_rows, v_rows, rows_layer_elems, block_tables, max_blk,
+                                 start_pos, nullptr, query_start_loc, path, lens, n_seq, n_tokens,
+                                 max_depth, row_elems, dtype, status, stream);
 }
 
 }  // extern "C"

@@ -138,6 +138,9 @@ _SIGNATURES = {
     "pkv_write_accepted": ([_c_vp, _c_vp, _c_i64, _c_int, _c_i64, _c_int, _c_vp, _c_vp, _c_i64,
                             _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int,
                             _c_i64, _c_int, _c_vp, _c_vp], _c_int),
+    "pkv_write_accepted_step": ([_c_vp, _c_vp, _c_i64, _c_int, _c_i64, _c_int, _c_vp, _c_vp,
+                                 _c_i64, _c_vp, _c_int] + [_c_vp] * 5 + [_c_int, _c_int, _c_int,
+                                 _c_i64, _c_int, _c_vp, _c_vp], _c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)

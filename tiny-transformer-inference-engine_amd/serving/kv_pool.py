@@ -196,11 +196,12 @@ class KVPool:
                        meta) -> None:
         """Every layer's K/V rows of the nodes a verification accepted, in one
         launch: row accepted.path[s, k] of sequence s's tree goes to position
-        meta.start_pos[s] + k, k < accepted.lens[s]. k_rows, v_rows [num_layers, T,
-        Hkv, D] as the tree's attention used them (serving.tree_decode); tree a
-        TreeMeta, accepted a TreeAccept, meta the accepted tokens' PagedBatchMeta
-        (build_batch_meta with q_lens = accepted.lens). The same bytes as write()
-        of those rows layer by layer."""
+        meta.start_pos[s] + k, k < accepted.lens[s] and below the tokens that meta has
+        for the sequence. k_rows, v_rows [num_layers, T, Hkv, D] as the tree's
+        attention used them (serving.tree_decode); tree a TreeMeta, accepted a
+        TreeAccept, meta the accepted tokens' PagedBatchMeta (build_batch_meta with
+        q_lens = accepted.lens, or less where a sequence is to take fewer). The same
+        bytes as write() of those rows layer by layer."""
         what = "KVPool.write_accepted"
         _native.require_device(self.kv, k_rows, v_rows, accepted.path, what=what)
         shape = (self.num_layers, tree.num_tokens, self.num_kv_heads, self.head_dim)
@@ -213,15 +214,16 @@ class KVPool:
         if meta.block_size != self.block_size:
             raise ValueError(f"{what}: blocks of {meta.block_size}, the pool's have {self.block_size}")
         path, lens, qsl = accepted.path, accepted.lens, tree.query_start_loc
-        table, start = meta.block_tables, meta.start_pos
+        table, start, step = meta.block_tables, meta.start_pos, meta.query_start_loc
         dev = self.device
         if not (k_rows.device == v_rows.device == path.device == lens.device == qsl.device
-                == table.device == start.device == dev):
+                == table.device == start.device == step.device == dev):
             raise RuntimeError(f"{what}: rows and metadata must be on {dev}")
-        for t in (path, lens, qsl, table, start):
+        for t in (path, lens, qsl, table, start, step):
             if t.dtype != torch.int32 or not t.is_contiguous():
                 raise ValueError(f"{what}: paths, lengths and metadata must be contiguous int32")
-        if table.shape[0] != n or start.numel() != n or qsl.numel() != n + 1:
+        if (table.shape[0] != n or start.numel() != n or qsl.numel() != n + 1
+                or step.numel() != n + 1):
             raise ValueError(f"{what}: the metadata's tensors are not those of {n} sequences")
         k = k_rows if k_rows.is_contiguous() else k_rows.contiguous()
         v = v_rows if v_rows.is_contiguous() else v_rows.contiguous()
@@ -229,16 +231,17 @@ class KVPool:
         status = self._status()
         previous = _native.make_current(dev)
         try:
-            rc = _native.calls().pkv_write_accepted(
+            rc = _native.calls().pkv_write_accepted_step(
                 self.flat_k[0].data_ptr(), self.flat_v[0].data_ptr(), 2 * self.num_slots * row,
                 self.num_layers, self.num_blocks, self.block_size, k.data_ptr(), v.data_ptr(),
                 tree.num_tokens * row, table.data_ptr(), table.shape[1], start.data_ptr(),
-                qsl.data_ptr(), path.data_ptr(), lens.data_ptr(), n, tree.num_tokens, depth, row,
+                step.data_ptr(), qsl.data_ptr(), path.data_ptr(), lens.data_ptr(), n,
+                tree.num_tokens, depth, row,
                 _native.kv_code(k.dtype, self.dtype), _native.ptr(status),
                 _native.stream_ptr(dev))
         finally:
             _native.restore(previous)
-        _native.check(rc, "pkv_write_accepted")
+        _native.check(rc, "pkv_write_accepted_step")
         self._raise_status(status, what)
 
     # ------------------------------------------------------------------
