@@ -365,3 +365,29 @@ def test_write_accepted_writes_the_steps_tokens_only(kv, packed):
         for flat, rows in ((want.flat_k[layer], k), (want.flat_v[layer], v)):
             bits(flat)[slots] = bits(rows[layer, [4, 5, 8, 9, 10, 11]].to(kv))
     assert torch.equal(bits(pool.kv), bits(want.kv))
+
+
+# ---- metadata that is not what the kernels read
+
+def tree_call(kv=F32, layers=1):
+    from serving.tree_decode import build_tree_meta
+    b = Batch([20, 5], [0, 0])
+    tree = build_tree_meta(b.tables(), i32([-1, 0, -1]), i32([0, 2, 3]), 2)
+    return b, tree, torch.ones(3, 8, 64, device=DEV), torch.ones(3, 1, 64, device=DEV), \
+        b.pool(1, 64, kv, layers)
+
+
+@pytest.mark.parametrize("name", ["block_tables", "ctx_lens", "query_start_loc"])
+def test_tree_attention_refuses_other_tensors(name):
+    """Tables and lengths of another type or device, or with gaps, before anything is
+    launched."""
+    from dataclasses import replace
+    from serving.tree_decode import paged_tree_attention
+    b, tree, q, k, pool = tree_call()
+    good = getattr(tree, name)
+    gaps = torch.stack([good, good], -1)[..., 0]
+    assert not gaps.is_contiguous()
+    for bad in (good.long(), good.float(), good.cpu(), gaps):
+        with pytest.raises((ValueError, RuntimeError), match=f"{name}|device"):
+            paged_tree_attention(q, k, k, *pool.kv[0], replace(tree, **{name: bad}))
+    paged_tree_attention(q, k, k, *pool.kv[0], tree)

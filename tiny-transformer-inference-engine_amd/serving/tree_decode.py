@@ -160,6 +160,9 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ctx, qsl = meta.ctx_lens, meta.query_start_loc
     if ctx.numel() != n or qsl.numel() != n + 1:
         raise ValueError(f"{what}: the metadata's tensors are not those of {n} sequences")
+    for t, name in ((table, "block_tables"), (ctx, "ctx_lens"), (qsl, "query_start_loc")):
+        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous int32 on {dev}")
     max_nodes, max_ctx = meta.max_nodes, meta.max_ctx_len
     calls = _native.calls()
     previous = _native.make_current(dev)
