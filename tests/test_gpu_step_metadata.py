@@ -391,3 +391,14 @@ def test_tree_attention_refuses_other_tensors(name):
         with pytest.raises((ValueError, RuntimeError), match=f"{name}|device"):
             paged_tree_attention(q, k, k, *pool.kv[0], replace(tree, **{name: bad}))
     paged_tree_attention(q, k, k, *pool.kv[0], tree)
+
+
+def test_tree_attention_refuses_a_smaller_pool():
+    """Tables that may name blocks which the pool does not have."""
+    from serving.tree_decode import paged_tree_attention
+    b, tree, q, k, pool = tree_call()
+    with pytest.raises(ValueError, match="blocks"):
+        paged_tree_attention(q, k, k, *pool.kv[0, :, :b.nb - 1], tree)
+    big = torch.cat([pool.kv[0], pool.kv[0]], 1)
+    assert torch.equal(paged_tree_attention(q, k, k, *big, tree),
+                       paged_tree_attention(q, k, k, *pool.kv[0], tree))

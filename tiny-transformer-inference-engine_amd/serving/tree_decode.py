@@ -47,7 +47,7 @@ class TreeMeta:
     max_nodes: int
     max_ctx_len: int
     block_size: int
-    num_blocks: int
+    num_blocks: int                # that the tables may name: the pools have as many, or more
 
 
 @dataclass
@@ -142,9 +142,9 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if pd != d or k.shape != (T, hkv, d) or v.shape != k.shape:
         raise ValueError(f"{what}: k and v must be [{T}, {hkv}, {d}] (got {tuple(k.shape)}, "
                          f"{tuple(v.shape)}), the pools' head dim {d} (got {pd})")
-    if T != meta.num_tokens or bs != meta.block_size:
-        raise ValueError(f"{what}: {T} rows and blocks of {bs}, the metadata has "
-                         f"{meta.num_tokens} and {meta.block_size}")
+    if T != meta.num_tokens or bs != meta.block_size or nb < meta.num_blocks:
+        raise ValueError(f"{what}: {T} rows and {nb} blocks of {bs}, the metadata has "
+                         f"{meta.num_tokens} and {meta.num_blocks} of {meta.block_size}")
     dtype = q.dtype
     if k.dtype != dtype or v.dtype != dtype or v_pool.dtype != k_pool.dtype:
         raise TypeError(f"{what}: q, k and v must share a dtype, and so must the pools")
