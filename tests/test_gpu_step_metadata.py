@@ -402,3 +402,13 @@ def test_tree_attention_refuses_a_smaller_pool():
     big = torch.cat([pool.kv[0], pool.kv[0]], 1)
     assert torch.equal(paged_tree_attention(q, k, k, *big, tree),
                        paged_tree_attention(q, k, k, *pool.kv[0], tree))
+
+
+def test_tree_context_bounds_of_any_size():
+    """A bound past what an int holds bounds nothing."""
+    from serving.tree_decode import build_tree_meta, paged_tree_attention
+    b, tree, q, k, pool = tree_call()
+    want = paged_tree_attention(q, k, k, *pool.kv[0], tree)
+    for bound in (1 << 31, 1 << 40, 1 << 70):
+        big = build_tree_meta(b.tables(), i32([-1, 0, -1]), i32([0, 2, 3]), 2, bound)
+        assert torch.equal(paged_tree_attention(q, k, k, *pool.kv[0], big), want)

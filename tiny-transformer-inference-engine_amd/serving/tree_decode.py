@@ -99,8 +99,9 @@ def build_tree_meta(tables: DeviceTables, parents: torch.Tensor, query_start_loc
     if rc:
         _native.check(rc, what)
     bs = tables.block_size
+    cap = max_blocks * bs  # contexts past the table do not exist
     return TreeMeta(bt, tables.ctx_lens, qsl, parents, masks, positions, n, T, max_nodes,
-                    int(max_ctx_len) if max_ctx_len > 0 else max_blocks * bs, bs,
+                    min(int(max_ctx_len), cap) if max_ctx_len > 0 else cap, bs,
                     tables.num_blocks)
 
 
