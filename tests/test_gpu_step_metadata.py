@@ -412,3 +412,55 @@ def test_tree_context_bounds_of_any_size():
     for bound in (1 << 31, 1 << 40, 1 << 70):
         big = build_tree_meta(b.tables(), i32([-1, 0, -1]), i32([0, 2, 3]), 2, bound)
         assert torch.equal(paged_tree_attention(q, k, k, *pool.kv[0], big), want)
+
+
+# ---- what a step's status tells
+
+def test_forward_tree_reports_bad_blocks_and_runs():
+    from serving import _native
+    from serving.tree_decode import build_tree_meta
+    cfg, model = small_model()
+    b = Batch([20, 5], [0, 0])
+    pool = b.pool(1, cfg.head_dim, F32, cfg.num_layers)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ids = torch.arange(3, device=DEV)
+    parents = i32([-1, 0, -1])
+
+    def run(dt, qsl, bound=2):
+        st.zero_()
+        tree = build_tree_meta(dt, parents, qsl, bound)  # reports to nobody
+        model.forward_tree(ids, pool, tree, status=st)
+        return int(st)
+
+    dt = b.tables()
+    assert run(dt, i32([0, 2, 3])) == 0
+    assert run(dt, i32([0, 2, 3]), 1) == _native.PKV_STATUS_BAD_QLOC
+    dt.block_tables[0, 1] = b.nb
+    assert run(dt, i32([0, 2, 3])) == _native.PKV_STATUS_BAD_BLOCK
+
+
+def test_generate_speculative_reports_bad_blocks():
+    """A block id past the pool that only the model's pass meets: the prompt's."""
+    from serving.allocator import BlockAllocator
+    from serving.generation import generate_speculative
+    cfg, model = small_model()
+    alloc = BlockAllocator(40)
+    pool = KVPool(cfg.num_layers, 16, 8, 1, cfg.head_dim, F32, DEV)
+    low = alloc.allocate_n(7)
+    high = alloc.allocate_n(1)  # block 8: the pool has 0 ... 7
+    assert high == [8] and low == list(range(1, 8))
+
+    class Ids:  # hands out the bad block first
+        ids = high + low
+
+        def allocate(self):
+            return self.ids.pop(0)
+
+        def allocate_n(self, n):
+            return [self.allocate() for _ in range(n)]
+
+        def free(self, blocks):
+            pass
+
+    with pytest.raises(AssertionError, match="block id"):
+        generate_speculative(model, [[1, 2, 3]], 5, pool, Ids(), lambda h: ([], []))

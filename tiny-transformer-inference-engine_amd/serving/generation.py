@@ -192,7 +192,7 @@ def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft,
                 ids = torch.tensor(tokens, dtype=torch.long, device=device)
                 tree = build_tree_meta(tables, i32[:len(parents)], i32[len(parents):],
                                        1 + max_drafts, max(len(r) for r in rows), status=status)
-                logits, k_rows, v_rows = model.forward_tree(ids, pool, tree)
+                logits, k_rows, v_rows = model.forward_tree(ids, pool, tree, status)
                 accepted = tree_accept(greedy(logits)[:, 0], ids, tree, max_depth, status=status)
                 meta, tables = build_batch_meta(tables, accepted.lens, len(rows) * max_depth,
                                                 max_depth, status=status)

@@ -106,12 +106,13 @@ class PagedTransformer(nn.Module):
             (qsl[1:] == qsl[:-1])[:, None], 0)
 
     @torch.no_grad()
-    def forward_tree(self, input_ids, pool, tree):
+    def forward_tree(self, input_ids, pool, tree, status=None):
         """The nodes of drafted trees in one pass on a ROCm device: input_ids [T]
         their tokens, tree a TreeMeta (serving.tree_decode). Returns the logits of
         every node [T, vocab] and the nodes' K and V rows of all layers, each
         [num_layers, T, Hkv, D] in the model's dtype, for KVPool.write_accepted;
-        the pool is read only."""
+        the pool is read only. `status` as in build_batch_meta: table entries outside
+        the pool, which read as zeros, and runs that were skipped."""
         x = self.embedding(input_ids).contiguous()
         if not x.is_cuda:
             raise RuntimeError("forward_tree requires the model on a ROCm GPU device")
@@ -121,7 +122,7 @@ class PagedTransformer(nn.Module):
         for i, layer in enumerate(self.layers):
             attr(layer, "attn").forward_tree_residual_(x, attr(layer, "attn_norm"), pool,
                                                        layer.layer_idx, tree, k_rows[i],
-                                                       v_rows[i])
+                                                       v_rows[i], status)
             attr(layer, "mlp").forward_residual_(x, attr(layer, "mlp_norm"))
         return self.lm_head(self.final_norm(x)), k_rows, v_rows
 

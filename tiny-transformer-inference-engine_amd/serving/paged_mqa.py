@@ -120,11 +120,13 @@ class MQA_Paged(nn.Module):
         return fused_ops.linear_residual_(x, out.view(T, d_model), attr(proj, "weight"),
                                           attr(proj, "bias"))
 
-    def forward_tree_residual_(self, x, norm, pool, layer_idx, tree, k_rows, v_rows):
+    def forward_tree_residual_(self, x, norm, pool, layer_idx, tree, k_rows, v_rows,
+                               status=None):
         """forward_meta_residual_ for the nodes of drafted trees (a TreeMeta,
         serving.tree_decode): RoPE at the nodes' positions, each node attending to
         its context in the pool, its ancestors and itself. The nodes' K/V rows are
-        written to k_rows, v_rows [T, Hkv, D] and not to the pool. Returns x."""
+        written to k_rows, v_rows [T, Hkv, D] and not to the pool; `status` as
+        paged_tree_attention's. Returns x."""
         T, d_model = x.shape
         w, b = self._qkv.get()
         attr = fused_ops.module_attr
@@ -133,7 +135,7 @@ class MQA_Paged(nn.Module):
             x, attr(norm, "weight"), norm.eps, w, b, tree.positions, cos, sin, self.num_heads,
             self.num_kv_heads, self.headdim, kv_out=(k_rows, v_rows))
         kp, vp = _get_kv_pool(pool, layer_idx)
-        out = paged_tree_attention(q, k, v, kp, vp, tree)
+        out = paged_tree_attention(q, k, v, kp, vp, tree, status=status)
         proj = attr(self, "out")
         return fused_ops.linear_residual_(x, out.view(T, d_model), attr(proj, "weight"),
                                           attr(proj, "bias"))

@@ -123,7 +123,8 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     type or float8_e4m3fn (the tree's rows then count as rounded to it). `out` /
     `lse` (float32 [T, Hq]): where to write, memory of no other operand; rows of no
     sequence are left as they were there. A row that sees no key gives 0 and lse +inf. part_tokens (0:
-    automatic) forces the length of the pieces a context is split into."""
+    automatic) forces the length of the pieces a context is split into. `status` as in
+    build_batch_meta."""
     what = "paged_tree_attention"
     masks, table = meta.masks, meta.block_tables
     dev = q.device
