@@ -464,3 +464,32 @@ def test_generate_speculative_reports_bad_blocks():
 
     with pytest.raises(AssertionError, match="block id"):
         generate_speculative(model, [[1, 2, 3]], 5, pool, Ids(), lambda h: ([], []))
+
+
+# ---- a pool of more layers than the model
+
+def test_generate_speculative_in_a_larger_pool():
+    from serving.allocator import BlockAllocator
+    from serving.generation import generate_batched, generate_speculative
+    cfg, model = small_model()
+    prompts = [[5, 6, 7], [9] * 20]
+    pool, alloc = KVPool(cfg.num_layers + 2, 16, 20, 1, cfg.head_dim, F32, DEV), BlockAllocator(20)
+    pool.kv[cfg.num_layers:].fill_(3.0)
+    truth = generate_batched(model, prompts, 20, pool, alloc)
+    draft = lambda h: ([(h[-1] + 1) % 97, h[0]], [-1, 0])  # noqa: E731
+    assert generate_speculative(model, prompts, 20, pool, alloc, draft) == truth
+    assert (pool.kv[cfg.num_layers:] == 3.0).all()
+
+
+def test_write_accepted_refuses_more_layers_than_the_pool_has():
+    from serving.tree_decode import tree_accept
+    b, tree, _, _, pool = tree_call(layers=2)
+    ids = torch.zeros(3, dtype=torch.long, device=DEV)
+    acc = tree_accept(ids, ids, tree, 2)
+    meta, _ = build_batch_meta(b.tables(), torch.zeros_like(acc.lens), 4, 2)
+    for layers in (1, 2):
+        rows = torch.ones(layers, 3, 1, 64, device=DEV)
+        pool.write_accepted(rows, rows, tree, acc, meta)
+    rows = torch.ones(3, 3, 1, 64, device=DEV)
+    with pytest.raises(AssertionError):
+        pool.write_accepted(rows, rows, tree, acc, meta)

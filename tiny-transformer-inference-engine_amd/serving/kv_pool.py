@@ -197,16 +197,20 @@ class KVPool:
         """Every layer's K/V rows of the nodes a verification accepted, in one
         launch: row accepted.path[s, k] of sequence s's tree goes to position
         meta.start_pos[s] + k, k < accepted.lens[s] and below the tokens that meta has
-        for the sequence. k_rows, v_rows [num_layers, T, Hkv, D] as the tree's
-        attention used them (serving.tree_decode); tree a TreeMeta, accepted a
+        for the sequence. k_rows, v_rows [layers, T, Hkv, D] as the tree's attention
+        used them (serving.tree_decode), for the pool's first layers, all of them or
+        the model's fewer; tree a TreeMeta, accepted a
         TreeAccept, meta the accepted tokens' PagedBatchMeta (build_batch_meta with
         q_lens = accepted.lens, or less where a sequence is to take fewer). The same
         bytes as write() of those rows layer by layer."""
         what = "KVPool.write_accepted"
         _native.require_device(self.kv, k_rows, v_rows, accepted.path, what=what)
-        shape = (self.num_layers, tree.num_tokens, self.num_kv_heads, self.head_dim)
+        layers = k_rows.shape[0]
+        shape = (layers, tree.num_tokens, self.num_kv_heads, self.head_dim)
         assert k_rows.shape == shape and v_rows.shape == shape, \
             f"k/v rows {tuple(k_rows.shape)}/{tuple(v_rows.shape)} != expected {shape}"
+        assert layers <= self.num_layers, \
+            f"rows of {layers} layers, the pool has {self.num_layers}"
         self._check_row_dtype(k_rows, v_rows)
         n, depth = accepted.path.shape
         if not (n == tree.num_seqs == meta.num_seqs == accepted.lens.numel()):
@@ -233,7 +237,7 @@ class KVPool:
         try:
             rc = _native.calls().pkv_write_accepted_step(
                 self.flat_k[0].data_ptr(), self.flat_v[0].data_ptr(), 2 * self.num_slots * row,
-                self.num_layers, self.num_blocks, self.block_size, k.data_ptr(), v.data_ptr(),
+                layers, self.num_blocks, self.block_size, k.data_ptr(), v.data_ptr(),
                 tree.num_tokens * row, table.data_ptr(), table.shape[1], start.data_ptr(),
                 step.data_ptr(), qsl.data_ptr(), path.data_ptr(), lens.data_ptr(), n,
                 tree.num_tokens, depth, row,
