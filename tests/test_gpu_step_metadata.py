@@ -1,7 +1,8 @@
 """Metadata that build_batch_meta makes on the device, handed on to what takes a
 step's metadata: appends, attention, the model's step, the accepted rows' way into
 the pool. num_tokens and max_q_len are bounds there, sequences may have no token, and
-a step may fail or be dropped and taken again. Copied rows are compared byte by byte;
+a step may fail or be dropped and taken again; and what the tree attention does with
+metadata and tree rows that are not as they should be. Copied rows are compared byte by byte;
 a token of one batch runs through the same kernels with the same partitions as the
 host-packed batch it is compared with, except where a tolerance says otherwise."""
 import numpy as np
@@ -493,3 +494,73 @@ def test_write_accepted_refuses_more_layers_than_the_pool_has():
     rows = torch.ones(3, 3, 1, 64, device=DEV)
     with pytest.raises(AssertionError):
         pool.write_accepted(rows, rows, tree, acc, meta)
+
+
+# ---- values that are not finite, in the trees' rows
+
+@pytest.mark.parametrize("dtype,kv,d,hkv", [(F32, F32, 64, 1), (BF, BF, 64, 2), (BF, BF, 128, 1),
+                                            (BF, F8, 64, 1), (torch.float16, torch.float16, 64, 2),
+                                            (BF, BF, 256, 1), (F32, F32, 8, 1)])
+@pytest.mark.parametrize("part", [0, 64])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), 470.0])
+def test_values_that_are_not_finite_reach_all_that_see_them(dtype, kv, d, hkv, part, bad):
+    """A tree value of NaN or infinity (with an fp8 pool also one past 464, which rounds to
+    NaN) makes that column of every row and head that sees its node not finite, and
+    changes nothing else; a key of NaN makes whole rows NaN. Contexts of several
+    partitions, and none."""
+    from serving.tree_decode import build_tree_meta, paged_tree_attention
+    print(f"[odd] {dtype} {kv} d={d} hkv={hkv} part={part} {bad}", flush=True)
+    if bad == 470.0 and kv != F8:  # finite in the operand's type
+        bad = -float("inf")
+    hq = 8
+    b = Batch([300, 0, 7], [0, 0, 0])
+    parents = [[-1, 0, 0, 1, 2, 2, 3, 4, 1], [-1, 0, 1, 1], [-1] + [0] * 69]
+    nodes = [len(p) for p in parents]
+    qsl = np.concatenate([[0], np.cumsum(nodes)])
+    T = int(qsl[-1])
+    g = torch.Generator().manual_seed(7)
+    q, k, v = (torch.randn(T, h, d, generator=g).to(dtype).to(DEV) for h in (hq, hkv, hkv))
+    pool = b.pool(hkv, d, kv)
+    tree = build_tree_meta(b.tables(), i32(np.concatenate(parents)), i32(qsl), max(nodes), 300)
+    vis = [tree_ref.visible_from_parents(p)[0] for p in parents]
+    run = lambda: paged_tree_attention(q, k, v, *pool.kv[0], tree, part_tokens=part)  # noqa: E731
+    clean = run().float().cpu()
+    assert torch.isfinite(clean).all()
+    sees = np.zeros((T, 3), dtype=bool)  # the node with the bad value, of each sequence
+    for s, node in enumerate((2, 1, 33)):
+        sees[qsl[s]:qsl[s + 1], s] = vis[s][:, node]
+        v[int(qsl[s]) + node, 0, 5] = bad
+    got = run().float().cpu()
+    hit = torch.from_numpy(sees.any(1))
+    heads = torch.arange(hq) < hq // hkv  # those of kv head 0
+    want = torch.zeros(T, hq, d, dtype=torch.bool)
+    want[:, :, 5] = hit[:, None] & heads
+    assert torch.equal(~torch.isfinite(got), want)
+    assert torch.equal(got[~want], clean[~want])
+    if kv != F8 and abs(bad) == float("inf"):
+        assert (got[want] == bad).all()
+    for s, node in enumerate((2, 1, 33)):  # and a key
+        k[int(qsl[s]) + node, 0, 3] = float("nan")
+    got = run().float().cpu()
+    rows = hit[:, None] & heads
+    assert torch.isnan(got[rows]).all() and torch.isfinite(got[~rows]).all()
+    # A row's weights are 2^(s - m), and m moves for the 32 rows of a wavefront together,
+    # at the largest of their new scores that passes it by the lazy step: a row of NaN never
+    # does, so the others may keep an earlier m, and each of their roundings falls
+    # elsewhere. Two results whose every weight (16-bit operands: u, fp16 steps of 2^-24)
+    # and sum are rounded anew differ by twice what one may be off by (the bounds are those
+    # of test_gpu_tree_attention.py): 2 (u A + 2 (d + 8) e S A + 2 (L + 16) e A +
+    # 2^-25 V1 + u |out|), A the weighted mean of |v|, S at most the scale times the
+    # largest norms of q and k, L at most 370 keys.
+    e, u = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    k, v = torch.nan_to_num(k, nan=0.0), v.nan_to_num(0.0, 0.0, 0.0).abs()
+    v[v > 464] = 0
+    pool.flat_v[0].copy_(pool.flat_v[0].float().abs().to(kv))
+    A = run().float().cpu()[~rows] * (1 + 2 * u + 1e-3)
+    S = d ** -0.5 * float(q.float().norm(dim=-1).max()) * max(
+        float(x.float().norm(dim=-1).max()) for x in (k, pool.flat_k[0]))
+    V1 = 370 * max(float(x.float().max()) for x in (v, pool.flat_v[0]))
+    tol = (2 * (d + 8) * e * S + 2 * (370 + 16) * e) * A + u * clean[~rows].abs() * (1 + 2.0 ** -6)
+    if dtype != F32:
+        tol += u * A + (2.0 ** -25 * V1 if dtype == torch.float16 else 0)
+    assert ((got - clean)[~rows].abs() <= 2 * tol).all()
