@@ -564,3 +564,25 @@ def test_values_that_are_not_finite_reach_all_that_see_them(dtype, kv, d, hkv, p
     if dtype != F32:
         tol += u * A + (2.0 ** -25 * V1 if dtype == torch.float16 else 0)
     assert ((got - clean)[~rows].abs() <= 2 * tol).all()
+
+
+# ---- the ends of a step's sizes
+
+def test_a_step_without_nodes():
+    """Every sequence finished: nothing to verify, nothing changes."""
+    from serving.tree_decode import build_tree_meta, tree_accept
+    cfg, model = small_model()
+    b = Batch([20, 5], [0, 0])
+    pool = b.pool(1, cfg.head_dim, F32, cfg.num_layers)
+    before, dt = pool.kv.clone(), b.tables()
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ids = torch.zeros(0, dtype=torch.long, device=DEV)
+    tree = build_tree_meta(dt, i32([]), i32([0, 0, 0]), 4, status=st)
+    logits, k, v = model.forward_tree(ids, pool, tree, st)
+    assert logits.shape == (0, 97) and k.shape == v.shape == (cfg.num_layers, 0, 1, cfg.head_dim)
+    acc = tree_accept(ids, ids, tree, 3, status=st)
+    assert acc.lens.tolist() == [0, 0] and (acc.path == -1).all()
+    meta, after = build_batch_meta(dt, acc.lens, 0, 3, status=st)
+    pool.write_accepted(k, v, tree, acc, meta)
+    assert int(st) == 0 and torch.equal(pool.kv, before)
+    assert after.ctx_lens.tolist() == [20, 5] and after.free_cursor.tolist() == [0]

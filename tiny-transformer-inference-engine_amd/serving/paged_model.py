@@ -118,6 +118,8 @@ class PagedTransformer(nn.Module):
             raise RuntimeError("forward_tree requires the model on a ROCm GPU device")
         shape = (len(self.layers), x.shape[0], pool.num_kv_heads, pool.head_dim)
         k_rows, v_rows = x.new_empty(shape), x.new_empty(shape)
+        if x.shape[0] == 0:  # every sequence finished
+            return x.new_empty((0, self.lm_head.out_features)), k_rows, v_rows
         attr = fused_ops.module_attr
         for i, layer in enumerate(self.layers):
             attr(layer, "attn").forward_tree_residual_(x, attr(layer, "attn_norm"), pool,
