@@ -130,17 +130,19 @@ def test_padded_steps_append_and_attend(ctx, q, dtype, kv, hq, hkv, d):
     T, pad = sum(q), 4
     g = torch.Generator().manual_seed(4)
     rows = [torch.randn(T + pad, h, d, generator=g).to(dtype).to(DEV) for h in (hq, hkv, hkv)]
-    got, want = b.pool(hkv, d, kv), b.pool(hkv, d, kv)
-    out = torch.full_like(rows[0], 9.0)
-    paged_attention_append_meta(*rows, got, 0, b.meta(pad), out=out)
+    want = b.pool(hkv, d, kv)
     ref = paged_attention_append_meta(*[x[:T].contiguous() for x in rows], want, 0, b.host_meta())
-    assert torch.equal(bits(got.kv), bits(want.kv))
     # other partitions of the contexts: sums of at most 5001 weights in another order, and
     # 16-bit probabilities against another maximum; values of at most 6
     u = torch.finfo(dtype).eps / 2
     tol = 6 * (2 * 5001 * 2.0 ** -24 + (2 * u if dtype != F32 else 0)) + 2 * u
-    assert float((out[:T].float() - ref.float()).abs().max()) <= tol
-    assert (out[T:] == 9).all()
+    for bound in (max(q), 9 + max(q)):  # looser, the prompt kernels' too
+        got = b.pool(hkv, d, kv)
+        out = torch.full_like(rows[0], 9.0)
+        paged_attention_append_meta(*rows, got, 0, b.meta(pad, bound), out=out)
+        assert torch.equal(bits(got.kv), bits(want.kv))
+        assert float((out[:T].float() - ref.float()).abs().max()) <= tol
+        assert (out[T:] == 9).all()
 
 
 # ---- sequences without a token in the model's step
@@ -586,3 +588,19 @@ def test_a_step_without_nodes():
     pool.write_accepted(k, v, tree, acc, meta)
     assert int(st) == 0 and torch.equal(pool.kv, before)
     assert after.ctx_lens.tolist() == [20, 5] and after.free_cursor.tolist() == [0]
+
+
+def test_generate_speculative_without_a_limit_on_depth():
+    """max_depth past what a step could keep costs nothing."""
+    from serving.allocator import BlockAllocator
+    from serving.generation import generate_batched, generate_speculative
+    cfg, model = small_model()
+    pool, alloc = KVPool(cfg.num_layers, 16, 20, 1, cfg.head_dim, F32, DEV), BlockAllocator(20)
+    prompts = [[5, 6, 7], [9] * 20]
+    truth = generate_batched(model, prompts, 12, pool, alloc)
+    right = lambda h: (next(p + t for p, t in zip(prompts, truth)  # noqa: E731
+                            if (p + t)[:len(h)] == h)[len(h):], list(range(-1, 11)))
+    draft = lambda h: (right(h)[0], right(h)[1][:len(right(h)[0])])  # noqa: E731
+    for depth in (8, 1 << 31, 1 << 62):
+        assert generate_speculative(model, prompts, 12, pool, alloc, draft, max_depth=depth) == truth
+    assert alloc.num_free == 19

@@ -163,6 +163,7 @@ def generate_speculative(model, prompts_ids, max_new_tokens, pool, alloc, draft,
         raise ValueError("every prompt must contain at least one token")
     if max_new_tokens == 0:
         return [[] for _ in prompts_ids]
+    max_depth = min(max_depth, 1 + max_drafts, max_new_tokens)  # no path is longer
     device = _model_device(model)
     vocab = model.lm_head.out_features
     stock = []
