@@ -604,3 +604,91 @@ def test_generate_speculative_without_a_limit_on_depth():
     for depth in (8, 1 << 31, 1 << 62):
         assert generate_speculative(model, prompts, 12, pool, alloc, draft, max_depth=depth) == truth
     assert alloc.num_free == 19
+
+
+# ---- captured
+
+def test_padded_step_in_a_graph():
+    """build_batch_meta and forward_step captured once and replayed over other lengths, a
+    sequence without a token, a step that fails and one that is taken after it: the
+    eager step's results, and nothing of the failed step in the pool."""
+    from serving import _native
+    cfg, model = small_model()
+    b = Batch([20, 3, 31], [9, 9, 9])
+    dt = b.tables()
+    pool, q = b.pool(1, cfg.head_dim, F32, cfg.num_layers), i32([2, 0, 1])
+    kv0, table0 = pool.kv.clone(), dt.block_tables.clone()
+    ids = torch.arange(12, device=DEV) * 7 % 97
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def step():
+        pool.kv.copy_(kv0)
+        dt.block_tables.copy_(table0)
+        st.zero_()
+        meta, after = build_batch_meta(dt, q, 12, 9, status=st)
+        logits = model.forward_step(ids, pool, meta)
+        return [logits, pool.kv, after.block_tables, after.blocks_held, after.ctx_lens,
+                after.free_cursor, meta.slot_mapping, st]
+
+    ws = _native.Workspace()
+    with _native.workspace_scope(ws):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured = step()
+    for lens, fails in (([2, 0, 1], 0), ([0, 9, 3], 0), ([9, 9, 0], 1), ([1, 1, 1], 0),
+                        ([0, 0, 0], 0), ([3, 10, 0], 1), ([4, 4, 4], 0)):
+        q.copy_(i32(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        want = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        for a, c in zip(got[1:], want[1:]):
+            assert torch.equal(a, c), lens
+        assert bool(int(got[-1])) == bool(fails), lens
+        if fails:
+            assert torch.equal(got[1], kv0) and torch.equal(got[2], table0)
+        else:
+            assert torch.equal(got[0], want[0]), lens
+            assert (got[0][[i for i, n in enumerate(lens) if n == 0]] == 0).all()
+
+
+def test_failed_tree_step_in_a_graph():
+    """The verification step captured, with too few blocks at some replays."""
+    from serving.tree_decode import TreeAccept, build_tree_meta
+    b = Batch([16, 10], [3, 3])
+    pool, dt = b.pool(2, 64, BF, 2), b.tables()
+    kv0, table0, cursor = pool.kv.clone(), dt.block_tables.clone(), dt.free_cursor
+    lens, rows = i32([2, 3]), torch.randn(2, 6, 2, 64, device=DEV).to(BF)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    parents, qsl, path = i32([-1, 0, 1] * 2), i32([0, 3, 6]), i32([0, 1, 2] * 2).view(2, 3)
+
+    def step():
+        pool.kv.copy_(kv0)
+        dt.block_tables.copy_(table0)
+        st.zero_()
+        tree = build_tree_meta(dt, parents, qsl, 3, status=st)
+        meta, after = build_batch_meta(dt, lens, 6, 3, status=st)
+        pool.write_accepted(rows, -rows, tree, TreeAccept(lens, path, None), meta)
+        return [pool.kv, after.block_tables, after.blocks_held, after.ctx_lens, st]
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for it, at in enumerate((0, len(b.free), 0, len(b.free) + 1, 0)):
+        cursor.fill_(at)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        want = [t.clone() for t in step()]
+        assert all(torch.equal(a, c) for a, c in zip(got, want)), it
+        assert bool(int(got[-1])) == (at > 0)
+        assert torch.equal(got[0], kv0) == (at > 0)
