@@ -32,6 +32,7 @@ from .paged_meta import DeviceTables, _status_ptr
 __all__ = ["TreeMeta", "TreeAccept", "build_tree_meta", "paged_tree_attention", "tree_accept"]
 
 MAX_TREE_NODES = 4096
+_I32 = torch.int32
 
 
 @dataclass
@@ -162,9 +163,11 @@ def paged_tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ctx, qsl = meta.ctx_lens, meta.query_start_loc
     if ctx.numel() != n or qsl.numel() != n + 1:
         raise ValueError(f"{what}: the metadata's tensors are not those of {n} sequences")
-    for t, name in ((table, "block_tables"), (ctx, "ctx_lens"), (qsl, "query_start_loc")):
-        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} must be contiguous int32 on {dev}")
+    if (table.dtype != _I32 or ctx.dtype != _I32 or qsl.dtype != _I32 or ctx.device != dev
+            or qsl.device != dev or not (table.is_contiguous() and ctx.is_contiguous()
+                                         and qsl.is_contiguous())):
+        raise ValueError(f"{what}: block_tables, ctx_lens and query_start_loc must be contiguous "
+                         f"int32 on {dev}")
     max_nodes, max_ctx = meta.max_nodes, meta.max_ctx_len
     calls = _native.calls()
     previous = _native.make_current(dev)
