@@ -585,8 +585,9 @@ size_t pkv_tree_attention_workspace_bytes(int n_seq, int max_nodes, int hq, int 
  * Values of keys that a row does not see do not reach it, infinities and NaN
  * included. Table entries outside [0, num_blocks) read as zeros
  * (PKV_STATUS_BAD_BLOCK); a run outside [0, n_tokens) or of more than max_nodes
- * nodes is skipped (PKV_STATUS_BAD_QLOC), and rows of no run are left as they
- * were. max_ctx_len (<= 0: the table's capacity) sizes the context's split, a
+ * nodes is skipped (PKV_STATUS_BAD_QLOC; max_nodes 0: nothing is launched or
+ * reported), and rows of no run are left as they were; the runs must not overlap.
+ * max_ctx_len (<= 0: the table's capacity) sizes the context's split, a
  * longer context is still computed whole; part_tokens forces the split's length
  * (0: automatic). bf16 / f16 / fp32 (fp8 pools: bf16 / f16), any hq a multiple
  * of hkv, d a multiple of 8 up to 256, at most 65536 trees of at most 4096 nodes, tensors
