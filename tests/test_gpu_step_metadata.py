@@ -692,3 +692,26 @@ def test_failed_tree_step_in_a_graph():
         assert all(torch.equal(a, c) for a, c in zip(got, want)), it
         assert bool(int(got[-1])) == (at > 0)
         assert torch.equal(got[0], kv0) == (at > 0)
+
+
+@pytest.mark.parametrize("dtype,kv,hq,hkv,d", [(F32, F32, 8, 1, 64), (BF, BF, 8, 1, 64),
+                                               (BF, BF, 16, 1, 64), (BF, BF, 32, 1, 128),
+                                               (BF, F8, 16, 1, 64), (F32, F32, 4, 4, 80)])
+@pytest.mark.parametrize("q", [[1, 1], [1, 9]])
+@pytest.mark.parametrize("width", [3, 300])
+def test_failed_decode_and_mixed_steps_write_nothing(dtype, kv, hq, hkv, d, q, width):
+    """Each form of the attention's own append (fused with decode partitions, the prompt
+    kernel or both in one launch, or a launch before the persistent kernel)."""
+    from serving.fake_paged_attn import paged_attention_append_meta
+    print(f"[failed] {dtype} {kv} {hq}x{hkv}x{d} q={q} width={width}", flush=True)
+    b = Batch([16, 10], q)
+    b.width = width
+    pool, want = b.pool(hkv, d, kv), b.pool(hkv, d, kv)
+    dt = b.tables()
+    dt.free_cursor.fill_(len(b.free))
+    meta, _ = build_batch_meta(dt, i32(q), sum(q), max(q))
+    g = torch.Generator().manual_seed(8)
+    rows = [torch.randn(sum(q), h, d, generator=g).to(dtype).to(DEV) for h in (hq, hkv, hkv)]
+    out = paged_attention_append_meta(*rows, pool, 0, meta)
+    assert torch.equal(bits(pool.kv), bits(want.kv))
+    assert (out == 0).all()  # it attends to nothing either
