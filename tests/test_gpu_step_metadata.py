@@ -715,3 +715,23 @@ def test_failed_decode_and_mixed_steps_write_nothing(dtype, kv, hq, hkv, d, q, w
     out = paged_attention_append_meta(*rows, pool, 0, meta)
     assert torch.equal(bits(pool.kv), bits(want.kv))
     assert (out == 0).all()  # it attends to nothing either
+
+
+def test_lengths_that_the_caller_knows():
+    """One token for every sequence, said to be so: a decode batch, captured and advanced
+    (within the blocks that the rows hold) as the host-packed one."""
+    from dataclasses import replace
+    from serving.graph_step import DecodeStepGraph
+    cfg, model = small_model()
+    b = Batch([20, 3, 34], [1, 1, 1])
+    ids = torch.tensor([3, 14, 15], device=DEV)
+    meta, host = replace(b.meta(), exact=True), b.host_meta()
+    assert meta.is_decode
+    pools = [b.pool(1, cfg.head_dim, F32, cfg.num_layers) for _ in range(2)]
+    graphs = [DecodeStepGraph(model, p, m, ids) for p, m in zip(pools, (meta, host))]
+    assert meta.slot_mapping.tolist() == [tree_ref.NO_SLOT] * 3
+    for it in range(4):
+        got, want = (g.replay().tolist() for g in graphs)
+        assert got == want, it
+    assert meta.seq_lens.tolist() == host.seq_lens.tolist()
+    assert float((pools[0].kv - pools[1].kv).abs().max()) <= 1e-4 * float(pools[1].kv.abs().max())

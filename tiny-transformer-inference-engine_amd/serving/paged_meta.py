@@ -52,9 +52,11 @@ class PagedBatchMeta:
     def advance_(self) -> None:
         """Every sequence one token further, on the device: seq_lens,
         start_pos and positions + 1 (one kernel when they share step_view).
-        With lengths from the device only sequences that have tokens, and their
-        rows; slot_mapping becomes NO_SLOT throughout, as the slots of later tokens
-        are another build_batch_meta's to give."""
+        Where the lengths are bounds (exact False) only sequences that have tokens,
+        and their rows. slot_mapping becomes NO_SLOT throughout, as the slots of later
+        tokens are another build_batch_meta's to give."""
+        if self.slot_mapping is not None:
+            self.slot_mapping.fill_(NO_SLOT)
         if not self.exact:
             some = (self.query_start_loc[1:] > self.query_start_loc[:-1]).int()
             self.seq_lens.add_(some)
@@ -62,8 +64,6 @@ class PagedBatchMeta:
             rows = torch.arange(self.num_tokens, dtype=torch.int32,
                                 device=self.positions.device)
             self.positions.add_((rows < self.query_start_loc[-1]).int())
-            if self.slot_mapping is not None:
-                self.slot_mapping.fill_(NO_SLOT)
             return
         v = self.step_view
         n, t = self.num_seqs, self.num_tokens
@@ -264,8 +264,9 @@ def build_batch_meta(tables: DeviceTables, q_lens: torch.Tensor, num_tokens: int
     Returns (PagedBatchMeta with slot_mapping, DeviceTables after the step).
     Values as pack_batch_meta gives them, and like its result the step can go to
     KVPool.write_from_table, paged_attention_append_meta and
-    PagedTransformer.forward_step, though never as a decode batch (is_decode): its
-    lengths are not the host's to know; the given tables' other tensors are not
+    PagedTransformer.forward_step, though not as a decode batch (is_decode): its
+    lengths are not the host's to know (a caller who knows that they are the bounds,
+    one token for every sequence, says so by dataclasses.replace(meta, exact=True)); the given tables' other tensors are not
     changed, so a step whose result is dropped can be taken again (the table itself
     is one for all states: its rows are those of the last step taken, zeros behind
     the blocks they hold). With too few
