@@ -204,7 +204,9 @@ class KVPool:
         q_lens = accepted.lens, or less where a sequence is to take fewer). The same
         bytes as write() of those rows layer by layer."""
         what = "KVPool.write_accepted"
-        _native.require_device(self.kv, k_rows, v_rows, accepted.path, what=what)
+        dev = self.device
+        if dev.type != "cuda":
+            _native.require_device(self.kv, what=what)
         layers = k_rows.shape[0]
         shape = (layers, tree.num_tokens, self.num_kv_heads, self.head_dim)
         assert k_rows.shape == shape and v_rows.shape == shape, \
@@ -219,13 +221,15 @@ class KVPool:
             raise ValueError(f"{what}: blocks of {meta.block_size}, the pool's have {self.block_size}")
         path, lens, qsl = accepted.path, accepted.lens, tree.query_start_loc
         table, start, step = meta.block_tables, meta.start_pos, meta.query_start_loc
-        dev = self.device
         if not (k_rows.device == v_rows.device == path.device == lens.device == qsl.device
                 == table.device == start.device == step.device == dev):
+            _native.require_device(k_rows, v_rows, path, what=what)
             raise RuntimeError(f"{what}: rows and metadata must be on {dev}")
-        for t in (path, lens, qsl, table, start, step):
-            if t.dtype != torch.int32 or not t.is_contiguous():
-                raise ValueError(f"{what}: paths, lengths and metadata must be contiguous int32")
+        if not (path.dtype == lens.dtype == qsl.dtype == table.dtype == start.dtype == step.dtype
+                == torch.int32 and path.is_contiguous() and lens.is_contiguous()
+                and qsl.is_contiguous() and table.is_contiguous() and start.is_contiguous()
+                and step.is_contiguous()):
+            raise ValueError(f"{what}: paths, lengths and metadata must be contiguous int32")
         if (table.shape[0] != n or start.numel() != n or qsl.numel() != n + 1
                 or step.numel() != n + 1):
             raise ValueError(f"{what}: the metadata's tensors are not those of {n} sequences")
