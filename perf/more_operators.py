@@ -105,6 +105,9 @@ def draw(rng):
     c = dict(kind=kind, batch=batch, lo=lo, hi=hi, adapters=_logint(rng, 1, 64),
              none=rng.choice([0.0, 0.1, 0.5, 1.0]) if rng.random() < 0.5 else 0.2, shape=shape)
     if kind == "plan":
+        # so many requests that their order, which the seed gives, shows in the plan
+        c.update(batch=max(batch, 12), hi=min(hi, 1300), lo=min(lo, 1300),
+                 adapters=max(c["adapters"], 4), none=min(c["none"], 0.5))
         return c
     c.update(k=8 * _logint(rng, 8, 512), rank=rng.choice([8, 8, 16, 16, 24, 32, 64, 128]),
              dtype=dtype)
@@ -371,7 +374,7 @@ def _plain_plan(st):
 def _plain_sum(st):
     """base plus every adapter's products, in 32 bits."""
     r, outs = st["case"]["rank"], _outs(st["case"])
-    y = st["base"].float()
+    y = st["base"].to(torch.float32, copy=True)
     for n, rows in st["rows"]:
         t = st["x"][rows].float() @ st["a"][n].float().t() * st["scale"][n]
         at, parts = 0, []
