@@ -142,6 +142,10 @@ extern "C" {
 #define PKV_STATUS_BAD_PARENT 2048 /* tree_masks: a parent that is neither -1 nor an
                                       earlier node of the tree; the node counts
                                       as a root                              */
+#define PKV_STATUS_BAD_TOKEN 4096 /* control_logits: a token or bias id outside the
+                                     vocabulary was skipped                  */
+#define PKV_STATUS_BAD_CONTROL 8192 /* a request's adapter, length, offset, mask or
+                                       sampling parameter is outside its range */
 
 /* Library version (PKV_VERSION). */
 int pkv_version(void);
@@ -649,6 +653,97 @@ int pkv_write_accepted_step(void* k_pool, void* v_pool, int64_t pool_layer_elems
                             const int32_t* path, const int32_t* lens, int n_seq, int n_tokens,
                             int max_depth, int64_t row_elems, int dtype, int* status,
                             void* stream);
+
+/*
+ * Rows of a step grouped by low-rank adapter (no counterpart in the reference).
+ * ids[t] (int32) is row t's adapter, -1 for none; any other value outside [0,
+ * n_adapters) counts as none (PKV_STATUS_BAD_CONTROL). order [n_tokens]: the rows
+ * sorted by adapter, in their own order within one, those without an adapter last;
+ * starts [n_adapters + 2]: the first place of each adapter's rows, of those without
+ * one, and n_tokens. tiles [max_tiles][4] (16-byte aligned): pieces of at most tile_rows
+ * (16 or 64) rows of one adapter, as {adapter or -1, first place, rows, 0}, unused
+ * entries with 0 rows; max_tiles at least n_tokens / tile_rows + min(n_adapters + 1,
+ * n_tokens). At most 1000 adapters and 2^24 rows.
+ */
+int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int max_tiles,
+                     const int32_t* ids, int n_tokens, int n_adapters, int tile_rows,
+                     int* status, void* stream);
+
+/*
+ * Workspace bytes of pkv_adapter_apply for a step of n_tokens rows whose plan has
+ * max_tiles tiles, k features in and `ranks` ranks of all parts together. It needs
+ * no initial state; calls in flight together need different memory.
+ */
+size_t pkv_adapter_workspace_bytes(int n_tokens, int max_tiles, int k, int ranks);
+
+/*
+ * Low-rank adapters beside a (fused) projection (no counterpart in the reference).
+ * base [n_tokens, n] is the projection's output, n = the sum of the features n0 ...
+ * of its 1 to 4 parts. With row t's adapter i of the plan (order, tiles):
+ *   y[t] = base[t] + scales[i] * b[i] (a[i] x[t])
+ * where a [n_adapters, parts * rank, k] (rows a_stride elements apart, a multiple of 8,
+ * zeros behind k) and b [n_adapters, n, rank]; the features of part s use the ranks
+ * s * rank ... (s + 1) * rank - 1. Rows without an adapter get y = base. All sums
+ * are fp32, also a[i] x[t], and y is rounded once. PKV_EPILOGUE_NONE: out [n_tokens, n] =
+ * y; out may be base itself (same address and stride). PKV_EPILOGUE_SWIGLU: two parts,
+ * out [n_tokens, n0] = silu(y of part 0) * y of part 1, rounded once. Except for that
+ * one case out shares no memory with an operand. rank is a multiple of 8 up to 128
+ * (PKV_ERR_UNSUPPORTED); any k, n and strides of rows; a, b 16-byte aligned.
+ */
+int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t base_stride,
+                      const void* x, int64_t x_stride, const void* a, int64_t a_stride,
+                      const void* b, const float* scales, const int32_t* order,
+                      const int32_t* tiles, int max_tiles, int tile_rows, int n_tokens,
+                      int n_adapters, int k, int rank, int parts, int n0, int n1, int n2, int n3,
+                      int epilogue, int dtype, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
+ * What requests ask of their next token, on rows of logits [rows, vocab] (fp32 / bf16 /
+ * f16, rows in_stride elements apart; no counterpart in the reference). In this order,
+ * in fp32, rounded once:
+ *   tokens[r][0 ... lens[r]) (int32, rows tok_stride apart, lens at most cap), the
+ *     first prompt_lens[r] (null: 0) of them the prompt. A token that is there: x > 0 ?
+ *     x / repetition[r] : x * repetition[r]; one that is there c > 0 times behind
+ *     the prompt: x -= frequency[r] * c + presence[r]. Null arrays: 1, 0 and 0.
+ *   x += bias_values[e] for every e in [bias_starts[r], bias_starts[r + 1]) (int32
+ *     [rows + 1], n_bias entries in all) with bias_ids[e] the id; an id named
+ *     more than once gets the sum, added up in the list's order.
+ *   mask_rows[r] >= 0: -infinity where bit id % 32 of word id / 32 of masks[mask_rows[r]]
+ *     ([n_masks, ceil(vocab / 32)] int32) is 0; -1: no mask.
+ * Null tokens, bias_starts, mask_rows: none of the kind. out may be logits itself (same
+ * address and stride), else it shares no memory with an operand. An id outside the
+ * vocabulary is skipped (PKV_STATUS_BAD_TOKEN); a length or offset outside its bounds is
+ * cut to them or counts as none, a mask row outside [-1, n_masks) as -1
+ * (PKV_STATUS_BAD_CONTROL).
+ */
+int pkv_control_logits(void* out, int64_t out_stride, const void* logits, int64_t in_stride,
+                       int64_t rows, int64_t vocab, const int32_t* tokens, int64_t tok_stride,
+                       int cap, const int32_t* lens, const int32_t* prompt_lens,
+                       const float* repetition, const float* presence, const float* frequency,
+                       const int32_t* bias_ids, const float* bias_values,
+                       const int32_t* bias_starts, int n_bias, const int32_t* masks, int n_masks,
+                       const int32_t* mask_rows, int dtype, int* status, void* stream);
+
+/*
+ * pkv_sample_rows with every row's own parameters and any top-k. Row r of logits l:
+ * temperature[r] = 0: the first of the largest (logprobs 0). Else the weights e_i =
+ * exp((l_i - max) / temperature[r]); top_k[r] > 0 keeps the ids with l_i at least the
+ * top_k-th largest (ties kept), top_p[r] < 1 of those, sorted descending (ties by ascending
+ * id), the ids with a sum of weights before them of at most top_p times the sum of
+ * all kept, min_p[r] > 0 of those the ids with e_i >= min_p. ids[r] (int64) = the first kept id,
+ * ascending, whose cumulative weight exceeds uniforms[r] times the sum, logprobs[r]
+ * (nullable) the logarithm of its share. Weights count in units of 2^-43 (in 64-bit
+ * integers: the draw does not depend on an order of summation). Null top_k, top_p, min_p:
+ * 0, 1, 0. Logits may be -infinity. ids[r] = -1, logprobs[r] NaN: PKV_STATUS_BAD_CONTROL
+ * (temperature not finite or negative, top_k < 0, top_p <= 0, min_p outside [0, 1], a
+ * uniform outside [0, 1)), PKV_STATUS_NONFINITE (a NaN or +infinity),
+ * PKV_STATUS_BAD_DISTRIBUTION (every logit -infinity). At most 2^20 logits a row.
+ */
+int pkv_sample_each(int64_t* ids, float* logprobs, const void* logits, int64_t rows,
+                    int64_t vocab, int64_t row_stride, const float* temperature,
+                    const int32_t* top_k, const float* top_p, const float* min_p,
+                    const float* uniforms, int dtype, int* status, void* stream);
 
 /*
  * Measurement helper, no counterpart in the reference: reads `bytes` bytes at

@@ -75,7 +75,8 @@ PyObject* checked(const char* name, R (*fn)(A...), PyObject* const* args, Py_ssi
   X(pkv_linear_tiles_rope_qkv) X(pkv_argmax_rows) X(pkv_sample_rows)                         \
   X(pkv_argmax_workspace_bytes) X(pkv_stream_read) X(pkv_build_step) X(pkv_tree_masks)        \
   X(pkv_tree_attention_workspace_bytes) X(pkv_paged_tree_attention) X(pkv_tree_accept)       \
-  X(pkv_write_accepted) X(pkv_write_accepted_step)
+  X(pkv_write_accepted) X(pkv_write_accepted_step) X(pkv_adapter_plan)                       \
+  X(pkv_adapter_workspace_bytes) X(pkv_adapter_apply) X(pkv_control_logits) X(pkv_sample_each)
 
 #define DEFINE(name)                                                                         \
   decltype(&::name) ptr_##name = nullptr;                                                    \

@@ -33,6 +33,15 @@ int check_launch(const char* what) {
   return PKV_OK;
 }
 
+int allow_lds(const void* kernel, size_t bytes) {
+  if (bytes <= 48 * 1024) return PKV_OK;
+  const hipError_t e =
+      hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != hipSuccess)
+    return fail(PKV_ERR_HIP, "%zu bytes of LDS: %s", bytes, hipGetErrorString(e));
+  return PKV_OK;
+}
+
 static bool valid_dtype(int dtype) {
   return dtype == PKV_DTYPE_F32 || dtype == PKV_DTYPE_F16 ||
          dtype == PKV_DTYPE_BF16;

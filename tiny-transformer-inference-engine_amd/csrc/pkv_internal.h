@@ -19,6 +19,9 @@ using f16 = _Float16;
 int fail(int code, const char* fmt, ...);
 int check_launch(const char* what);
 
+// Lets a kernel be launched with that many bytes of dynamic LDS (capi.hip).
+int allow_lds(const void* kernel, size_t bytes);
+
 inline int elem_bytes(int dtype) {
   return dtype == PKV_DTYPE_F32 ? 4 : 2;
 }

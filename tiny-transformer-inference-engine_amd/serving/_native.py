@@ -42,6 +42,8 @@ PKV_STATUS_DIRTY_WORKSPACE = 256
 PKV_STATUS_STALLED = 512
 PKV_STATUS_OUT_OF_BLOCKS = 1024
 PKV_STATUS_BAD_PARENT = 2048
+PKV_STATUS_BAD_TOKEN = 4096
+PKV_STATUS_BAD_CONTROL = 8192
 # part_tokens values selecting a persistent decode kernel (every workgroup an
 # equal share of all sequences' chunks): PART_PERSISTENT and PART_STATIC the
 # register-staged kernel (also the automatic choice for long context
@@ -141,6 +143,16 @@ _SIGNATURES = {
     "pkv_write_accepted_step": ([_c_vp, _c_vp, _c_i64, _c_int, _c_i64, _c_int, _c_vp, _c_vp,
                                  _c_i64, _c_vp, _c_int] + [_c_vp] * 5 + [_c_int, _c_int, _c_int,
                                  _c_i64, _c_int, _c_vp, _c_vp], _c_int),
+    "pkv_adapter_plan": ([_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_int, _c_vp,
+                          _c_vp], _c_int),
+    "pkv_adapter_workspace_bytes": ([_c_int] * 4, _c_size),
+    "pkv_adapter_apply": ([_c_vp, _c_i64] * 4 + [_c_vp] * 4 + [_c_int] * 13 + [_c_vp, _c_size,
+                                                                              _c_vp], _c_int),
+    "pkv_control_logits": ([_c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_int]
+                           + [_c_vp] * 8 + [_c_int, _c_vp, _c_int, _c_vp, _c_int, _c_vp, _c_vp],
+                           _c_int),
+    "pkv_sample_each": ([_c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64] + [_c_vp] * 5
+                        + [_c_int, _c_vp, _c_vp], _c_int),
 }
 
 EXPORTED = tuple(_SIGNATURES)

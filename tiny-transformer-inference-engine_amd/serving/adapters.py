@@ -1,0 +1,252 @@
+"""Low-rank adapters of many requests beside the shared projections.
+
+Row t of a step may name an adapter i; a projection's output of that row is then
+y = W x + scale_i B_i (A_i x). AdapterWeights holds the A and B of several adapters
+for one (fused) projection, build_adapter_plan groups a step's rows by adapter once
+for all layers, and adapter_add / adapter_swiglu take the projection's output and
+finish it (csrc/adapters.hip):
+
+  weights = AdapterWeights(d_model, (hq * d, hkv * d, hkv * d), num_adapters=16, max_rank=16)
+  weights.load(3, [(A_q, B_q), (A_k, B_k), None], scale=alpha / r)
+  plan = build_adapter_plan(ids, 16)                  # int32 [T], -1: no adapter
+  qkv = adapter_add(linear(x, w_qkv), x, weights, plan)
+
+AdapterSet holds the weights of every projection of a PagedTransformer; its
+forward_batch, forward_step and generate_batched, and the Scheduler's requests, take
+adapters by index. No counterpart in the reference. Nothing here synchronises the
+host, and every call's scratch is its own.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _native
+from .paged_meta import _status_ptr
+
+__all__ = ["AdapterWeights", "AdapterPlan", "build_adapter_plan", "adapter_add", "adapter_swiglu"]
+
+MAX_ADAPTERS = 1000
+MAX_RANK = 128
+_I32 = torch.int32
+# Rows a tile: 16 leaves no empty matrix rows where most adapters have a few rows;
+# 64 reads an adapter's weights a quarter as often where a step holds prompts.
+TILE_ROWS_FEW, TILE_ROWS_MANY, TILE_MANY_FROM = 16, 64, 1024
+
+
+class AdapterWeights:
+    """A and B of num_adapters adapters beside a projection of in_features features
+    to the parts out_features (one, or those of a fused projection, at most 4), of at
+    most max_rank ranks a part. a [num_adapters, parts * rank, in_features rounded up
+    to 8], b [num_adapters, sum(out_features), rank] and scales (float32) are what the
+    kernels read, rank being max_rank rounded up to a multiple of 8; unused ranks are 0,
+    and so is an adapter that was not loaded."""
+
+    def __init__(self, in_features: int, out_features, num_adapters: int, max_rank: int,
+                 dtype: torch.dtype = torch.float32, device="cuda"):
+        outs = (out_features,) if isinstance(out_features, int) else tuple(out_features)
+        _native.dtype_code(dtype)
+        if in_features < 1 or not 1 <= len(outs) <= 4 or min(outs) < 1:
+            raise ValueError("AdapterWeights: needs features in and 1 to 4 parts of features out")
+        if not 1 <= num_adapters <= MAX_ADAPTERS or not 1 <= max_rank <= MAX_RANK:
+            raise ValueError(f"AdapterWeights: 1 to {MAX_ADAPTERS} adapters of rank 1 to {MAX_RANK}")
+        self.in_features, self.out_features = int(in_features), outs
+        self.num_adapters, self.rank, self.dtype = int(num_adapters), -(-max_rank // 8) * 8, dtype
+        self.a = torch.zeros((num_adapters, len(outs) * self.rank, -(-in_features // 8) * 8),
+                             dtype=dtype, device=device)
+        self.b = torch.zeros((num_adapters, sum(outs), self.rank), dtype=dtype, device=device)
+        self.scales = torch.zeros(num_adapters, dtype=torch.float32, device=device)
+        self.device = self.a.device
+        self._ns = outs + (0,) * (4 - len(outs))
+
+    def _index(self, index):
+        if not 0 <= index < self.num_adapters:
+            raise IndexError(f"adapter {index} of {self.num_adapters}")
+        return index
+
+    @torch.no_grad()
+    def load(self, index: int, parts, scale: float = 1.0) -> None:
+        """Puts an adapter in place `index`: per part (A [r, in_features], B
+        [out_features, r]) with r up to the rank, or None for a part without one."""
+        self._index(index)
+        if len(parts) != len(self.out_features):
+            raise ValueError(f"AdapterWeights.load: {len(self.out_features)} parts, "
+                             f"got {len(parts)}")
+        for n, pair in zip(self.out_features, parts):
+            if pair is None:
+                continue
+            a, b = pair
+            r = a.shape[0] if a.dim() == 2 else -1
+            if (not 0 <= r <= self.rank or a.shape != (r, self.in_features)
+                    or b.shape != (n, r)):
+                raise ValueError(
+                    f"AdapterWeights.load: A {tuple(a.shape)} and B {tuple(b.shape)} are not "
+                    f"[r, {self.in_features}] and [{n}, r] with r up to {self.rank}")
+        R, k, at = self.rank, self.in_features, 0
+        if self.a.shape[2] != k or any(pair is None or pair[0].shape[0] < R for pair in parts):
+            self.clear(index)
+        dst, src = [], []
+        for s, (n, pair) in enumerate(zip(self.out_features, parts)):
+            if pair is not None:
+                r = pair[0].shape[0]
+                dst += [self.a[index, s * R:s * R + r, :k], self.b[index, at:at + n, :r]]
+                src += pair
+            at += n
+        if dst:
+            torch._foreach_copy_(dst, src)  # one launch where types and layouts agree
+        self.scales[index] = float(scale)
+
+    @torch.no_grad()
+    def clear(self, index: int) -> None:
+        """Takes adapter `index` out: rows that name it get the projection alone."""
+        index = self._index(index)
+        self.a[index].zero_()
+        self.b[index].zero_()
+        self.scales[index] = 0.0
+
+
+@dataclass(frozen=True)
+class AdapterPlan:
+    order: torch.Tensor   # int32 [T] rows sorted by adapter, those without one last
+    starts: torch.Tensor  # int32 [num_adapters + 2] first place of each adapter's rows
+    tiles: torch.Tensor   # int32 [max_tiles, 4] adapter or -1, first place, rows, 0
+    num_tokens: int
+    num_adapters: int
+    tile_rows: int
+
+
+def build_adapter_plan(ids: torch.Tensor, num_adapters: int,
+                       status: Optional[torch.Tensor] = None) -> AdapterPlan:
+    """Groups the rows of a step by adapter: ids int32 [T], -1 for a row without
+    one. Any other id outside [0, num_adapters) counts as none and is reported in
+    `status` (int32 [1], zeroed by the caller, read with raise_step_status)."""
+    what = "build_adapter_plan"
+    _native.require_device(ids, what=what)
+    if ids.dtype != _I32 or ids.dim() != 1:
+        raise ValueError(f"{what}: ids must be int32 [T]")
+    n = int(num_adapters)
+    if not 0 <= n <= MAX_ADAPTERS:
+        raise ValueError(f"{what}: at most {MAX_ADAPTERS} adapters")
+    T, dev = ids.shape[0], ids.device
+    rows = TILE_ROWS_MANY if T >= TILE_MANY_FROM else TILE_ROWS_FEW
+    max_tiles = T // rows + min(n + 1, T)
+    previous = _native.make_current(dev)
+    try:
+        if not ids.is_contiguous():
+            ids = ids.contiguous()
+        # one allocation; the tiles lead, their rows are 16 bytes
+        buf = ids.new_empty(4 * max_tiles + T + n + 2)
+        tiles, order, starts = buf.split_with_sizes((4 * max_tiles, T, n + 2))
+        rc = _native.calls().pkv_adapter_plan(
+            order.data_ptr(), starts.data_ptr(), tiles.data_ptr(), max_tiles, ids.data_ptr(), T,
+            n, rows, None if status is None else _status_ptr(status, dev, what),
+            _native.stream_ptr(dev))
+    finally:
+        _native.restore(previous)
+    if rc:
+        _native.check(rc, what)
+    return AdapterPlan(order, starts, tiles.view(max_tiles, 4), T, n, rows)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two 2-D tensors with unit column stride share memory."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    es = a.element_size()
+    pa, pb = a.data_ptr(), b.data_ptr()
+    wa, wb = a.shape[1] * es, b.shape[1] * es
+    if (pa + (a.shape[0] - 1) * a.stride(0) * es + wa <= pb
+            or pb + (b.shape[0] - 1) * b.stride(0) * es + wb <= pa):
+        return False
+    if a.stride(0) == b.stride(0):  # columns of one buffer
+        pitch = a.stride(0) * es
+        off = (pa - pb) % pitch
+        return not (off >= wb and off + wa <= pitch)
+    return True
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with unit column stride and rows that do not overlap."""
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        return t.contiguous()
+    return t
+
+
+def _apply(base, x, weights, plan, out, written, epilogue, what):
+    dev, dtype, T = weights.device, weights.dtype, plan.num_tokens
+    _native.require_device(base, x, plan.order, weights.a, what=what)
+    if base.device != dev or x.device != dev or plan.order.device != dev:
+        raise RuntimeError(f"{what}: base, x, the weights and the plan must share a device")
+    if base.dtype != dtype or x.dtype != dtype:
+        raise TypeError(f"{what}: base and x must be {dtype}, as the weights are")
+    if (base.requires_grad or x.requires_grad) and torch.is_grad_enabled():
+        raise NotImplementedError(
+            f"{what} is forward-only (inference); run it under torch.no_grad()")
+    outs = weights.out_features
+    n, k = sum(outs), weights.in_features
+    if base.shape != (T, n) or x.shape != (T, k):
+        raise ValueError(f"{what}: base must be [{T}, {n}] and x [{T}, {k}] for this plan and "
+                         f"these weights (got {tuple(base.shape)}, {tuple(x.shape)})")
+    if plan.num_adapters != weights.num_adapters:
+        raise ValueError(f"{what}: a plan of {plan.num_adapters} adapters, weights of "
+                         f"{weights.num_adapters}")
+    in_place = out is base
+    base, x = _rows(base), _rows(x)
+    previous = _native.make_current(dev)
+    try:
+        if out is None:
+            out = base.new_empty((T, written))
+        else:
+            if out.shape != (T, written) or out.dtype != dtype or out.device != dev:
+                raise ValueError(f"{what}: out must be [{T}, {written}] {dtype} on {dev}")
+            if _rows(out) is not out:
+                raise ValueError(f"{what}: out needs unit column stride and rows of its own")
+            if out.requires_grad and torch.is_grad_enabled():
+                raise NotImplementedError(f"{what} is forward-only (inference)")
+            same = (out.data_ptr() == base.data_ptr() and written == n
+                    and _row_stride(out) == _row_stride(base))
+            if (not same and _overlap(out, base)) or _overlap(out, x):
+                raise ValueError(f"{what}: out shares memory with base or x")
+        tiles, calls = plan.tiles, _native.calls()
+        nbytes = calls.pkv_adapter_workspace_bytes(T, tiles.shape[0], k, len(outs) * weights.rank)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        rc = calls.pkv_adapter_apply(
+            out.data_ptr(), _row_stride(out), base.data_ptr(), _row_stride(base), x.data_ptr(),
+            _row_stride(x), weights.a.data_ptr(), weights.a.shape[2], weights.b.data_ptr(),
+            weights.scales.data_ptr(), plan.order.data_ptr(), tiles.data_ptr(), tiles.shape[0],
+            plan.tile_rows, T, weights.num_adapters, k, weights.rank, len(outs), *weights._ns,
+            epilogue, _native.DTYPE_CODES[dtype], None if ws is None else ws.data_ptr(), nbytes,
+            _native.stream_ptr(dev))
+        if rc:
+            _native.check(rc, what)
+        if in_place:
+            torch.autograd.graph.increment_version(out)
+    finally:
+        _native.restore(previous)
+    return out
+
+
+def adapter_add(base: torch.Tensor, x: torch.Tensor, weights: AdapterWeights, plan: AdapterPlan,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """base [T, sum(out_features)] plus each row's adapter's product with x [T,
+    in_features]; float32, float16 or bfloat16, sums in fp32, rounded once. Rows without
+    an adapter are base's. out: where to write, base itself (in place) or memory of no
+    operand."""
+    return _apply(base, x, weights, plan, out, sum(weights.out_features),
+                  _native.EPILOGUE_NONE, "adapter_add")
+
+
+def adapter_swiglu(base: torch.Tensor, x: torch.Tensor, weights: AdapterWeights,
+                   plan: AdapterPlan, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """silu(gate) * up [T, H] of adapter_add(base, ...) = [gate, up], base [T, 2 H],
+    without rounding in between. Rows without an adapter are silu_mul of base."""
+    outs = weights.out_features
+    if len(outs) != 2 or outs[0] != outs[1]:
+        raise ValueError("adapter_swiglu: the weights need two parts of one size (gate, up)")
+    return _apply(base, x, weights, plan, out, outs[0], _native.EPILOGUE_SWIGLU, "adapter_swiglu")

@@ -1,0 +1,209 @@
+"""What each request of a batch asks of its next token: penalties of tokens that are
+there already, biases, a grammar's mask, and its own sampling parameters
+(csrc/controls.hip). No counterpart in the reference, whose sample() takes one set of
+parameters for all rows (sampling.py:94-137).
+
+  logits = control_logits(logits, LogitControls(tokens=history, lens=lens, ...), out=logits)
+  ids, logprobs = sample_each(logits, temperature, top_k, top_p, min_p)
+
+Nothing here synchronises the host, so both calls can be captured in a HIP graph.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass, fields
+from typing import Optional
+
+import torch
+
+from . import _native
+from .adapters import _overlap, _row_stride, _rows
+from .paged_meta import _status_ptr
+
+__all__ = ["LogitControls", "control_logits", "sample_each"]
+
+MAX_SAMPLE_VOCAB = 1 << 20
+
+
+def _check(t, dtype, shape, name, what):
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be contiguous {dtype} {list(shape)} "
+                         f"(got {t.dtype} {list(t.shape)})")
+
+
+@dataclass(frozen=True)
+class LogitControls:
+    """The controls of a batch's rows, on the device; each kind may be left out.
+
+    tokens       int32 [rows, capacity] each row's tokens so far, the first lens[r]
+    lens         int32 [rows]
+    prompt_lens  int32 [rows] how many of them are the prompt (None: 0)
+    repetition   float32 [rows] > 0: of a token that is there, x / r where x > 0, else x * r
+    presence     float32 [rows] taken off a token that is there behind the prompt
+    frequency    float32 [rows] the same, times how often it is there
+    bias_ids, bias_values, bias_starts
+                 int32 [n], float32 [n], int32 [rows + 1]: row r adds bias_values[e] to id
+                 bias_ids[e], bias_starts[r] <= e < bias_starts[r + 1]; what is named
+                 twice is added up
+    masks        int32 [masks, ceil(vocab / 32)] bit id % 32 of word id / 32: id is allowed
+    mask_rows    int32 [rows] the row's mask, -1 for none
+    """
+    tokens: Optional[torch.Tensor] = None
+    lens: Optional[torch.Tensor] = None
+    prompt_lens: Optional[torch.Tensor] = None
+    repetition: Optional[torch.Tensor] = None
+    presence: Optional[torch.Tensor] = None
+    frequency: Optional[torch.Tensor] = None
+    bias_ids: Optional[torch.Tensor] = None
+    bias_values: Optional[torch.Tensor] = None
+    bias_starts: Optional[torch.Tensor] = None
+    masks: Optional[torch.Tensor] = None
+    mask_rows: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        what = "LogitControls"
+        given = {f.name: getattr(self, f.name) for f in fields(self)
+                 if getattr(self, f.name) is not None}
+        if len({t.device for t in given.values()}) > 1:
+            raise ValueError(f"{what}: the tensors must share a device")
+        for group in (("tokens", "lens"), ("bias_ids", "bias_values", "bias_starts"),
+                      ("masks", "mask_rows")):
+            if len([n for n in group if n in given]) not in (0, len(group)):
+                raise ValueError(f"{what}: {', '.join(group)} go together")
+        history = [n for n in ("prompt_lens", "repetition", "presence", "frequency")
+                   if n in given]
+        if history and "tokens" not in given:
+            raise ValueError(f"{what}: {history[0]} needs tokens and lens")
+        rows = set()
+        if "tokens" in given:
+            t = self.tokens
+            if t.dtype != torch.int32 or t.dim() != 2 or (t.numel() > 0 and (
+                    t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]))):
+                raise ValueError(f"{what}: tokens must be int32 [rows, capacity] with unit "
+                                 "column stride")
+            rows.add(t.shape[0])
+            _check(self.lens, torch.int32, (t.shape[0],), "lens", what)
+            for n in history:
+                _check(given[n], torch.int32 if n == "prompt_lens" else torch.float32,
+                       (t.shape[0],), n, what)
+        if "bias_ids" in given:
+            n = self.bias_starts.numel() - 1
+            _check(self.bias_starts, torch.int32, (n + 1,), "bias_starts", what)
+            _check(self.bias_ids, torch.int32, (self.bias_ids.numel(),), "bias_ids", what)
+            _check(self.bias_values, torch.float32, (self.bias_ids.numel(),), "bias_values", what)
+            rows.add(n)
+        if "masks" in given:
+            if self.masks.dtype != torch.int32 or self.masks.dim() != 2 \
+                    or not self.masks.is_contiguous():
+                raise ValueError(f"{what}: masks must be contiguous int32 [masks, words]")
+            _check(self.mask_rows, torch.int32, (self.mask_rows.numel(),), "mask_rows", what)
+            rows.add(self.mask_rows.numel())
+        if len(rows) > 1:
+            raise ValueError(f"{what}: the tensors disagree on the rows ({sorted(rows)})")
+        object.__setattr__(self, "_rows", rows.pop() if rows else None)
+        object.__setattr__(self, "_device", next(iter(given.values())).device if given else None)
+
+
+def control_logits(logits: torch.Tensor, controls: LogitControls,
+                   out: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """logits [rows, vocab] (float32, float16, bfloat16) with every row's penalties, then
+    biases, then its mask (-infinity where an id is not allowed), in fp32 and rounded
+    once. out: where to write, logits itself or memory of no operand. `status` as in
+    build_adapter_plan: ids outside the vocabulary, which are skipped, and lengths, offsets
+    and mask rows outside their bounds. A mask may leave a row nothing: all -infinity."""
+    what = "control_logits"
+    _native.require_device(logits, what=what)
+    code = _native.dtype_code(logits.dtype)
+    if logits.dim() != 2:
+        raise ValueError(f"{what}: expected [rows, vocab], got {tuple(logits.shape)}")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(
+            f"{what} is forward-only (inference); run it under torch.no_grad()")
+    c, dev = controls, logits.device
+    rows, vocab = logits.shape
+    if c._rows is not None and (c._rows != rows or c._device != dev):
+        raise ValueError(f"{what}: controls of {c._rows} rows on {c._device}, logits of {rows} "
+                         f"on {dev}")
+    masks, tokens, bias = c.masks, c.tokens, c.bias_ids
+    if masks is not None and masks.shape[1] != -(-vocab // 32):
+        raise ValueError(f"{what}: masks of {masks.shape[1]} words, {-(-vocab // 32)} needed")
+    previous = _native.make_current(dev)
+    try:
+        src = _rows(logits)
+        in_place = out is logits
+        if out is None:
+            out = src.new_empty((rows, vocab))
+        elif not in_place or src is not logits:
+            if (out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev
+                    or _rows(out) is not out):
+                raise ValueError(f"{what}: out must be {tuple(logits.shape)} {logits.dtype} on "
+                                 f"{dev} with unit column stride and rows of its own")
+            if out.requires_grad and torch.is_grad_enabled():
+                raise NotImplementedError(f"{what} is forward-only (inference)")
+            same = out.data_ptr() == src.data_ptr() and _row_stride(out) == _row_stride(src)
+            if not same and _overlap(out, src):
+                raise ValueError(f"{what}: out shares memory with logits")
+        ptr = _native.ptr
+        rc = _native.calls().pkv_control_logits(
+            out.data_ptr(), _row_stride(out), src.data_ptr(), _row_stride(src), rows, vocab,
+            ptr(tokens), 0 if tokens is None else _row_stride(tokens),
+            0 if tokens is None else tokens.shape[1], ptr(c.lens), ptr(c.prompt_lens),
+            ptr(c.repetition), ptr(c.presence), ptr(c.frequency), ptr(bias), ptr(c.bias_values),
+            ptr(c.bias_starts), 0 if bias is None else bias.numel(), ptr(masks),
+            0 if masks is None else masks.shape[0], ptr(c.mask_rows), code,
+            None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
+        if rc:
+            _native.check(rc, what)
+        if in_place:
+            torch.autograd.graph.increment_version(out)
+    finally:
+        _native.restore(previous)
+    return out
+
+
+def sample_each(logits: torch.Tensor, temperature: torch.Tensor,
+                top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                min_p: Optional[torch.Tensor] = None, uniforms: Optional[torch.Tensor] = None,
+                status: Optional[torch.Tensor] = None):
+    """One draw a row of logits [rows, vocab] (up to 2^20 of them) with the row's
+    temperature (float32 [rows], 0: the largest), top_k (int32, 0: off), top_p (float32, 1:
+    off) and min_p (float32, 0: off; a share of the largest probability), by inverse CDF,
+    ids ascending, at its uniform in [0, 1) (None: from torch's generator). top-k and top-p
+    as in sampling.sample. Logits may be -infinity. Returns (ids int64 [rows], logprobs
+    float32 [rows] of the distribution drawn from). A row that cannot be drawn has id -1
+    and log-probability NaN, and is reported in `status` (PKV_STATUS_NONFINITE: NaN or
+    +infinity; PKV_STATUS_BAD_DISTRIBUTION: all -infinity; PKV_STATUS_BAD_CONTROL: a
+    parameter outside its range)."""
+    what = "sample_each"
+    _native.require_device(logits, what=what)
+    code = _native.dtype_code(logits.dtype)
+    if logits.dim() != 2 or not 0 < logits.shape[1] <= MAX_SAMPLE_VOCAB:
+        raise ValueError(f"{what}: expected [rows, 1 to {MAX_SAMPLE_VOCAB}] logits, "
+                         f"got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    dev = logits.device
+    for t, dtype, name in ((temperature, torch.float32, "temperature"),
+                           (top_k, torch.int32, "top_k"), (top_p, torch.float32, "top_p"),
+                           (min_p, torch.float32, "min_p"),
+                           (uniforms, torch.float32, "uniforms")):
+        if t is not None:
+            if t.device != dev:
+                raise ValueError(f"{what}: {name} must be on {dev} (got {t.device})")
+            _check(t, dtype, (rows,), name, what)
+    previous = _native.make_current(dev)
+    try:
+        if uniforms is None:
+            uniforms = torch.rand(rows, device=dev, dtype=torch.float32)
+        src = _rows(logits)
+        ids = torch.empty(rows, dtype=torch.int64, device=dev)
+        logprobs = temperature.new_empty(rows)
+        ptr = _native.ptr
+        rc = _native.calls().pkv_sample_each(
+            ids.data_ptr(), logprobs.data_ptr(), src.data_ptr(), rows, vocab, _row_stride(src),
+            temperature.data_ptr(), ptr(top_k), ptr(top_p), ptr(min_p), uniforms.data_ptr(), code,
+            None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
+        if rc:
+            _native.check(rc, what)
+    finally:
+        _native.restore(previous)
+    return ids, logprobs

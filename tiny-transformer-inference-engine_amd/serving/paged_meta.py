@@ -242,6 +242,15 @@ def raise_step_status(status: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what}: a node's parent is neither -1 nor an earlier node")
     if bits & _native.PKV_STATUS_BAD_BLOCK:
         raise AssertionError(f"{what}: a block id is block 0 or outside the pool")
+    if bits & _native.PKV_STATUS_BAD_TOKEN:
+        raise ValueError(f"{what}: a token or bias id is outside the vocabulary")
+    if bits & _native.PKV_STATUS_BAD_CONTROL:
+        raise ValueError(f"{what}: an adapter, length, mask or sampling parameter is outside "
+                         "its range")
+    if bits & _native.PKV_STATUS_NONFINITE:
+        raise ValueError(f"{what}: logits contain NaN or infinity")
+    if bits & _native.PKV_STATUS_BAD_DISTRIBUTION:
+        raise ValueError(f"{what}: a row has no token left to draw")
     if bits:
         raise RuntimeError(f"{what}: status {bits}")
 
