@@ -26,7 +26,8 @@ import torch
 from . import _native
 from .paged_meta import _status_ptr
 
-__all__ = ["AdapterWeights", "AdapterPlan", "build_adapter_plan", "adapter_add", "adapter_swiglu"]
+__all__ = ["AdapterWeights", "AdapterPlan", "AdapterSet", "StepAdapters", "build_adapter_plan",
+           "adapter_add", "adapter_swiglu", "step_adapters"]
 
 MAX_ADAPTERS = 1000
 MAX_RANK = 128
@@ -250,3 +251,83 @@ def adapter_swiglu(base: torch.Tensor, x: torch.Tensor, weights: AdapterWeights,
     if len(outs) != 2 or outs[0] != outs[1]:
         raise ValueError("adapter_swiglu: the weights need two parts of one size (gate, up)")
     return _apply(base, x, weights, plan, out, outs[0], _native.EPILOGUE_SWIGLU, "adapter_swiglu")
+
+
+# The adapted projections of a block: its module, the parts of its fused projection, and
+# what the parts read and write, as attributes of the attention or the MLP
+_PROJECTIONS = {"qkv": ("attn", ("q_proj", "k_proj", "v_proj")), "out": ("attn", ("out",)),
+                "gate_up": ("mlp", ("gate_proj", "up_proj")), "down": ("mlp", ("down_proj",))}
+
+
+class AdapterSet:
+    """Adapters of a PagedTransformer, by index: layers[i] holds the AdapterWeights of
+    layer i's fused projections ("qkv", "out", "gate_up", "down"), of those in
+    `projections`."""
+
+    def __init__(self, model, num_adapters: int, max_rank: int, projections=tuple(_PROJECTIONS)):
+        unknown = set(projections) - set(_PROJECTIONS)
+        if unknown:
+            raise ValueError(f"AdapterSet: no projection {sorted(unknown)[0]!r}")
+        self.num_adapters = int(num_adapters)
+        self.layers = []
+        for layer in model.layers:
+            ws = {}
+            for name in projections:
+                owner, parts = _PROJECTIONS[name]
+                lins = [getattr(getattr(layer, owner), p) for p in parts]
+                ws[name] = AdapterWeights(lins[0].in_features, [m.out_features for m in lins],
+                                          num_adapters, max_rank, dtype=lins[0].weight.dtype,
+                                          device=lins[0].weight.device)
+            self.layers.append(ws)
+
+    def load(self, index: int, state: dict, scale: float = 1.0) -> None:
+        """Puts an adapter in place `index`. state: for each adapted nn.Linear of the
+        model, by its name ("layers.0.attn.q_proj"), "<name>.lora_A.weight" [r,
+        in_features] and "<name>.lora_B.weight" [out_features, r]; scale is usually
+        alpha / r. Linears that are not named have no adapter."""
+        left = set(state)
+        found = []
+        for i, ws in enumerate(self.layers):
+            for name, w in ws.items():
+                owner, parts = _PROJECTIONS[name]
+                pairs = []
+                for p in parts:
+                    keys = [f"layers.{i}.{owner}.{p}.lora_{m}.weight" for m in "AB"]
+                    here = [k for k in keys if k in state]
+                    if len(here) == 1:
+                        raise ValueError(f"AdapterSet.load: {here[0]} comes without the other")
+                    pairs.append(tuple(state[k] for k in keys) if here else None)
+                    left -= set(here)
+                found.append((w, pairs))
+        if left:
+            raise ValueError(f"AdapterSet.load: {sorted(left)[0]!r} is no projection of this set")
+        for w, pairs in found:
+            w.load(index, pairs, scale)
+
+    def clear(self, index: int) -> None:
+        for ws in self.layers:
+            for w in ws.values():
+                w.clear(index)
+
+
+@dataclass(frozen=True)
+class StepAdapters:
+    """The adapters of one step's rows."""
+    weights: AdapterSet
+    plan: AdapterPlan
+
+
+def step_adapters(weights: AdapterSet, ids, query_start_loc, device) -> Optional[StepAdapters]:
+    """The adapters of a ragged step from one id a sequence (-1: none) and the host's
+    query_start_loc; None where no sequence has one."""
+    ids = [int(i) for i in ids]
+    if len(ids) != len(query_start_loc) - 1:
+        raise ValueError(f"{len(ids)} adapter ids for {len(query_start_loc) - 1} sequences")
+    for i in ids:
+        if not -1 <= i < weights.num_adapters:
+            raise ValueError(f"adapter {i} of {weights.num_adapters}")
+    if all(i < 0 for i in ids):
+        return None
+    rows = [i for i, a, b in zip(ids, query_start_loc, query_start_loc[1:]) for _ in range(a, b)]
+    return StepAdapters(weights, build_adapter_plan(
+        torch.tensor(rows, dtype=_I32, device=device), weights.num_adapters))

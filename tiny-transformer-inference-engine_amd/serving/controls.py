@@ -6,20 +6,23 @@ parameters for all rows (sampling.py:94-137).
   logits = control_logits(logits, LogitControls(tokens=history, lens=lens, ...), out=logits)
   ids, logprobs = sample_each(logits, temperature, top_k, top_p, min_p)
 
-Nothing here synchronises the host, so both calls can be captured in a HIP graph.
+Neither synchronises the host, so both can be captured in a HIP graph. RequestParams is
+what a request of the Scheduler may ask for, draw_tokens its step over those requests.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, fields
-from typing import Optional
+import math
+from dataclasses import dataclass, field, fields
+from typing import Optional, Protocol
 
 import torch
 
 from . import _native
 from .adapters import _overlap, _row_stride, _rows
-from .paged_meta import _status_ptr
+from .paged_meta import _status_ptr, raise_step_status
 
-__all__ = ["LogitControls", "control_logits", "sample_each"]
+__all__ = ["LogitControls", "RequestParams", "Grammar", "TokenHistory", "control_logits",
+           "sample_each", "pack_mask", "draw_tokens"]
 
 MAX_SAMPLE_VOCAB = 1 << 20
 
@@ -207,3 +210,165 @@ def sample_each(logits: torch.Tensor, temperature: torch.Tensor,
     finally:
         _native.restore(previous)
     return ids, logprobs
+
+
+def pack_mask(allowed: torch.Tensor) -> torch.Tensor:
+    """bool [..., vocab] -> int32 [..., ceil(vocab / 32)], the words of LogitControls.masks."""
+    v = allowed.shape[-1]
+    bits = torch.nn.functional.pad(allowed.bool(), (0, -v % 32)).view(*allowed.shape[:-1], -1, 32)
+    weights = torch.tensor([1 << i for i in range(31)] + [-(1 << 31)], dtype=torch.int64,
+                           device=allowed.device)
+    return (bits * weights).sum(-1).to(torch.int32)
+
+
+class Grammar(Protocol):
+    """What a request's tokens may be: a state that its tokens advance."""
+
+    def mask(self) -> torch.Tensor:
+        """int32 [ceil(vocab / 32)] (pack_mask): the tokens allowed next."""
+
+    def advance(self, token: int) -> None:
+        """The request took `token`."""
+
+
+@dataclass
+class RequestParams:
+    """What one request of a batch asks for beyond its prompt (Scheduler.add_request);
+    the defaults ask for nothing but a draw at temperature 1."""
+    temperature: float = 1.0         # 0: the most likely token
+    top_k: int = 0                   # 0: off
+    top_p: float = 1.0
+    min_p: float = 0.0
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: dict = field(default_factory=dict)  # id -> value
+    grammar: Optional[Grammar] = None
+    adapter: int = -1                # of the scheduler's AdapterSet
+
+    def __post_init__(self):
+        if not math.isfinite(self.temperature) or self.temperature < 0:
+            raise ValueError("temperature must be finite and >= 0")
+        if self.top_k < 0:
+            raise ValueError("top_k must be >= 0")
+        if not 0 < self.top_p <= 1:
+            raise ValueError("top_p must be in (0, 1]")
+        if not 0 <= self.min_p <= 1:
+            raise ValueError("min_p must be in [0, 1]")
+        if not math.isfinite(self.repetition_penalty) or self.repetition_penalty <= 0:
+            raise ValueError("repetition_penalty must be finite and > 0")
+        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
+            raise ValueError("presence_penalty and frequency_penalty must be finite")
+
+    @property
+    def has_penalties(self) -> bool:
+        return (self.repetition_penalty != 1.0 or self.presence_penalty != 0.0
+                or self.frequency_penalty != 0.0)
+
+
+class TokenHistory:
+    """The tokens of running requests on the device, a row each: a step uploads the
+    tokens that are new, not the histories."""
+
+    def __init__(self, device):
+        self.device = device
+        self._buf = torch.zeros((0, 0), dtype=torch.int32, device=device)
+        self._row: dict = {}    # request -> row
+        self._len: dict = {}    # request -> (tokens, of which the prompt)
+        self._free: list = []
+        self._new: list = []    # (row, position, token) that are not on the device yet
+
+    def put(self, key, tokens, prompt_len: int) -> None:
+        """A request that starts, or starts again, with these tokens."""
+        if key not in self._row:
+            if not self._free:
+                n = self._buf.shape[0]
+                self._grow(max(8, 2 * n), self._buf.shape[1])
+                self._free = list(range(self._buf.shape[0] - 1, n - 1, -1))
+            self._row[key] = self._free.pop()
+        r, n = self._row[key], len(tokens)
+        self._fit(n)
+        self._new = [e for e in self._new if e[0] != r]
+        if n:
+            self._buf[r, :n] = torch.tensor(tokens, dtype=torch.int32, device=self.device)
+        self._len[key] = (n, int(prompt_len))
+
+    def append(self, key, token: int) -> None:
+        n, p = self._len[key]
+        self._new.append((self._row[key], n, int(token)))
+        self._len[key] = (n + 1, p)
+
+    def drop(self, key) -> None:
+        if key in self._row:
+            r = self._row.pop(key)
+            del self._len[key]
+            self._new = [e for e in self._new if e[0] != r]
+            self._free.append(r)
+
+    def rows(self, keys):
+        """(tokens [n, capacity], lens [n], prompt_lens [n]) of these requests; a request
+        that was never put has none."""
+        if self._new:
+            self._fit(max(p for _, p, _ in self._new) + 1)
+            row, pos, tok = torch.tensor(self._new, device=self.device).unbind(1)
+            self._buf[row, pos] = tok.to(torch.int32)
+            self._new = []
+        lens = [self._len.get(k, (0, 0)) for k in keys]
+        i = torch.tensor([[self._row.get(k, 0), *n] for k, n in zip(keys, lens)],
+                         device=self.device)
+        if self._buf.numel() == 0:
+            tokens = torch.zeros((len(keys), 1), dtype=torch.int32, device=self.device)
+        else:
+            tokens = self._buf.index_select(0, i[:, 0])
+        counts = i[:, 1:].to(torch.int32).t().contiguous()
+        return tokens, counts[0], counts[1]
+
+    def _fit(self, n):
+        if n > self._buf.shape[1]:
+            self._grow(self._buf.shape[0], max(n, 2 * self._buf.shape[1], 256))
+
+    def _grow(self, rows, cap):
+        buf = torch.zeros((rows, cap), dtype=torch.int32, device=self.device)
+        buf[:self._buf.shape[0], :self._buf.shape[1]] = self._buf
+        self._buf = buf
+
+
+def draw_tokens(logits: torch.Tensor, params, history: TokenHistory, keys):
+    """One token a row of logits [rows, vocab] on a ROCm device: row i by params[i]
+    (RequestParams) with the tokens of request keys[i] in `history`. Returns (ids,
+    log-probabilities) as lists; raises where a row has no token left to draw."""
+    n, dev, f32 = len(params), logits.device, torch.float32
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    # one upload of what is a number a row
+    nums = torch.tensor([[p.temperature, p.top_p, p.min_p, p.repetition_penalty,
+                          p.presence_penalty, p.frequency_penalty, min(p.top_k, 1 << 30)]
+                         for p in params], dtype=torch.float64).t().contiguous().to(dev)
+    temperature, top_p, min_p, rep, pres, freq = nums[:6].to(f32).unbind(0)
+    kw = {}
+    if any(p.has_penalties for p in params):
+        tokens, lens, prompt_lens = history.rows(keys)
+        kw.update(tokens=tokens, lens=lens, prompt_lens=prompt_lens, repetition=rep,
+                  presence=pres, frequency=freq)
+    if any(p.logit_bias for p in params):
+        starts = [0]
+        for p in params:
+            starts.append(starts[-1] + len(p.logit_bias))
+        flat = [(t, v) for p in params for t, v in p.logit_bias.items()]
+        kw.update(bias_ids=torch.tensor([t for t, _ in flat], dtype=torch.int32, device=dev),
+                  bias_values=torch.tensor([v for _, v in flat], dtype=f32, device=dev),
+                  bias_starts=torch.tensor(starts, dtype=torch.int32, device=dev))
+    masks = [(i, p.grammar.mask()) for i, p in enumerate(params) if p.grammar is not None]
+    if masks:
+        rows = [-1] * n
+        for m, (i, _) in enumerate(masks):
+            rows[i] = m
+        kw.update(masks=torch.stack([m.to(dev, torch.int32) for _, m in masks]),
+                  mask_rows=torch.tensor(rows, dtype=torch.int32, device=dev))
+    if kw:
+        logits = control_logits(logits, LogitControls(**kw), status=status)
+    ids, logprobs = sample_each(logits, temperature, nums[6].to(torch.int32), top_p, min_p,
+                                status=status)
+    got = torch.cat([ids.double(), logprobs.double(), status.double()]).tolist()  # one copy
+    if got[-1]:
+        raise_step_status(status, "draw_tokens")
+    return [int(i) for i in got[:n]], got[n:2 * n]

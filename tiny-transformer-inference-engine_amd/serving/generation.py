@@ -83,12 +83,18 @@ class _Cohort:
         self.running = still
 
 
-def _drive(model, pool, cohort, max_new_tokens, pick, stop_id=None):
-    cohort.accept(pick(model.forward_batch(cohort.prefill_batch(), pool)), stop_id)
+def _drive(model, pool, cohort, max_new_tokens, pick, stop_id=None, adapters=None,
+           adapter_ids=None):
+    def forward(batch):
+        if adapter_ids is None:
+            return model.forward_batch(batch, pool)
+        return model.forward_batch(batch, pool, adapters, [adapter_ids[n] for n in cohort.running])
+
+    cohort.accept(pick(forward(cohort.prefill_batch())), stop_id)
     for _ in range(max_new_tokens - 1):
         if not cohort.running:
             break
-        cohort.accept(pick(model.forward_batch(cohort.decode_batch(), pool)), stop_id)
+        cohort.accept(pick(forward(cohort.decode_batch())), stop_id)
     return cohort.produced
 
 
@@ -101,9 +107,13 @@ def _greedy_ids(logits):
 
 
 @torch.no_grad()
-def generate_batched(model, prompts_ids, max_new_tokens, pool, alloc, block_size=16):
+def generate_batched(model, prompts_ids, max_new_tokens, pool, alloc, block_size=16,
+                     adapters=None, adapter_ids=None):
     """prompts_ids: list of token-id lists. Returns the greedy continuation of
-    each (max_new_tokens tokens, no EOS stop), in prompt order."""
+    each (max_new_tokens tokens, no EOS stop), in prompt order. adapters: an AdapterSet
+    (serving.adapters), adapter_ids one index of it a prompt, -1 for none."""
+    if adapter_ids is not None and len(adapter_ids) != len(prompts_ids):
+        raise ValueError("adapter_ids must name one adapter (or -1) a prompt")
     if max_new_tokens < 0:
         raise ValueError("max_new_tokens must be >= 0")
     if not prompts_ids:
@@ -113,7 +123,8 @@ def generate_batched(model, prompts_ids, max_new_tokens, pool, alloc, block_size
     if max_new_tokens == 0:
         return [[] for _ in prompts_ids]
     with _Cohort(prompts_ids, block_size, alloc, _model_device(model)) as cohort:
-        return _drive(model, pool, cohort, max_new_tokens, _greedy_ids)
+        return _drive(model, pool, cohort, max_new_tokens, _greedy_ids, adapters=adapters,
+                      adapter_ids=adapter_ids)
 
 
 def _draft_tree(draft, history, limit, depth, vocab):

@@ -37,17 +37,18 @@ class DecodeStepGraph:
     each replay, `ids` holds the argmax tokens (the next step's input) and
     `logits` the step's logits [N, vocab]. `meta` is advanced by one token
     per sequence on the device by every replay (its Python-side max_kv_len is
-    not touched).
+    not touched). adapters: the rows' low-rank adapters (serving.adapters.StepAdapters),
+    fixed for the graph; their weights are read at replay time.
     """
 
-    def __init__(self, model, pool, meta, ids: torch.Tensor, warmup: int = 0):
+    def __init__(self, model, pool, meta, ids: torch.Tensor, warmup: int = 0, adapters=None):
         if not ids.is_cuda or ids.dtype != torch.long or ids.dim() != 1:
             raise ValueError("ids must be a 1-D int64 device tensor")
         if ids.shape[0] != meta.num_tokens or not meta.is_decode:
             raise ValueError("DecodeStepGraph needs a decode batch: one token per sequence")
         if getattr(pool, "debug", False):
             raise ValueError("KVPool debug checks synchronise the host; disable them to capture")
-        self.model, self.pool, self.meta = model, pool, meta
+        self.model, self.pool, self.meta, self.adapters = model, pool, meta, adapters
         self.ids = ids.clone()
         self.logits = None
         self.workspace = _native.Workspace()
@@ -66,7 +67,7 @@ class DecodeStepGraph:
                 self.logits = self._step()
 
     def _step(self):
-        logits = self.model.forward_step(self.ids, self.pool, self.meta)
+        logits = self.model.forward_step(self.ids, self.pool, self.meta, self.adapters)
         fused_ops.argmax_rows(logits, out=self.ids)
         self.meta.advance_()
         return logits

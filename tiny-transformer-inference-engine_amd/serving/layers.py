@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import fused_ops
+from . import adapters, fused_ops
 
 
 class RoPE(nn.Module):
@@ -132,6 +132,23 @@ class SwiGLU(nn.Module):
         h = fused_ops.linear_swiglu_rmsnorm(x, attr(norm, "weight"), norm.eps, w, b)
         down = attr(self, "down_proj")
         return fused_ops.linear_residual_(x, h, attr(down, "weight"), attr(down, "bias"))
+
+
+    def forward_adapted_residual_(self, x, norm, weights, plan):
+        """forward_residual_ with low-rank adapters (serving.adapters): weights holds
+        those of the "gate_up" and "down" projections, either may be missing."""
+        w, b = self._gate_up.get()
+        attr = fused_ops.module_attr
+        h = fused_ops.rms_norm(x, attr(norm, "weight"), norm.eps)
+        if "gate_up" in weights:
+            h = adapters.adapter_swiglu(fused_ops.linear(h, w, b), h, weights["gate_up"], plan)
+        else:
+            h = fused_ops.linear_swiglu(h, w, b)
+        down = attr(self, "down_proj")
+        fused_ops.linear_residual_(x, h, attr(down, "weight"), attr(down, "bias"))
+        if "down" in weights:
+            adapters.adapter_add(x, h, weights["down"], plan, out=x)
+        return x
 
 
 fused_ops.PLAIN_MODULES.update((RoPE, RMSNorm, SwiGLU))

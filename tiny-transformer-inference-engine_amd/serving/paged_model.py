@@ -12,6 +12,7 @@ import torch
 import torch.nn as nn
 
 from . import fused_ops
+from .adapters import step_adapters
 from .layers import ModelConfig, RMSNorm, SwiGLU, TokenEmbedding
 from .paged_meta import pack_batch_meta
 from .paged_mqa import MQA_Paged
@@ -57,16 +58,23 @@ class PagedTransformer(nn.Module):
         return self.lm_head(self.final_norm(x))
 
     @torch.no_grad()
-    def forward_batch(self, batch, pool):
+    def forward_batch(self, batch, pool, adapters=None, adapter_ids=None):
         """Ragged batch step (reference: paged_model.py:50-67): logits of each
-        sequence's last new token, [num_seqs, vocab]."""
+        sequence's last new token, [num_seqs, vocab]. adapters: an AdapterSet
+        (serving.adapters), adapter_ids one index of it a sequence, -1 for none."""
         T = batch.input_ids.numel()
         meta = pack_batch_meta(batch.block_tables, batch.query_start_loc, batch.positions,
                                T, batch.input_ids.device, pool.block_size)
-        return self.forward_step(batch.input_ids, pool, meta)
+        step = None
+        if adapter_ids is not None and any(i != -1 for i in adapter_ids):
+            if adapters is None:
+                raise ValueError("forward_batch: adapter_ids needs an AdapterSet")
+            step = step_adapters(adapters, adapter_ids, batch.query_start_loc,
+                                 batch.input_ids.device)
+        return self.forward_step(batch.input_ids, pool, meta, step)
 
     @torch.no_grad()
-    def forward_step(self, input_ids, pool, meta):
+    def forward_step(self, input_ids, pool, meta, adapters=None):
         """forward_batch with pre-packed metadata (PagedBatchMeta). With lengths
         from the device (build_batch_meta) input_ids has num_tokens rows, those
         behind the last token of any value, and a sequence without a token gets
@@ -78,9 +86,15 @@ class PagedTransformer(nn.Module):
         and one attention call: norm + qkv GEMM + RoPE, append + attention,
         out GEMM + add, norm + gate/up GEMM + SwiGLU gate, down GEMM + add.
         The arithmetic is that of PagedBlock.forward_meta: each sum is
-        rounded to the model dtype before it is normalised or carried on."""
+        rounded to the model dtype before it is normalised or carried on.
+
+        adapters: the rows' low-rank adapters (StepAdapters, on a ROCm device). The
+        norms, RoPE and the gate then run beside the projections, with the same
+        rounded values for rows without an adapter."""
         x = self.embedding(input_ids)
         if not x.is_cuda:
+            if adapters is not None:
+                raise RuntimeError("adapters require the model on a ROCm GPU device")
             for layer in self.layers:
                 x = layer.forward_meta(x, pool, meta)
             last = meta.query_start_loc[1:].long() - 1
@@ -89,10 +103,17 @@ class PagedTransformer(nn.Module):
             return x.new_zeros((meta.num_seqs, self.lm_head.out_features))
         x = x.contiguous()
         attr = fused_ops.module_attr
-        for layer in self.layers:
-            attr(layer, "attn").forward_meta_residual_(x, attr(layer, "attn_norm"), pool,
-                                                       layer.layer_idx, meta)
-            attr(layer, "mlp").forward_residual_(x, attr(layer, "mlp_norm"))
+        for i, layer in enumerate(self.layers):
+            attn, mlp = attr(layer, "attn"), attr(layer, "mlp")
+            if adapters is None:
+                attn.forward_meta_residual_(x, attr(layer, "attn_norm"), pool, layer.layer_idx,
+                                            meta)
+                mlp.forward_residual_(x, attr(layer, "mlp_norm"))
+            else:
+                weights = adapters.weights.layers[i]
+                attn.forward_adapted_residual_(x, attr(layer, "attn_norm"), pool,
+                                               layer.layer_idx, meta, weights, adapters.plan)
+                mlp.forward_adapted_residual_(x, attr(layer, "mlp_norm"), weights, adapters.plan)
         if not meta.exact:
             return self._logits_of_last(x, meta.query_start_loc)
         if not meta.is_decode:

@@ -19,6 +19,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from .adapters import adapter_add
 from .fake_paged_attn import paged_attention_append_meta, paged_attention_meta
 from . import fused_ops
 from .fused_ops import FusedRows
@@ -119,6 +120,28 @@ class MQA_Paged(nn.Module):
         proj = attr(self, "out")
         return fused_ops.linear_residual_(x, out.view(T, d_model), attr(proj, "weight"),
                                           attr(proj, "bias"))
+
+    def forward_adapted_residual_(self, x, norm, pool, layer_idx, meta: PagedBatchMeta, weights,
+                                  plan):
+        """forward_meta_residual_ with low-rank adapters (serving.adapters): weights
+        holds those of the "qkv" and "out" projections, either may be missing. A row
+        without an adapter is computed as forward_meta_residual_'s separate calls do."""
+        T, d_model = x.shape
+        w, b = self._qkv.get()
+        attr = fused_ops.module_attr
+        cos, sin = attr(self, "rope")._tables_fp32()
+        h = fused_ops.rms_norm(x, attr(norm, "weight"), norm.eps)
+        qkv = fused_ops.linear(h, w, b)
+        if "qkv" in weights:
+            adapter_add(qkv, h, weights["qkv"], plan, out=qkv)
+        nq, nk = self.num_heads * self.headdim, self.num_kv_heads * self.headdim
+        q, k, v = fused_ops.rope(qkv[:, :nq], qkv[:, nq:nq + nk], meta.positions, cos, sin,
+                                 v=qkv[:, nq + nk:], hq=self.num_heads, hkv=self.num_kv_heads,
+                                 d=self.headdim)
+        out = paged_attention_append_meta(q, k, v, pool, layer_idx, meta).view(T, d_model)
+        proj = attr(self, "out")
+        fused_ops.linear_residual_(x, out, attr(proj, "weight"), attr(proj, "bias"))
+        return adapter_add(x, out, weights["out"], plan, out=x) if "out" in weights else x
 
     def forward_tree_residual_(self, x, norm, pool, layer_idx, tree, k_rows, v_rows,
                                status=None):

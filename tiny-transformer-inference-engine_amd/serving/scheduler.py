@@ -36,6 +36,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 from .batch import BatchStep, build_batch_step
+from .controls import RequestParams, TokenHistory, draw_tokens
 from .sampling import sample
 from .sequence import Sequence, blocks_for
 
@@ -49,6 +50,8 @@ class _Request:
     max_new_tokens: int
     generated: int = 0
     seq_id: int | None = None
+    params: RequestParams | None = None
+    asked_len: int = 0  # tokens of the prompt as it was asked
 
 
 @dataclass
@@ -59,7 +62,7 @@ class _Running:
 
 class Scheduler:
     def __init__(self, model, pool, alloc, cfg, block_size=16,
-                 temperature=1.0, top_k=32, top_p=0.9, sched_cfg=None):
+                 temperature=1.0, top_k=32, top_p=0.9, sched_cfg=None, adapters=None):
         self.model = model
         self.pool = pool
         self.alloc = alloc
@@ -70,6 +73,8 @@ class Scheduler:
         self.top_p = top_p
         self.device = next(model.parameters()).device
         self.sched_cfg = sched_cfg
+        self.adapters = adapters  # AdapterSet that the requests' params name
+        self._history: TokenHistory | None = None
         self.waiting: list[_Request] = []
         self.running: list[Sequence] = []
         self._state: dict[int, _Running] = {}  # seq_id -> state of a running sequence
@@ -79,7 +84,14 @@ class Scheduler:
 
     # ---- requests ---------------------------------------------------------
 
-    def add_request(self, prompt_ids, max_new_tokens):
+    def add_request(self, prompt_ids, max_new_tokens, params=None):
+        """params (controls.RequestParams): the request's own sampling parameters,
+        penalties, biases, grammar and adapter, on a ROCm device; without it the
+        scheduler's temperature, top_k and top_p."""
+        if params is not None and params.adapter != -1 and not (
+                self.adapters is not None
+                and 0 <= params.adapter < self.adapters.num_adapters):
+            raise ValueError(f"the scheduler has no adapter {params.adapter}")
         if self.sched_cfg is not None:
             sc = self.sched_cfg
             # without chunking a recomputed (preempted) request is prefilled whole,
@@ -94,7 +106,8 @@ class Scheduler:
             if need + 1 > self.alloc.num_usable:
                 raise ValueError(f"request needs {need} blocks; the pool has "
                                  f"{self.alloc.num_usable} usable")
-        self.waiting.append(_Request(list(prompt_ids), max_new_tokens))
+        self.waiting.append(_Request(list(prompt_ids), max_new_tokens, params=params,
+                                     asked_len=len(prompt_ids)))
 
     def computed_tokens(self, seq: Sequence) -> int:
         """Tokens of a running sequence whose K/V are in the pool."""
@@ -116,22 +129,54 @@ class Scheduler:
         seq.ensure_blocks(self.alloc)
         self.running.append(seq)
         self._state[seq.seq_id] = _Running(req)
+        if req.params is not None and req.params.has_penalties:
+            if self._history is None:
+                self._history = TokenHistory(self.device)
+            self._history.put(seq.seq_id, seq.token_ids, req.asked_len)
         return seq
 
     def _finish(self, seq: Sequence) -> None:
         seq.release(self.alloc)
         del self._state[seq.seq_id]
+        if self._history is not None:
+            self._history.drop(seq.seq_id)
+
+    def _forward(self, batch, seqs):
+        params = [self._state[seq.seq_id].req.params for seq in seqs]
+        ids = [-1 if p is None else p.adapter for p in params]
+        if all(i == -1 for i in ids):
+            return self.model.forward_batch(batch, self.pool)
+        return self.model.forward_batch(batch, self.pool, self.adapters, ids)
 
     def _pick(self, row):
         return int(sample(row.unsqueeze(0), self.temperature, self.top_k, self.top_p))
 
-    def _sampled(self, seq: Sequence, row):
-        """Sample the next token of a sequence whose tokens are all computed;
-        returns (token, done)."""
-        tok = self._pick(row)
+    def _draws(self, seqs, logits, rows):
+        """The next token of every sequence in seqs, whose tokens are all computed, from
+        row rows[i] of logits: those with parameters of their own by one draw together,
+        the others each by the scheduler's."""
+        own = [i for i, seq in enumerate(seqs) if self._state[seq.seq_id].req.params is not None]
+        toks = [None] * len(seqs)
+        if own:
+            at = [rows[i] for i in own]
+            picked, _ = draw_tokens(logits if at == list(range(len(logits))) else logits[at],
+                                    [self._state[seqs[i].seq_id].req.params for i in own],
+                                    self._history, [seqs[i].seq_id for i in own])
+            for i, tok in zip(own, picked):
+                toks[i] = tok
+        return [self._pick(logits[r]) if t is None else t for r, t in zip(rows, toks)]
+
+    def _sampled(self, seq: Sequence, tok):
+        """The sequence takes tok; returns whether it is done."""
         req = self._state[seq.seq_id].req
         req.generated += 1
-        return tok, tok == self.cfg.eos_token_id or req.generated >= req.max_new_tokens
+        done = tok == self.cfg.eos_token_id or req.generated >= req.max_new_tokens
+        if req.params is not None and not done:
+            if req.params.has_penalties:
+                self._history.append(seq.seq_id, tok)
+            if req.params.grammar is not None:
+                req.params.grammar.advance(tok)
+        return done
 
     # ---- a step -----------------------------------------------------------
 
@@ -146,12 +191,13 @@ class Scheduler:
         if not self.running:
             return []
         batch = [(seq, seq.token_ids[self._state[seq.seq_id].computed:]) for seq in self.running]
-        logits = self.model.forward_batch(build_batch_step(batch, self.device), self.pool)
+        logits = self._forward(build_batch_step(batch, self.device), self.running)
 
+        toks = self._draws(self.running, logits, range(len(self.running)))
         results, kept = [], []
-        for i, seq in enumerate(self.running):
+        for seq, tok in zip(self.running, toks):
             self._state[seq.seq_id].computed = seq.num_tokens
-            tok, done = self._sampled(seq, logits[i])
+            done = self._sampled(seq, tok)
             results.append((seq.seq_id, tok, done))
             if done:
                 self._finish(seq)
@@ -223,14 +269,17 @@ class Scheduler:
                           query_start_loc=qsl, block_tables=[seq.block_table for seq, _, _ in plan],
                           seq_lens=[b for _, _, b in plan])
         self.last_batch_tokens = len(ids)
-        logits = self.model.forward_batch(batch, self.pool)
+        logits = self._forward(batch, [seq for seq, _, _ in plan])
 
         results = []
-        for i, (seq, _, b) in enumerate(plan):
+        # a prefill chunk that does not finish its prompt samples nothing
+        whole = [i for i, (seq, _, b) in enumerate(plan) if b == seq.num_tokens]
+        drawn = [plan[i][0] for i in whole]
+        toks = self._draws(drawn, logits, whole)
+        for seq, _, b in plan:
             self._state[seq.seq_id].computed = b
-            if b < seq.num_tokens:
-                continue  # prefill chunk: the prompt is not finished yet
-            tok, done = self._sampled(seq, logits[i])
+        for seq, tok in zip(drawn, toks):
+            done = self._sampled(seq, tok)
             results.append((seq.seq_id, tok, done))
             if done:
                 self._finish(seq)
