@@ -234,10 +234,12 @@ int launch_control(ControlArgs a, hipStream_t st) {
 // rounding moves a border by is below 2^-23 of the sum for the widest vocabulary and
 // 2^-40 for usual ones, under the spacing of the fp32 uniforms.
 //
-// A workgroup a row, passes over the row from L2 after the first: the largest logit; a
-// histogram of counts over 2048 bins of (max - l) / T (1/64 each) where top-k is asked,
-// its bin refined by the bits of the keys until one key is left; the same with weights for
-// top-p; the kept weights' sums per wavefront and round, and the place in them.
+// A workgroup a row; its passes over it are: the
+// largest logit; where top-k is asked, counts over 2048 bins of the distance to it and
+// the k-th's bin once more by the bits of its keys, until one key is left; the same with
+// weights for top-p; the kept weights' sum per wavefront, and the place in one wavefront's
+// ids (a wavefront's ids are consecutive). What binds is the weights' arithmetic: some
+// twenty 64-bit operations each, at the rate of 32-bit ones here.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
   int64_t* ids;
@@ -262,249 +264,545 @@ constexpr int kSampMaxVocab = 1 << 20;
 // rounds of a row: 1024 threads x 4 (fp32) ids each, and one for a misaligned end
 constexpr int kMaxRounds = kSampMaxVocab / (kSampThreads * 4) + 1;
 constexpr double kOne = 8796093022208.0;  // 2^43: the weight of the largest logit
-constexpr double kFar = 31.0;             // exp(-31) 2^43 < 1/2: weight 0
+// Distances to the largest logit count in 1 / kStep octaves of the weight; from kFar on
+// (44 octaves, where a weight is half a unit) all weights are 0.
+constexpr int kStep = 4096, kStepBits = 12;
+constexpr double kFar = 44.0 * kStep;
+// 32 bins an octave, 2048 in all
+constexpr int kBinShift = kStepBits - 5;
+
+// A wavefront's part of the list of values that can be kept; with it the workgroup takes
+// 155 KB of a CU's 160.
+constexpr int kListCap = 768;
 
 struct SampShared {
-  unsigned count[kBins];
+  u32x4 edge[3];
+  int listed[kSampWaves];
+  double pow[kStep];  // 2^43 2^(-j / kStep)
   u64 mass[kBins];
-  u64 sums[kMaxRounds * kSampWaves];
+  unsigned count[kBins];
   u64 wsum[kSampWaves];
-  float wmax[kSampWaves];
-  int warg[kSampWaves];
+  u64 rsum[kMaxRounds];
   u64 found[3];
   int at[2];
-  unsigned kmin, kmax;
+  float list_value[kSampWaves][kListCap];
+  int list_id[kSampWaves][kListCap];
 };
 
-__device__ __forceinline__ unsigned sort_key(float x) {
-  const unsigned b = __float_as_uint(x + 0.f);  // -0 and 0 are one value
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+// Keys in the order of the values, as short as the type (fp32 values of 16-bit ones end
+// in zeros).
+template <typename T>
+struct Key {
+  static constexpr int kDrop = sizeof(T) == 4 ? 0 : __is_same(T, f16) ? 13 : 16;
+  static constexpr unsigned kTop = ~0u >> kDrop;
+  static __device__ __forceinline__ unsigned of(float x) {
+    const unsigned b = __float_as_uint(x + 0.f);  // -0 and 0 are one value
+    return (b ^ (unsigned)((int)b >> 31 | (int)0x80000000)) >> kDrop;
+  }
+  static __device__ __forceinline__ float value(unsigned k) {
+    const unsigned b = k << kDrop;
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~(b | ((1u << kDrop) - 1)));
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ float piece_value(u32x4 v, int j) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(v[j]);
+  else if constexpr (__is_same(T, bf16))
+    return __uint_as_float(j & 1 ? v[j / 2] & 0xffff0000u : v[j / 2] << 16);
+  else
+    return (float)__builtin_bit_cast(f16, (unsigned short)(j & 1 ? v[j / 2] >> 16 : v[j / 2]));
 }
-__device__ __forceinline__ float key_value(unsigned k) {
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
+
+// A row of logits: wavefront w has the pieces w * rounds * 64 ..., lane l the l-th of each
+// 64. Every pass reads them again (from L2, a round ahead), so that any vocabulary takes
+// the same short code. Places outside the row hold -infinity, whose weight is 0.
+__device__ const u32x4 kNoPiece[1] = {};
 
 template <typename T>
 struct Row {
+  static constexpr int E = kPiece<T>;
   const T* p;
   int vocab;
-  int mis;
   int rounds;
-  // f(value, id, round) for every id of this thread
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    constexpr int E = kPiece<T>;
-    for (int k = 0; k < rounds; ++k) {
-      const int id0 = (k * kSampThreads + (int)threadIdx.x) * E - mis;
-      T v[E];
-      if (id0 < vocab) load_piece(p, id0, vocab, (T)-INFINITY, v);
+  int first, last;  // ids at which the first and the last piece inside the row begin
+  const T* from;    // what read() reads
+  int from_first, from_last;
+
+  __device__ __forceinline__ Row(const T* row, int n) : p(row), vocab(n) {
+    const int mis = misaligned(row);
+    rounds = (n + mis + kSampThreads * E - 1) / (kSampThreads * E);
+    first = mis ? E - mis : 0;
+    last = (n + mis) / E * E - mis - E;
+    const bool some = first <= last;
+    from = some ? row : reinterpret_cast<const T*>(kNoPiece);
+    from_first = some ? first : 0;
+    from_last = some ? last : 0;
+  }
+  __device__ __forceinline__ int first_id(int w, int k) const {
+    return ((w * rounds + k) * 64 + (int)(threadIdx.x & 63)) * E - (first ? E - first : 0);
+  }
+  // The piece at id0; for one that is not all inside the row some piece that is (or any
+  // 16 bytes, where the row holds none), without a branch before the load, and whole()
+  // puts it right.
+  __device__ __forceinline__ u32x4 read(int id0) const {
+    return *reinterpret_cast<const u32x4*>(from + min(max(id0, from_first), from_last));
+  }
+  // The pieces over the row's ends, as edge[0] and edge[1], and edge[2] behind it.
+  __device__ __forceinline__ void edges(u32x4* edge) const {
+    const int i = threadIdx.x;
+    if (i < 3 * E) {
+      const int id = i < E ? first - E + i : i < 2 * E ? max(last, first - E) + i : -1;
+      reinterpret_cast<T*>(edge)[i] = (unsigned)id < (unsigned)vocab ? p[id] : (T)-INFINITY;
+    }
+  }
+  __device__ __forceinline__ u32x4 whole(u32x4 v, int id0, const u32x4* edge) const {
+    if (id0 < first || id0 > last)
+      v = edge[id0 < first ? 0 : id0 == max(last, first - E) + E ? 1 : 2];
+    return v;
+  }
+  static __device__ __forceinline__ void values(u32x4 v, float (&x)[E]) {
 #pragma unroll
-      for (int j = 0; j < E; ++j)
-        if ((unsigned)(id0 + j) < (unsigned)vocab) f((float)v[j], id0 + j, k);
+    for (int j = 0; j < E; ++j) x[j] = piece_value<T>(v, j);
+  }
+  // Round k of wavefront w: this lane's values and the first one's id.
+  __device__ __forceinline__ void get(const SampShared& s, int w, int k, float (&x)[E],
+                                      int& id0) const {
+    id0 = first_id(w, k);
+    values(whole(read(id0), id0, s.edge), x);
+  }
+  __device__ __forceinline__ int rounds_of(const SampShared&, int) const { return rounds; }
+  // f(values, first id) for every piece of this thread, kAhead rounds in flight (each in
+  // registers of its own: handing them on would wait for them)
+  static constexpr int kAhead = 2;
+  template <typename F>
+  __device__ __forceinline__ void each(const SampShared& s, F f) const {
+    const int w = threadIdx.x >> 6;
+    u32x4 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) v[i] = read(first_id(w, i));
+#pragma nounroll
+    for (int k = 0; k < rounds; k += kAhead) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        if (k + i >= rounds) break;
+        const int id0 = first_id(w, k + i);
+        float x[E];
+        values(whole(v[i], id0, s.edge), x);
+        v[i] = read(first_id(w, k + i + kAhead));  // past the end: some piece inside
+        f(x, id0);
+      }
     }
   }
 };
 
-__device__ __forceinline__ u64 wave_sum(u64 x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
-}
-__device__ __forceinline__ u64 wave_prefix(u64 x) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 y = __shfl_up(x, d);
-    if (lane >= d) x += y;
+// The values of a row that can still be kept, in LDS: what Row is for all of them.
+struct List {
+  static constexpr int E = 1;
+  __device__ __forceinline__ void get(const SampShared& s, int w, int k, float (&x)[1],
+                                      int& id0) const {
+    const int i = 64 * k + (threadIdx.x & 63);
+    const bool in = i < s.listed[w];
+    x[0] = in ? s.list_value[w][i] : -INFINITY;
+    id0 = in ? s.list_id[w][i] : -1;
   }
-  return x;
-}
+  __device__ __forceinline__ int rounds_of(const SampShared& s, int w) const {
+    return (s.listed[w] + 63) / 64;
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(const SampShared& s, F f) const {
+    const int w = threadIdx.x >> 6;
+    const int n = rounds_of(s, w);
+    for (int k = 0; k < n; ++k) {
+      float x[1];
+      int id0;
+      get(s, w, k, x, id0);
+      f(x, id0);
+    }
+  }
+};
 
-// The first entry of v [n] at which the inclusive prefix sum exceeds target; found[0] is
-// that entry, found[1] the sum before it, found[2] the entry itself. found[0] = n: none.
+// x of another lane by VALU data movement: the DPP control CTRL on the rows of RM, 0 for
+// lanes it gives nothing.
+template <int CTRL, int RM>
+__device__ __forceinline__ u64 lanes(u64 x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, RM, 0xF, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, RM, 0xF, true);
+  return (u64)(unsigned)hi << 32 | (unsigned)lo;
+}
+// op over lanes 0 ... l for lane l (all lanes active), 0 being op's neutral value: row
+// shifts by 1, 2, 4, 8, then the last lane of each row of 16 and of each half handed on. The
+// same by LDS permutes waits some ten times as long.
+template <typename Op>
+__device__ __forceinline__ u64 wave_scan(u64 x, Op op) {
+  x = op(x, lanes<0x111, 0xF>(x));
+  x = op(x, lanes<0x112, 0xF>(x));
+  x = op(x, lanes<0x114, 0xF>(x));
+  x = op(x, lanes<0x118, 0xF>(x));
+  x = op(x, lanes<0x142, 0xA>(x));
+  return op(x, lanes<0x143, 0xC>(x));
+}
+__device__ __forceinline__ u64 last_lane(u64 x) {
+  return (u64)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 |
+         (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+}
+__device__ __forceinline__ u64 wave_prefix(u64 x) {
+  return wave_scan(x, [](u64 p, u64 q) { return p + q; });
+}
+__device__ __forceinline__ u64 wave_sum(u64 x) { return last_lane(wave_prefix(x)); }
+
+// The first of the n <= kBins entries of v at which the inclusive prefix sum exceeds
+// target: found[0] is that entry (n: none), found[1] the sum before it, found[2] itself.
 template <typename V>
 __device__ void find_prefix(const V* v, int n, u64 target, SampShared& s) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (tid == 0) s.found[0] = n, s.found[1] = 0, s.found[2] = 0;
-  u64 carry = 0;
-  for (int base = 0; base < n; base += kSampThreads) {
-    const int i = base + tid;
-    const u64 x = i < n ? (u64)v[i] : 0;
-    const u64 inc = wave_prefix(x);
-    __syncthreads();
+  const int i = 2 * tid;
+  const u64 x0 = i < n ? (u64)v[i] : 0, x1 = i + 1 < n ? (u64)v[i + 1] : 0;
+  u64 before = 0;
+  if (n > 128) {
+    const u64 inc = wave_prefix(x0 + x1);
+    if (tid == 0) s.found[0] = n, s.found[1] = 0, s.found[2] = 0;
     if (lane == 63) s.wsum[w] = inc;
     __syncthreads();
-    u64 before = carry;
-    for (int j = 0; j < kSampWaves; ++j) {
-      before += j < w ? s.wsum[j] : 0;
-      carry += s.wsum[j];
-    }
-    const u64 upto = before + inc;
-    if (i < n && upto > target && upto - x <= target)
-      s.found[0] = i, s.found[1] = upto - x, s.found[2] = x;
+    for (int j = 0; j < kSampWaves; ++j) before += j < w ? s.wsum[j] : 0;
+    before += inc - x0 - x1;
+  } else {  // one wavefront's entries
+    if (tid == 0) s.found[0] = n, s.found[1] = 0, s.found[2] = 0;
+    if (w == 0) before = wave_prefix(x0 + x1) - x0 - x1;
+    __builtin_amdgcn_wave_barrier();
   }
+  if (before <= target && target < before + x0)
+    s.found[0] = i, s.found[1] = before, s.found[2] = x0;
+  else if (before + x0 <= target && target < before + x0 + x1)
+    s.found[0] = i + 1, s.found[1] = before + x0, s.found[2] = x1;
   __syncthreads();
 }
 
 template <typename T>
 struct Sampler {
   SampShared& s;
-  Row<T> row;
-  float top;       // the largest logit
-  double inv_t;
-  float inv_t_bin; // 64 / T: bins of 1/64
+  double top;    // the largest logit
+  double steps;  // steps of distance for one of logits
 
-  // The weight of x, 0 where it is below `least` of the largest.
-  __device__ __forceinline__ u64 mass(float x, double least = 0.) const {
-    const double z = ((double)top - (double)x) * inv_t;
-    if (!(z < kFar)) return 0;
-    const double e = exp(-z);
-    return e < least ? 0 : (u64)rint(e * kOne);
+  __device__ __forceinline__ double distance(float x) const { return (top - (double)x) * steps; }
+  // The whole steps of a distance below 2^31, rounded: adding 3 2^51 leaves them in the
+  // low bits, at the rate of an addition (a conversion runs at a quarter of it).
+  static constexpr double kShift = 6755399441055744.;
+  // 2^43 2^(-z / kStep) for a distance z of at most 60 octaves, and the steps n of z: the
+  // whole steps from the table and by the exponent, the rest r, at most half a step, as a
+  // polynomial whose next term is below 2^-43.
+  __device__ __forceinline__ double weight(double z, int& n) const {
+    constexpr double c = 0.69314718055994530942 / kStep;
+    const double y = z + kShift;
+    n = __double2loint(y);
+    const double r = z - (y - kShift);
+    const double q = fma(r, fma(r, c * c / 2., -c), 1.);
+    const double t = s.pow[n & (kStep - 1)] * q;
+    return __hiloint2double(__double2hiint(t) - ((n >> kStepBits) << 20), __double2loint(t));
   }
-  __device__ __forceinline__ int bin(float x) const {
-    return (int)fminf((top - x) * inv_t_bin, (float)(kBins - 1));
+  // The nearest whole number to w < 2^52 in the low 52 bits, under the bits kUnit.
+  static constexpr u64 kUnit = 0x4330000000000000ull;
+  static __device__ __forceinline__ u64 unit_bits(double w) {
+    return __builtin_bit_cast(u64, w + 4503599627370496.);
   }
-  __device__ __forceinline__ void clear() {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kSampThreads) s.count[i] = 0, s.mass[i] = 0;
-    __syncthreads();
+  // The weight of x, under kUnit. No branches, so that those of a piece are computed side
+  // by side; two octaves past kFar 1/8 rounds to 0.
+  __device__ __forceinline__ u64 mass_bits(float x, int& bin) const {
+    int n;
+    const u64 e = unit_bits(weight(fmin(distance(x), kFar + 2. * kStep), n));
+    bin = n >> kBinShift;
+    return e;
+  }
+  __device__ __forceinline__ u64 mass(float x, int& bin) const { return mass_bits(x, bin) - kUnit; }
+  // Bins of counts (weights have their steps).
+  __device__ __forceinline__ int count_bin(float x) const {
+    return (int)fminf(((float)top - x) * (float)steps, (float)((kBins << kBinShift) - 1)) >> kBinShift;
   }
 
-  // The key in bin b at which the sum of weights (by_mass: masses, else counts) of the
-  // bin's larger keys and its own exceeds rest; `before` the sum of the larger keys,
-  // `own` that of the key. Only ids with key >= floor count.
-  __device__ unsigned refine(int b, u64 rest, bool by_mass, unsigned floor, u64& before, u64& own) {
-    if (threadIdx.x == 0) s.kmin = ~0u, s.kmax = 0;
-    __syncthreads();
-    row.each([&](float x, int, int) {
-      const unsigned k = sort_key(x);
-      if (k >= floor && bin(x) == b) {
-        if (k < s.kmin) atomicMin(&s.kmin, k);
-        if (k > s.kmax) atomicMax(&s.kmax, k);
+  // Keys around bin b: its ends as values (a step more), and some for their rounding.
+  __device__ __forceinline__ void around(int b, unsigned& k0, unsigned& k1) const {
+    const double at0 = top - ((b << kBinShift) - 1) / steps;
+    const double at1 = top - (((b + 1) << kBinShift) + 1) / steps;
+    const unsigned hi = Key<T>::of((float)(T)(float)at0), lo = Key<T>::of((float)(T)(float)at1);
+    k1 = min(hi < Key<T>::kTop - 4 ? hi + 4 : Key<T>::kTop, Key<T>::of((float)top));
+    const unsigned least = Key<T>::of(-INFINITY);  // below it are no numbers
+    k0 = b == kBins - 1 || lo < least + 4 ? least : lo - 4;
+  }
+
+  // The values of at least `from` into the list; false where they are too many for it.
+  __device__ bool list_up(const Row<T>& row, float from) {
+    constexpr int E = Row<T>::E;
+    const int w = threadIdx.x >> 6;
+    int n = 0;
+    row.each(s, [&](const float (&x)[E], int id0) {
+      if (n > kListCap) return;
+      int c = 0;
+#pragma unroll
+      for (int j = 0; j < E; ++j) c += x[j] >= from;
+      if (__ballot(c != 0) == 0) return;
+      const int upto = (int)wave_prefix((u64)c);
+      int at = n + upto - c;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        if (x[j] >= from) {
+          if (at < kListCap) s.list_value[w][at] = x[j], s.list_id[w][at] = id0 + j;
+          ++at;
+        }
       }
+      n += __builtin_amdgcn_readlane(upto, 63);
     });
-    __syncthreads();
-    unsigned k0 = s.kmin, k1 = s.kmax;
+    if ((threadIdx.x & 63) == 0) s.listed[w] = n;
+    return !__syncthreads_or(n > kListCap);
+  }
+
+  // The value in bin b at which the sum of weights (by_mass: masses, else counts) of the
+  // bin's larger values and its own exceeds rest; `before` the sum of the larger ones,
+  // `own` that of the value. Only values of at least `floor` count.
+  template <bool by_mass, typename S>
+  __device__ float refine(const S& src, int b, u64 rest, float floor, u64& before, u64& own) {
+    unsigned k0, k1;
+    around(b, k0, k1);
+    k0 = max(k0, Key<T>::of(floor));
     before = 0;
     for (;;) {
-      const int bits = k1 == k0 ? 0 : 32 - __clz(k1 - k0);
+      const int bits = k1 <= k0 ? 0 : 32 - __clz(k1 - k0);
       const int shift = max(0, bits - 11);
-      clear();
-      row.each([&](float x, int, int) {
-        const unsigned k = sort_key(x);
-        if (k >= floor && k >= k0 && k <= k1 && bin(x) == b) {
-          const int at = (k1 - k) >> shift;  // descending
-          if (by_mass) atomicAdd(&s.mass[at], mass(x));
-          else atomicAdd(&s.count[at], 1u);
+      const int n = k1 <= k0 ? 1 : (int)((k1 - k0) >> shift) + 1;
+      __syncthreads();
+      for (int i = threadIdx.x; i < n; i += kSampThreads) {
+        if constexpr (by_mass) s.mass[i] = 0;
+        else s.count[i] = 0;
+      }
+      __syncthreads();
+      const float v0 = Key<T>::value(k0), v1 = Key<T>::value(k1);
+      src.each(s, [&](const float (&x)[S::E], int) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < S::E; ++j) any |= x[j] >= v0 && x[j] <= v1;
+        if (!any) return;
+        for (int j = 0; j < S::E; ++j) {
+          if (!(x[j] >= v0 && x[j] <= v1)) continue;
+          const int at = (k1 - Key<T>::of(x[j])) >> shift;  // descending
+          if constexpr (by_mass) {
+            int bin;
+            const u64 e = mass(x[j], bin);
+            if (bin == b) atomicAdd(&s.mass[at], e);
+          } else {
+            if (count_bin(x[j]) == b) atomicAdd(&s.count[at], 1u);
+          }
         }
       });
       __syncthreads();
-      if (by_mass) find_prefix(s.mass, kBins, rest - before, s);
-      else find_prefix(s.count, kBins, rest - before, s);
+      if constexpr (by_mass) find_prefix(s.mass, n, rest - before, s);
+      else find_prefix(s.count, n, rest - before, s);
       const unsigned i = (unsigned)s.found[0];
       before += s.found[1];
       own = s.found[2];
-      __syncthreads();
-      if (i >= kBins) return k0;  // only where the row changed under the call
-      const unsigned top_of = k1 - (i << shift);
-      if (shift == 0) return top_of;
-      const unsigned low = top_of - ((1u << shift) - 1);
-      k0 = low > k1 ? k0 : max(k0, low);  // the last bin may reach below 0
-      k1 = top_of;
+      if (i >= (unsigned)n) return v0;  // only where the row changed under the call
+      k1 -= i << shift;
+      if (shift == 0) return Key<T>::value(k1);
+      const unsigned span = (1u << shift) - 1;
+      k0 = k1 - k0 > span ? k1 - span : k0;  // the last bin may be short
     }
   }
 
-  // The first id at which the cumulative weight exceeds target; f(value, id) the weight.
-  template <typename F>
-  __device__ int locate(u64 target, F f) {
-    find_prefix(s.sums, row.rounds * kSampWaves, target, s);
-    const int e = (int)s.found[0];
-    const u64 rest = target - s.found[1];
-    if (threadIdx.x == 0) s.at[0] = -1;
+  // top-p over the values of at least `floor`, from the sums by bin in s.mass and their
+  // total: the smallest value kept and the last id of its ties that is.
+  template <typename S>
+  __device__ void nucleus(const S& src, int b, u64 rest, float floor, float& cut, int& cut_id) {
+    u64 before, own;
+    cut = refine<true>(src, b, rest, floor, before, own);
+    int bin;
+    const u64 each = max(mass(cut, bin), (u64)1);
+    const u64 kept = (rest - before) / each + 1;  // ids of the last value
+    if (kept * each < own) {
+      const float c = cut;
+      auto tie = [=](const float (&x)[S::E], int, u64 (&n)[S::E]) {
+#pragma unroll
+        for (int j = 0; j < S::E; ++j) n[j] = kUnit + (x[j] == c);
+        return true;
+      };
+      sum_up(src, tie);
+      cut_id = locate(src, kept - 1, tie);
+    }
+  }
+
+  // The sums of the weights of at least `near` by bin in s.mass (cleared before), and the
+  // total of those of at least `floor`: atomics for the few that can matter.
+  template <typename S>
+  __device__ u64 histogram(const S& src, float floor, float near) {
+    u64 sum = 0;
+    src.each(s, [&](const float (&x)[S::E], int) {
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < S::E; ++j) any |= x[j] >= floor;
+      if (!any) return;
+      u64 e[S::E];
+      int at[S::E];
+#pragma unroll
+      for (int j = 0; j < S::E; ++j) {
+        e[j] = mass_bits(x[j] >= floor ? x[j] : -INFINITY, at[j]);
+        sum += e[j];
+      }
+      sum -= S::E * kUnit;  // modulo 2^64
+#pragma unroll
+      for (int j = 0; j < S::E; ++j)
+        if (x[j] >= near && e[j] != kUnit) atomicAdd(&s.mass[at[j]], e[j] - kUnit);
+    });
+    sum = wave_sum(sum);
     __syncthreads();
-    const int k = e / kSampWaves, w = e % kSampWaves;
-    if ((int)(threadIdx.x >> 6) == w && k < row.rounds) {
-      constexpr int E = kPiece<T>;
-      const int id0 = (k * kSampThreads + (int)threadIdx.x) * E - row.mis;
-      T v[E];
-      if (id0 < row.vocab) load_piece(row.p, id0, row.vocab, (T)-INFINITY, v);
-      u64 m[E], sum = 0;
+    if ((threadIdx.x & 63) == 0) s.wsum[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    const u64 all = total();
+    __syncthreads();
+    return all;
+  }
+
+  // The draw: the first kept id at which the cumulative weight exceeds u times the sum.
+  template <typename S>
+  __device__ u64 draw(const S& src, float cut, int cut_id, double u) {
+    auto kept = [&](const float (&x)[S::E], int id0, u64 (&e)[S::E]) {
+      bool any = false;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        m[j] = (unsigned)(id0 + j) < (unsigned)row.vocab ? f((float)v[j], id0 + j) : 0;
-        sum += m[j];
+      for (int j = 0; j < S::E; ++j) any |= x[j] >= cut;
+      if (!any) return false;
+      float y[S::E];
+#pragma unroll
+      for (int j = 0; j < S::E; ++j) y[j] = x[j] >= cut ? x[j] : -INFINITY;
+      if (cut_id != 0x7fffffff) {
+#pragma unroll
+        for (int j = 0; j < S::E; ++j)
+          if (x[j] == cut && id0 + j > cut_id) y[j] = -INFINITY;
       }
-      u64 c = wave_prefix(sum) - sum;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        if (m[j] && c <= rest && c + m[j] > rest) {
-          s.at[0] = id0 + j;
-          s.at[1] = __float_as_int((float)v[j]);
+      for (int j = 0; j < S::E; ++j) {
+        int bin;
+        e[j] = mass_bits(y[j], bin);
+      }
+      return true;
+    };
+    sum_up(src, kept);
+    const u64 all = total();
+    locate(src, (u64)(u * (double)all), kept);
+    return all;
+  }
+
+  // The sums of f's weights by wavefront, for total() and locate(): f(values, first id,
+  // weights) gives a piece's weights, each under kUnit.
+  template <typename S, typename F>
+  __device__ void sum_up(const S& src, F f) {
+    u64 sum = 0;
+    src.each(s, [&](const float (&x)[S::E], int id0) {
+      u64 m[S::E];
+      if (!f(x, id0, m)) return;
+#pragma unroll
+      for (int j = 0; j < S::E; ++j) sum += m[j];
+      sum -= S::E * kUnit;  // modulo 2^64
+    });
+    sum = wave_sum(sum);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wsum[threadIdx.x >> 6] = sum;
+    __syncthreads();
+  }
+  __device__ u64 total() const {
+    u64 t = 0;
+    for (int j = 0; j < kSampWaves; ++j) t += s.wsum[j];
+    return t;
+  }
+  // After sum_up(f): the first id at which the cumulative sum exceeds target, in at[0]
+  // (-1: none), its value in at[1]. The wavefronts share the rounds of the one it is in.
+  template <typename S, typename F>
+  __device__ int locate(const S& src, u64 target, F f) {
+    constexpr int E = S::E;
+    const int w = threadIdx.x >> 6;
+    u64 rest = target;
+    int mine = 0;
+    while (mine < kSampWaves && rest >= s.wsum[mine]) rest -= s.wsum[mine++];
+    if (threadIdx.x == 0) s.at[0] = -1;
+    if (mine == kSampWaves) mine = 0, rest = ~0ull;  // only where the row changed
+    const int rounds = src.rounds_of(s, mine);
+    // first the sums of the rounds, then the one that the place is in
+    int k = w, end = rounds;
+#pragma nounroll
+    for (int turn = 0; turn < 2; ++turn) {
+#pragma nounroll
+      for (; k < end; k += kSampWaves) {
+        float x[E];
+        u64 m[E], sum = 0;
+        int id0;
+        src.get(s, mine, k, x, id0);
+        const bool some = f(x, id0, m);
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum += m[j] = some ? m[j] - kUnit : 0;
+        const u64 upto = wave_prefix(sum);
+        if (turn == 0) {
+          if ((threadIdx.x & 63) == 63) s.rsum[k] = upto;
+        } else {
+          u64 c = upto - sum;
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            if (c <= rest && c + m[j] > rest) {
+              s.at[0] = id0 + j;
+              s.at[1] = __float_as_int(x[j]);
+            }
+            c += m[j];
+          }
         }
-        c += m[j];
       }
+      if (turn == 1) break;
+      __syncthreads();
+      k = 0;
+      while (k < rounds && rest >= s.rsum[k]) rest -= s.rsum[k++];
+      end = k < rounds && w == k % kSampWaves ? k + 1 : 0;
     }
     __syncthreads();
     return s.at[0];
-  }
-
-  // The sums of f over this row's rounds and wavefronts, for locate().
-  template <typename F>
-  __device__ void sum_up(F f) {
-    constexpr int E = kPiece<T>;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    __syncthreads();
-    for (int k = 0; k < row.rounds; ++k) {
-      const int id0 = (k * kSampThreads + (int)threadIdx.x) * E - row.mis;
-      T v[E];
-      if (id0 < row.vocab) load_piece(row.p, id0, row.vocab, (T)-INFINITY, v);
-      u64 sum = 0;
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if ((unsigned)(id0 + j) < (unsigned)row.vocab) sum += f((float)v[j], id0 + j);
-      sum = wave_sum(sum);
-      if (lane == 0) s.sums[k * kSampWaves + w] = sum;
-    }
-    __syncthreads();
   }
 };
 
 template <typename T>
 __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a) {
-  __shared__ SampShared s;
-  constexpr int E = kPiece<T>;
+  extern __shared__ __attribute__((aligned(16))) char samp_lds[];
+  SampShared& s = *reinterpret_cast<SampShared*>(samp_lds);
   const int r = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  Row<T> row;
-  row.p = static_cast<const T*>(a.logits) + (int64_t)r * a.stride;
-  row.vocab = a.vocab;
-  row.mis = misaligned(row.p);
-  row.rounds = (a.vocab + row.mis + kSampThreads * E - 1) / (kSampThreads * E);
-
-  // the largest logit, its first id, and whether all are numbers below infinity
-  float best = -INFINITY;
-  int arg = 0x7fffffff;
-  int bad = 0;
-  row.each([&](float x, int id, int) {
-    if (!(x < INFINITY)) bad = 1;
-    if (x > best) best = x, arg = id;
-  });
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const float x = __shfl_xor(best, d);
-    const int i = __shfl_xor(arg, d);
-    if (x > best || (x == best && i < arg)) best = x, arg = i;
-  }
-  if (lane == 0) s.wmax[w] = best, s.warg[w] = arg;
-  bad = __syncthreads_or(bad);
-  for (int j = 0; j < kSampWaves; ++j)
-    if (s.wmax[j] > best || (s.wmax[j] == best && s.warg[j] < arg)) best = s.wmax[j], arg = s.warg[j];
-
+  constexpr int E = kPiece<T>;
+  const Row<T> row(static_cast<const T*>(a.logits) + (int64_t)r * a.stride, a.vocab);
+  row.edges(s.edge);
   const float temp = a.temperature[r];
   const int top_k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.f;
   const float min_p = a.min_p ? a.min_p[r] : 0.f;
   const float u = a.uniforms[r];
+  {
+    static_assert(kStep == 4 * kSampThreads, "four entries a thread");
+    const double e = kOne * exp2(-(double)tid / kStep);  // and 2^(-1/4), 2^(-1/2), 2^(-3/4) of it
+    s.pow[tid] = e;
+    s.pow[tid + kSampThreads] = e * 0.84089641525371454303;
+    s.pow[tid + 2 * kSampThreads] = e * 0.70710678118654752440;
+    s.pow[tid + 3 * kSampThreads] = e * 0.59460355750136053336;
+  }
+  for (int i = tid; i < kBins; i += kSampThreads) s.count[i] = 0, s.mass[i] = 0;
+
+  __syncthreads();
+
+  // the largest logit, and whether all are numbers below infinity
+  float best = -INFINITY;
+  bool bad = false;
+  row.each(s, [&](const float (&x)[E], int) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      bad |= !(x[j] < INFINITY);
+      best = fmaxf(best, x[j]);
+    }
+  });
+  auto larger = [](u64 p, u64 q) { return p > q ? p : q; };
+  u64 key = last_lane(wave_scan((u64)Key<float>::of(best), larger));
+  if (lane == 0) s.wsum[w] = key;
+  bad = __syncthreads_or(bad);
+  for (int j = 0; j < kSampWaves; ++j) key = larger(key, s.wsum[j]);
+  best = Key<float>::value((unsigned)key);
+
   int err = 0;
   if (!(temp >= 0.f && temp < INFINITY) || top_k < 0 || !(top_p > 0.f) ||
       !(min_p >= 0.f && min_p <= 1.f) || !(u >= 0.f && u < 1.f))
@@ -513,86 +811,120 @@ __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a)
     err = PKV_STATUS_NONFINITE;
   else if (best == -INFINITY)
     err = PKV_STATUS_BAD_DISTRIBUTION;
-  if (err || temp == 0.f) {
+  if (err) {
     if (tid == 0) {
-      a.ids[r] = err ? -1 : arg;
-      if (a.logprobs) a.logprobs[r] = err ? NAN : 0.f;
-      if (err && a.status) atomicOr(a.status, err);
+      a.ids[r] = -1;
+      if (a.logprobs) a.logprobs[r] = NAN;
+      if (a.status) atomicOr(a.status, err);
+    }
+    return;
+  }
+  if (temp == 0.f) {  // its first id
+    u64 near = 0;
+    row.each(s, [&](const float (&x)[E], int id0) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (x[j] == best) near = larger(near, (u64)(unsigned)~(id0 + j));
+    });
+    near = last_lane(wave_scan(near, larger));
+    __syncthreads();
+    if (lane == 0) s.wsum[w] = near;
+    __syncthreads();
+    for (int j = 0; j < kSampWaves; ++j) near = larger(near, s.wsum[j]);
+    if (tid == 0) {
+      a.ids[r] = (int)~(unsigned)near;
+      if (a.logprobs) a.logprobs[r] = 0.f;
     }
     return;
   }
 
-  // a finite factor: the largest logit is in bin 0 at any temperature
-  Sampler<T> m{s, row, best, 1.0 / (double)temp, fminf(64.f / temp, 1e30f)};
-  unsigned floor = 0;  // keys below it are out
+  constexpr double kLog2e = 1.4426950408889634074;
+  Sampler<T> m{s, (double)best, kLog2e * kStep / (double)temp};
+  // min-p as the smallest value it keeps: near max + T log(min_p), the lanes try the keys
+  // around it. Below half a unit it drops nothing that weighs.
+  float min_cut = -INFINITY;
+  const double least = (double)min_p * kOne;
+  if (least >= 0.5) {
+    const float about = (float)(T)(float)((double)best + log((double)min_p) * (double)temp);
+    const unsigned none = Key<T>::of(-INFINITY), k = Key<T>::of(about);
+    const unsigned first = k < none + 32 ? none : k - 32;
+    int n;
+    const float x = Key<T>::value(min(first + lane, Key<T>::of(INFINITY)));
+    const double z = fmin(fmax(m.distance(x), 0.), kFar + 2. * kStep);
+    const uint64_t in = __ballot(x >= best || m.weight(z, n) >= least);
+    min_cut = __shfl(x, in ? __ffsll((unsigned long long)in) - 1 : 63);
+  }
+  const List list;
+  bool listed = false;     // what can be kept is in the list
+  float cut = -INFINITY;   // values below it are out, and so are its own ids behind cut_id
+  int cut_id = 0x7fffffff;
+  unsigned k0, k1;
   if (top_k > 0 && top_k < a.vocab) {
-    m.clear();
-    row.each([&](float x, int, int) { atomicAdd(&s.count[m.bin(x)], 1u); });
+    row.each(s, [&](const float (&x)[E], int) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) atomicAdd(&s.count[m.count_bin(x[j])], 1u);
+    });
     __syncthreads();
     find_prefix(s.count, kBins, (u64)top_k - 1, s);
     const int b = (int)s.found[0];
     const u64 rest = (u64)top_k - 1 - s.found[1];
-    __syncthreads();
-    // the last bin's weights are 0: a threshold in it keeps all that can be drawn
-    if (b < kBins - 1) {
-      u64 before, own;
-      floor = m.refine(b, rest, false, 0, before, own);
-    }
+    m.around(b, k0, k1);
+    listed = m.list_up(row, Key<T>::value(k0));
+    u64 before, own;
+    cut = listed ? m.template refine<false>(list, b, rest, -INFINITY, before, own)
+                 : m.template refine<false>(row, b, rest, -INFINITY, before, own);
   }
-  unsigned cut_key = floor;     // keys above it are kept, and its own ids up to cut_id
-  int cut_id = 0x7fffffff;
   if (top_p < 1.f) {
-    m.clear();
-    u64 sum = 0;
-    row.each([&](float x, int, int) {
-      if (sort_key(x) >= floor) {
-        const u64 e = m.mass(x);
-        if (e) atomicAdd(&s.mass[m.bin(x)], e);
-        sum += e;
-      }
-    });
-    sum = wave_sum(sum);
-    __syncthreads();
-    if (lane == 0) s.wsum[w] = sum;
-    __syncthreads();
-    u64 total = 0;
-    for (int j = 0; j < kSampWaves; ++j) total += s.wsum[j];
-    __syncthreads();
-    // kept: a sum before of at most p * total
-    const u64 most = (u64)((double)top_p * (double)total);
-    if (most < total) {
+    // Most borders are within 16 octaves of the largest, a border below min-p's does not
+    // matter; only where neither holds are the weights of all values binned.
+    float near = fmaxf(min_cut, (float)((double)best - 16. * kStep / m.steps));
+    u64 all = listed ? m.histogram(list, cut, near) : m.histogram(row, cut, near);
+    // kept: a sum before of at most p times all
+    const u64 most = (u64)((double)top_p * (double)all);
+    if (most < all) {
       find_prefix(s.mass, kBins, most, s);
+      if (s.found[0] == kBins && near > min_cut) {
+        __syncthreads();
+        for (int i = tid; i < kBins; i += kSampThreads) s.mass[i] = 0;
+        __syncthreads();
+        if (listed) m.histogram(list, cut, min_cut);
+        else m.histogram(row, cut, min_cut);
+        find_prefix(s.mass, kBins, most, s);
+      }
       const int b = (int)s.found[0];
       const u64 rest = most - s.found[1];
-      __syncthreads();
-      u64 before, own;
-      cut_key = m.refine(b, rest, true, floor, before, own);
-      const u64 each = m.mass(key_value(cut_key));
-      const u64 kept = (rest - before) / each + 1;  // ids of the last key
-      if (kept * each < own) {
-        auto tie = [&](float x, int) -> u64 { return sort_key(x) == cut_key; };
-        m.sum_up(tie);
-        cut_id = m.locate(kept - 1, tie);
+      if (b < kBins) {
+        if (!listed) {
+          m.around(b, k0, k1);
+          listed = m.list_up(row, fmaxf(Key<T>::value(k0), cut));
+        }
+        const float floor = cut;
+        if (listed) m.nucleus(list, b, rest, floor, cut, cut_id);
+        else m.nucleus(row, b, rest, floor, cut, cut_id);
       }
     }
   }
-  const double least = (double)min_p;
-  auto kept = [&](float x, int id) -> u64 {
-    const unsigned k = sort_key(x);
-    return k < cut_key || (k == cut_key && id > cut_id) ? 0 : m.mass(x, least);
-  };
-  m.sum_up(kept);
-  u64 total = 0;
-  for (int i = lane; i < row.rounds * kSampWaves; i += 64) total += s.sums[i];
-  total = wave_sum(total);
-  const int id = m.locate((u64)((double)u * (double)total), kept);
+  if (min_cut > cut) {
+    cut = min_cut;
+    cut_id = 0x7fffffff;
+    if (!listed) listed = m.list_up(row, cut);
+  }
+  const u64 all = listed ? m.draw(list, cut, cut_id, (double)u) : m.draw(row, cut, cut_id, (double)u);
   if (tid == 0) {
-    a.ids[r] = id;
+    a.ids[r] = s.at[0];
     if (a.logprobs) {
-      const double z = ((double)best - (double)__int_as_float(s.at[1])) * m.inv_t;
-      a.logprobs[r] = (float)(-z - log((double)total / kOne));
+      const double z = ((double)best - (double)__int_as_float(s.at[1])) / (double)temp;
+      a.logprobs[r] = (float)(-z - log((double)all / kOne));
     }
   }
+}
+
+template <typename T>
+int launch_sample(const SampleArgs& a, int64_t rows, hipStream_t st) {
+  const int rc = allow_lds(reinterpret_cast<const void*>(sample_each_kernel<T>), sizeof(SampShared));
+  if (rc) return rc;
+  sample_each_kernel<T><<<(unsigned)rows, kSampThreads, sizeof(SampShared), st>>>(a);
+  return check_launch("sample_each");
 }
 
 bool ok_dtype(int dtype) {
@@ -675,10 +1007,9 @@ int pkv_sample_each(int64_t* ids, float* logprobs, const void* logits, int64_t r
   const SampleArgs a{ids,   logprobs, logits, row_stride, (int)vocab, temperature,
                      top_k, top_p,    min_p,  uniforms,   status};
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == PKV_DTYPE_F32) sample_each_kernel<float><<<(unsigned)rows, kSampThreads, 0, st>>>(a);
-  else if (dtype == PKV_DTYPE_F16) sample_each_kernel<f16><<<(unsigned)rows, kSampThreads, 0, st>>>(a);
-  else sample_each_kernel<bf16><<<(unsigned)rows, kSampThreads, 0, st>>>(a);
-  return check_launch("sample_each");
+  if (dtype == PKV_DTYPE_F32) return launch_sample<float>(a, rows, st);
+  if (dtype == PKV_DTYPE_F16) return launch_sample<f16>(a, rows, st);
+  return launch_sample<bf16>(a, rows, st);
 }
 
 }  // extern "C"
