@@ -662,38 +662,39 @@ int pkv_write_accepted_step(void* k_pool, void* v_pool, int64_t pool_layer_elems
  * starts [n_adapters + 2]: the first place of each adapter's rows, of those without
  * one, and n_tokens. tiles [max_tiles][4] (16-byte aligned): pieces of at most tile_rows
  * (16 or 64) rows of one adapter, as {adapter or -1, first place, rows, 0}, unused
- * entries with 0 rows; max_tiles at least n_tokens / tile_rows + min(n_adapters + 1,
- * n_tokens). At most 1000 adapters and 2^24 rows.
+ * entries with 0 rows; rows [max_tiles][tile_rows]: the tiles' rows, the last one
+ * repeated; max_tiles at least n_tokens / tile_rows + min(n_adapters + 1, n_tokens). At most 1000 adapters and 2^24 rows.
  */
-int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int max_tiles,
-                     const int32_t* ids, int n_tokens, int n_adapters, int tile_rows,
+int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int32_t* rows,
+                     int max_tiles, const int32_t* ids, int n_tokens, int n_adapters, int tile_rows,
                      int* status, void* stream);
 
 /*
- * Workspace bytes of pkv_adapter_apply for a step of n_tokens rows whose plan has
- * max_tiles tiles, k features in and `ranks` ranks of all parts together. It needs
- * no initial state; calls in flight together need different memory.
+ * Workspace bytes of pkv_adapter_apply for a step of n_tokens rows. It needs no
+ * initial state; calls in flight together need different memory.
  */
-size_t pkv_adapter_workspace_bytes(int n_tokens, int max_tiles, int k, int ranks);
+size_t pkv_adapter_workspace_bytes(int n_tokens, int max_tiles, int tile_rows, int k, int rank,
+                                   int parts);
 
 /*
  * Low-rank adapters beside a (fused) projection (no counterpart in the reference).
  * base [n_tokens, n] is the projection's output, n = the sum of the features n0 ...
- * of its 1 to 4 parts. With row t's adapter i of the plan (order, tiles):
+ * of its 1 to 4 parts. With row t's adapter i of the plan (tiles, rows):
  *   y[t] = base[t] + scales[i] * b[i] (a[i] x[t])
- * where a [n_adapters, parts * rank, k] (rows a_stride elements apart, a multiple of 8,
+ * where a [n_adapters, parts * rank, k] (rows a_stride elements apart, a multiple of 32,
  * zeros behind k) and b [n_adapters, n, rank]; the features of part s use the ranks
  * s * rank ... (s + 1) * rank - 1. Rows without an adapter get y = base. All sums
  * are fp32, also a[i] x[t], and y is rounded once. PKV_EPILOGUE_NONE: out [n_tokens, n] =
  * y; out may be base itself (same address and stride). PKV_EPILOGUE_SWIGLU: two parts,
  * out [n_tokens, n0] = silu(y of part 0) * y of part 1, rounded once. Except for that
  * one case out shares no memory with an operand. rank is a multiple of 8 up to 128
- * (PKV_ERR_UNSUPPORTED); any k, n and strides of rows; a, b 16-byte aligned.
+ * (PKV_ERR_UNSUPPORTED), max_tiles at most 65535; any k, n and strides of rows; a, b
+ * 16-byte aligned.
  */
 int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t base_stride,
                       const void* x, int64_t x_stride, const void* a, int64_t a_stride,
-                      const void* b, const float* scales, const int32_t* order,
-                      const int32_t* tiles, int max_tiles, int tile_rows, int n_tokens,
+                      const void* b, const float* scales, const int32_t* tiles,
+                      const int32_t* rows, int max_tiles, int tile_rows, int n_tokens,
                       int n_adapters, int k, int rank, int parts, int n0, int n1, int n2, int n3,
                       int epilogue, int dtype, void* workspace, size_t workspace_bytes,
                       void* stream);

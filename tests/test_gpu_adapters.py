@@ -43,6 +43,10 @@ def check_plan(ids, n):
     got = plan.tiles.tolist()
     assert got[:len(tiles)] == tiles
     assert all(t[2] == 0 for t in got[len(tiles):])
+    rows = plan.rows.tolist()
+    for (_, first, n_rows, _), places in zip(tiles, rows):
+        want = order[first:first + n_rows]
+        assert places == want + want[-1:] * (plan.tile_rows - n_rows)
     return plan
 
 

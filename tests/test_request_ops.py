@@ -14,37 +14,39 @@ from serving.controls import LogitControls, control_logits, sample_each
 def test_plan_refusals():
     L = _native.lib()
 
-    def plan(order=16, starts=16, tiles=16, max_tiles=8, ids=16, T=4, n=3, rows=16):
-        return L.pkv_adapter_plan(order, starts, tiles, max_tiles, ids, T, n, rows, None, None)
+    def plan(order=16, starts=16, tiles=16, places=16, max_tiles=8, ids=16, T=4, n=3, rows=16):
+        return L.pkv_adapter_plan(order, starts, tiles, places, max_tiles, ids, T, n, rows, None,
+                                  None)
 
     assert plan(T=-1) == -1 and plan(n=-1) == -1 and plan(rows=32) == -1
     assert plan(max_tiles=3) == -1 and b"max_tiles" in L.pkv_last_error()
     assert plan(ids=None) == -1 and plan(order=None) == -1 and plan(starts=None) == -1
+    assert plan(places=None) == -1
     assert plan(tiles=8) == -1 and b"aligned" in L.pkv_last_error()
     assert plan(n=1001, max_tiles=2000) == -2
 
 
 def test_apply_refusals():
     L = _native.lib()
-    good = dict(out=16, os=16, base=32, bs=16, x=48, xs=32, a=64, astr=32, b=80, sc=16, order=16,
-                tiles=16, mt=4, rows=16, T=4, N=2, k=32, r=8, parts=1, n0=16, n1=0, n2=0, n3=0,
+    good = dict(out=16, os=16, base=32, bs=16, x=48, xs=32, a=64, astr=32, b=80, sc=16, tiles=16,
+                places=16, mt=4, rows=16, T=4, N=2, k=32, r=8, parts=1, n0=16, n1=0, n2=0, n3=0,
                 epi=0, dt=0, ws=16, wsb=1 << 20)
 
     def apply(**kw):
         return L.pkv_adapter_apply(*{**good, **kw}.values(), None)
 
     for kw in (dict(dt=7), dict(epi=2), dict(T=-1), dict(parts=0), dict(parts=5), dict(n0=0),
-               dict(k=0), dict(r=0), dict(rows=8), dict(astr=24), dict(astr=36), dict(os=15),
+               dict(k=0), dict(r=0), dict(rows=8), dict(astr=31), dict(astr=40), dict(os=15),
                dict(bs=15), dict(xs=31), dict(out=None), dict(x=None), dict(a=None),
-               dict(order=None), dict(sc=None), dict(a=65), dict(tiles=24), dict(epi=1),
-               dict(epi=1, parts=2, n1=17, bs=40), dict(ws=24), dict(mt=1 << 28),
+               dict(places=None), dict(sc=None), dict(a=65), dict(tiles=24), dict(epi=1),
+               dict(epi=1, parts=2, n1=17, bs=40), dict(ws=24),
                dict(epi=1, parts=2, n1=16, bs=32, out=32)):
         assert apply(**kw) == -1, kw
-    assert apply(r=12) == -2 and apply(r=136) == -2
+    assert apply(r=12) == -2 and apply(r=136) == -2 and apply(mt=65536) == -2
     assert apply(ws=None) == -3 and apply(wsb=64) == -3
     assert apply(T=0) == 0 and apply(mt=0) == 0  # nothing to do
-    assert L.pkv_adapter_workspace_bytes(0, 4, 32, 8) == 0
-    assert L.pkv_adapter_workspace_bytes(4, 4, 32, 8) >= 4 * 8 * 4
+    assert L.pkv_adapter_workspace_bytes(0, 4, 16, 32, 8, 1) == 0
+    assert L.pkv_adapter_workspace_bytes(4, 4, 16, 32, 8, 1) >= 4 * 8 * 4
 
 
 def test_control_and_draw_refusals():

@@ -5,15 +5,16 @@
 // features of part s use ranks s R ... (s + 1) R - 1. Three kernels:
 //   adapter_plan_kernel  once a step: rows sorted by adapter and cut into tiles of
 //                        one adapter (all layers and projections share it);
-//   adapter_down_kernel  t = A x per tile, fp32 partial sums over pieces of k;
-//   adapter_up_kernel    sums the partials, scales, multiplies by B and writes
-//                        base + product, or silu(gate) * up of the two sums.
+//   adapter_down_kernel  t = scale A x per tile;
+//   adapter_up_kernel    multiplies by B and writes base + product, or silu(gate) * up
+//                        of the two sums.
 // The ranks are few, so both products are far below the ridge of the matrix cores
 // and the bytes bind: the used adapters' A and B for a decode step, the
 // activations for prompts.
 #include "mfma_decode_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace pkv {
 namespace {
@@ -23,6 +24,7 @@ using namespace mfma;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kMaxAdapters = 1000;  // a counter per wavefront and adapter in 64 KiB of LDS
+constexpr int kBatch = 8;           // rounds of a plan's pass
 constexpr int kMaxSlices = 4;
 
 // ---------------------------------------------------------------------------
@@ -37,6 +39,7 @@ struct PlanArgs {
   int32_t* order;   // [T]
   int32_t* starts;  // [N + 2]
   int4* tiles;      // [max_tiles]: adapter (-1: none), first place in order, rows
+  int32_t* rows;    // [max_tiles][tile_rows]: the tiles' rows, the last one repeated
   int max_tiles;
   const int32_t* ids;
   int T;
@@ -79,11 +82,38 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
   const int per = ((a.T + kPlanWaves - 1) / kPlanWaves + 63) & ~63;
   const int t0 = min(w * per, a.T), t1 = min(t0 + per, a.T);
   auto group = [&](int id) { return (unsigned)id < (unsigned)a.N ? id : a.N; };
-  for (int t = t0 + lane; t < t1; t += 64) {
-    const int id = a.ids[t];
-    if (id < -1 || id >= a.N) bad = PKV_STATUS_BAD_CONTROL;
-    atomicAdd(&cnt[w * G + group(id)], 1);
-  }
+  // f(row or -1, its group, the lanes of the same group) for the wavefront's rows, 64 at a
+  // time; the ids of kBatch rounds are requested together
+  auto each = [&](auto f) {
+    for (int base = t0; base < t1; base += 64 * kBatch) {
+      int id[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) id[i] = a.ids[min(base + 64 * i + lane, a.T - 1)];
+#pragma nounroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (base + 64 * i >= t1) break;
+        const int t = base + 64 * i + lane;
+        const bool in = t < t1;
+        const int g = in ? group(id[0]) : G;  // G: no group of a row
+        uint64_t same = __ballot(g == __builtin_amdgcn_readfirstlane(g));
+        if (same != ~0ull) {  // rows of a prompt mostly are of one group
+          same = ~0ull;
+          for (int bit = 1; bit <= G; bit <<= 1) {
+            const uint64_t set = __ballot((g & bit) != 0);
+            same &= (g & bit) ? set : ~set;
+          }
+        }
+        f(in ? t : -1, id[0], g, same);
+#pragma unroll
+        for (int k = 0; k + 1 < kBatch; ++k) id[k] = id[k + 1];
+      }
+    }
+  };
+  each([&](int t, int id, int g, uint64_t same) {
+    if (t >= 0 && (id < -1 || id >= a.N)) bad = PKV_STATUS_BAD_CONTROL;
+    if (t >= 0 && lane == __ffsll((unsigned long long)same) - 1)
+      atomicAdd(&cnt[w * G + g], __popcll(same));
+  });
   __syncthreads();
   int mine = 0;  // rows of group tid
   if (tid < G)
@@ -92,15 +122,10 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
   const int start = plan_scan(mine, sh, total);
   const int ntiles = (mine + a.tile_rows - 1) / a.tile_rows;
   const int tile0 = plan_scan(ntiles, sh, total);
+  __shared__ int first_row[kMaxAdapters + 2], first_tile[kMaxAdapters + 2];
   if (tid < G) {
-    a.starts[tid] = start;
-    if (tid == a.N) a.starts[G] = a.T;
-    for (int j = 0; j < ntiles; ++j) {
-      const int first = j * a.tile_rows;
-      if (tile0 + j < a.max_tiles)
-        a.tiles[tile0 + j] = make_int4(tid < a.N ? tid : -1, start + first,
-                                       min(a.tile_rows, mine - first), 0);
-    }
+    a.starts[tid] = first_row[tid] = start;
+    first_tile[tid] = tile0;
     int run = start;
     for (int i = 0; i < kPlanWaves; ++i) {
       const int c = cnt[i * G + tid];
@@ -108,22 +133,40 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
       run += c;
     }
   }
-  for (int i = total + tid; i < a.max_tiles; i += kPlanThreads) a.tiles[i] = make_int4(-1, 0, 0, 0);
+  if (tid == 0) {
+    a.starts[G] = first_row[G] = a.T;
+    first_tile[G] = total;
+  }
   __syncthreads();
-  for (int base = t0; base < t1; base += 64) {
-    const int t = base + lane;
-    const bool in = t < t1;
-    const int g = in ? group(a.ids[t]) : G;  // G: no group of a row
-    uint64_t same = ~0ull;                   // the lanes of this lane's group
-    for (int bit = 1; bit <= G; bit <<= 1) {
-      const uint64_t set = __ballot((g & bit) != 0);
-      same &= (g & bit) ? set : ~set;
-    }
+  const int rows_log = a.tile_rows == 16 ? 4 : 6;
+  each([&](int t, int, int g, uint64_t same) {
     const int leader = __ffsll((unsigned long long)same) - 1;
     int at = 0;
-    if (in && lane == leader) at = atomicAdd(&cnt[w * G + g], __popcll(same));
+    if (t >= 0 && lane == leader) at = atomicAdd(&cnt[w * G + g], __popcll(same));
     at = __shfl(at, leader);
-    if (in) a.order[at + __popcll(same & ((1ull << lane) - 1))] = t;
+    if (t >= 0) {
+      at += __popcll(same & ((1ull << lane) - 1));
+      a.order[at] = t;
+      const int place = at - first_row[g], tile = first_tile[g] + (place >> rows_log);
+      if (tile < a.max_tiles) {
+        int32_t* rows = a.rows + (int64_t)tile * a.tile_rows;
+        const int i = place & (a.tile_rows - 1);
+        rows[i] = t;
+        if (at + 1 == first_row[g + 1])  // the group's last row fills its last tile
+          for (int j = i + 1; j < a.tile_rows; ++j) rows[j] = t;
+      }
+    }
+  });
+  for (int i = tid; i < a.max_tiles; i += kPlanThreads) {
+    int lo = 0, hi = G;  // the last group whose first tile is at most i
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first_tile[mid] <= i) lo = mid; else hi = mid - 1;
+    }
+    const int first = first_row[min(lo, G)] + (i - first_tile[lo]) * a.tile_rows;
+    a.tiles[i] = i < total ? make_int4(lo < a.N ? lo : -1, first,
+                                       min(a.tile_rows, first_row[lo + 1] - first), 0)
+                           : make_int4(-1, 0, 0, 0);
   }
   if (tid == 0 && bad && a.status) atomicOr(a.status, bad);
 }
@@ -141,36 +184,51 @@ struct ApplyArgs {
   const void* a;        // [N, SR, ka]
   const void* b;        // [N, n, R]
   const float* scales;  // [N]
-  const int32_t* order;
   const int4* tiles;
+  const int32_t* rows;  // [max_tiles][tile_rows]
+  int tile_rows;
   int T;
   int N;
   int k;
-  int ka;   // pitch of A's rows: k rounded up to 8, zeros behind k
-  int R;    // ranks a part, a multiple of 8
+  int ka;      // pitch of A's rows: k rounded up to 32 at least, zeros behind k
+  int R;       // ranks a part, a multiple of 8
   int SR;
-  int n;    // features of all parts
+  int blocks;  // of 16 ranks, a part: t's unit
+  int n;       // features of all parts
   int slices;
   int at[kMaxSlices + 1];      // first feature of each part
   int chunk0[kMaxSlices + 1];  // first column chunk of each part
-  int ksplit;
-  int k_steps;  // 32-wide steps of k per piece
-  float* part;  // [ksplit][T][SR], rows in the plan's order
+  int pieces;   // of k
+  int k_steps;  // 32-wide steps of k a piece
+  int max_tiles;
+  float* low;   // t's sums over each piece: [pieces][T][slices * blocks][16]
   int vec;      // base and out can be moved in 16-byte pieces
-  int xvec;     // so can x
   int copy;     // out is other memory than base: rows without an adapter are copied
 };
 
-__device__ __forceinline__ bool load_tile(const ApplyArgs& a, int i, int rows_max, int4& t) {
+// The tile of workgroup b, of max_tiles and up to 7 more, which have none: each XCD, whose
+// workgroups are every eighth, gets a run of tiles, so that few adapters share its L2.
+__device__ __forceinline__ int tile_of(const ApplyArgs& a, int b) {
+  const int per = (a.max_tiles + 7) / 8;
+  return (b & 7) * per + (b >> 3);
+}
+// The tile and, in the same round trip, rows [row0, row0 + 16 MR) of it: lane l has row
+// l % 16 of each 16. False where there are none.
+template <int MR>
+__device__ __forceinline__ bool load_tile(const ApplyArgs& a, int i, int row0, int4& t,
+                                          int (&row)[MR]) {
+  if (i >= a.max_tiles) return false;
   t = a.tiles[i];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+    row[m] = a.rows[(int64_t)i * a.tile_rows + row0 + 16 * m + (threadIdx.x & 15)];
   t.x = __builtin_amdgcn_readfirstlane(t.x);
   t.y = __builtin_amdgcn_readfirstlane(t.y);
   t.z = __builtin_amdgcn_readfirstlane(t.z);
   // a plan of other sizes would lead out of bounds
-  return t.z > 0 && t.z <= rows_max && t.y >= 0 && t.y <= a.T - t.z && t.x < a.N;
-}
-__device__ __forceinline__ int tile_row(const ApplyArgs& a, const int4& t, int i) {
-  return min((unsigned)a.order[t.y + min(i, t.z - 1)], (unsigned)(a.T - 1));
+#pragma unroll
+  for (int m = 0; m < MR; ++m) row[m] = min((unsigned)row[m], (unsigned)(a.T - 1));
+  return t.z > row0 && t.z <= a.tile_rows && t.y >= 0 && t.y <= a.T - t.z && t.x < a.N;
 }
 
 template <typename T>
@@ -188,29 +246,39 @@ __device__ __forceinline__ void load8(typename Ops<T>::v8& v, const T* p) {
 constexpr int kDownWaves = 4;
 constexpr int kDownThreads = 64 * kDownWaves;
 
-// t = A x of one tile (16 MR rows), RB blocks of 16 ranks and one piece of k; the
-// wavefronts split the piece, so that each reads 16 MR rows of x and 16 RB of A once,
-// and their sums meet in LDS in a fixed order. D[rank][token]: lane l has token l % 16
-// and four consecutive ranks.
-template <typename T, int MR, int RB>
+// t = A x of one tile (16 MR rows), RB blocks of 16 ranks and one piece of k. The wavefronts
+// split the piece (each a contiguous range of its 32-wide steps, so each reads its part of
+// the rows of x and A once) and their sums meet in LDS in the wavefronts' order; the pieces'
+// are added up, in order, by whoever needs t: no workgroup waits for another and the
+// results have one order. D[rank][token]: lane l has token l % 16 and four consecutive
+// ranks. XV: x's rows are read in 16-byte pieces, all but the last step's without a
+// condition.
+template <typename T, int MR, int RB, bool XV>
 __global__ __launch_bounds__(kDownThreads) void adapter_down_kernel(ApplyArgs a) {
   using v8 = typename Ops<T>::v8;
-  __shared__ float red[2][16 * MR][16 * RB + 4];
+  constexpr int W = kDownWaves;
+  constexpr int kPitch = 16 * RB + 4;
+  __shared__ __attribute__((aligned(16))) float red[W][16][kPitch];
   int4 t;
-  if (!load_tile(a, blockIdx.x, 16 * MR, t) || t.x < 0) return;
-  const int lane = threadIdx.x & 63;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int row[MR];
+  if (!load_tile<MR>(a, tile_of(a, blockIdx.x), 0, t, row) || t.x < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const int rank0 = blockIdx.y * 16 * RB;
+  const int block0 = blockIdx.y * RB;  // of all parts' blocks
+  const int all = a.slices * a.blocks;
   const T* xp[MR];
 #pragma unroll
   for (int m = 0; m < MR; ++m)
-    xp[m] = static_cast<const T*>(a.x) + (int64_t)tile_row(a, t, 16 * m + l16) * a.x_stride;
+    xp[m] = static_cast<const T*>(a.x) + (int64_t)row[m] * a.x_stride + g * 8;
   const T* ap[RB];
 #pragma unroll
-  for (int r = 0; r < RB; ++r)
-    ap[r] = static_cast<const T*>(a.a) +
-            ((int64_t)t.x * a.SR + min(rank0 + 16 * r + l16, a.SR - 1)) * a.ka;
+  for (int r = 0; r < RB; ++r) {
+    const int b = min(block0 + r, all - 1);
+    // ranks behind the part's last read its last row, and are dropped below
+    const int rank = b / a.blocks * a.R + min(b % a.blocks * 16 + l16, a.R - 1);
+    ap[r] = static_cast<const T*>(a.a) + ((int64_t)t.x * a.SR + rank) * a.ka + g * 8;
+  }
   floatx4 acc[MR][RB];
 #pragma unroll
   for (int m = 0; m < MR; ++m)
@@ -218,28 +286,51 @@ __global__ __launch_bounds__(kDownThreads) void adapter_down_kernel(ApplyArgs a)
     for (int r = 0; r < RB; ++r) acc[m][r] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   const int steps = (a.k + 31) / 32;
-  const int s0 = blockIdx.z * a.k_steps;
-  const int s1 = min(s0 + a.k_steps, steps);
-  const int per = (s1 - s0 + kDownWaves - 1) / kDownWaves;
-  const int w0 = s0 + w * per, w1 = min(w0 + per, s1);
-  for (int s = w0; s < w1; ++s) {
-    const int kk = s * 32 + g * 8;
+  const int full = XV ? a.k / 32 : 0;  // steps that lie inside x's rows
+  const int p0 = blockIdx.z * a.k_steps, p1 = min(p0 + a.k_steps, steps);
+  const int per = (a.k_steps + W - 1) / W;
+  const int s0 = min(p0 + w * per, p1), s1 = min(s0 + per, p1);
+  // U steps whose loads are in flight together
+  constexpr int U = MR * RB == 1 ? (sizeof(T) == 2 ? 4 : 2) : (sizeof(T) == 2 ? 2 : 1);
+  int s = s0;
+  if constexpr (XV) {
+    const int e = min(s1, full);
+    auto run = [&](auto n) {
+      constexpr int N = decltype(n)::value;
+      v8 xv[N][MR], av[N][RB];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int r = 0; r < RB; ++r) load8<T>(av[i][r], ap[r] + (s + i) * 32);
+#pragma unroll
+        for (int m = 0; m < MR; ++m) load8<T>(xv[i][m], xp[m] + (s + i) * 32);
+      }
+      // the scheduler would hand each load to its product to save registers
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+          for (int r = 0; r < RB; ++r) acc[m][r] = Ops<T>::mma(av[i][r], xv[i][m], acc[m][r]);
+      s += N;
+    };
+#pragma nounroll
+    while (s + U <= e) run(std::integral_constant<int, U>{});
+#pragma nounroll
+    while (s < e) run(std::integral_constant<int, 1>{});
+  }
+#pragma nounroll
+  for (; s < s1; ++s) {
     v8 xv[MR], av[RB];
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      av[r] = v8{};
-      if (kk < a.ka) load8<T>(av[r], ap[r] + kk);
-    }
+    for (int r = 0; r < RB; ++r) load8<T>(av[r], ap[r] + s * 32);
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
       xv[m] = v8{};
-      if (a.xvec) {
-        if (kk < a.k) load8<T>(xv[m], xp[m] + kk);
-      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (kk + j < a.k) xv[m][j] = xp[m][kk + j];
-      }
+      for (int j = 0; j < 8; ++j)
+        if (s * 32 + g * 8 + j < a.k) xv[m][j] = xp[m][s * 32 + j];
     }
 #pragma unroll
     for (int m = 0; m < MR; ++m)
@@ -247,195 +338,217 @@ __global__ __launch_bounds__(kDownThreads) void adapter_down_kernel(ApplyArgs a)
       for (int r = 0; r < RB; ++r) acc[m][r] = Ops<T>::mma(av[r], xv[m], acc[m][r]);
   }
 
-  // (w0 + w2) + (w1 + w3)
-  auto put = [&](int slot) {
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-        *reinterpret_cast<floatx4*>(&red[slot][16 * m + l16][16 * r + 4 * g]) = acc[m][r];
-  };
-  auto add = [&](int slot) {
-#pragma unroll
-    for (int m = 0; m < MR; ++m)
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-        acc[m][r] += *reinterpret_cast<const floatx4*>(&red[slot][16 * m + l16][16 * r + 4 * g]);
-  };
-  if (w >= 2) put(w - 2);
-  __syncthreads();
-  if (w < 2) add(w);
-  __syncthreads();
-  if (w == 1) put(0);
-  __syncthreads();
-  if (w != 0) return;
-  add(0);
-  float* part = a.part + (int64_t)blockIdx.z * a.T * a.SR;
+  float* low = a.low + (int64_t)blockIdx.z * a.T * all * 16;
 #pragma unroll
   for (int m = 0; m < MR; ++m) {
-    const int i = 16 * m + l16;
-    if (i >= t.z) continue;
+    if (m) __syncthreads();
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const int rank = rank0 + 16 * r + 4 * g;
-      if (rank < a.SR)  // SR is a multiple of 8
-        *reinterpret_cast<floatx4*>(part + (int64_t)(t.y + i) * a.SR + rank) = acc[m][r];
+    for (int r = 0; r < RB; ++r)
+      *reinterpret_cast<floatx4*>(&red[w][l16][16 * r + 4 * g]) = acc[m][r];
+    __syncthreads();
+    for (int i = tid; i < 16 * RB * 4; i += kDownThreads) {  // four ranks each
+      const int rank = (i & 3) * 4, r = (i >> 2) % RB, tok = i / (4 * RB);
+      floatx4 v = *reinterpret_cast<const floatx4*>(&red[0][tok][16 * r + rank]);
+#pragma unroll
+      for (int q = 1; q < W; ++q)
+        v += *reinterpret_cast<const floatx4*>(&red[q][tok][16 * r + rank]);
+      const int b = block0 + r, row = 16 * m + tok;
+      if (b >= all || row >= t.z) continue;
+      if (b % a.blocks * 16 + rank >= a.R) v = floatx4{0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<floatx4*>(low + ((int64_t)(t.y + row) * all + b) * 16 + rank) = v;
     }
   }
 }
 
 constexpr int kUpWaves = 4;
 constexpr int kUpThreads = 64 * kUpWaves;
-constexpr int kUpCols = 64 * kUpWaves;  // features of a workgroup, 64 a wavefront
+constexpr int kUpCols = 64 * kUpWaves;  // features of a workgroup
 enum { kEpiAdd = 0, kEpiSwiglu = 1 };
 
-// The products with B of one tile and kUpCols features of a part (swiglu: of both
-// parts), added to base. D[feature][token]: lane l has token l % 16 and, over the four
-// MFMA of its 64 features, 8 consecutive features twice, so rows move in 16-byte pieces.
-// 16-bit types: t (fp32) is the sum of two 16-bit values, t = hi + lo to 2^-16 of t,
-// which share one MFMA of 32: k-values 0-15 are 16 ranks of hi, 16-31 the same ranks of
-// lo, both against the same B. fp16's narrow exponents are met by a power of two a row.
-template <typename T, int MR, int EPI>
+// silu(g) u by the exponential and reciprocal instructions, each within a step of fp32: a
+// third of swiglu_gate's operations, which bind a prompt's gate. Rows without an adapter
+// keep swiglu_gate, and with it the bits of the gate by itself.
+__device__ __forceinline__ float gate(float g, float u) {
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
+}
+
+// The products with B of 16 rows of a tile and, a wavefront, 64 features of a part (swiglu: of
+// both parts), added to base. First the workgroup adds up t over the P pieces of k and puts
+// it into LDS as what the products multiply: for 16-bit types the sum of two 16-bit values,
+// t = hi + lo to 2^-18 of t (bf16) or 2^-24 of the largest of 32 ranks (fp16, whose narrow
+// exponents are met by a power of two a row and 32 ranks), each a product with the same
+// operand of B. D[feature][token]: lane l has token l % 16 and, over the four products of 64
+// features, 8 consecutive features twice, so rows move in 16-byte pieces; those of base are
+// requested before t. 16 rows and 64 features a wavefront leave many wavefronts in flight,
+// which a prompt's rows need: 32 rows, or several times 64 features with the next one's rows
+// requested ahead, were slower (7400 rows, gate of 4096, rank 32: 50 us against 55 and 67-84).
+template <typename T, int P, int EPI>
 __global__ __launch_bounds__(kUpThreads) void adapter_up_kernel(ApplyArgs a) {
   using v8 = typename Ops<T>::v8;
-  constexpr bool SPLIT = sizeof(T) == 2;
   constexpr int NS = EPI == kEpiSwiglu ? 2 : 1;
-  constexpr int KR = SPLIT ? 16 : 32;  // ranks a step of 32 k-values
+  constexpr bool HALF = __is_same(T, f16);
+  constexpr bool SPLIT = sizeof(T) == 2;
   extern __shared__ __attribute__((aligned(16))) char dyn[];
   int4 t;
-  if (!load_tile(a, blockIdx.x, 16 * MR, t)) return;
+  int rows[1];
+  const int row0 = blockIdx.z * 16;
+  if (!load_tile<1>(a, blockIdx.y, row0, t, rows)) return;
   if (t.x < 0 && EPI == kEpiAdd && !a.copy) return;
+  const int row = rows[0];
   int slice = 0;
   if (EPI == kEpiAdd)
-    while (slice + 1 < a.slices && (int)blockIdx.y >= a.chunk0[slice + 1]) ++slice;
-  const int steps = (a.R + KR - 1) / KR;
-  const int pitch = steps * 32 + 16 / (int)sizeof(T);  // elements; spreads the rows over banks
-  T* const low = reinterpret_cast<T*>(dyn);            // [NS][16 MR][pitch]
-  float* const rowf = reinterpret_cast<float*>(low + NS * 16 * MR * pitch);  // [NS][16 MR]
+    while (slice + 1 < a.slices && (int)blockIdx.x >= a.chunk0[slice + 1]) ++slice;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
+  const int width = a.at[slice + 1] - a.at[slice];
+  const int c0 = ((int)blockIdx.x - a.chunk0[slice]) * kUpCols + w * 64;
+  const int f0 = c0 + g * 8, f1 = f0 + 32;  // lane's features: two runs of 8
+  const int steps = (a.R + 31) / 32;        // of 32 ranks
+  const int half = steps * 32;              // t's hi, then its lo
+  const int pitch = (SPLIT ? 2 : 1) * half + 16 / (int)sizeof(T);  // spreads the rows over the banks
+  T* const low = reinterpret_cast<T*>(dyn);                        // [NS][16][pitch]
+  float* const pow = reinterpret_cast<float*>(low + NS * 16 * pitch);  // [NS][16][steps]
 
+  T yv[NS][16];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const T* p =
+        static_cast<const T*>(a.base) + (int64_t)row * a.base_stride + a.at[slice] + s * width;
+    if (a.vec) {
+      load8<T>(*reinterpret_cast<v8*>(&yv[s][0]), p + min(f0, width - 8));
+      load8<T>(*reinterpret_cast<v8*>(&yv[s][8]), p + min(f1, width - 8));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        yv[s][j] = p[min(f0 + j, width - 1)];
+        yv[s][8 + j] = p[min(f1 + j, width - 1)];
+      }
+    }
+  }
+  // the operands of B of BB steps from c on
+  constexpr int BB = NS == 1 ? 2 : 1;
+  v8 bv[BB][NS][4];
+  auto request = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < BB; ++i) {
+      if (i && c + i >= steps) break;
+      const int r = min((c + i) * 32 + g * 8, a.R - 8);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const T* b = static_cast<const T*>(a.b) + ((int64_t)t.x * a.n + a.at[slice + s]) * a.R + r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // product j, row l16: the feature whose sum lane (l16 / 4) gets in element l16 % 4
+          const int f = c0 + (j >> 1) * 32 + (l16 >> 2) * 8 + (j & 1) * 4 + (l16 & 3);
+          load8<T>(bv[i][s][j], b + (int64_t)min(f, width - 1) * a.R);
+        }
+      }
+    }
+  };
   if (t.x >= 0) {
+    request(0);
+    const int all = a.slices * a.blocks;
     const float scale = a.scales[t.x];
-    // 16 lanes a row (they share its exponent), one rank each at a time
-    for (int r = tid >> 4; r < NS * 16 * MR; r += kUpThreads / 16) {
-      const int s = NS == 2 ? r / (16 * MR) : slice;
-      const int i = r % (16 * MR);
-      const float* p = a.part + (int64_t)(t.y + min(i, t.z - 1)) * a.SR + s * a.R;
-      auto value = [&](int c) {
-        float v = 0.f;
-        if (c < a.R && i < t.z)
-          for (int z = 0; z < a.ksplit; ++z) v += p[(int64_t)z * a.T * a.SR + c];
-        return v * scale;
-      };
-      T* row = low + r * pitch;
-      if constexpr (SPLIT) {
-        float f = 1.f;
-        if constexpr (__is_same(T, f16)) {
-          float m = 0.f;
-          for (int c = l16; c < steps * KR; c += 16) m = fmaxf(m, fabsf(value(c)));
-          m = fmaxf(m, lane_xor<1>(m));
-          m = fmaxf(m, lane_xor<2>(m));
-          m = fmaxf(m, lane_xor<4>(m));
-          m = fmaxf(m, lane_xor<8>(m));
-          // 2^e with the row's largest in [1, 2) after dividing by it; not a number or
-          // infinite stays as it is
-          const int e = (int)((__float_as_uint(m) >> 23) & 255);
-          if (e > 0 && e < 254) f = __uint_as_float((unsigned)e << 23);
-          if (l16 == 0) rowf[r] = f;
-        }
-        const float inv = 1.f / f;
-        for (int c = l16; c < steps * KR; c += 16) {
-          const float v = value(c) * inv;
-          const T hi = (T)v;
-          const float rest = v - (float)hi;
-          const int at = (c / 16) * 32 + (c & 15);
-          row[at] = hi;
-          // the rest of an infinite value is not a number: it has none
-          row[at + 16] = fabsf((float)hi) < INFINITY ? (T)rest : (T)0.f;
-        }
+    const int64_t piece = (int64_t)a.T * all * 16;
+    // four ranks a thread, 8 threads a step; t is 0 behind the last rank
+    for (int i = tid; i < NS * 16 * steps * 8; i += kUpThreads) {
+      const int q = i & 7, c = (i >> 3) % steps, r = (i >> 3) / steps;
+      const int s = r / 16, tok = min(row0 + r % 16, t.z - 1);
+      const int block = min(c * 2 + (q >> 2), a.blocks - 1);
+      const float* p =
+          a.low + ((int64_t)(t.y + tok) * all + (slice + s) * a.blocks + block) * 16 + (q & 3) * 4;
+      floatx4 z[P];
+#pragma unroll
+      for (int k = 0; k < P; ++k)
+        z[k] = *reinterpret_cast<const floatx4*>(p + min(k, a.pieces - 1) * piece);
+      floatx4 v = z[0];
+#pragma unroll
+      for (int k = 1; k < P; ++k)
+        if (k < a.pieces) v += z[k];
+      v *= scale;
+      if (c * 2 + (q >> 2) >= a.blocks) v = floatx4{0.f, 0.f, 0.f, 0.f};
+      T* to = low + r * pitch + c * 32 + q * 4;
+      if constexpr (!SPLIT) {
+        *reinterpret_cast<floatx4*>(to) = v;
       } else {
-        for (int c = l16; c < steps * KR; c += 16) row[c] = value(c);
+        if constexpr (HALF) {
+          float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+          most = fmaxf(most, lane_xor<1>(most));
+          most = fmaxf(most, lane_xor<2>(most));
+          most = fmaxf(most, lane_xor<4>(most));
+          // 2^e with the step's largest in [1, 2) after dividing by it; not where it is 0, not
+          // a number or infinite
+          const int e = (int)((__float_as_uint(most) >> 23) & 255);
+          const float f = e > 0 && e < 254 ? __uint_as_float((unsigned)e << 23) : 1.f;
+          if (q == 0) pow[r * steps + c] = f;
+          v *= 1.f / f;
+        }
+        T hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          hi[j] = (T)v[j];
+          // the rest of an infinite value is not a number: it has none
+          lo[j] = fabsf((float)hi[j]) < INFINITY ? (T)(v[j] - (float)hi[j]) : (T)0.f;
+        }
+        __builtin_memcpy(to, hi, 8);
+        __builtin_memcpy(to + half, lo, 8);
       }
     }
   }
   __syncthreads();
-
-  // this wavefront's features within its part
-  const int chunk = EPI == kEpiAdd ? (int)blockIdx.y - a.chunk0[slice] : (int)blockIdx.y;
-  const int width = a.at[slice + 1] - a.at[slice];
-  const int c0 = chunk * kUpCols + w * 64;
   if (c0 >= width) return;
-  const T* bp[NS];
+
+  floatx4 acc[NS][4];  // the sums begin with base
 #pragma unroll
   for (int s = 0; s < NS; ++s)
-    bp[s] = static_cast<const T*>(a.b) +
-            ((int64_t)max(t.x, 0) * a.n + a.at[slice + s]) * a.R;
-  // lane's features: two runs of 8
-  const int f0 = c0 + g * 8, f1 = f0 + 32;
-  for (int m = 0; m < MR; ++m) {
-    if (16 * m >= t.z) break;
-    const int i = 16 * m + l16;
-    const int row = tile_row(a, t, i);
-    const T* base = static_cast<const T*>(a.base) + (int64_t)row * a.base_stride + a.at[slice];
-    T yv[NS][16];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const T* p = base + (s ? width : 0);
-      if (a.vec) {
-        if (f0 < width) load8<T>(*reinterpret_cast<v8*>(&yv[s][0]), p + f0);
-        if (f1 < width) load8<T>(*reinterpret_cast<v8*>(&yv[s][8]), p + f1);
-      } else {
+    for (int j = 0; j < 16; ++j) acc[s][j >> 2][j & 3] = (float)yv[s][j];
+  if (t.x >= 0) {
+#pragma nounroll
+    for (int cb = 0; cb < steps; cb += BB) {
+      if (cb) request(cb);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          yv[s][j] = f0 + j < width ? p[f0 + j] : (T)0.f;
-          yv[s][8 + j] = f1 + j < width ? p[f1 + j] : (T)0.f;
+      for (int i = 0; i < BB; ++i) {
+        const int c = cb + i;
+        if (c >= steps) break;
+        if (c * 32 + g * 8 >= a.R) {  // t's 0 times what is no number is none
+#pragma unroll
+          for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bv[i][s][j] = v8{};
         }
-      }
-    }
-    floatx4 acc[NS][4];
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[s][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-    if (t.x >= 0) {
-      for (int c = 0; c < steps; ++c) {
-        const int r = SPLIT ? c * 16 + (g & 1) * 8 : c * 32 + g * 8;  // lane's first rank
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          v8 tv;
-          load8<T>(tv, low + (s * 16 * MR + i) * pitch + c * 32 + g * 8);
+          const int r = s * 16 + l16;
+          v8 hi, lo;
+          load8<T>(hi, low + r * pitch + c * 32 + g * 8);
+          if constexpr (SPLIT) load8<T>(lo, low + r * pitch + half + c * 32 + g * 8);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            // MFMA j, row l16: the feature whose sum lane (l16 / 4) gets in element l16 % 4
-            const int f = c0 + (j >> 1) * 32 + (l16 >> 2) * 8 + (j & 1) * 4 + (l16 & 3);
-            v8 bv = v8{};
-            if (r < a.R) load8<T>(bv, bp[s] + (int64_t)min(f, width - 1) * a.R + r);
-            acc[s][j] = Ops<T>::mma(bv, tv, acc[s][j]);
+            if constexpr (HALF) {
+              const floatx4 v = Ops<T>::mma(bv[i][s][j], hi, floatx4{0.f, 0.f, 0.f, 0.f});
+              acc[s][j] += Ops<T>::mma(bv[i][s][j], lo, v) * pow[r * steps + c];
+            } else {
+              acc[s][j] = Ops<T>::mma(bv[i][s][j], hi, acc[s][j]);
+              if constexpr (SPLIT) acc[s][j] = Ops<T>::mma(bv[i][s][j], lo, acc[s][j]);
+            }
           }
         }
       }
-      if constexpr (__is_same(T, f16)) {
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[s][j] *= rowf[s * 16 * MR + i];
-      }
     }
-    if (i >= t.z) continue;
+  }
+  if (row0 + l16 >= t.z) return;
+  auto finish = [&](auto fn) {
     T* out = static_cast<T*>(a.out) + (int64_t)row * a.out_stride + a.at[slice];
     T o[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      float v = (float)yv[0][j] + acc[0][j >> 2][j & 3];
-      if constexpr (EPI == kEpiSwiglu)
-        v = swiglu_gate(v, (float)yv[NS - 1][j] + acc[NS - 1][j >> 2][j & 3]);
-      o[j] = (T)v;
-    }
+    for (int j = 0; j < 16; ++j) o[j] = (T)fn(acc[0][j >> 2][j & 3], acc[NS - 1][j >> 2][j & 3]);
     if (a.vec) {
-      if (f0 < width) __builtin_memcpy(__builtin_assume_aligned(out + f0, 16), &o[0], 8 * sizeof(T));
-      if (f1 < width) __builtin_memcpy(__builtin_assume_aligned(out + f1, 16), &o[8], 8 * sizeof(T));
+      if (f0 < width)
+        __builtin_memcpy(__builtin_assume_aligned(out + f0, 16), &o[0], 8 * sizeof(T));
+      if (f1 < width)
+        __builtin_memcpy(__builtin_assume_aligned(out + f1, 16), &o[8], 8 * sizeof(T));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -443,57 +556,68 @@ __global__ __launch_bounds__(kUpThreads) void adapter_up_kernel(ApplyArgs a) {
         if (f1 + j < width) out[f1 + j] = o[8 + j];
       }
     }
-  }
+  };
+  if constexpr (EPI == kEpiAdd) finish([](float y, float) { return y; });
+  else if (t.x >= 0) finish([](float y, float u) { return gate(y, u); });
+  else finish([](float y, float u) { return swiglu_gate(y, u); });
 }
 
 int cdiv(int a, int b) { return (a + b - 1) / b; }
 
-// Pieces of k: enough workgroups to fill the chip, at least two steps a wavefront.
-int down_rank_blocks(int SR) { return std::min(cdiv(SR, 16), 4); }
-int down_pieces(int max_tiles, int SR, int k) {
-  const int groups = max_tiles * cdiv(cdiv(SR, 16), down_rank_blocks(SR));
-  const int most = std::max(1, cdiv(k, 32) / (2 * kDownWaves));
-  return std::max(1, std::min({8, most, cdiv(512, std::max(groups, 1))}));
+// How a call is cut up. Few rows (tiles of 16): a workgroup a tile, block of ranks and piece
+// of k, up to 8 pieces, so that the adapters are read by many CUs. Prompts (tiles of 64): up to
+// 4 blocks, so that x is read once.
+constexpr int kMaxPieces = 8, kPromptPieces = 2;
+struct ApplyPlan {
+  int rb;       // blocks of ranks a workgroup
+  int pieces;
+  int k_steps;
+};
+ApplyPlan plan_apply(int max_tiles, int tile_rows, int blocks, int k) {
+  ApplyPlan p;
+  const int steps = cdiv(k, 32);
+  p.rb = tile_rows == 16 ? 1 : std::min(blocks, 4);
+  const int groups = std::max(1, max_tiles * cdiv(blocks, p.rb));
+  const int most = tile_rows == 16 ? kMaxPieces : kPromptPieces;
+  p.pieces = std::max(1, std::min({most, cdiv(steps, 16), cdiv(1024, groups)}));
+  p.k_steps = cdiv(steps, p.pieces);
+  p.pieces = cdiv(steps, p.k_steps);
+  return p;
 }
 
-template <typename T, int MR>
-int launch_down(const ApplyArgs& a, int max_tiles, hipStream_t st) {
-  const int rb = down_rank_blocks(a.SR);
-  const dim3 grid(max_tiles, cdiv(cdiv(a.SR, 16), rb), a.ksplit);
-  switch (rb) {
-    case 1: adapter_down_kernel<T, MR, 1><<<grid, kDownThreads, 0, st>>>(a); break;
-    case 2: adapter_down_kernel<T, MR, 2><<<grid, kDownThreads, 0, st>>>(a); break;
-    case 3: adapter_down_kernel<T, MR, 3><<<grid, kDownThreads, 0, st>>>(a); break;
-    default: adapter_down_kernel<T, MR, 4><<<grid, kDownThreads, 0, st>>>(a); break;
-  }
+template <typename T, int MR, int RB>
+int launch_down(const ApplyArgs& a, bool xvec, hipStream_t st) {
+  const dim3 grid((a.max_tiles + 7) / 8 * 8, cdiv(a.slices * a.blocks, RB), a.pieces);
+  if (xvec) adapter_down_kernel<T, MR, RB, true><<<grid, kDownThreads, 0, st>>>(a);
+  else adapter_down_kernel<T, MR, RB, false><<<grid, kDownThreads, 0, st>>>(a);
   return check_launch("adapter_down");
 }
 
-template <typename T, int MR, int EPI>
-int launch_up(const ApplyArgs& a, int max_tiles, hipStream_t st) {
+template <typename T, int P, int EPI>
+int launch_up(const ApplyArgs& a, hipStream_t st) {
   const int ns = EPI == kEpiSwiglu ? 2 : 1;
-  const int steps = cdiv(a.R, sizeof(T) == 2 ? 16 : 32);
-  const size_t pitch = steps * 32 + 16 / sizeof(T);
-  const size_t lds = ns * 16 * MR * (pitch * sizeof(T) + sizeof(float));
-  const int rc = allow_lds(reinterpret_cast<const void*>(adapter_up_kernel<T, MR, EPI>), lds);
-  if (rc) return rc;
-  const dim3 grid(max_tiles, EPI == kEpiSwiglu ? cdiv(a.at[1], kUpCols) : a.chunk0[a.slices]);
-  adapter_up_kernel<T, MR, EPI><<<grid, kUpThreads, lds, st>>>(a);
+  const int steps = cdiv(a.R, 32);
+  const size_t pitch = steps * (sizeof(T) == 2 ? 64 : 32) + 16 / sizeof(T);
+  const size_t lds = ns * 16 * (pitch * sizeof(T) + steps * sizeof(float));
+  const dim3 grid(a.chunk0[a.slices] / ns, a.max_tiles, a.tile_rows / 16);
+  adapter_up_kernel<T, P, EPI><<<grid, kUpThreads, lds, st>>>(a);
   return check_launch("adapter_up");
 }
 
-template <typename T, int MR>
-int launch_apply(const ApplyArgs& a, int max_tiles, int epilogue, hipStream_t st) {
-  const int rc = launch_down<T, MR>(a, max_tiles, st);
-  if (rc) return rc;
-  return epilogue == PKV_EPILOGUE_SWIGLU ? launch_up<T, MR, kEpiSwiglu>(a, max_tiles, st)
-                                         : launch_up<T, MR, kEpiAdd>(a, max_tiles, st);
-}
-
 template <typename T>
-int launch_apply(const ApplyArgs& a, int max_tiles, int tile_rows, int epilogue, hipStream_t st) {
-  return tile_rows == 16 ? launch_apply<T, 1>(a, max_tiles, epilogue, st)
-                         : launch_apply<T, 4>(a, max_tiles, epilogue, st);
+int launch_apply(const ApplyArgs& a, bool xvec, int rb, int tile_rows, int epilogue, hipStream_t st) {
+  int rc;
+  if (tile_rows == 16) rc = launch_down<T, 1, 1>(a, xvec, st);
+  else if (rb == 1) rc = launch_down<T, 4, 1>(a, xvec, st);
+  else if (rb == 2) rc = launch_down<T, 4, 2>(a, xvec, st);
+  else if (rb == 3) rc = launch_down<T, 4, 3>(a, xvec, st);
+  else rc = launch_down<T, 4, 4>(a, xvec, st);
+  if (rc) return rc;
+  const bool gate = epilogue == PKV_EPILOGUE_SWIGLU;
+  if (tile_rows == 16)
+    return gate ? launch_up<T, kMaxPieces, kEpiSwiglu>(a, st) : launch_up<T, kMaxPieces, kEpiAdd>(a, st);
+  return gate ? launch_up<T, kPromptPieces, kEpiSwiglu>(a, st)
+              : launch_up<T, kPromptPieces, kEpiAdd>(a, st);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -505,8 +629,8 @@ using namespace pkv;
 
 extern "C" {
 
-int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int max_tiles,
-                     const int32_t* ids, int n_tokens, int n_adapters, int tile_rows,
+int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int32_t* rows,
+                     int max_tiles, const int32_t* ids, int n_tokens, int n_adapters, int tile_rows,
                      int* status, void* stream) {
   fail(PKV_OK, "%s", "");
   if (n_tokens < 0 || n_adapters < 0) return fail(PKV_ERR_INVALID, "bad sizes");
@@ -516,11 +640,11 @@ int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int max_ti
     return fail(PKV_ERR_UNSUPPORTED, "at most %d adapters and 2^24 rows", kMaxAdapters);
   if (max_tiles < n_tokens / tile_rows + std::min(n_adapters + 1, n_tokens))
     return fail(PKV_ERR_INVALID, "max_tiles %d is too small", max_tiles);
-  if (!starts || (n_tokens > 0 && (!order || !ids)) || (max_tiles > 0 && !tiles))
+  if (!starts || (n_tokens > 0 && (!order || !ids)) || (max_tiles > 0 && (!tiles || !rows)))
     return fail(PKV_ERR_INVALID, "null pointer argument");
   if (!aligned16(tiles)) return fail(PKV_ERR_INVALID, "tiles must be 16-byte aligned");
-  PlanArgs a{order, starts,   reinterpret_cast<int4*>(tiles), max_tiles, ids, n_tokens,
-             n_adapters, tile_rows, status};
+  PlanArgs a{order,    starts,     reinterpret_cast<int4*>(tiles), rows,   max_tiles, ids,
+             n_tokens, n_adapters, tile_rows,                      status};
   const size_t lds = kPlanWaves * (n_adapters + 1) * sizeof(int);
   const int rc = allow_lds(reinterpret_cast<const void*>(adapter_plan_kernel), lds);
   if (rc) return rc;
@@ -528,15 +652,17 @@ int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int max_ti
   return check_launch("adapter_plan");
 }
 
-size_t pkv_adapter_workspace_bytes(int n_tokens, int max_tiles, int k, int ranks) {
-  if (n_tokens <= 0 || max_tiles <= 0 || k <= 0 || ranks <= 0) return 0;
-  return (size_t)down_pieces(max_tiles, ranks, k) * n_tokens * ranks * sizeof(float);
+size_t pkv_adapter_workspace_bytes(int n_tokens, int max_tiles, int tile_rows, int k, int rank,
+                                   int parts) {
+  if (n_tokens <= 0 || max_tiles <= 0 || k <= 0 || rank <= 0 || parts <= 0) return 0;
+  const int blocks = parts * cdiv(rank, 16);
+  return (size_t)plan_apply(max_tiles, tile_rows, blocks, k).pieces * n_tokens * blocks * 64;
 }
 
 int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t base_stride,
                       const void* x, int64_t x_stride, const void* a, int64_t a_stride,
-                      const void* b, const float* scales, const int32_t* order,
-                      const int32_t* tiles, int max_tiles, int tile_rows, int n_tokens,
+                      const void* b, const float* scales, const int32_t* tiles,
+                      const int32_t* rows, int max_tiles, int tile_rows, int n_tokens,
                       int n_adapters, int k, int rank, int parts, int n0, int n1, int n2, int n3,
                       int epilogue, int dtype, void* workspace, size_t workspace_bytes,
                       void* stream) {
@@ -553,8 +679,8 @@ int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t b
     return fail(PKV_ERR_INVALID, "tile_rows must be 16 or 64 (got %d)", tile_rows);
   if (rank % 8 || rank > 128)
     return fail(PKV_ERR_UNSUPPORTED, "rank %d is not a multiple of 8 up to 128", rank);
-  if (a_stride < k || a_stride % 8 || a_stride > (1 << 24) || k > (1 << 24))
-    return fail(PKV_ERR_INVALID, "A's rows must be a multiple of 8 elements, at least k, apart");
+  if (a_stride < k || a_stride % 32 || a_stride > (1 << 24) || k > (1 << 24))
+    return fail(PKV_ERR_INVALID, "A's rows must be a multiple of 32 elements, at least k, apart");
   ApplyArgs p{};
   int64_t n = 0;
   int chunks = 0;
@@ -572,12 +698,10 @@ int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t b
   const int64_t written = epilogue == PKV_EPILOGUE_SWIGLU ? n0 : n;
   if (n_tokens > 1 && (out_stride < written || base_stride < n || x_stride < k))
     return fail(PKV_ERR_INVALID, "row strides are smaller than the rows");
-  if (chunks > 65535 || n_tokens > (1 << 24))
-    return fail(PKV_ERR_UNSUPPORTED, "too many features or rows");
-  if (max_tiles > (1 << 24) / 16 + kMaxAdapters + 1)
-    return fail(PKV_ERR_INVALID, "max_tiles %d is no plan's", max_tiles);
+  if (max_tiles > 65535 || n_tokens > (1 << 24) || chunks > (1 << 20))
+    return fail(PKV_ERR_UNSUPPORTED, "at most 65535 tiles, 2^24 rows and 2^28 features");
   if (n_tokens == 0 || max_tiles == 0) return PKV_OK;
-  if (!out || !base || !x || !order || !tiles || (n_adapters > 0 && (!a || !b || !scales)))
+  if (!out || !base || !x || !tiles || !rows || (n_adapters > 0 && (!a || !b || !scales)))
     return fail(PKV_ERR_INVALID, "null pointer argument");
   if (!aligned16(a) || !aligned16(b) || !aligned16(tiles))
     return fail(PKV_ERR_INVALID, "the adapters and tiles must be 16-byte aligned");
@@ -594,8 +718,9 @@ int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t b
   p.a = a;
   p.b = b;
   p.scales = scales;
-  p.order = order;
   p.tiles = reinterpret_cast<const int4*>(tiles);
+  p.rows = rows;
+  p.tile_rows = tile_rows;
   p.T = n_tokens;
   p.N = n_adapters;
   p.k = k;
@@ -604,23 +729,26 @@ int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t b
   p.SR = rank * parts;
   p.n = (int)n;
   p.slices = parts;
-  p.ksplit = down_pieces(max_tiles, p.SR, k);
-  p.k_steps = cdiv(cdiv(k, 32), p.ksplit);
+  p.blocks = cdiv(rank, 16);
+  p.max_tiles = max_tiles;
+  const ApplyPlan cut = plan_apply(max_tiles, tile_rows, parts * p.blocks, k);
+  p.pieces = cut.pieces;
+  p.k_steps = cut.k_steps;
   p.copy = out != base || out_stride != base_stride;
   bool vec = aligned16(out) && aligned16(base) && out_stride % piece == 0 &&
              base_stride % piece == 0;
   for (int s = 0; s < parts; ++s) vec = vec && ns[s] % 8 == 0;
   p.vec = vec;
-  p.xvec = aligned16(x) && x_stride % piece == 0 && k % 8 == 0;
-  const size_t need = (size_t)p.ksplit * n_tokens * p.SR * sizeof(float);
+  const bool xvec = aligned16(x) && x_stride % piece == 0;
+  const size_t need = pkv_adapter_workspace_bytes(n_tokens, max_tiles, tile_rows, k, rank, parts);
   if (!workspace || workspace_bytes < need)
     return fail(PKV_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   if (!aligned16(workspace)) return fail(PKV_ERR_INVALID, "workspace must be 16-byte aligned");
-  p.part = static_cast<float*>(workspace);
+  p.low = static_cast<float*>(workspace);
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == PKV_DTYPE_F32) return launch_apply<float>(p, max_tiles, tile_rows, epilogue, st);
-  if (dtype == PKV_DTYPE_F16) return launch_apply<f16>(p, max_tiles, tile_rows, epilogue, st);
-  return launch_apply<bf16>(p, max_tiles, tile_rows, epilogue, st);
+  if (dtype == PKV_DTYPE_F32) return launch_apply<float>(p, xvec, cut.rb, tile_rows, epilogue, st);
+  if (dtype == PKV_DTYPE_F16) return launch_apply<f16>(p, xvec, cut.rb, tile_rows, epilogue, st);
+  return launch_apply<bf16>(p, xvec, cut.rb, tile_rows, epilogue, st);
 }
 
 }  // extern "C"

@@ -143,9 +143,9 @@ _SIGNATURES = {
     "pkv_write_accepted_step": ([_c_vp, _c_vp, _c_i64, _c_int, _c_i64, _c_int, _c_vp, _c_vp,
                                  _c_i64, _c_vp, _c_int] + [_c_vp] * 5 + [_c_int, _c_int, _c_int,
                                  _c_i64, _c_int, _c_vp, _c_vp], _c_int),
-    "pkv_adapter_plan": ([_c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_int, _c_vp,
+    "pkv_adapter_plan": ([_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_int, _c_int, _c_vp,
                           _c_vp], _c_int),
-    "pkv_adapter_workspace_bytes": ([_c_int] * 4, _c_size),
+    "pkv_adapter_workspace_bytes": ([_c_int] * 6, _c_size),
     "pkv_adapter_apply": ([_c_vp, _c_i64] * 4 + [_c_vp] * 4 + [_c_int] * 13 + [_c_vp, _c_size,
                                                                               _c_vp], _c_int),
     "pkv_control_logits": ([_c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_int]

@@ -41,7 +41,7 @@ class AdapterWeights:
     """A and B of num_adapters adapters beside a projection of in_features features
     to the parts out_features (one, or those of a fused projection, at most 4), of at
     most max_rank ranks a part. a [num_adapters, parts * rank, in_features rounded up
-    to 8], b [num_adapters, sum(out_features), rank] and scales (float32) are what the
+    to 32], b [num_adapters, sum(out_features), rank] and scales (float32) are what the
     kernels read, rank being max_rank rounded up to a multiple of 8; unused ranks are 0,
     and so is an adapter that was not loaded."""
 
@@ -55,12 +55,14 @@ class AdapterWeights:
             raise ValueError(f"AdapterWeights: 1 to {MAX_ADAPTERS} adapters of rank 1 to {MAX_RANK}")
         self.in_features, self.out_features = int(in_features), outs
         self.num_adapters, self.rank, self.dtype = int(num_adapters), -(-max_rank // 8) * 8, dtype
-        self.a = torch.zeros((num_adapters, len(outs) * self.rank, -(-in_features // 8) * 8),
+        self.a = torch.zeros((num_adapters, len(outs) * self.rank, -(-in_features // 32) * 32),
                              dtype=dtype, device=device)
         self.b = torch.zeros((num_adapters, sum(outs), self.rank), dtype=dtype, device=device)
         self.scales = torch.zeros(num_adapters, dtype=torch.float32, device=device)
         self.device = self.a.device
-        self._ns = outs + (0,) * (4 - len(outs))
+        # what every call hands on
+        self._place, self._features, self._parts = self.a.get_device(), sum(outs), len(outs)
+        self._a_stride, self._ns = self.a.shape[2], outs + (0,) * (4 - len(outs))
 
     def _index(self, index):
         if not 0 <= index < self.num_adapters:
@@ -113,6 +115,7 @@ class AdapterPlan:
     order: torch.Tensor   # int32 [T] rows sorted by adapter, those without one last
     starts: torch.Tensor  # int32 [num_adapters + 2] first place of each adapter's rows
     tiles: torch.Tensor   # int32 [max_tiles, 4] adapter or -1, first place, rows, 0
+    rows: torch.Tensor    # int32 [max_tiles, tile_rows] the tiles' rows
     num_tokens: int
     num_adapters: int
     tile_rows: int
@@ -138,17 +141,18 @@ def build_adapter_plan(ids: torch.Tensor, num_adapters: int,
         if not ids.is_contiguous():
             ids = ids.contiguous()
         # one allocation; the tiles lead, their rows are 16 bytes
-        buf = ids.new_empty(4 * max_tiles + T + n + 2)
-        tiles, order, starts = buf.split_with_sizes((4 * max_tiles, T, n + 2))
+        sizes = (4 * max_tiles, rows * max_tiles, T, n + 2)
+        tiles, places, order, starts = ids.new_empty(sum(sizes)).split_with_sizes(sizes)
         rc = _native.calls().pkv_adapter_plan(
-            order.data_ptr(), starts.data_ptr(), tiles.data_ptr(), max_tiles, ids.data_ptr(), T,
-            n, rows, None if status is None else _status_ptr(status, dev, what),
+            order.data_ptr(), starts.data_ptr(), tiles.data_ptr(), places.data_ptr(), max_tiles,
+            ids.data_ptr(), T, n, rows, None if status is None else _status_ptr(status, dev, what),
             _native.stream_ptr(dev))
     finally:
         _native.restore(previous)
     if rc:
         _native.check(rc, what)
-    return AdapterPlan(order, starts, tiles.view(max_tiles, 4), T, n, rows)
+    return AdapterPlan(order, starts, tiles.view(max_tiles, 4), places.view(max_tiles, rows), T, n,
+                       rows)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -168,29 +172,29 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     return True
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t with unit column stride and rows that do not overlap."""
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        return t.contiguous()
-    return t
+def _rows(t: torch.Tensor):
+    """A 2-D tensor with unit column stride and rows that do not overlap, t where it is
+    one, and its row stride."""
+    n, width = t.shape
+    stride, one = t.stride()
+    if one != 1 or (n > 1 and stride < width):
+        return t.contiguous(), width
+    return t, stride if n > 1 else width
 
 
 def _apply(base, x, weights, plan, out, written, epilogue, what):
-    dev, dtype, T = weights.device, weights.dtype, plan.num_tokens
-    _native.require_device(base, x, plan.order, weights.a, what=what)
-    if base.device != dev or x.device != dev or plan.order.device != dev:
+    a, dev, dtype, T = weights.a, weights.device, weights.dtype, plan.num_tokens
+    place, tiles = weights._place, plan.tiles
+    if not (place >= 0 and base.get_device() == place and x.get_device() == place
+            and tiles.get_device() == place):
+        _native.require_device(base, x, tiles, a, what=what)
         raise RuntimeError(f"{what}: base, x, the weights and the plan must share a device")
     if base.dtype != dtype or x.dtype != dtype:
         raise TypeError(f"{what}: base and x must be {dtype}, as the weights are")
     if (base.requires_grad or x.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError(
             f"{what} is forward-only (inference); run it under torch.no_grad()")
-    outs = weights.out_features
-    n, k = sum(outs), weights.in_features
+    n, k = weights._features, weights.in_features
     if base.shape != (T, n) or x.shape != (T, k):
         raise ValueError(f"{what}: base must be [{T}, {n}] and x [{T}, {k}] for this plan and "
                          f"these weights (got {tuple(base.shape)}, {tuple(x.shape)})")
@@ -198,32 +202,35 @@ def _apply(base, x, weights, plan, out, written, epilogue, what):
         raise ValueError(f"{what}: a plan of {plan.num_adapters} adapters, weights of "
                          f"{weights.num_adapters}")
     in_place = out is base
-    base, x = _rows(base), _rows(x)
+    (base, base_stride), (x, x_stride) = _rows(base), _rows(x)
+    calls, max_tiles = _native.calls(), tiles.shape[0]
     previous = _native.make_current(dev)
     try:
         if out is None:
-            out = base.new_empty((T, written))
+            out, out_stride = base.new_empty((T, written)), written
         else:
-            if out.shape != (T, written) or out.dtype != dtype or out.device != dev:
+            if out.shape != (T, written) or out.dtype != dtype or out.get_device() != place:
                 raise ValueError(f"{what}: out must be [{T}, {written}] {dtype} on {dev}")
-            if _rows(out) is not out:
+            dst, out_stride = _rows(out)
+            if dst is not out:
                 raise ValueError(f"{what}: out needs unit column stride and rows of its own")
             if out.requires_grad and torch.is_grad_enabled():
                 raise NotImplementedError(f"{what} is forward-only (inference)")
             same = (out.data_ptr() == base.data_ptr() and written == n
-                    and _row_stride(out) == _row_stride(base))
+                    and out_stride == base_stride)
             if (not same and _overlap(out, base)) or _overlap(out, x):
                 raise ValueError(f"{what}: out shares memory with base or x")
-        tiles, calls = plan.tiles, _native.calls()
-        nbytes = calls.pkv_adapter_workspace_bytes(T, tiles.shape[0], k, len(outs) * weights.rank)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        nbytes = calls.pkv_adapter_workspace_bytes(T, max_tiles, plan.tile_rows, k, weights.rank,
+                                                   weights._parts)
+        # this call's own scratch, from the allocator's pool of the current stream (or of
+        # the graph being captured): nothing is shared between calls
+        ws = base.new_empty(nbytes, dtype=torch.uint8)
         rc = calls.pkv_adapter_apply(
-            out.data_ptr(), _row_stride(out), base.data_ptr(), _row_stride(base), x.data_ptr(),
-            _row_stride(x), weights.a.data_ptr(), weights.a.shape[2], weights.b.data_ptr(),
-            weights.scales.data_ptr(), plan.order.data_ptr(), tiles.data_ptr(), tiles.shape[0],
-            plan.tile_rows, T, weights.num_adapters, k, weights.rank, len(outs), *weights._ns,
-            epilogue, _native.DTYPE_CODES[dtype], None if ws is None else ws.data_ptr(), nbytes,
-            _native.stream_ptr(dev))
+            out.data_ptr(), out_stride, base.data_ptr(), base_stride, x.data_ptr(), x_stride,
+            a.data_ptr(), weights._a_stride, weights.b.data_ptr(), weights.scales.data_ptr(),
+            tiles.data_ptr(), plan.rows.data_ptr(), max_tiles, plan.tile_rows, T,
+            weights.num_adapters, k, weights.rank, weights._parts, *weights._ns, epilogue,
+            _native.DTYPE_CODES[dtype], ws.data_ptr(), nbytes, _native.stream_ptr(dev))
         if rc:
             _native.check(rc, what)
         if in_place:
@@ -239,8 +246,8 @@ def adapter_add(base: torch.Tensor, x: torch.Tensor, weights: AdapterWeights, pl
     in_features]; float32, float16 or bfloat16, sums in fp32, rounded once. Rows without
     an adapter are base's. out: where to write, base itself (in place) or memory of no
     operand."""
-    return _apply(base, x, weights, plan, out, sum(weights.out_features),
-                  _native.EPILOGUE_NONE, "adapter_add")
+    return _apply(base, x, weights, plan, out, weights._features, _native.EPILOGUE_NONE,
+                  "adapter_add")
 
 
 def adapter_swiglu(base: torch.Tensor, x: torch.Tensor, weights: AdapterWeights,

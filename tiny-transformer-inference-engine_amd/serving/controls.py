@@ -18,7 +18,7 @@ from typing import Optional, Protocol
 import torch
 
 from . import _native
-from .adapters import _overlap, _row_stride, _rows
+from .adapters import _overlap, _rows
 from .paged_meta import _status_ptr, raise_step_status
 
 __all__ = ["LogitControls", "RequestParams", "Grammar", "TokenHistory", "control_logits",
@@ -103,6 +103,10 @@ class LogitControls:
         if len(rows) > 1:
             raise ValueError(f"{what}: the tensors disagree on the rows ({sorted(rows)})")
         object.__setattr__(self, "_rows", rows.pop() if rows else None)
+        # row stride and capacity, as the call hands them on
+        t = self.tokens
+        object.__setattr__(self, "_history", (0, 0) if t is None else (
+            t.stride(0) if t.shape[0] > 1 else t.shape[1], t.shape[1]))
         object.__setattr__(self, "_device", next(iter(given.values())).device if given else None)
 
 
@@ -132,25 +136,27 @@ def control_logits(logits: torch.Tensor, controls: LogitControls,
         raise ValueError(f"{what}: masks of {masks.shape[1]} words, {-(-vocab // 32)} needed")
     previous = _native.make_current(dev)
     try:
-        src = _rows(logits)
+        src, stride = _rows(logits)
         in_place = out is logits
         if out is None:
-            out = src.new_empty((rows, vocab))
-        elif not in_place or src is not logits:
-            if (out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev
-                    or _rows(out) is not out):
+            out, out_stride = src.new_empty((rows, vocab)), vocab
+        elif in_place and src is logits:
+            out_stride = stride
+        else:
+            dst, out_stride = _rows(out) if out.dim() == 2 else (None, 0)
+            if (dst is not out or out.shape != logits.shape or out.dtype != logits.dtype
+                    or out.device != dev):
                 raise ValueError(f"{what}: out must be {tuple(logits.shape)} {logits.dtype} on "
                                  f"{dev} with unit column stride and rows of its own")
             if out.requires_grad and torch.is_grad_enabled():
                 raise NotImplementedError(f"{what} is forward-only (inference)")
-            same = out.data_ptr() == src.data_ptr() and _row_stride(out) == _row_stride(src)
+            same = out.data_ptr() == src.data_ptr() and out_stride == stride
             if not same and _overlap(out, src):
                 raise ValueError(f"{what}: out shares memory with logits")
         ptr = _native.ptr
         rc = _native.calls().pkv_control_logits(
-            out.data_ptr(), _row_stride(out), src.data_ptr(), _row_stride(src), rows, vocab,
-            ptr(tokens), 0 if tokens is None else _row_stride(tokens),
-            0 if tokens is None else tokens.shape[1], ptr(c.lens), ptr(c.prompt_lens),
+            out.data_ptr(), out_stride, src.data_ptr(), stride, rows, vocab, ptr(tokens),
+            *c._history, ptr(c.lens), ptr(c.prompt_lens),
             ptr(c.repetition), ptr(c.presence), ptr(c.frequency), ptr(bias), ptr(c.bias_values),
             ptr(c.bias_starts), 0 if bias is None else bias.numel(), ptr(masks),
             0 if masks is None else masks.shape[0], ptr(c.mask_rows), code,
@@ -197,12 +203,12 @@ def sample_each(logits: torch.Tensor, temperature: torch.Tensor,
     try:
         if uniforms is None:
             uniforms = torch.rand(rows, device=dev, dtype=torch.float32)
-        src = _rows(logits)
-        ids = torch.empty(rows, dtype=torch.int64, device=dev)
+        src, stride = _rows(logits)
+        ids = logits.new_empty(rows, dtype=torch.int64)
         logprobs = temperature.new_empty(rows)
         ptr = _native.ptr
         rc = _native.calls().pkv_sample_each(
-            ids.data_ptr(), logprobs.data_ptr(), src.data_ptr(), rows, vocab, _row_stride(src),
+            ids.data_ptr(), logprobs.data_ptr(), src.data_ptr(), rows, vocab, stride,
             temperature.data_ptr(), ptr(top_k), ptr(top_p), ptr(min_p), uniforms.data_ptr(), code,
             None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
         if rc:
