@@ -8,6 +8,7 @@
 namespace pkv {
 namespace {
 
+using mfma::floatx4;
 using mfma::u32x4;
 
 // ---------------------------------------------------------------------------
@@ -36,20 +37,19 @@ __device__ __forceinline__ void load_piece(const T* row, int id0, int vocab, T f
 }
 
 // ---------------------------------------------------------------------------
-// Penalties, biases, masks. A workgroup takes one row and a range of kRange ids: it
-// counts the row's history over that range in LDS, adds up the biases there, and then
-// passes over the logits once. Bytes bind (logits in and out); the history is read once
-// per range, from L2 after the first.
+// Penalties, biases, masks. A workgroup takes one row and a range of its ids: it requests
+// the range's logits, counts the row's history over the range in LDS, adds up the biases
+// there, and changes what it holds. Bytes bind (logits in and out, once); the history
+// is read once per range, from L2 after the first. What is in the way is a chain of round
+// trips (lengths, then ids, then barriers), so ranges are small and many workgroups share a
+// CU.
 // ---------------------------------------------------------------------------
 struct ControlArgs {
   void* out;
   int64_t out_stride;
   const void* in;
   int64_t in_stride;
-  int rows;
   int vocab;
-  int range;  // ids of a workgroup, a multiple of 32
-  int ranges;
   const int32_t* tokens;  // [rows, cap], tok_stride apart
   int64_t tok_stride;
   int cap;
@@ -69,70 +69,42 @@ struct ControlArgs {
   int* status;
 };
 
-constexpr int kCtlThreads = 512;
-constexpr unsigned kInPrompt = 0x80000000u;  // a count's top bit: the prompt holds the token
+// An id's record: how often it is behind the prompt, and whether the prompt holds it.
+constexpr unsigned kInPrompt = 0x80000000u;
+constexpr int kMaxHistory = 1 << 30;
+constexpr int kAlike = 1024;  // counters of biases whose ids are alike modulo as much
 
-template <typename T>
-__global__ __launch_bounds__(kCtlThreads) void control_kernel(ControlArgs a) {
+// TH threads, S pieces each: a range of TH S pieces.
+template <typename T, int TH, int S>
+__global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
   constexpr int E = kPiece<T>;
-  extern __shared__ __attribute__((aligned(16))) unsigned dyn[];
-  unsigned* const cnt = dyn;                                   // [range]
-  float* const bias = reinterpret_cast<float*>(dyn + a.range);  // [range], with biases
+  constexpr int R = TH * S * E;
+  static_assert(S * E <= 32, "a bit an id");
+  __shared__ __attribute__((aligned(16))) unsigned cnt[R];  // records, then the biases' claims
+  __shared__ __attribute__((aligned(16))) float vals[R];
+  __shared__ unsigned alike[kAlike];
   const int tid = threadIdx.x;
   const int r = blockIdx.x;
   const T* in = static_cast<const T*>(a.in) + (int64_t)r * a.in_stride;
   T* out = static_cast<T*>(a.out) + (int64_t)r * a.out_stride;
   const int mis = misaligned(in);
   const bool same = mis == misaligned(static_cast<const T*>(out));
-  const int lo = (int)blockIdx.y * a.range - mis;  // first id of the range (its piece 0)
-  const int hi = min(lo + a.range, a.vocab);
+  const int lo = (int)blockIdx.y * R - mis;  // first id of the range (its piece 0)
+  const int hi = min(lo + R, a.vocab);
   if (hi <= 0 || lo >= a.vocab) return;
+
+  T v[S][E];
+#pragma unroll
+  for (int s = 0; s < S; ++s) load_piece(in, lo + (s * TH + tid) * E, a.vocab, (T)0.f, v[s]);
+  // the first ids of the history, before it is known how many there are
+  constexpr int U = 8;  // ids requested together
+  const int32_t* tok = a.tokens + (int64_t)r * a.tok_stride;
+  int id[U];
+  if (a.tokens) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = tok[min(tid + u * TH, a.cap - 1)];
+  }
   int bad = 0;
-
-  // Biases, in the order of the list where it names an id twice: the entries of a
-  // batch claim their ids, the first of each adds its value, and so on until all have.
-  int b0 = 0, b1 = 0;
-  if (a.bias_starts) {
-    b0 = ld_meta(a.bias_starts, r);
-    b1 = ld_meta(a.bias_starts, r + 1);
-    if (b0 < 0 || b1 < b0 || b1 > a.n_bias) {
-      bad |= PKV_STATUS_BAD_CONTROL;
-      b0 = b1 = 0;
-    }
-  }
-  const bool biased = b1 > b0;
-  if (biased) {
-    for (int i = tid; i < a.range; i += kCtlThreads) {
-      cnt[i] = ~0u;
-      bias[i] = 0.f;
-    }
-    __syncthreads();
-    for (int base = b0; base < b1; base += kCtlThreads) {
-      const int e = base + tid;
-      int id = -1;
-      float v = 0.f;
-      if (e < b1) {
-        id = a.bias_ids[e];
-        v = a.bias_values[e];
-        if ((unsigned)id >= (unsigned)a.vocab) {
-          bad |= PKV_STATUS_BAD_TOKEN;
-          id = -1;
-        }
-      }
-      bool todo = id >= lo && id >= 0 && id < hi;
-      const int at = id - lo;
-      while (__syncthreads_or(todo)) {
-        if (todo) atomicMin(&cnt[at], (unsigned)tid);
-        __syncthreads();
-        if (todo && cnt[at] == (unsigned)tid) {
-          bias[at] += v;
-          cnt[at] = ~0u;
-          todo = false;
-        }
-      }
-    }
-  }
-
   int n = 0, prompt = 0;
   if (a.tokens) {
     n = ld_meta(a.lens, r);
@@ -143,82 +115,190 @@ __global__ __launch_bounds__(kCtlThreads) void control_kernel(ControlArgs a) {
       prompt = min(max(prompt, 0), n);
     }
   }
-  if (n > 0) {
-    for (int i = tid; i < a.range; i += kCtlThreads) cnt[i] = 0;
-    __syncthreads();
-    const int32_t* tok = a.tokens + (int64_t)r * a.tok_stride;
-    for (int i = tid; i < n; i += kCtlThreads) {
-      const int id = tok[i];
-      if ((unsigned)id >= (unsigned)a.vocab) {
-        bad |= PKV_STATUS_BAD_TOKEN;
-      } else if (id >= lo && id < hi) {
-        if (i < prompt) atomicOr(&cnt[id - lo], kInPrompt);
-        else atomicAdd(&cnt[id - lo], 1u);
-      }
+  int b0 = 0, b1 = 0;
+  if (a.bias_starts) {
+    b0 = ld_meta(a.bias_starts, r);
+    b1 = ld_meta(a.bias_starts, r + 1);
+    if (b0 < 0 || b1 < b0 || b1 > a.n_bias) {
+      bad |= PKV_STATUS_BAD_CONTROL;
+      b0 = b1 = 0;
     }
   }
+  // a batch of biases, the first before the history is counted
+  int bid = -1;
+  float badd = 0.f;
+  auto request = [&](int base) {
+    const int e = base + tid;
+    bid = -1;
+    if (e < b1) {
+      bid = a.bias_ids[e];
+      badd = a.bias_values[e];
+    }
+  };
+  request(b0);
   const int32_t* mask = nullptr;
   if (a.mask_rows) {
     const int m = ld_meta(a.mask_rows, r);
     if (m >= 0 && m < a.n_masks) mask = a.masks + (int64_t)m * a.words;
     else if (m != -1) bad |= PKV_STATUS_BAD_CONTROL;
   }
-  __syncthreads();
+  unsigned allowed[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    allowed[s] = ~0u;
+    if (mask) {
+      const int id0 = lo + (s * TH + tid) * E;
+      const int f = min(max(id0, 0), a.vocab - 1);
+      const int q = f >> 5;
+      const uint64_t two = (uint64_t)(uint32_t)mask[q] |
+                           ((uint64_t)(uint32_t)mask[min(q + 1, a.words - 1)] << 32);
+      allowed[s] = (unsigned)(two >> (f & 31)) << min(max(f - id0, 0), 31);
+    }
+  }
   const float rep = a.repetition ? a.repetition[r] : 1.f;
   const float pres = a.presence ? a.presence[r] : 0.f;
   const float freq = a.frequency ? a.frequency[r] : 0.f;
 
-  for (int p = tid * E; p < a.range; p += kCtlThreads * E) {
+  bool staged = false;  // the range's logits are in vals
+  auto stage = [&]() {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int j = 0; j < E; j += 4)
+        *reinterpret_cast<floatx4*>(&vals[(s * TH + tid) * E + j]) =
+            floatx4{(float)v[s][j], (float)v[s][j + 1], (float)v[s][j + 2], (float)v[s][j + 3]};
+    staged = true;
+  };
+  const bool biased = b1 > b0;
+  bool todo = bid >= lo && bid >= 0 && bid < hi;
+  if (n > 0)
+    for (int i = tid * 4; i < R; i += TH * 4) *reinterpret_cast<u32x4*>(&cnt[i]) = u32x4{};
+  if (biased)
+    for (int i = tid; i < kAlike; i += TH) alike[i] = 0;
+  if (n > 0 || biased) __syncthreads();
+  if (todo) atomicAdd(&alike[bid & (kAlike - 1)], 1u);
+  if (n > 0) {
+    for (int base = tid; base < n; base += U * TH) {
+      if (base != tid) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) id[u] = tok[min(base + u * TH, n - 1)];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = base + u * TH;
+        if (i >= n) break;
+        if (blockIdx.y == 0 && (unsigned)id[u] >= (unsigned)a.vocab) bad |= PKV_STATUS_BAD_TOKEN;
+        const unsigned at = (unsigned)(id[u] - lo);
+        if (at < (unsigned)(hi - lo) && id[u] >= 0) {
+          if (i < prompt) atomicOr(&cnt[at], kInPrompt);
+          else atomicAdd(&cnt[at], 1u);
+        }
+      }
+    }
+    __syncthreads();
+    // Few ids change, and a change is some thirty operations (a division among them): each
+    // thread finds its own by their bits and changes them in LDS one by one, not all of a
+    // piece where it stands.
+    unsigned bits = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int j = 0; j < E; j += 4) {
+        const u32x4 c = *reinterpret_cast<const u32x4*>(&cnt[(s * TH + tid) * E + j]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bits |= (c[k] != 0u ? 1u : 0u) << (s * E + j + k);
+      }
+    stage();
+    while (bits) {
+      const int k = __ffs(bits) - 1;
+      bits &= bits - 1;
+      const int at = (k / E * TH + tid) * E + k % E;
+      const unsigned c = cnt[at];
+      float x = vals[at];
+      x = x > 0.f ? x / rep : x * rep;
+      const unsigned made = c & ~kInPrompt;
+      if (made) x -= freq * (float)made + pres;
+      vals[at] = x;
+    }
+  }
+  // Biases. The first batch's that no other is alike are added at once. The others, in the
+  // order of the list where it names an id twice: the entries of a batch claim their ids, the
+  // first of each adds its value, and so on until all have.
+  bool claims = false;  // cnt is ready for claims
+  for (int base = b0; base < b1; base += TH) {
+    if (base != b0) {
+      request(base);
+      todo = bid >= lo && bid >= 0 && bid < hi;
+    } else {
+      if (!staged) stage();
+      __syncthreads();
+      if (todo && alike[bid & (kAlike - 1)] == 1) {
+        vals[bid - lo] += badd;
+        todo = false;
+      }
+    }
+    if (blockIdx.y == 0 && base + tid < b1 && (unsigned)bid >= (unsigned)a.vocab)
+      bad |= PKV_STATUS_BAD_TOKEN;
+    if (!__syncthreads_or(todo)) continue;
+    if (!claims) {
+      for (int i = tid; i < R; i += TH) cnt[i] = ~0u;
+      claims = true;
+      __syncthreads();
+    }
+    const int at = bid - lo;
+    do {
+      if (todo) atomicMin(&cnt[at], (unsigned)tid);
+      __syncthreads();
+      if (todo && cnt[at] == (unsigned)tid) {
+        vals[at] += badd;
+        cnt[at] = ~0u;
+        todo = false;
+      }
+    } while (__syncthreads_or(todo));
+  }
+  if (bad && a.status) atomicOr(a.status, bad);
+  if (!staged && !mask && out == in) return;  // as it was
+
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const int p = (s * TH + tid) * E;
     const int id0 = lo + p;
     if (id0 >= hi) break;
-    T v[E];
-    load_piece(in, id0, a.vocab, (T)0.f, v);
-    unsigned c[E];
-    float b[E];
+    if (staged) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      c[j] = n > 0 ? cnt[p + j] : 0u;
-      b[j] = biased ? bias[p + j] : 0.f;
-    }
-    unsigned allowed = (1u << E) - 1;
-    if (mask) {
-      const int f = max(id0, 0);
-      const int q = f >> 5;
-      const uint64_t two = (uint64_t)(uint32_t)mask[q] |
-                           ((uint64_t)(uint32_t)(q + 1 < a.words ? mask[q + 1] : 0) << 32);
-      allowed = (unsigned)(two >> (f & 31)) << (f - id0);
-    }
+      for (int j = 0; j < E; j += 4) {
+        const floatx4 x = *reinterpret_cast<const floatx4*>(&vals[p + j]);
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-      if (c[j] != 0u || b[j] != 0.f) {
-        float x = (float)v[j];
-        const unsigned made = c[j] & ~kInPrompt;
-        if (c[j] != 0u) {
-          x = x > 0.f ? x / rep : x * rep;
-          if (made) x -= freq * (float)made + pres;
-        }
-        v[j] = (T)(x + b[j]);
+        for (int k = 0; k < 4; ++k) v[s][j + k] = (T)x[k];
       }
-      if (!(allowed >> j & 1)) v[j] = (T)-INFINITY;
+    }
+    if (mask) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (!(allowed[s] >> j & 1)) v[s][j] = (T)-INFINITY;
     }
     if (same && id0 >= 0 && id0 + E <= a.vocab) {
-      __builtin_memcpy(__builtin_assume_aligned(out + id0, 16), v, 16);
+      __builtin_memcpy(__builtin_assume_aligned(out + id0, 16), v[s], 16);
     } else {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        if ((unsigned)(id0 + j) < (unsigned)a.vocab) out[id0 + j] = v[j];
+        if ((unsigned)(id0 + j) < (unsigned)a.vocab) out[id0 + j] = v[s][j];
     }
   }
-  if (bad && a.status) atomicOr(a.status, bad);
+}
+
+template <typename T, int TH, int S>
+int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
+  constexpr int R = TH * S * kPiece<T>;
+  const dim3 grid((unsigned)rows, (unsigned)((a.vocab + kPiece<T> - 1 + R - 1) / R));
+  control_kernel<T, TH, S><<<grid, TH, 0, st>>>(a);
+  return check_launch("control_logits");
 }
 
 template <typename T>
-int launch_control(ControlArgs a, hipStream_t st) {
-  const size_t lds = (size_t)a.range * 4 * (a.bias_starts ? 2 : 1);
-  const int rc = allow_lds(reinterpret_cast<const void*>(control_kernel<T>), lds);
-  if (rc) return rc;
-  control_kernel<T><<<dim3(a.rows, a.ranges), kCtlThreads, lds, st>>>(a);
-  return check_launch("control_logits");
+int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
+  constexpr int S = 8 / kPiece<T>;
+  return launch_control<T, 512, S>(a, rows, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -947,7 +1027,7 @@ int pkv_control_logits(void* out, int64_t out_stride, const void* logits, int64_
                        const int32_t* mask_rows, int dtype, int* status, void* stream) {
   fail(PKV_OK, "%s", "");
   if (!ok_dtype(dtype)) return fail(PKV_ERR_INVALID, "unknown dtype %d", dtype);
-  if (rows < 0 || vocab < 0 || cap < 0 || n_bias < 0 || n_masks < 0)
+  if (rows < 0 || vocab < 0 || cap < 0 || cap >= kMaxHistory || n_bias < 0 || n_masks < 0)
     return fail(PKV_ERR_INVALID, "bad sizes");
   if (rows > (1 << 20) || vocab > (1 << 24))
     return fail(PKV_ERR_UNSUPPORTED, "at most 2^20 rows of 2^24 logits");
@@ -963,7 +1043,6 @@ int pkv_control_logits(void* out, int64_t out_stride, const void* logits, int64_
   a.out_stride = out_stride;
   a.in = logits;
   a.in_stride = in_stride;
-  a.rows = (int)rows;
   a.vocab = (int)vocab;
   a.tokens = cap > 0 ? tokens : nullptr;
   a.tok_stride = tok_stride;
@@ -982,12 +1061,10 @@ int pkv_control_logits(void* out, int64_t out_stride, const void* logits, int64_
   a.words = (int)((vocab + 31) / 32);
   a.mask_rows = mask_rows;
   a.status = status;
-  a.range = rows >= 32 ? 8192 : 2048;
-  a.ranges = (int)((vocab + 7 + a.range - 1) / a.range);
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == PKV_DTYPE_F32) return launch_control<float>(a, st);
-  if (dtype == PKV_DTYPE_F16) return launch_control<f16>(a, st);
-  return launch_control<bf16>(a, st);
+  if (dtype == PKV_DTYPE_F32) return launch_control<float>(a, rows, st);
+  if (dtype == PKV_DTYPE_F16) return launch_control<f16>(a, rows, st);
+  return launch_control<bf16>(a, rows, st);
 }
 
 int pkv_sample_each(int64_t* ids, float* logprobs, const void* logits, int64_t rows,
