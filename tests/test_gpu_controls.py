@@ -296,6 +296,24 @@ def test_ties(dtype):
     assert ids == [0, 0, 1, 1]  # weights 1 1 1 0.37: before the third it is 0.59 of the sum
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_values_than_are_listed(dtype):
+    """Wide nuclei and large top_k, with few values near the border and with many; and borders
+    further from the largest logit than the bins of the counts reach."""
+    rng = np.random.default_rng(21)
+    rows, vocab = 20, 50257
+    u = rng.random(rows, dtype=np.float32)
+    t = [1.0, 1.4, 0.7, 3.0] * 5
+    k = [0] * 8 + [9000, 20000, 50256, 50257, 12000, 30000] * 2
+    p = [0.95, 0.9, 0.999, 0.99] * 4 + [1.0] * 4
+    m = [0.0, 0.0, 1e-3, 1e-6, 0.0] * 4
+    for x in (rng.normal(0, 2, (rows, vocab)), rng.integers(-6, 7, (rows, vocab)) / 2.0,
+              np.sort(rng.normal(0, 2, (rows, vocab)), axis=1)):
+        draw_and_check(torch.from_numpy(x).to(dtype).to(DEV), t, k, p, m, u, least_checked=0.6)
+    x = torch.from_numpy(rng.normal(0, 2, (rows, vocab))).to(dtype).to(DEV)
+    draw_and_check(x, [0.01, 0.05, 0.2, 0.3] * 5, [40000, 1000, 300, 50000] * 5, p, m, u)
+
+
 def test_far_apart_and_extreme_parameters():
     rng = np.random.default_rng(5)
     x = torch.from_numpy(rng.normal(0, 1, (32, 500)) * 1e4).float().to(DEV)

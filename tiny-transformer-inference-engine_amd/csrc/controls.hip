@@ -351,13 +351,14 @@ constexpr double kFar = 44.0 * kStep;
 // 32 bins an octave, 2048 in all
 constexpr int kBinShift = kStepBits - 5;
 
-// A wavefront's part of the list of values that can be kept; with it the workgroup takes
-// 155 KB of a CU's 160.
-constexpr int kListCap = 768;
+// A wavefront's parts of the list of values that can be kept and of that of the values near
+// a border (some 30 of a row's bin); with them the workgroup takes 155 KB of a CU's 160.
+constexpr int kListCap = 640;
+constexpr int kBorderCap = 128;
 
 struct SampShared {
   u32x4 edge[3];
-  int listed[kSampWaves];
+  int listed[2][kSampWaves];  // entries of list and border list
   double pow[kStep];  // 2^43 2^(-j / kStep)
   u64 mass[kBins];
   unsigned count[kBins];
@@ -365,8 +366,8 @@ struct SampShared {
   u64 rsum[kMaxRounds];
   u64 found[3];
   int at[2];
-  float list_value[kSampWaves][kListCap];
-  int list_id[kSampWaves][kListCap];
+  float list_value[kSampWaves][kListCap + kBorderCap];
+  int list_id[kSampWaves][kListCap + kBorderCap];
 };
 
 // Keys in the order of the values, as short as the type (fp32 values of 16-bit ones end
@@ -476,18 +477,21 @@ struct Row {
   }
 };
 
-// The values of a row that can still be kept, in LDS: what Row is for all of them.
+// The values of a row that can still be kept (kPart 0) or are near the border (1), in LDS
+// in the order of the ids: what Row is for all of them.
+template <int kPart>
 struct List {
   static constexpr int E = 1;
+  static constexpr int kFrom = kPart ? kListCap : 0;
   __device__ __forceinline__ void get(const SampShared& s, int w, int k, float (&x)[1],
                                       int& id0) const {
     const int i = 64 * k + (threadIdx.x & 63);
-    const bool in = i < s.listed[w];
-    x[0] = in ? s.list_value[w][i] : -INFINITY;
-    id0 = in ? s.list_id[w][i] : -1;
+    const bool in = i < s.listed[kPart][w];
+    x[0] = in ? s.list_value[w][kFrom + i] : -INFINITY;
+    id0 = in ? s.list_id[w][kFrom + i] : -1;
   }
   __device__ __forceinline__ int rounds_of(const SampShared& s, int w) const {
-    return (s.listed[w] + 63) / 64;
+    return (s.listed[kPart][w] + 63) / 64;
   }
   template <typename F>
   __device__ __forceinline__ void each(const SampShared& s, F f) const {
@@ -570,7 +574,8 @@ struct Sampler {
   static constexpr double kShift = 6755399441055744.;
   // 2^43 2^(-z / kStep) for a distance z of at most 60 octaves, and the steps n of z: the
   // whole steps from the table and by the exponent, the rest r, at most half a step, as a
-  // polynomial whose next term is below 2^-43.
+  // polynomial whose next term is below 2^-43. (A pass is bound by its instructions: a table
+  // of 32 entries, without bank conflicts, and three more terms took 1 us more for 128 rows.)
   __device__ __forceinline__ double weight(double z, int& n) const {
     constexpr double c = 0.69314718055994530942 / kStep;
     const double y = z + kShift;
@@ -609,30 +614,44 @@ struct Sampler {
     k0 = b == kBins - 1 || lo < least + 4 ? least : lo - 4;
   }
 
-  // The values of at least `from` into the list; false where they are too many for it.
-  __device__ bool list_up(const Row<T>& row, float from) {
+  // The values of at least `from` into the list, those within [v0, v1], v0 >= from, into the
+  // border list (kBorder). The bits of the result: 1, all are in the list; 2, in the border
+  // list.
+  template <bool kBorder>
+  __device__ int list_up(const Row<T>& row, float from, float v0, float v1) {
     constexpr int E = Row<T>::E;
     const int w = threadIdx.x >> 6;
-    int n = 0;
+    float* const value = s.list_value[w];
+    int* const id = s.list_id[w];
+    int n = 0, border = 0;
     row.each(s, [&](const float (&x)[E], int id0) {
-      if (n > kListCap) return;
-      int c = 0;
+      int c = 0, d = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) c += x[j] >= from;
-      if (__ballot(c != 0) == 0) return;
-      const int upto = (int)wave_prefix((u64)c);
-      int at = n + upto - c;
+      for (int j = 0; j < E; ++j) {
+        c += x[j] >= from;
+        if constexpr (kBorder) d += x[j] >= v0 && x[j] <= v1;
+      }
+      if (__ballot(n > kListCap ? d != 0 : c != 0) == 0) return;
+      const u64 upto = wave_prefix((u64)d << 32 | (unsigned)c);
+      int at = n + (int)upto - c, at1 = border + (int)(upto >> 32) - d;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         if (x[j] >= from) {
-          if (at < kListCap) s.list_value[w][at] = x[j], s.list_id[w][at] = id0 + j;
+          if (at < kListCap) value[at] = x[j], id[at] = id0 + j;
           ++at;
         }
+        if (kBorder && x[j] >= v0 && x[j] <= v1) {
+          if (at1 < kBorderCap) value[kListCap + at1] = x[j], id[kListCap + at1] = id0 + j;
+          ++at1;
+        }
       }
-      n += __builtin_amdgcn_readlane(upto, 63);
+      n += __builtin_amdgcn_readlane((int)upto, 63);
+      border += __builtin_amdgcn_readlane((int)(upto >> 32), 63);
     });
-    if ((threadIdx.x & 63) == 0) s.listed[w] = n;
-    return !__syncthreads_or(n > kListCap);
+    if ((threadIdx.x & 63) == 0) s.listed[0][w] = n, s.listed[1][w] = border;
+    const int in = __syncthreads_or(n > kListCap) ? 0 : 1;
+    if constexpr (!kBorder) return in;
+    return in | (__syncthreads_or(border > kBorderCap) ? 0 : 2);
   }
 
   // The value in bin b at which the sum of weights (by_mass: masses, else counts) of the
@@ -934,22 +953,29 @@ __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a)
     const uint64_t in = __ballot(x >= best || m.weight(z, n) >= least);
     min_cut = __shfl(x, in ? __ffsll((unsigned long long)in) - 1 : 63);
   }
-  const List list;
-  bool listed = false;     // what can be kept is in the list
+  const List<0> list;
+  const List<1> border;
+  int listed = 0;          // 1: what can be kept is in the list
   float cut = -INFINITY;   // values below it are out, and so are its own ids behind cut_id
   int cut_id = 0x7fffffff;
   unsigned k0, k1;
   if (top_k > 0 && top_k < a.vocab) {
     row.each(s, [&](const float (&x)[E], int) {
 #pragma unroll
-      for (int j = 0; j < E; ++j) atomicAdd(&s.count[m.count_bin(x[j])], 1u);
+      for (int j = 0; j < E; ++j) {
+        // not the last bin, whose values would queue for one place (a third of the time
+        // at temperature 0.3); it has what the others lack
+        const int b = m.count_bin(x[j]);
+        if (b < kBins - 1) atomicAdd(&s.count[b], 1u);
+      }
     });
     __syncthreads();
     find_prefix(s.count, kBins, (u64)top_k - 1, s);
-    const int b = (int)s.found[0];
-    const u64 rest = (u64)top_k - 1 - s.found[1];
+    const bool past = s.found[0] == kBins;
+    const int b = past ? kBins - 1 : (int)s.found[0];
+    const u64 rest = (u64)top_k - 1 - (past ? m.total() : s.found[1]);
     m.around(b, k0, k1);
-    listed = m.list_up(row, Key<T>::value(k0));
+    listed = m.template list_up<false>(row, Key<T>::value(k0), 0.f, 0.f);
     u64 before, own;
     cut = listed ? m.template refine<false>(list, b, rest, -INFINITY, before, own)
                  : m.template refine<false>(row, b, rest, -INFINITY, before, own);
@@ -976,18 +1002,21 @@ __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a)
       if (b < kBins) {
         if (!listed) {
           m.around(b, k0, k1);
-          listed = m.list_up(row, fmaxf(Key<T>::value(k0), cut));
+          const float v0 = fmaxf(Key<T>::value(k0), cut);
+          listed = m.template list_up<true>(row, v0, v0, Key<T>::value(k1));
         }
         const float floor = cut;
-        if (listed) m.nucleus(list, b, rest, floor, cut, cut_id);
+        if (listed & 1) m.nucleus(list, b, rest, floor, cut, cut_id);
+        else if (listed) m.nucleus(border, b, rest, floor, cut, cut_id);
         else m.nucleus(row, b, rest, floor, cut, cut_id);
       }
     }
   }
+  listed &= 1;
   if (min_cut > cut) {
     cut = min_cut;
     cut_id = 0x7fffffff;
-    if (!listed) listed = m.list_up(row, cut);
+    if (!listed) listed = m.template list_up<false>(row, cut, 0.f, 0.f);
   }
   const u64 all = listed ? m.draw(list, cut, cut_id, (double)u) : m.draw(row, cut, cut_id, (double)u);
   if (tid == 0) {
