@@ -355,6 +355,10 @@ constexpr int kBinShift = kStepBits - 5;
 // a border (some 30 of a row's bin); with them the workgroup takes 155 KB of a CU's 160.
 constexpr int kListCap = 640;
 constexpr int kBorderCap = 128;
+// The most values that a nucleus is listed with: 4/5 of the list, for the wavefronts differ.
+// 128 rows of 50257 with some 5600 each take 43 us by the list and 49 by the border alone,
+// whose time does not rise with the number (22000: 57 us by a list that overflows).
+constexpr int kListMost = kSampWaves * kListCap / 5 * 4;
 
 struct SampShared {
   u32x4 edge[3];
@@ -614,44 +618,30 @@ struct Sampler {
     k0 = b == kBins - 1 || lo < least + 4 ? least : lo - 4;
   }
 
-  // The values of at least `from` into the list, those within [v0, v1], v0 >= from, into the
-  // border list (kBorder). The bits of the result: 1, all are in the list; 2, in the border
-  // list.
-  template <bool kBorder>
-  __device__ int list_up(const Row<T>& row, float from, float v0, float v1) {
+  // The values of at least `from` into the list; false where they are too many for it.
+  __device__ bool list_up(const Row<T>& row, float from) {
     constexpr int E = Row<T>::E;
     const int w = threadIdx.x >> 6;
-    float* const value = s.list_value[w];
-    int* const id = s.list_id[w];
-    int n = 0, border = 0;
+    int n = 0;
     row.each(s, [&](const float (&x)[E], int id0) {
-      int c = 0, d = 0;
+      if (n > kListCap) return;
+      int c = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        c += x[j] >= from;
-        if constexpr (kBorder) d += x[j] >= v0 && x[j] <= v1;
-      }
-      if (__ballot(n > kListCap ? d != 0 : c != 0) == 0) return;
-      const u64 upto = wave_prefix((u64)d << 32 | (unsigned)c);
-      int at = n + (int)upto - c, at1 = border + (int)(upto >> 32) - d;
+      for (int j = 0; j < E; ++j) c += x[j] >= from;
+      if (__ballot(c != 0) == 0) return;
+      const int upto = (int)wave_prefix((u64)c);
+      int at = n + upto - c;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         if (x[j] >= from) {
-          if (at < kListCap) value[at] = x[j], id[at] = id0 + j;
+          if (at < kListCap) s.list_value[w][at] = x[j], s.list_id[w][at] = id0 + j;
           ++at;
         }
-        if (kBorder && x[j] >= v0 && x[j] <= v1) {
-          if (at1 < kBorderCap) value[kListCap + at1] = x[j], id[kListCap + at1] = id0 + j;
-          ++at1;
-        }
       }
-      n += __builtin_amdgcn_readlane((int)upto, 63);
-      border += __builtin_amdgcn_readlane((int)(upto >> 32), 63);
+      n += __builtin_amdgcn_readlane(upto, 63);
     });
-    if ((threadIdx.x & 63) == 0) s.listed[0][w] = n, s.listed[1][w] = border;
-    const int in = __syncthreads_or(n > kListCap) ? 0 : 1;
-    if constexpr (!kBorder) return in;
-    return in | (__syncthreads_or(border > kBorderCap) ? 0 : 2);
+    if ((threadIdx.x & 63) == 0) s.listed[0][w] = n;
+    return !__syncthreads_or(n > kListCap);
   }
 
   // The value in bin b at which the sum of weights (by_mass: masses, else counts) of the
@@ -727,7 +717,8 @@ struct Sampler {
   }
 
   // The sums of the weights of at least `near` by bin in s.mass (cleared before), and the
-  // total of those of at least `floor`: atomics for the few that can matter.
+  // total of those of at least `floor`. (The atomics cost nothing beside the weights: the
+  // same time with those of 16 octaves alone, or of 3.)
   template <typename S>
   __device__ u64 histogram(const S& src, float floor, float near) {
     u64 sum = 0;
@@ -757,39 +748,100 @@ struct Sampler {
     return all;
   }
 
-  // The draw: the first kept id at which the cumulative weight exceeds u times the sum.
-  template <typename S>
-  __device__ u64 draw(const S& src, float cut, int cut_id, double u) {
-    auto kept = [&](const float (&x)[S::E], int id0, u64 (&e)[S::E]) {
+  // The weights of kept values, for sum_up() and locate().
+  __device__ __forceinline__ auto kept(float cut, int cut_id) const {
+    return [=](const auto& x, int id0, auto& e) {
+      constexpr int E = sizeof(x) / sizeof(float);
       bool any = false;
 #pragma unroll
-      for (int j = 0; j < S::E; ++j) any |= x[j] >= cut;
+      for (int j = 0; j < E; ++j) any |= x[j] >= cut;
       if (!any) return false;
-      float y[S::E];
+      float y[E];
 #pragma unroll
-      for (int j = 0; j < S::E; ++j) y[j] = x[j] >= cut ? x[j] : -INFINITY;
+      for (int j = 0; j < E; ++j) y[j] = x[j] >= cut ? x[j] : -INFINITY;
       if (cut_id != 0x7fffffff) {
 #pragma unroll
-        for (int j = 0; j < S::E; ++j)
+        for (int j = 0; j < E; ++j)
           if (x[j] == cut && id0 + j > cut_id) y[j] = -INFINITY;
       }
 #pragma unroll
-      for (int j = 0; j < S::E; ++j) {
+      for (int j = 0; j < E; ++j) {
         int bin;
         e[j] = mass_bits(y[j], bin);
       }
       return true;
     };
-    sum_up(src, kept);
+  }
+  // The draw: the first kept id at which the cumulative weight exceeds u times the sum. The
+  // sums are those over `some` and each wavefront's own `above`.
+  template <typename S, typename U>
+  __device__ u64 draw(const S& src, const U& some, u64 above, float cut, int cut_id, double u) {
+    sum_up(some, kept(cut, cut_id), above);
     const u64 all = total();
-    locate(src, (u64)(u * (double)all), kept);
+    locate(src, (u64)(u * (double)all), kept(cut, cut_id));
     return all;
+  }
+
+  // About how many values are in bins 0 ... b, by their masses (some percent off).
+  __device__ int about(int b) {
+    float n = 0;
+    for (int i = threadIdx.x; i <= b; i += kSampThreads)
+      n += (float)s.mass[i] * exp2f((i + 0.5f) / (kStep >> kBinShift) - 43.f);
+    const u64 sum = wave_sum((u64)n);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wsum[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    return (int)total();
+  }
+
+  // The values within [v0, v1] into the border list (false: too many), and the wavefront's
+  // sum of the weights above them.
+  __device__ bool split(const Row<T>& row, float v0, float v1, u64& above) {
+    constexpr int E = Row<T>::E;
+    const int w = threadIdx.x >> 6;
+    float* const value = s.list_value[w] + kListCap;
+    int* const id = s.list_id[w] + kListCap;
+    int n = 0;
+    u64 sum = 0;
+    row.each(s, [&](const float (&x)[E], int id0) {
+      int c = 0;
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        c += x[j] >= v0 && x[j] <= v1;
+        any |= x[j] > v1;
+      }
+      if (any) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          int bin;
+          sum += mass_bits(x[j] > v1 ? x[j] : -INFINITY, bin);
+        }
+        sum -= E * kUnit;  // modulo 2^64
+      }
+      if (__ballot(c != 0) == 0) return;
+      const int upto = (int)wave_prefix((u64)c);
+      int at = n + upto - c;
+      if (c != 0) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          if (x[j] >= v0 && x[j] <= v1) {
+            if (at < kBorderCap) value[at] = x[j], id[at] = id0 + j;
+            ++at;
+          }
+        }
+      }
+      n += __builtin_amdgcn_readlane(upto, 63);
+    });
+    above = wave_sum(sum);
+    if ((threadIdx.x & 63) == 0) s.listed[1][w] = n;
+    return !__syncthreads_or(n > kBorderCap);
   }
 
   // The sums of f's weights by wavefront, for total() and locate(): f(values, first id,
   // weights) gives a piece's weights, each under kUnit.
   template <typename S, typename F>
-  __device__ void sum_up(const S& src, F f) {
+  __device__ void sum_up(const S& src, F f, u64 above = 0) {
     u64 sum = 0;
     src.each(s, [&](const float (&x)[S::E], int id0) {
       u64 m[S::E];
@@ -798,7 +850,7 @@ struct Sampler {
       for (int j = 0; j < S::E; ++j) sum += m[j];
       sum -= S::E * kUnit;  // modulo 2^64
     });
-    sum = wave_sum(sum);
+    sum = wave_sum(sum) + above;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s.wsum[threadIdx.x >> 6] = sum;
     __syncthreads();
@@ -955,7 +1007,9 @@ __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a)
   }
   const List<0> list;
   const List<1> border;
-  int listed = 0;          // 1: what can be kept is in the list
+  bool listed = false;     // what can be kept is in the list
+  bool wide = false;       // no: near the border, and its sums are `above` and that list's
+  u64 above = 0;
   float cut = -INFINITY;   // values below it are out, and so are its own ids behind cut_id
   int cut_id = 0x7fffffff;
   unsigned k0, k1;
@@ -975,50 +1029,43 @@ __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a)
     const int b = past ? kBins - 1 : (int)s.found[0];
     const u64 rest = (u64)top_k - 1 - (past ? m.total() : s.found[1]);
     m.around(b, k0, k1);
-    listed = m.template list_up<false>(row, Key<T>::value(k0), 0.f, 0.f);
+    listed = m.list_up(row, Key<T>::value(k0));
     u64 before, own;
     cut = listed ? m.template refine<false>(list, b, rest, -INFINITY, before, own)
                  : m.template refine<false>(row, b, rest, -INFINITY, before, own);
   }
   if (top_p < 1.f) {
-    // Most borders are within 16 octaves of the largest, a border below min-p's does not
-    // matter; only where neither holds are the weights of all values binned.
-    float near = fmaxf(min_cut, (float)((double)best - 16. * kStep / m.steps));
-    u64 all = listed ? m.histogram(list, cut, near) : m.histogram(row, cut, near);
+    // a border below min-p's does not matter
+    const u64 all = listed ? m.histogram(list, cut, min_cut) : m.histogram(row, cut, min_cut);
     // kept: a sum before of at most p times all
     const u64 most = (u64)((double)top_p * (double)all);
     if (most < all) {
       find_prefix(s.mass, kBins, most, s);
-      if (s.found[0] == kBins && near > min_cut) {
-        __syncthreads();
-        for (int i = tid; i < kBins; i += kSampThreads) s.mass[i] = 0;
-        __syncthreads();
-        if (listed) m.histogram(list, cut, min_cut);
-        else m.histogram(row, cut, min_cut);
-        find_prefix(s.mass, kBins, most, s);
-      }
       const int b = (int)s.found[0];
       const u64 rest = most - s.found[1];
       if (b < kBins) {
+        const float floor = cut;
         if (!listed) {
           m.around(b, k0, k1);
-          const float v0 = fmaxf(Key<T>::value(k0), cut);
-          listed = m.template list_up<true>(row, v0, v0, Key<T>::value(k1));
+          const float v0 = fmaxf(Key<T>::value(k0), floor), v1 = Key<T>::value(k1);
+          if (m.about(b) <= kListMost) listed = m.list_up(row, v0);
+          if (!listed) wide = m.split(row, v0, v1, above);
         }
-        const float floor = cut;
-        if (listed & 1) m.nucleus(list, b, rest, floor, cut, cut_id);
-        else if (listed) m.nucleus(border, b, rest, floor, cut, cut_id);
+        if (listed) m.nucleus(list, b, rest, floor, cut, cut_id);
+        else if (wide) m.nucleus(border, b, rest, floor, cut, cut_id);
         else m.nucleus(row, b, rest, floor, cut, cut_id);
       }
     }
   }
-  listed &= 1;
   if (min_cut > cut) {
     cut = min_cut;
     cut_id = 0x7fffffff;
-    if (!listed) listed = m.template list_up<false>(row, cut, 0.f, 0.f);
+    wide = false;
+    if (!listed) listed = m.list_up(row, cut);
   }
-  const u64 all = listed ? m.draw(list, cut, cut_id, (double)u) : m.draw(row, cut, cut_id, (double)u);
+  const u64 all = listed ? m.draw(list, list, 0, cut, cut_id, (double)u)
+                  : wide ? m.draw(row, border, above, cut, cut_id, (double)u)
+                         : m.draw(row, row, 0, cut, cut_id, (double)u);
   if (tid == 0) {
     a.ids[r] = s.at[0];
     if (a.logprobs) {
