@@ -379,6 +379,10 @@ def test_sample_refusals():
         sample_each(x[:, :0], t)
     with pytest.raises(RuntimeError):
         sample_each(x.cpu(), t)
+    with pytest.raises(NotImplementedError):
+        sample_each(x.clone().requires_grad_(), t)
+    with torch.no_grad():
+        sample_each(x.clone().requires_grad_(), t)
     with pytest.raises(TypeError):
         sample_each(x.double(), t)
     ids, lp = sample_each(x[:0], t[:0])

@@ -273,6 +273,39 @@ def test_scheduler_refusals(served):
                          adapter_ids=[0, 0])
 
 
+def test_a_request_that_no_step_could_serve_is_refused_when_it_is_added(served):
+    model, cfg, _, _ = served
+    sched = Scheduler(model, pool_of(cfg), BlockAllocator(64), SimpleNamespace(eos_token_id=-1))
+    with pytest.raises(ValueError, match="outside the vocabulary"):
+        sched.add_request([1], 2, params=RequestParams(logit_bias={VOCAB: 1.0}))
+    with pytest.raises(ValueError, match="infinite logit"):
+        sched.add_request([1], 2, params=RequestParams(logit_bias={1: 3e38}))
+    sched.add_request([1], 3, params=RequestParams(logit_bias={VOCAB - 1: -float("inf")}))
+    words = Words([[3, 5], [4]])
+    sched.add_request([1, 2], 3, params=RequestParams(grammar=words))
+    with pytest.raises(ValueError, match="another request"):  # waiting
+        sched.add_request([3], 3, params=RequestParams(grammar=words))
+    sched.step()
+    with pytest.raises(ValueError, match="another request"):  # running
+        sched.add_request([3], 3, params=RequestParams(grammar=words, temperature=0))
+    while sched.running or sched.waiting:
+        sched.step()
+    sched.add_request([3], 3, params=RequestParams(grammar=words))  # that one is done
+
+
+def test_a_set_loads_all_of_an_adapter_or_nothing(served):
+    model, _, _, _ = served
+    few = AdapterSet(model, 1, 4)
+    state = adapter_state(model, 1, 4)
+    state["layers.2.mlp.down_proj.lora_B.weight"] = torch.zeros(128, 3)
+    with pytest.raises(ValueError, match="are not"):
+        few.load(0, state)
+    with pytest.raises(IndexError):
+        few.load(1, adapter_state(model, 1, 4))
+    assert not any(w.a.any() or w.b.any() or w.scales.any()
+                   for ws in few.layers for w in ws.values())
+
+
 def test_adapter_set_names(served):
     model, cfg, _, _ = served
     few = AdapterSet(model, 1, 4, projections=("qkv",))

@@ -8,7 +8,8 @@ import torch
 from oracle import requests_ref as ref
 from serving import _native
 from serving.adapters import AdapterWeights, _overlap, build_adapter_plan
-from serving.controls import LogitControls, control_logits, sample_each
+from serving.controls import LogitControls, RequestParams, control_logits, sample_each
+from serving.scheduler import Scheduler
 
 
 def test_plan_refusals():
@@ -93,6 +94,33 @@ def test_cpu_tensors_are_refused():
         AdapterWeights(32, (16,), 1001, 8, device="cpu")
     with pytest.raises(TypeError):
         AdapterWeights(32, (16,), 2, 8, dtype=torch.float64, device="cpu")
+
+
+def test_parameters_are_checked_as_the_kernels_get_them():
+    for kw in (dict(temperature=-1), dict(temperature=float("nan")), dict(temperature=1e39),
+               dict(top_k=-1), dict(top_p=0.0), dict(top_p=1e-60), dict(top_p=1.5),
+               dict(min_p=-0.1), dict(min_p=1.5), dict(repetition_penalty=0.0),
+               dict(repetition_penalty=1e-60), dict(repetition_penalty=1e39),
+               dict(presence_penalty=float("inf")), dict(frequency_penalty=1e39),
+               dict(logit_bias={-1: 1.0}), dict(logit_bias={1 << 31: 1.0}),
+               dict(logit_bias={3: float("nan")}), dict(logit_bias={3: 1e39})):
+        with pytest.raises(ValueError):
+            RequestParams(**kw)
+    bias = {3: -1e39, 4: 2}
+    p = RequestParams(temperature=0, top_p=1, repetition_penalty=1e-30, logit_bias=bias)
+    bias[4] = float("nan")  # the request keeps its own
+    assert p.logit_bias[4] == 2
+    with pytest.raises(AttributeError):
+        p.top_p = 2.0
+
+
+def test_a_model_on_the_cpu_takes_no_params():
+    model = torch.nn.Module()
+    model.lm_head = torch.nn.Linear(4, 8)
+    sched = Scheduler(model, None, None, None)
+    with pytest.raises(RuntimeError, match="ROCm"):
+        sched.add_request([1], 2, params=RequestParams())
+    sched.add_request([1], 2)
 
 
 def test_overlap():

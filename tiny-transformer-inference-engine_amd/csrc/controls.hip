@@ -188,7 +188,7 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
         const int i = base + u * TH;
         if (i >= n) break;
         if (blockIdx.y == 0 && (unsigned)id[u] >= (unsigned)a.vocab) bad |= PKV_STATUS_BAD_TOKEN;
-        const unsigned at = (unsigned)(id[u] - lo);
+        const unsigned at = (unsigned)id[u] - (unsigned)lo;
         if (at < (unsigned)(hi - lo) && id[u] >= 0) {
           if (i < prompt) atomicOr(&cnt[at], kInPrompt);
           else atomicAdd(&cnt[at], 1u);

@@ -69,10 +69,7 @@ class AdapterWeights:
             raise IndexError(f"adapter {index} of {self.num_adapters}")
         return index
 
-    @torch.no_grad()
-    def load(self, index: int, parts, scale: float = 1.0) -> None:
-        """Puts an adapter in place `index`: per part (A [r, in_features], B
-        [out_features, r]) with r up to the rank, or None for a part without one."""
+    def _check_parts(self, index, parts):
         self._index(index)
         if len(parts) != len(self.out_features):
             raise ValueError(f"AdapterWeights.load: {len(self.out_features)} parts, "
@@ -87,6 +84,12 @@ class AdapterWeights:
                 raise ValueError(
                     f"AdapterWeights.load: A {tuple(a.shape)} and B {tuple(b.shape)} are not "
                     f"[r, {self.in_features}] and [{n}, r] with r up to {self.rank}")
+
+    @torch.no_grad()
+    def load(self, index: int, parts, scale: float = 1.0) -> None:
+        """Puts an adapter in place `index`: per part (A [r, in_features], B
+        [out_features, r]) with r up to the rank, or None for a part without one."""
+        self._check_parts(index, parts)
         R, k, at = self.rank, self.in_features, 0
         if self.a.shape[2] != k or any(pair is None or pair[0].shape[0] < R for pair in parts):
             self.clear(index)
@@ -308,6 +311,8 @@ class AdapterSet:
                 found.append((w, pairs))
         if left:
             raise ValueError(f"AdapterSet.load: {sorted(left)[0]!r} is no projection of this set")
+        for w, pairs in found:  # all before the first is changed
+            w._check_parts(index, pairs)
         for w, pairs in found:
             w.load(index, pairs, scale)
 

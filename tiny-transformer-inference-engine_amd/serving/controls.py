@@ -189,6 +189,9 @@ def sample_each(logits: torch.Tensor, temperature: torch.Tensor,
     if logits.dim() != 2 or not 0 < logits.shape[1] <= MAX_SAMPLE_VOCAB:
         raise ValueError(f"{what}: expected [rows, 1 to {MAX_SAMPLE_VOCAB}] logits, "
                          f"got {tuple(logits.shape)}")
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise NotImplementedError(
+            f"{what} is forward-only (inference); run it under torch.no_grad()")
     rows, vocab = logits.shape
     dev = logits.device
     for t, dtype, name in ((temperature, torch.float32, "temperature"),
@@ -237,10 +240,15 @@ class Grammar(Protocol):
         """The request took `token`."""
 
 
-@dataclass
+def _f32(x) -> float:
+    return float(torch.tensor(float(x), dtype=torch.float32))
+
+
+@dataclass(frozen=True)
 class RequestParams:
     """What one request of a batch asks for beyond its prompt (Scheduler.add_request);
-    the defaults ask for nothing but a draw at temperature 1."""
+    the defaults ask for nothing but a draw at temperature 1. Numbers are checked as the
+    float32 that the kernels get: a step that fails would fail for the whole batch."""
     temperature: float = 1.0         # 0: the most likely token
     top_k: int = 0                   # 0: off
     top_p: float = 1.0
@@ -248,23 +256,30 @@ class RequestParams:
     repetition_penalty: float = 1.0
     presence_penalty: float = 0.0
     frequency_penalty: float = 0.0
-    logit_bias: dict = field(default_factory=dict)  # id -> value
+    logit_bias: dict = field(default_factory=dict)  # id -> value (-infinity: never)
     grammar: Optional[Grammar] = None
     adapter: int = -1                # of the scheduler's AdapterSet
 
     def __post_init__(self):
-        if not math.isfinite(self.temperature) or self.temperature < 0:
+        f32 = {f.name: _f32(getattr(self, f.name)) for f in fields(self)
+               if isinstance(f.default, float)}
+        if not math.isfinite(f32["temperature"]) or self.temperature < 0:
             raise ValueError("temperature must be finite and >= 0")
         if self.top_k < 0:
             raise ValueError("top_k must be >= 0")
-        if not 0 < self.top_p <= 1:
+        if not 0 < f32["top_p"] <= 1:
             raise ValueError("top_p must be in (0, 1]")
         if not 0 <= self.min_p <= 1:
             raise ValueError("min_p must be in [0, 1]")
-        if not math.isfinite(self.repetition_penalty) or self.repetition_penalty <= 0:
+        if not 0 < f32["repetition_penalty"] < math.inf:
             raise ValueError("repetition_penalty must be finite and > 0")
-        if not (math.isfinite(self.presence_penalty) and math.isfinite(self.frequency_penalty)):
+        if not (math.isfinite(f32["presence_penalty"]) and math.isfinite(f32["frequency_penalty"])):
             raise ValueError("presence_penalty and frequency_penalty must be finite")
+        object.__setattr__(self, "logit_bias", dict(self.logit_bias))
+        for i, v in self.logit_bias.items():
+            if not 0 <= int(i) < 1 << 31 or not _f32(v) < math.inf:
+                raise ValueError("logit_bias names an id below 0, or a value that is NaN or "
+                                 f"infinity ({i}: {v})")
 
     @property
     def has_penalties(self) -> bool:

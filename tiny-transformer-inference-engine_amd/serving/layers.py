@@ -133,7 +133,6 @@ class SwiGLU(nn.Module):
         down = attr(self, "down_proj")
         return fused_ops.linear_residual_(x, h, attr(down, "weight"), attr(down, "bias"))
 
-
     def forward_adapted_residual_(self, x, norm, weights, plan):
         """forward_residual_ with low-rank adapters (serving.adapters): weights holds
         those of the "gate_up" and "down" projections, either may be missing."""

@@ -35,6 +35,8 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import torch
+
 from .batch import BatchStep, build_batch_step
 from .controls import RequestParams, TokenHistory, draw_tokens
 from .sampling import sample
@@ -86,12 +88,11 @@ class Scheduler:
 
     def add_request(self, prompt_ids, max_new_tokens, params=None):
         """params (controls.RequestParams): the request's own sampling parameters,
-        penalties, biases, grammar and adapter, on a ROCm device; without it the
-        scheduler's temperature, top_k and top_p."""
-        if params is not None and params.adapter != -1 and not (
-                self.adapters is not None
-                and 0 <= params.adapter < self.adapters.num_adapters):
-            raise ValueError(f"the scheduler has no adapter {params.adapter}")
+        penalties, biases, grammar (no other request's: it follows this one's tokens) and
+        adapter, on a ROCm device; without it the scheduler's temperature, top_k and
+        top_p."""
+        if params is not None:
+            self._check_params(params)
         if self.sched_cfg is not None:
             sc = self.sched_cfg
             # without chunking a recomputed (preempted) request is prefilled whole,
@@ -108,6 +109,25 @@ class Scheduler:
                                  f"{self.alloc.num_usable} usable")
         self.waiting.append(_Request(list(prompt_ids), max_new_tokens, params=params,
                                      asked_len=len(prompt_ids)))
+
+    def _check_params(self, params: RequestParams) -> None:
+        if self.device.type != "cuda":
+            raise RuntimeError("a request's params require the model on a ROCm GPU device")
+        if params.adapter != -1 and not (
+                self.adapters is not None
+                and 0 <= params.adapter < self.adapters.num_adapters):
+            raise ValueError(f"the scheduler has no adapter {params.adapter}")
+        vocab = self.model.lm_head.out_features
+        if any(i >= vocab for i in params.logit_bias):
+            raise ValueError(f"logit_bias names an id outside the vocabulary of {vocab}")
+        most = torch.finfo(self.model.lm_head.weight.dtype).max / 2
+        if any(v > most for v in params.logit_bias.values()):
+            raise ValueError(f"a logit_bias above {most} would leave an infinite logit")
+        if params.grammar is not None and any(
+                p is not None and p.grammar is params.grammar
+                for p in [r.params for r in self.waiting]
+                + [st.req.params for st in self._state.values()]):
+            raise ValueError("the grammar follows the tokens of another request")
 
     def computed_tokens(self, seq: Sequence) -> int:
         """Tokens of a running sequence whose K/V are in the pool."""
@@ -259,7 +279,6 @@ class Scheduler:
         if not plan:
             self.last_batch_tokens = 0
             return []
-        import torch
         ids = [t for seq, a, b in plan for t in seq.token_ids[a:b]]
         qsl = [0]
         for _, a, b in plan:
