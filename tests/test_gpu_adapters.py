@@ -335,6 +335,55 @@ def test_the_same_bits_every_time_and_on_another_stream():
     assert all(torch.equal(first, o) for o in got)
 
 
+def test_two_streams_and_two_graphs_at_once():
+    """Plans and scratch of calls in flight together are their own."""
+    work, want, graphs, outs = [], [], [], []
+    for T, n, k, parts, rank in ((200, 6, 1024, (512, 512), 16), (1500, 3, 512, (256, 256), 40)):
+        ids, w, x, base, R = problem(T, n, k, parts, rank, torch.bfloat16)
+        work.append((i32(ids), x.to(DEV), base.to(DEV), w, n))
+
+    def step(ids, x, base, w, n):
+        plan = build_adapter_plan(ids, n)
+        return adapter_add(base, x, w, plan), adapter_swiglu(base, x, w, plan)
+
+    want = [step(*a) for a in work]
+    torch.cuda.synchronize()
+    for a in work:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(*a))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        eager = [None, None]
+        for o in outs:
+            for t in o:
+                t.zero_()
+        torch.cuda.synchronize()
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+                eager[1 - i] = step(*work[1 - i])
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(want[i], outs[i]))
+            assert all(torch.equal(a, b) for a, b in zip(want[i], eager[i]))
+
+
+def test_rows_that_are_gigabytes_apart():
+    T, n, k, parts, rank = 5, 2, 96, (64, 32), 8
+    ids, w, x, base, R = problem(T, n, k, parts, rank, torch.bfloat16)
+    far = (1 << 30) - 8  # the last rows begin past 2^31 elements
+    buf = torch.empty(4 * far + 512, dtype=torch.bfloat16, device=DEV)
+    xd, bd = buf.as_strided((T, k), (far, 1)), buf[256:].as_strided((T, sum(parts)), (far, 1))
+    xd.copy_(x)
+    bd.copy_(base)
+    plan = build_adapter_plan(i32(ids), n)
+    want = adapter_add(base.to(DEV), x.to(DEV), w, plan)
+    assert torch.equal(adapter_add(bd, xd, w, plan), want)
+    assert torch.equal(adapter_add(bd, xd, w, plan, out=bd), want)
+
+
 def test_in_a_graph_with_the_plan():
     """Ids, x and base change between replays; eager calls run in between."""
     T, n, k, outs, rank = 64, 5, 256, (128, 128), 16

@@ -392,6 +392,59 @@ def test_sample_refusals():
     assert sample_each(x[:1].expand(3, 20), f32([0.0] * 3))[0].tolist() == [int(x[0].argmax())] * 3
 
 
+def test_the_widest_rows():
+    rng = np.random.default_rng(31)
+    wide = torch.zeros(2, (1 << 20) + 3, device=DEV)
+    x = wide[:, 3:]
+    x.copy_(torch.from_numpy(rng.normal(0, 2, (2, 1 << 20))).float())
+    for k, p, m in ((0, 1.0, 0.0), (0, 0.9, 0.0), (1000, 0.9, 0.0), (0, 1.0, 0.3)):
+        draw_and_check(x, [1.0, 0.6], [k] * 2, [p] * 2, [m] * 2, rng.random(2, dtype=np.float32),
+                       least_checked=0.5)
+    with pytest.raises(ValueError, match="logits"):
+        sample_each(wide, f32([1.0, 1.0]))
+
+
+def test_rows_that_are_gigabytes_apart():
+    rows, vocab, far = 4, 1009, 1 << 30  # the last row begins past 2^31 elements
+    buf = torch.empty(rows - 1, far, dtype=torch.bfloat16, device=DEV)
+    x = buf.view(-1).as_strided((rows, vocab), (far - 1000, 1))
+    p = Problem(rows, vocab, 30, 5, 2, torch.bfloat16)
+    x.copy_(p.logits)
+    t, u = f32([0.0, 0.7, 1.0, 1.0]), f32([0.1, 0.9, 0.5, 0.2])
+    want = sample_each(p.logits.to(DEV), t, i32([0, 5, 0, 9]), None, None, u)
+    got = sample_each(x, t, i32([0, 5, 0, 9]), None, None, u)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    p.check(control_logits(x, p.controls()))
+    p.check(control_logits(x, p.controls(), out=x))
+
+
+def test_two_streams_at_once():
+    p = Problem(40, 20011, 300, 20, 4, torch.bfloat16)
+    q = Problem(24, 20011, 300, 20, 4, torch.bfloat16, seed=1)
+    rng = np.random.default_rng(9)
+    work = []
+    for a in (p, q):
+        t, k, tp, mp, u = params(rng, a.rows)
+        work.append((a.logits.to(DEV), a.controls(), f32(t), i32(k), f32(tp), f32(mp), f32(u)))
+
+    def step(x, c, *pars):
+        y = control_logits(x, c)
+        return (y,) + sample_each(y, *pars)
+
+    want = [step(*a) for a in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*work[i]))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        assert all(torch.equal(a, b) for r in runs for a, b in zip(w[:2], r[:2]))
+        assert all(torch.equal(w[2].nan_to_num(9), r[2].nan_to_num(9)) for r in runs)
+
+
 def test_both_in_a_graph():
     """Histories, parameters and logits change between replays."""
     p = Problem(6, 5003, 50, 10, 3, torch.bfloat16)
