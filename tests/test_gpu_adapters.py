@@ -65,6 +65,21 @@ def test_plan_of_one_adapter_and_of_many_rows():
     check_plan(random_ids(100003, 999, 0.2, g), 999)
 
 
+@pytest.mark.parametrize("lens", [[256] * 16, [4096, 1, 255, 257, 4096], [512, 300, 1200, 64] * 4,
+                                  [16384], [16383, 1], [1000] * 17])
+def test_plan_of_prompts(lens):
+    """Runs of rows of one adapter, some of them of the same."""
+    ids = [a for i, n in enumerate(lens) for a in [(5 * i) % 7 - 1] * n]
+    check_plan(ids, 6)
+    bad = list(ids)
+    bad[len(ids) // 2] = 6
+    st = status()
+    plan = build_adapter_plan(i32(bad), 6, status=st)
+    assert int(st) == _native.PKV_STATUS_BAD_CONTROL
+    bad[len(ids) // 2] = -1
+    assert plan.order.tolist() == ref.plan(bad, 6, plan.tile_rows)[0]
+
+
 def test_plan_reports_ids_of_no_adapter():
     ids = [0, 5, -1, 2, -7, 1, 2 ** 31 - 1, -2 ** 31]
     st = status()

@@ -24,7 +24,7 @@ using namespace mfma;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kMaxAdapters = 1000;  // a counter per wavefront and adapter in 64 KiB of LDS
-constexpr int kBatch = 8;           // rounds of a plan's pass
+constexpr int kBatch = 2;           // rounds of 64 rows that a plan's pass takes together
 constexpr int kMaxSlices = 4;
 
 // ---------------------------------------------------------------------------
@@ -33,7 +33,10 @@ constexpr int kMaxSlices = 4;
 // the rows' order: per-wavefront histograms, a scan over (adapter, wavefront),
 // and a second pass in which the lanes of one adapter find their rank among
 // themselves by ballots. Whole numbers: the result does not depend on the order
-// of the LDS atomics. Latency binds: three passes over ids that stay in L2.
+// of the LDS atomics. A decode step's plan is latency (64 rows: 5.1 us, three round
+// trips and their barriers); a prompts' one is the instructions of the two passes on one CU,
+// so kBatch times 64 rows of one adapter are taken at once (16160 rows of 24 prompts:
+// 12.8 us; 13.5 with 64 at a time, 14.0 with 256, which meet two prompts too often, 19 before).
 // ---------------------------------------------------------------------------
 struct PlanArgs {
   int32_t* order;   // [T]
@@ -82,38 +85,62 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
   const int per = ((a.T + kPlanWaves - 1) / kPlanWaves + 63) & ~63;
   const int t0 = min(w * per, a.T), t1 = min(t0 + per, a.T);
   auto group = [&](int id) { return (unsigned)id < (unsigned)a.N ? id : a.N; };
-  // f(row or -1, its group, the lanes of the same group) for the wavefront's rows, 64 at a
-  // time; the ids of kBatch rounds are requested together
-  auto each = [&](auto f) {
-    for (int base = t0; base < t1; base += 64 * kBatch) {
-      int id[kBatch];
+  // The wavefront's rows, kBatch times 64 at a time, the next ones' ids requested ahead:
+  // all(first row, group) where they are of one group, as a prompt's rows mostly are, else
+  // some(row or -1, its group, the lanes of the same group) for each 64. bad: whether any id
+  // was out of range.
+  auto each = [&](auto all, auto some) {
+    int id[kBatch];
+    bool out = false;
+    auto request = [&](int base) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) id[i] = a.ids[min(base + 64 * i + lane, a.T - 1)];
+    };
+    if (t0 < t1) request(t0);
+    for (int base = t0; base < t1; base += 64 * kBatch) {
+      int g[kBatch];
+      bool differ = base + 64 * kBatch > t1;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        out |= (unsigned)id[i] + 1u > (unsigned)a.N;
+        g[i] = group(id[i]);
+        differ |= g[i] != __builtin_amdgcn_readfirstlane(g[0]);
+      }
+      if (base + 64 * kBatch < t1) request(base + 64 * kBatch);
+      if (__ballot(differ) == 0) {
+        all(base, __builtin_amdgcn_readfirstlane(g[0]));
+        continue;
+      }
 #pragma nounroll
       for (int i = 0; i < kBatch; ++i) {
-        if (base + 64 * i >= t1) break;
         const int t = base + 64 * i + lane;
-        const bool in = t < t1;
-        const int g = in ? group(id[0]) : G;  // G: no group of a row
-        uint64_t same = __ballot(g == __builtin_amdgcn_readfirstlane(g));
-        if (same != ~0ull) {  // rows of a prompt mostly are of one group
+        if (base + 64 * i >= t1) break;
+        int mine = g[0];
+#pragma unroll
+        for (int k = 1; k < kBatch; ++k) mine = i == k ? g[k] : mine;
+        if (t >= t1) mine = G;  // no group of a row
+        uint64_t same = __ballot(mine == __builtin_amdgcn_readfirstlane(mine));
+        if (same != ~0ull) {
           same = ~0ull;
           for (int bit = 1; bit <= G; bit <<= 1) {
-            const uint64_t set = __ballot((g & bit) != 0);
-            same &= (g & bit) ? set : ~set;
+            const uint64_t set = __ballot((mine & bit) != 0);
+            same &= (mine & bit) ? set : ~set;
           }
         }
-        f(in ? t : -1, id[0], g, same);
-#pragma unroll
-        for (int k = 0; k + 1 < kBatch; ++k) id[k] = id[k + 1];
+        some(t < t1 ? t : -1, mine, same);
       }
     }
+    return out;
   };
-  each([&](int t, int id, int g, uint64_t same) {
-    if (t >= 0 && (id < -1 || id >= a.N)) bad = PKV_STATUS_BAD_CONTROL;
-    if (t >= 0 && lane == __ffsll((unsigned long long)same) - 1)
-      atomicAdd(&cnt[w * G + g], __popcll(same));
-  });
+  const bool out_of_range = each(
+      [&](int, int g) {
+        if (lane == 0) atomicAdd(&cnt[w * G + g], 64 * kBatch);
+      },
+      [&](int t, int g, uint64_t same) {
+        if (t >= 0 && lane == __ffsll((unsigned long long)same) - 1)
+          atomicAdd(&cnt[w * G + g], __popcll(same));
+      });
+  if (out_of_range) bad = PKV_STATUS_BAD_CONTROL;
   __syncthreads();
   int mine = 0;  // rows of group tid
   if (tid < G)
@@ -139,24 +166,54 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(PlanArgs a) 
   }
   __syncthreads();
   const int rows_log = a.tile_rows == 16 ? 4 : 6;
-  each([&](int t, int, int g, uint64_t same) {
-    const int leader = __ffsll((unsigned long long)same) - 1;
-    int at = 0;
-    if (t >= 0 && lane == leader) at = atomicAdd(&cnt[w * G + g], __popcll(same));
-    at = __shfl(at, leader);
-    if (t >= 0) {
-      at += __popcll(same & ((1ull << lane) - 1));
-      a.order[at] = t;
-      const int place = at - first_row[g], tile = first_tile[g] + (place >> rows_log);
-      if (tile < a.max_tiles) {
-        int32_t* rows = a.rows + (int64_t)tile * a.tile_rows;
-        const int i = place & (a.tile_rows - 1);
-        rows[i] = t;
-        if (at + 1 == first_row[g + 1])  // the group's last row fills its last tile
-          for (int j = i + 1; j < a.tile_rows; ++j) rows[j] = t;
-      }
-    }
-  });
+  const int last = a.tile_rows - 1;
+  // row t at place `at` of the order, which is of group g
+  auto put = [&](int t, int at, int first, int tile0) {
+    a.order[at] = t;
+    const int place = at - first, tile = tile0 + (place >> rows_log);
+    if (tile < a.max_tiles) a.rows[((int64_t)tile << rows_log) + (place & last)] = t;
+  };
+  // the rows of a group's last tile behind its last row t, at place `at`: t as well
+  auto fill = [&](int t, int at, int first, int tile0) {
+    const int place = at - first, tile = tile0 + (place >> rows_log);
+    const int i = (place & last) + 1 + lane;
+    if (i <= last && tile < a.max_tiles) a.rows[((int64_t)tile << rows_log) + i] = t;
+  };
+  each(
+      [&](int base, int g) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&cnt[w * G + g], 64 * kBatch);
+        at = __builtin_amdgcn_readfirstlane(at);
+        const int first = first_row[g], tile0 = first_tile[g];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) put(base + 64 * i + lane, at + 64 * i + lane, first, tile0);
+        const int n = at + 64 * kBatch;
+        if (n == first_row[g + 1]) fill(base + 64 * kBatch - 1, n - 1, first, tile0);
+      },
+      [&](int t, int g, uint64_t same) {
+        const int leader = __ffsll((unsigned long long)same) - 1;
+        int at = 0;
+        if (t >= 0 && lane == leader) at = atomicAdd(&cnt[w * G + g], __popcll(same));
+        at = __shfl(at, leader) + __popcll(same & ((1ull << lane) - 1));
+        const int of = t >= 0 ? g : 0;
+        const int first = first_row[of], tile0 = first_tile[of];
+        if (t >= 0) put(t, at, first, tile0);
+        const bool end = t >= 0 && at + 1 == first_row[of + 1];
+        uint64_t ends = __ballot(end);
+        if (4 * __popcll(ends) > a.tile_rows) {  // each lane its own tile
+          const int place = at - first, tile = tile0 + (place >> rows_log);
+          int32_t* const rows = a.rows + ((int64_t)tile << rows_log);
+          if (end && tile < a.max_tiles)
+            for (int i = (place & last) + 1; i <= last; ++i) rows[i] = t;
+          ends = 0;
+        }
+        while (ends) {  // all lanes one tile
+          const int l = __ffsll((unsigned long long)ends) - 1;
+          ends &= ends - 1;
+          fill(__builtin_amdgcn_readlane(t, l), __builtin_amdgcn_readlane(at, l),
+               __builtin_amdgcn_readlane(first, l), __builtin_amdgcn_readlane(tile0, l));
+        }
+      });
   for (int i = tid; i < a.max_tiles; i += kPlanThreads) {
     int lo = 0, hi = G;  // the last group whose first tile is at most i
     while (lo < hi) {
