@@ -663,7 +663,8 @@ int pkv_write_accepted_step(void* k_pool, void* v_pool, int64_t pool_layer_elems
  * one, and n_tokens. tiles [max_tiles][4] (16-byte aligned): pieces of at most tile_rows
  * (16 or 64) rows of one adapter, as {adapter or -1, first place, rows, 0}, unused
  * entries with 0 rows; rows [max_tiles][tile_rows]: the tiles' rows, the last one
- * repeated; max_tiles at least n_tokens / tile_rows + min(n_adapters + 1, n_tokens). At most 1000 adapters and 2^24 rows.
+ * repeated; max_tiles at least n_tokens / tile_rows + min(n_adapters + 1, n_tokens). At
+ * most 1000 adapters and 2^24 rows.
  */
 int pkv_adapter_plan(int32_t* order, int32_t* starts, int32_t* tiles, int32_t* rows,
                      int max_tiles, const int32_t* ids, int n_tokens, int n_adapters, int tile_rows,
