@@ -314,6 +314,34 @@ def test_more_values_than_are_listed(dtype):
     draw_and_check(x, [0.01, 0.05, 0.2, 0.3] * 5, [40000, 1000, 300, 50000] * 5, p, m, u)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("order", ["mixed", "sorted", "ties"])
+def test_a_row_draws_the_same_in_any_batch(dtype, order):
+    """Few long rows are split over workgroups, many are not."""
+    rng = np.random.default_rng(77)
+    rows, vocab, times = 24, 50257, 26
+    x = rng.normal(0, 2.5, (rows, vocab))
+    if order == "sorted":  # what is kept lies together
+        x = np.sort(x, axis=1)
+    elif order == "ties":
+        x = np.round(x)
+    x = torch.from_numpy(x).to(dtype).to(DEV)
+    t = [1.0, 0.7, 1.4, 0.0, 0.3, 3.0] * 4
+    k = [0, 0, 0, 5, 400, 20000] * 2 + [0, 50, 0, 0, 0, 9000] * 2
+    p = [1.0, 0.9, 0.95, 0.5] * 6
+    m = [0.0, 0.0, 0.02, 0.0, 0.0, 0.1] * 4
+    u = rng.random(rows, dtype=np.float32)
+    few = sample_each(x, f32(t), i32(k), f32(p), f32(m), f32(u))
+    many = sample_each(x.repeat(times, 1), f32(t * times), i32(k * times), f32(p * times),
+                       f32(m * times), f32(u).repeat(times))
+    assert torch.equal(few[0].repeat(times), many[0])
+    assert torch.equal(few[1].repeat(times), many[1])
+    for i in range(rows):  # and alone
+        one = sample_each(x[i:i + 1], f32(t[i:i + 1]), i32(k[i:i + 1]), f32(p[i:i + 1]),
+                          f32(m[i:i + 1]), f32(u[i:i + 1]))
+        assert torch.equal(one[0], few[0][i:i + 1]) and torch.equal(one[1], few[1][i:i + 1])
+
+
 def test_far_apart_and_extreme_parameters():
     rng = np.random.default_rng(5)
     x = torch.from_numpy(rng.normal(0, 1, (32, 500)) * 1e4).float().to(DEV)
