@@ -319,12 +319,12 @@ int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
 // the values that can be kept, or, where they are many, those near the border and the sum above
 // them, into LDS, where the border's bin is looked at by the bits of its keys until one is
 // left; the place in the ids at which the cumulative weight passes. What binds is the weights'
-// arithmetic: some twenty 64-bit operations each, at the rate of 32-bit ones here, 10 to 14 us a
-// pass over 50257 on one CU. 128 such rows (bf16): greedy 12 us, without a filter 25, top_k of 50
-// 22, with top_p as well 30, a nucleus of 5600 41, of 22000 49; rows of every kind 49.5, the
-// slowest of them. Splitting a row over workgroups takes a launch a pass, each with its own
-// tables, dispatch and round trips: 83 us for the 128 rows, the same for 4 rows, so it is not
-// done.
+// arithmetic: 22 instructions each, half of them of 64 bits at the rate of 32-bit ones here, 9
+// to 13 us a pass over 50257 on one CU, whose issue slots are two thirds full. 128 such rows
+// (bf16): greedy 12 us, without a filter 24, top_k of 50 22, with top_p as well 30, a nucleus
+// of 5600 39, of 22000 46; rows of every kind 42 to 46, the slowest of them. Splitting a row over
+// workgroups takes a launch a pass, each with its own tables, dispatch and round trips: 83 us
+// for the 128 rows when this took 49, the same for 4 rows, so it is not done.
 // ---------------------------------------------------------------------------
 struct SampleArgs {
   int64_t* ids;
@@ -360,15 +360,16 @@ constexpr int kBinShift = kStepBits - 5;
 // a border (some 30 of a row's bin); with them the workgroup takes 155 KB of a CU's 160.
 constexpr int kListCap = 640;
 constexpr int kBorderCap = 128;
-// The most values that a nucleus is listed with: 4/5 of the list, for the wavefronts differ.
-// 128 rows of 50257 with some 5600 each take 43 us by the list and 49 by the border alone,
-// whose time does not rise with the number (22000: 57 us by a list that overflows).
-constexpr int kListMost = kSampWaves * kListCap / 5 * 4;
+// The most values that a nucleus is listed with: 7/10 of the list, for the wavefronts differ and
+// the border's bin comes with some keys around it. 128 rows of 50257 with some 5600 each take
+// 39 us by the list and 46 by the border alone, whose time does not rise with the number (22000:
+// 51 us by a list that overflows first).
+constexpr int kListMost = kSampWaves * kListCap / 10 * 7;
 
 struct SampShared {
   u32x4 edge[3];
   int listed[2][kSampWaves];  // entries of list and border list
-  double pow[kStep];  // 2^43 2^(-j / kStep)
+  double pow[kStep];  // 2^43 2^(j / kStep) less j in its exponent's low bits (weight())
   u64 mass[kBins];
   unsigned count[kBins];
   u64 wsum[kSampWaves];
@@ -535,6 +536,18 @@ __device__ __forceinline__ u64 wave_scan(u64 x, Op op) {
   x = op(x, lanes<0x142, 0xA>(x));
   return op(x, lanes<0x143, 0xC>(x));
 }
+template <int CTRL, int RM>
+__device__ __forceinline__ int lanes(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, RM, 0xF, true);
+}
+__device__ __forceinline__ int wave_prefix(int x) {
+  x += lanes<0x111, 0xF>(x);
+  x += lanes<0x112, 0xF>(x);
+  x += lanes<0x114, 0xF>(x);
+  x += lanes<0x118, 0xF>(x);
+  x += lanes<0x142, 0xA>(x);
+  return x + lanes<0x143, 0xC>(x);
+}
 __device__ __forceinline__ u64 last_lane(u64 x) {
   return (u64)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), 63) << 32 |
          (unsigned)__builtin_amdgcn_readlane((int)x, 63);
@@ -581,18 +594,21 @@ struct Sampler {
   // The whole steps of a distance below 2^31, rounded: adding 3 2^51 leaves them in the
   // low bits, at the rate of an addition (a conversion runs at a quarter of it).
   static constexpr double kShift = 6755399441055744.;
-  // 2^43 2^(-z / kStep) for a distance z of at most 60 octaves, and the steps n of z: the
-  // whole steps from the table and by the exponent, the rest r, at most half a step, as a
-  // polynomial whose next term is below 2^-43. (A pass is bound by its instructions: a table
-  // of 32 entries, without bank conflicts, and three more terms took 1 us more for 128 rows.)
+  // 2^43 2^(-z / kStep) for a distance z of at most 60 octaves, and the steps n of z: of
+  // -n = kStep o + j the j steps from the table and the octaves o by its exponent (the entry has
+  // j taken off there, so that adding -n at once adds o), the rest r, at most half a step,
+  // as a polynomial whose next term is below 2^-43. (A pass is bound by its instructions: a
+  // table of 32 entries, without bank conflicts, and three more terms took 1 us more for 128
+  // rows.)
   __device__ __forceinline__ double weight(double z, int& n) const {
     constexpr double c = 0.69314718055994530942 / kStep;
-    const double y = z + kShift;
-    n = __double2loint(y);
-    const double r = z - (y - kShift);
+    const double y = kShift - z;
+    const int less = __double2loint(y);
+    n = -less;
+    const double r = z + (y - kShift);
     const double q = fma(r, fma(r, c * c / 2., -c), 1.);
-    const double t = s.pow[n & (kStep - 1)] * q;
-    return __hiloint2double(__double2hiint(t) - ((n >> kStepBits) << 20), __double2loint(t));
+    const double t = s.pow[less & (kStep - 1)];
+    return __hiloint2double(__double2hiint(t) + (less << (20 - kStepBits)), __double2loint(t)) * q;
   }
   // The nearest whole number to w < 2^52 in the low 52 bits, under the bits kUnit.
   static constexpr u64 kUnit = 0x4330000000000000ull;
@@ -634,7 +650,7 @@ struct Sampler {
 #pragma unroll
       for (int j = 0; j < E; ++j) c += x[j] >= from;
       if (__ballot(c != 0) == 0) return;
-      const int upto = (int)wave_prefix((u64)c);
+      const int upto = wave_prefix(c);
       int at = n + upto - c;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -724,11 +740,12 @@ struct Sampler {
   // The sums of the weights of at least `near` by bin in s.mass (cleared before), and the
   // total of those of at least `floor`. (The atomics cost nothing beside the weights: the
   // same time with those of 16 octaves alone, or of 3.)
-  template <typename S>
+  // kAll: without a floor.
+  template <bool kAll, typename S>
   __device__ u64 histogram(const S& src, float floor, float near) {
     u64 sum = 0;
     src.each(s, [&](const float (&x)[S::E], int) {
-      bool any = false;
+      bool any = kAll;
 #pragma unroll
       for (int j = 0; j < S::E; ++j) any |= x[j] >= floor;
       if (!any) return;
@@ -736,7 +753,7 @@ struct Sampler {
       int at[S::E];
 #pragma unroll
       for (int j = 0; j < S::E; ++j) {
-        e[j] = mass_bits(x[j] >= floor ? x[j] : -INFINITY, at[j]);
+        e[j] = mass_bits(kAll || x[j] >= floor ? x[j] : -INFINITY, at[j]);
         sum += e[j];
       }
       sum -= S::E * kUnit;  // modulo 2^64
@@ -809,11 +826,11 @@ struct Sampler {
     int n = 0;
     u64 sum = 0;
     row.each(s, [&](const float (&x)[E], int id0) {
-      int c = 0;
+      unsigned bits = 0;  // the few near the border
       bool any = false;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        c += x[j] >= v0 && x[j] <= v1;
+        bits |= (x[j] >= v0 && x[j] <= v1 ? 1u : 0u) << j;
         any |= x[j] > v1;
       }
       if (any) {
@@ -824,17 +841,14 @@ struct Sampler {
         }
         sum -= E * kUnit;  // modulo 2^64
       }
-      if (__ballot(c != 0) == 0) return;
-      const int upto = (int)wave_prefix((u64)c);
-      int at = n + upto - c;
-      if (c != 0) {
+      if (__ballot(bits != 0) == 0) return;
+      const int c = __popc(bits), upto = wave_prefix(c);
+      for (int at = n + upto - c; bits; bits &= bits - 1, ++at) {
+        const int k = __ffs(bits) - 1;
+        float y = x[0];
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-          if (x[j] >= v0 && x[j] <= v1) {
-            if (at < kBorderCap) value[at] = x[j], id[at] = id0 + j;
-            ++at;
-          }
-        }
+        for (int j = 1; j < E; ++j) y = k == j ? x[j] : y;
+        if (at < kBorderCap) value[at] = y, id[at] = id0 + k;
       }
       n += __builtin_amdgcn_readlane(upto, 63);
     });
@@ -932,11 +946,16 @@ __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a)
   const float u = a.uniforms[r];
   {
     static_assert(kStep == 4 * kSampThreads, "four entries a thread");
-    const double e = kOne * exp2(-(double)tid / kStep);  // and 2^(-1/4), 2^(-1/2), 2^(-3/4) of it
-    s.pow[tid] = e;
-    s.pow[tid + kSampThreads] = e * 0.84089641525371454303;
-    s.pow[tid + 2 * kSampThreads] = e * 0.70710678118654752440;
-    s.pow[tid + 3 * kSampThreads] = e * 0.59460355750136053336;
+    // 2^43 2^(j / kStep), and 2^(1/4), 2^(1/2), 2^(3/4) of it
+    const double e = kOne * exp2((double)tid / kStep);
+    const double f[4] = {e, e * 1.18920711500272106672, e * 1.41421356237309504880,
+                         e * 1.68179283050742908606};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = tid + i * kSampThreads;
+      s.pow[j] = __hiloint2double(__double2hiint(f[i]) - (j << (20 - kStepBits)),
+                                  __double2loint(f[i]));
+    }
   }
   for (int i = tid; i < kBins; i += kSampThreads) s.count[i] = 0, s.mass[i] = 0;
 
@@ -1041,7 +1060,9 @@ __global__ __launch_bounds__(kSampThreads) void sample_each_kernel(SampleArgs a)
   }
   if (top_p < 1.f) {
     // a border below min-p's does not matter
-    const u64 all = listed ? m.histogram(list, cut, min_cut) : m.histogram(row, cut, min_cut);
+    const u64 all = listed            ? m.template histogram<false>(list, cut, min_cut)
+                    : cut > -INFINITY ? m.template histogram<false>(row, cut, min_cut)
+                                      : m.template histogram<true>(row, cut, min_cut);
     // kept: a sum before of at most p times all
     const u64 most = (u64)((double)top_p * (double)all);
     if (most < all) {
