@@ -132,6 +132,34 @@ def test_control_logits(shape, dtype):
     assert torch.equal(control_logits(x, LogitControls()), x)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1100, 90, 20, 4, 2), (85, 50257, 300, 40, 2)])
+def test_control_logits_of_many_workgroups(shape, dtype):
+    print(f"[controls] {shape} {dtype}", flush=True)
+    p = Problem(*shape, dtype)
+    x = p.logits.to(DEV)
+    p.check(control_logits(x, p.controls()))
+    wide = torch.zeros(p.rows, p.vocab + 5, dtype=dtype, device=DEV)
+    y = wide[:, 3:3 + p.vocab]
+    y.copy_(x)
+    p.check(control_logits(y, p.controls(), out=y))
+    assert not wide[:, :3].any() and not wide[:, 3 + p.vocab:].any()
+
+
+def test_biases_that_share_places():
+    """Ids whose places collide, each of them several times, more than a batch of them."""
+    rng = np.random.default_rng(12)
+    vocab = 60000
+    ids = rng.choice(np.arange(0, vocab, 1024), 1500)
+    values = rng.choice([1.0, -3.0, 1e-3, 1e4], 1500).astype(np.float32)
+    x = torch.zeros(1, vocab, device=DEV)
+    c = LogitControls(bias_ids=i32(ids), bias_values=f32(values), bias_starts=i32([0, 1500]))
+    want = np.zeros(vocab, dtype=np.float32)
+    for i, v in zip(ids, values):
+        want[i] = np.float32(want[i] + v)  # in the list's order, rounded at every step
+    assert np.array_equal(control_logits(x, c)[0].cpu().numpy(), want)
+
+
 def test_an_id_named_many_times_is_added_up_in_order():
     """Values whose sum depends on the order: 1e8, 1, -1e8, 1 in fp32 gives 1; and lists
     longer than a workgroup, of one id and of two in turn."""

@@ -281,6 +281,9 @@ def test_a_request_that_no_step_could_serve_is_refused_when_it_is_added(served):
     with pytest.raises(ValueError, match="infinite logit"):
         sched.add_request([1], 2, params=RequestParams(logit_bias={1: 3e38}))
     sched.add_request([1], 3, params=RequestParams(logit_bias={VOCAB - 1: -float("inf")}))
+    short = SimpleNamespace(mask=lambda: torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="words"):
+        sched.add_request([1], 2, params=RequestParams(grammar=short))
     words = Words([[3, 5], [4]])
     sched.add_request([1, 2], 3, params=RequestParams(grammar=words))
     with pytest.raises(ValueError, match="another request"):  # waiting

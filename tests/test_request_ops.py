@@ -110,6 +110,7 @@ def test_parameters_are_checked_as_the_kernels_get_them():
     p = RequestParams(temperature=0, top_p=1, repetition_penalty=1e-30, logit_bias=bias)
     bias[4] = float("nan")  # the request keeps its own
     assert p.logit_bias[4] == 2
+    assert RequestParams(logit_bias={"7": np.float32(1.5)}).logit_bias == {7: 1.5}
     with pytest.raises(AttributeError):
         p.top_p = 2.0
 

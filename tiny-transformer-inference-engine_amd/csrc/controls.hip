@@ -39,10 +39,10 @@ __device__ __forceinline__ void load_piece(const T* row, int id0, int vocab, T f
 // ---------------------------------------------------------------------------
 // Penalties, biases, masks. A workgroup takes one row and a range of its ids: it requests
 // the range's logits, counts the row's history over the range in LDS, adds up the biases
-// there, and changes what it holds. Bytes bind (logits in and out, once); the history
-// is read once per range, from L2 after the first. What is in the way is a chain of round
-// trips (lengths, then ids, then barriers), so ranges are small and many workgroups share a
-// CU.
+// there, and changes what it holds. Bytes bind at least (logits in and out, once: 5 us for 128
+// rows of 50257 in bf16); the history is read once per range, from L2 after the first. What
+// is in the way is a chain of round trips and barriers: of those rows' 14.9 us, 7 remain without
+// any control, a history of some 1150 tokens adds 4.5, 40 biases 2.5, a mask 1.
 // ---------------------------------------------------------------------------
 struct ControlArgs {
   void* out;
@@ -72,7 +72,11 @@ struct ControlArgs {
 // An id's record: how often it is behind the prompt, and whether the prompt holds it.
 constexpr unsigned kInPrompt = 0x80000000u;
 constexpr int kMaxHistory = 1 << 30;
-constexpr int kAlike = 1024;  // counters of biases whose ids are alike modulo as much
+// Places for the ids of a batch of biases, by a hash of them.
+constexpr int kPlaceBits = 10, kPlaces = 1 << kPlaceBits;
+__device__ __forceinline__ int place_of(int id) {
+  return (int)((unsigned)id * 2654435761u >> (32 - kPlaceBits));
+}
 
 // TH threads, S pieces each: a range of TH S pieces.
 template <typename T, int TH, int S>
@@ -80,9 +84,9 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
   constexpr int E = kPiece<T>;
   constexpr int R = TH * S * E;
   static_assert(S * E <= 32, "a bit an id");
-  __shared__ __attribute__((aligned(16))) unsigned cnt[R];  // records, then the biases' claims
-  __shared__ __attribute__((aligned(16))) float vals[R];
-  __shared__ unsigned alike[kAlike];
+  __shared__ __attribute__((aligned(16))) unsigned cnt[R];  // records, then the changed logits
+  __shared__ unsigned alike[kPlaces];  // how many biases have a place, then their claims on it
+  float* const vals = reinterpret_cast<float*>(cnt);
   const int tid = threadIdx.x;
   const int r = blockIdx.x;
   const T* in = static_cast<const T*>(a.in) + (int64_t)r * a.in_stride;
@@ -159,14 +163,20 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
   const float pres = a.presence ? a.presence[r] : 0.f;
   const float freq = a.frequency ? a.frequency[r] : 0.f;
 
-  bool staged = false;  // the range's logits are in vals
+  unsigned bits = 0;    // this thread's ids that the history changed; theirs are in vals
+  bool staged = false;  // the range's logits are
   auto stage = [&]() {
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
-      for (int j = 0; j < E; j += 4)
-        *reinterpret_cast<floatx4*>(&vals[(s * TH + tid) * E + j]) =
-            floatx4{(float)v[s][j], (float)v[s][j + 1], (float)v[s][j + 2], (float)v[s][j + 3]};
+      for (int j = 0; j < E; j += 4) {
+        floatx4& to = *reinterpret_cast<floatx4*>(&vals[(s * TH + tid) * E + j]);
+        floatx4 x = to;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (!(bits >> (s * E + j + k) & 1)) x[k] = (float)v[s][j + k];
+        to = x;
+      }
     staged = true;
   };
   const bool biased = b1 > b0;
@@ -174,9 +184,9 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
   if (n > 0)
     for (int i = tid * 4; i < R; i += TH * 4) *reinterpret_cast<u32x4*>(&cnt[i]) = u32x4{};
   if (biased)
-    for (int i = tid; i < kAlike; i += TH) alike[i] = 0;
+    for (int i = tid; i < kPlaces; i += TH) alike[i] = 0;
   if (n > 0 || biased) __syncthreads();
-  if (todo) atomicAdd(&alike[bid & (kAlike - 1)], 1u);
+  if (todo) atomicAdd(&alike[place_of(bid)], 1u);
   if (n > 0) {
     for (int base = tid; base < n; base += U * TH) {
       if (base != tid) {
@@ -197,9 +207,8 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
     }
     __syncthreads();
     // Few ids change, and a change is some thirty operations (a division among them): each
-    // thread finds its own by their bits and changes them in LDS one by one, not all of a
-    // piece where it stands.
-    unsigned bits = 0;
+    // thread finds its own by their bits and changes them one by one, the results where the
+    // records were, not all of a piece.
 #pragma unroll
     for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -208,23 +217,24 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) bits |= (c[k] != 0u ? 1u : 0u) << (s * E + j + k);
       }
-    stage();
-    while (bits) {
-      const int k = __ffs(bits) - 1;
-      bits &= bits - 1;
+    for (unsigned left = bits; left; left &= left - 1) {
+      const int k = __ffs(left) - 1;
       const int at = (k / E * TH + tid) * E + k % E;
       const unsigned c = cnt[at];
-      float x = vals[at];
+      float x = (float)v[0][0];
+#pragma unroll
+      for (int i = 1; i < S * E; ++i) x = k == i ? (float)v[i / E][i % E] : x;
       x = x > 0.f ? x / rep : x * rep;
       const unsigned made = c & ~kInPrompt;
       if (made) x -= freq * (float)made + pres;
       vals[at] = x;
     }
+    stage();
   }
-  // Biases. The first batch's that no other is alike are added at once. The others, in the
-  // order of the list where it names an id twice: the entries of a batch claim their ids, the
-  // first of each adds its value, and so on until all have.
-  bool claims = false;  // cnt is ready for claims
+  // Biases. The first batch's that have a place of their own are added at once. The others, in
+  // the order of the list where it names an id twice: the entries of a batch claim their places,
+  // the first of each adds its value, and so on until all have.
+  bool claims = false;  // alike is ready for claims
   for (int base = b0; base < b1; base += TH) {
     if (base != b0) {
       request(base);
@@ -232,7 +242,7 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
     } else {
       if (!staged) stage();
       __syncthreads();
-      if (todo && alike[bid & (kAlike - 1)] == 1) {
+      if (todo && alike[place_of(bid)] == 1) {
         vals[bid - lo] += badd;
         todo = false;
       }
@@ -241,17 +251,17 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
       bad |= PKV_STATUS_BAD_TOKEN;
     if (!__syncthreads_or(todo)) continue;
     if (!claims) {
-      for (int i = tid; i < R; i += TH) cnt[i] = ~0u;
+      for (int i = tid; i < kPlaces; i += TH) alike[i] = ~0u;
       claims = true;
       __syncthreads();
     }
-    const int at = bid - lo;
+    unsigned& claim = alike[place_of(bid)];
     do {
-      if (todo) atomicMin(&cnt[at], (unsigned)tid);
+      if (todo) atomicMin(&claim, (unsigned)tid);
       __syncthreads();
-      if (todo && cnt[at] == (unsigned)tid) {
-        vals[at] += badd;
-        cnt[at] = ~0u;
+      if (todo && claim == (unsigned)tid) {
+        vals[bid - lo] += badd;
+        claim = ~0u;
         todo = false;
       }
     } while (__syncthreads_or(todo));
@@ -295,10 +305,16 @@ int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
   return check_launch("control_logits");
 }
 
+// 8 ids a thread, 4096 a workgroup, where the chip's 1024 places for workgroups of 512 threads
+// hold all of them (4 rows of 50257, fp32: 4.2 us against 5.1); else 16, half the workgroups,
+// which read and count a row's history half as often (64 rows of 131072, histories to 8192: 20.6
+// us against 23.5; 128 rows of 50257, to 2048: 15.9 and 15.8). 256 threads: 15.5 and 29.8 for the
+// last two, 1024: 19.8 and 26.4.
 template <typename T>
 int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
   constexpr int S = 8 / kPiece<T>;
-  return launch_control<T, 512, S>(a, rows, st);
+  if (rows * ((a.vocab + 4095) / 4096) <= 1024) return launch_control<T, 512, S>(a, rows, st);
+  return launch_control<T, 512, 2 * S>(a, rows, st);
 }
 
 // ---------------------------------------------------------------------------

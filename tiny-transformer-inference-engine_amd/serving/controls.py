@@ -275,9 +275,10 @@ class RequestParams:
             raise ValueError("repetition_penalty must be finite and > 0")
         if not (math.isfinite(f32["presence_penalty"]) and math.isfinite(f32["frequency_penalty"])):
             raise ValueError("presence_penalty and frequency_penalty must be finite")
-        object.__setattr__(self, "logit_bias", dict(self.logit_bias))
+        object.__setattr__(self, "logit_bias",
+                           {int(i): float(v) for i, v in self.logit_bias.items()})
         for i, v in self.logit_bias.items():
-            if not 0 <= int(i) < 1 << 31 or not _f32(v) < math.inf:
+            if not 0 <= i < 1 << 31 or not _f32(v) < math.inf:
                 raise ValueError("logit_bias names an id below 0, or a value that is NaN or "
                                  f"infinity ({i}: {v})")
 

@@ -123,11 +123,15 @@ class Scheduler:
         most = torch.finfo(self.model.lm_head.weight.dtype).max / 2
         if any(v > most for v in params.logit_bias.values()):
             raise ValueError(f"a logit_bias above {most} would leave an infinite logit")
-        if params.grammar is not None and any(
-                p is not None and p.grammar is params.grammar
-                for p in [r.params for r in self.waiting]
-                + [st.req.params for st in self._state.values()]):
-            raise ValueError("the grammar follows the tokens of another request")
+        if params.grammar is not None:
+            if any(p is not None and p.grammar is params.grammar
+                   for p in [r.params for r in self.waiting]
+                   + [st.req.params for st in self._state.values()]):
+                raise ValueError("the grammar follows the tokens of another request")
+            words = tuple(params.grammar.mask().shape)
+            if words != (-(-vocab // 32),):
+                raise ValueError(f"the grammar's mask must be [{-(-vocab // 32)}] words "
+                                 f"(got {list(words)})")
 
     def computed_tokens(self, seq: Sequence) -> int:
         """Tokens of a running sequence whose K/V are in the pool."""
