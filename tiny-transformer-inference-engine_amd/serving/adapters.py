@@ -211,6 +211,10 @@ def _apply(base, x, weights, plan, out, written, epilogue, what):
     try:
         if out is None:
             out, out_stride = base.new_empty((T, written)), written
+        elif in_place and out is base and written == n:  # and not a copy of its rows
+            out_stride = base_stride
+            if _overlap(out, x):
+                raise ValueError(f"{what}: out shares memory with base or x")
         else:
             if out.shape != (T, written) or out.dtype != dtype or out.get_device() != place:
                 raise ValueError(f"{what}: out must be [{T}, {written}] {dtype} on {dev}")
