@@ -682,9 +682,13 @@ size_t pkv_adapter_workspace_bytes(int n_tokens, int max_tiles, int tile_rows, i
  * base [n_tokens, n] is the projection's output, n = the sum of the features n0 ...
  * of its 1 to 4 parts. With row t's adapter i of the plan (tiles, rows):
  *   y[t] = base[t] + scales[i] * b[i] (a[i] x[t])
- * where a [n_adapters, parts * rank, k] (rows a_stride elements apart, a multiple of 32,
- * zeros behind k) and b [n_adapters, n, rank]; the features of part s use the ranks
- * s * rank ... (s + 1) * rank - 1. Rows without an adapter get y = base. All sums
+ * where a is [parts * rank, k] and b [n, rank]; the features of part s use the ranks
+ * s * rank ... (s + 1) * rank - 1. Both are laid out as the kernels' lanes read them: a
+ * [n_adapters][parts][rank * a_stride], a_stride at least k and a multiple of 32, zeros behind
+ * k, of each part the ranks in blocks of 16 (the last may have 8): block, 8s of k, rank of
+ * the block, element; b [n_adapters][features of each part rounded up to 64, zeros there][rank],
+ * of each 64 features: 8s of ranks, feature in the order 32 h + 8 q + 4 l + e of h < 2, l < 2,
+ * q < 4, e < 4, rank of the 8. Rows without an adapter get y = base. All sums
  * are fp32, also a[i] x[t], and y is rounded once. PKV_EPILOGUE_NONE: out [n_tokens, n] =
  * y; out may be base itself (same address and stride). PKV_EPILOGUE_SWIGLU: two parts,
  * out [n_tokens, n0] = silu(y of part 0) * y of part 1, rounded once. Except for that

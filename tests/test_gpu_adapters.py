@@ -110,7 +110,8 @@ def problem(T, n, k, outs, rank, dtype, none=0.3, r=None):
 
 def expected(ids, w, x, base, R):
     """(64-bit result, what an fp32 computation of it may be off before its rounding)."""
-    a, b, sc = w.a.cpu()[..., :w.in_features], w.b.cpu(), w.scales.cpu()
+    a, b = (torch.stack(t).cpu() for t in zip(*(w.unpack(i) for i in range(w.num_adapters))))
+    sc = w.scales.cpu()
     outs, k = w.out_features, w.in_features
     y = ref.adapted(base, x, a, b, sc, ids, outs, R)
     terms = ref.adapted_bound(torch.zeros_like(base), x, a, b, sc, ids, outs, R)

@@ -79,7 +79,7 @@ def test_control_and_draw_refusals():
 
 def test_cpu_tensors_are_refused():
     w = AdapterWeights(32, (16,), 2, 4, device="cpu")
-    assert w.rank == 8 and w.a.shape == (2, 8, 32) and w.b.shape == (2, 16, 8)
+    assert w.rank == 8 and w.a.shape == (2, 8, 32) and w.b.shape == (2, 64, 8)
     with pytest.raises(RuntimeError, match="ROCm"):
         build_adapter_plan(torch.zeros(3, dtype=torch.int32), 2)
     with pytest.raises(RuntimeError, match="ROCm"):
@@ -94,6 +94,36 @@ def test_cpu_tensors_are_refused():
         AdapterWeights(32, (16,), 1001, 8, device="cpu")
     with pytest.raises(TypeError):
         AdapterWeights(32, (16,), 2, 8, dtype=torch.float64, device="cpu")
+
+
+@pytest.mark.parametrize("k,outs,rank", [(32, (64,), 8), (33, (1, 70, 16), 16), (96, (130,), 24),
+                                         (64, (64, 64), 128), (5, (200, 8), 40)])
+def test_weights_are_laid_out_as_the_lanes_read_them(k, outs, rank):
+    g = torch.Generator().manual_seed(k)
+    w = AdapterWeights(k, outs, 2, rank, dtype=torch.float16, device="cpu")
+    pairs = [(torch.randn(rank, k, generator=g), torch.randn(n, rank, generator=g)) for n in outs]
+    w.load(1, pairs, 2.0)
+    a, b = w.unpack(1)
+    assert torch.equal(a, torch.cat([p[0] for p in pairs]).half())
+    assert torch.equal(b, torch.cat([p[1] for p in pairs]).half())
+    ka, flat_a, flat_b = -(-k // 32) * 32, w.a[1].view(-1), w.b[1].view(-1)
+    at = 0
+    for s, (pa, pb) in enumerate(pairs):
+        for r in range(rank):
+            r0 = r // 16 * 16
+            nr = min(16, rank - r0)
+            for c in range(0, k, 7):
+                place = (s * rank + r0) * ka + ((c // 8) * nr + r - r0) * 8 + c % 8
+                assert flat_a[place] == pa[r, c].half()
+        for f in range(pb.shape[0]):
+            h, q, l, e = f % 64 // 32, f % 32 // 8, f % 8 // 4, f % 4
+            for r in range(0, rank, 3):
+                place = ((at + f // 64 * 64) * rank + (r // 8) * 512
+                         + ((2 * h + l) * 16 + 4 * q + e) * 8 + r % 8)
+                assert flat_b[place] == pb[f, r].half()
+        at += -(-pb.shape[0] // 64) * 64
+    w.load(1, [None] * len(outs))
+    assert not w.a.any() and not w.b.any()
 
 
 def test_parameters_are_checked_as_the_kernels_get_them():

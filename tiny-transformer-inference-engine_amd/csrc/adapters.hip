@@ -10,7 +10,9 @@
 //                        of the two sums.
 // The ranks are few, so both products are far below the ridge of the matrix cores
 // and the bytes bind: the used adapters' A and B for a decode step, the
-// activations for prompts.
+// activations for prompts. A and B are laid out once as the lanes of a product read them, 16
+// lanes in a row: from row-major weights, whose neighbouring lanes are rows apart, the two
+// products of 256 rows over 4 adapters of rank 64 took 13.3 us in place of 11.3.
 #include "mfma_decode_common.h"
 
 #include <algorithm>
@@ -238,8 +240,8 @@ struct ApplyArgs {
   int64_t base_stride;
   const void* x;
   int64_t x_stride;
-  const void* a;        // [N, SR, ka]
-  const void* b;        // [N, n, R]
+  const void* a;        // [N, SR, ka], each part in blocks of 16 ranks: [step of 32][8s][rank][8]
+  const void* b;        // [N, nb, R], in blocks of 64 features: [8s of ranks][product][l16][8]
   const float* scales;  // [N]
   const int4* tiles;
   const int32_t* rows;  // [max_tiles][tile_rows]
@@ -247,7 +249,7 @@ struct ApplyArgs {
   int T;
   int N;
   int k;
-  int ka;      // pitch of A's rows: k rounded up to 32 at least, zeros behind k
+  int ka;      // of A: k rounded up to 32 at least, zeros behind k
   int R;       // ranks a part, a multiple of 8
   int SR;
   int blocks;  // of 16 ranks, a part: t's unit
@@ -255,6 +257,8 @@ struct ApplyArgs {
   int slices;
   int at[kMaxSlices + 1];      // first feature of each part
   int chunk0[kMaxSlices + 1];  // first column chunk of each part
+  int b_at[kMaxSlices];        // first feature of each in b, where they have whole 64s
+  int nb;                      // all features there
   int pieces;   // of k
   int k_steps;  // 32-wide steps of k a piece
   int max_tiles;
@@ -309,9 +313,10 @@ constexpr int kDownThreads = 64 * kDownWaves;
 // are added up, in order, by whoever needs t: no workgroup waits for another and the
 // results have one order. D[rank][token]: lane l has token l % 16 and four consecutive
 // ranks. XV: x's rows are read in 16-byte pieces, all but the last step's without a
-// condition. Round trips bind: 7400 rows of 4096 (bf16, 64 ranks, 64 MB) take 20.8 us, 3.1
-// TB/s of the copy's 5.2, and the same with eight wavefronts or four steps in flight; 64 rows
-// over 24 adapters of rank 16 (8 MB) 5.7 us; 256 over 4 of rank 64 (fp16) 6.0.
+// condition. 7400 rows of 4096 (bf16, 64 ranks, 64 MB) take 19.8 us, 3.2 TB/s of the copy's
+// 5.2, and the same with eight wavefronts, four steps in flight or four pieces: a CU takes x's
+// rows, 64 bytes of each at a time, no faster. 64 rows over 24 adapters of rank 16 (8 MB) 5.1 us,
+// 256 over 4 of rank 64 (fp16) 5.2, in round trips.
 template <typename T, int MR, int RB, bool XV>
 __global__ __launch_bounds__(kDownThreads) void adapter_down_kernel(ApplyArgs a) {
   using v8 = typename Ops<T>::v8;
@@ -331,12 +336,15 @@ __global__ __launch_bounds__(kDownThreads) void adapter_down_kernel(ApplyArgs a)
   for (int m = 0; m < MR; ++m)
     xp[m] = static_cast<const T*>(a.x) + (int64_t)row[m] * a.x_stride + g * 8;
   const T* ap[RB];
+  int next[RB];  // elements of a block's step
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     const int b = min(block0 + r, all - 1);
-    // ranks behind the part's last read its last row, and are dropped below
-    const int rank = b / a.blocks * a.R + min(b % a.blocks * 16 + l16, a.R - 1);
-    ap[r] = static_cast<const T*>(a.a) + ((int64_t)t.x * a.SR + rank) * a.ka + g * 8;
+    // ranks behind the part's last read its last, and are dropped below
+    const int r0 = b % a.blocks * 16, nr = min(16, a.R - r0);
+    ap[r] = static_cast<const T*>(a.a) + ((int64_t)t.x * a.SR + b / a.blocks * a.R + r0) * a.ka +
+            (g * nr + min(l16, nr - 1)) * 8;
+    next[r] = nr * 32;
   }
   floatx4 acc[MR][RB];
 #pragma unroll
@@ -360,7 +368,7 @@ __global__ __launch_bounds__(kDownThreads) void adapter_down_kernel(ApplyArgs a)
 #pragma unroll
       for (int i = 0; i < N; ++i) {
 #pragma unroll
-        for (int r = 0; r < RB; ++r) load8<T>(av[i][r], ap[r] + (s + i) * 32);
+        for (int r = 0; r < RB; ++r) load8<T>(av[i][r], ap[r] + (int64_t)(s + i) * next[r]);
 #pragma unroll
         for (int m = 0; m < MR; ++m) load8<T>(xv[i][m], xp[m] + (s + i) * 32);
       }
@@ -383,7 +391,7 @@ __global__ __launch_bounds__(kDownThreads) void adapter_down_kernel(ApplyArgs a)
   for (; s < s1; ++s) {
     v8 xv[MR], av[RB];
 #pragma unroll
-    for (int r = 0; r < RB; ++r) load8<T>(av[r], ap[r] + s * 32);
+    for (int r = 0; r < RB; ++r) load8<T>(av[r], ap[r] + (int64_t)s * next[r]);
 #pragma unroll
     for (int m = 0; m < MR; ++m) {
       xv[m] = v8{};
@@ -441,9 +449,9 @@ __device__ __forceinline__ float gate(float g, float u) {
 // requested before t. 16 rows and 64 features a wavefront leave many wavefronts in flight,
 // which a prompt's rows need: 32 rows, or several times 64 features with the next one's rows
 // requested ahead, were slower (7400 rows, gate of 4096, rank 32: 50 us against 55 and 67-84).
-// Now 47.5 us for 182 MB of base and out, 3.8 TB/s, with the VALU's issue slots two thirds full;
-// B's rows shared by 32 or 64 rows of a workgroup take 48 and 59 us, and addresses kept in
-// scalars for features that are all there the same. 64 rows of q/k/v 5.3 us, 256 of rank 64 7.1.
+// Now 46.7 us for 182 MB of base and out, 3.9 TB/s, with the VALU's issue slots two thirds full;
+// B shared by 32 or 64 rows of a workgroup took 48 and 59 us when this took 47.5. 64 rows of
+// q/k/v 5.0 us, 256 of rank 64 6.1.
 template <typename T, int P, int EPI>
 __global__ __launch_bounds__(kUpThreads) void adapter_up_kernel(ApplyArgs a) {
   using v8 = typename Ops<T>::v8;
@@ -495,16 +503,15 @@ __global__ __launch_bounds__(kUpThreads) void adapter_up_kernel(ApplyArgs a) {
 #pragma unroll
     for (int i = 0; i < BB; ++i) {
       if (i && c + i >= steps) break;
-      const int r = min((c + i) * 32 + g * 8, a.R - 8);
+      const int r8 = min((c + i) * 4 + g, a.R / 8 - 1);
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const T* b = static_cast<const T*>(a.b) + ((int64_t)t.x * a.n + a.at[slice + s]) * a.R + r;
+        // product j, row l16: the feature whose sum lane (l16 / 4) gets in element l16 % 4,
+        // 32 (j / 2) + 8 (l16 / 4) + 4 (j % 2) + l16 % 4 of the 64
+        const T* b = static_cast<const T*>(a.b) + ((int64_t)t.x * a.nb + a.b_at[slice + s]) * a.R +
+                     ((int64_t)(min(c0, width - 1) / 64) * (a.R / 8) + r8) * 512 + l16 * 8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // product j, row l16: the feature whose sum lane (l16 / 4) gets in element l16 % 4
-          const int f = c0 + (j >> 1) * 32 + (l16 >> 2) * 8 + (j & 1) * 4 + (l16 & 3);
-          load8<T>(bv[i][s][j], b + (int64_t)min(f, width - 1) * a.R);
-        }
+        for (int j = 0; j < 4; ++j) load8<T>(bv[i][s][j], b + j * 128);
       }
     }
   };
@@ -750,6 +757,8 @@ int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t b
     if (ns[s] <= 0 || ns[s] > (1 << 24)) return fail(PKV_ERR_INVALID, "bad features of part %d", s);
     p.at[s] = (int)n;
     p.chunk0[s] = chunks;
+    p.b_at[s] = p.nb;
+    p.nb += cdiv(ns[s], 64) * 64;
     n += ns[s];
     chunks += cdiv(ns[s], kUpCols);
   }

@@ -41,9 +41,10 @@ class AdapterWeights:
     """A and B of num_adapters adapters beside a projection of in_features features
     to the parts out_features (one, or those of a fused projection, at most 4), of at
     most max_rank ranks a part. a [num_adapters, parts * rank, in_features rounded up
-    to 32], b [num_adapters, sum(out_features), rank] and scales (float32) are what the
-    kernels read, rank being max_rank rounded up to a multiple of 8; unused ranks are 0,
-    and so is an adapter that was not loaded."""
+    to 32], b [num_adapters, out_features each rounded up to 64, rank] and scales (float32)
+    are what the kernels read, rank being max_rank rounded up to a multiple of 8, a and b in
+    the order of their lanes (unpack() gives them in plain order); unused ranks are 0, and
+    so is an adapter that was not loaded."""
 
     def __init__(self, in_features: int, out_features, num_adapters: int, max_rank: int,
                  dtype: torch.dtype = torch.float32, device="cuda"):
@@ -57,7 +58,8 @@ class AdapterWeights:
         self.num_adapters, self.rank, self.dtype = int(num_adapters), -(-max_rank // 8) * 8, dtype
         self.a = torch.zeros((num_adapters, len(outs) * self.rank, -(-in_features // 32) * 32),
                              dtype=dtype, device=device)
-        self.b = torch.zeros((num_adapters, sum(outs), self.rank), dtype=dtype, device=device)
+        self.b = torch.zeros((num_adapters, sum(-(-n // 64) * 64 for n in outs), self.rank),
+                             dtype=dtype, device=device)
         self.scales = torch.zeros(num_adapters, dtype=torch.float32, device=device)
         self.device = self.a.device
         # what every call hands on
@@ -90,19 +92,53 @@ class AdapterWeights:
         """Puts an adapter in place `index`: per part (A [r, in_features], B
         [out_features, r]) with r up to the rank, or None for a part without one."""
         self._check_parts(index, parts)
-        R, k, at = self.rank, self.in_features, 0
-        if self.a.shape[2] != k or any(pair is None or pair[0].shape[0] < R for pair in parts):
-            self.clear(index)
-        dst, src = [], []
-        for s, (n, pair) in enumerate(zip(self.out_features, parts)):
-            if pair is not None:
-                r = pair[0].shape[0]
-                dst += [self.a[index, s * R:s * R + r, :k], self.b[index, at:at + n, :r]]
-                src += pair
-            at += n
-        if dst:
-            torch._foreach_copy_(dst, src)  # one launch where types and layouts agree
+        for (dst_a, dst_b), n, pair in zip(self._parts_of(index), self.out_features, parts):
+            r = 0 if pair is None else pair[0].shape[0]
+            if r == 0:
+                for d in (*dst_a, dst_b):
+                    d.zero_()
+                continue
+            a, b = self._whole(pair[0], self.rank, self.a.shape[2]), self._whole(
+                pair[1], -(-n // 64) * 64, self.rank)
+            at = 0
+            for d in dst_a:
+                d.copy_(a[at:at + d.shape[0] * d.shape[1]].view(d.shape))
+                at += d.shape[0] * d.shape[1]
+            dst_b.copy_(b.view(dst_b.shape))
         self.scales[index] = float(scale)
+
+    def _whole(self, t, rows, cols):
+        """t on the device, in the type and with zeros up to [rows, cols]."""
+        if t.shape == (rows, cols):
+            return t.to(self.device, self.dtype).contiguous()
+        out = torch.zeros((rows, cols), dtype=self.dtype, device=self.device)
+        out[:t.shape[0], :t.shape[1]] = t
+        return out
+
+    def _parts_of(self, index):
+        """Views of each part's A, ranks in blocks of 16 and then of 8 ([blocks, ranks, steps,
+        4, 8]), and B ([blocks of 64 features, 2, 4, 2, 4, 8s of ranks, 8]), whose elements in
+        order are the rows in order."""
+        R, steps, at = self.rank, self.a.shape[2] // 32, 0
+        for s, n in enumerate(self.out_features):
+            a, full = self.a[index, s * R:(s + 1) * R], R // 16 * 16
+            views = []
+            for rows, of in ((a[:full], 16), (a[full:], 8)):
+                if len(rows):
+                    views.append(rows.view(-1, steps, 4, of, 8).permute(0, 3, 1, 2, 4))
+            wide = -(-n // 64) * 64
+            b = self.b[index, at:at + wide].view(-1, R // 8, 2, 2, 4, 4, 8)
+            at += wide
+            yield views, b.permute(0, 2, 4, 3, 5, 1, 6)
+
+    def unpack(self, index: int):
+        """(A [parts * rank, in_features], B [sum(out_features), rank]) of an adapter, copies
+        in plain order."""
+        a_rows, b_rows = [], []
+        for (views, b), n in zip(self._parts_of(self._index(index)), self.out_features):
+            a_rows += [v.reshape(-1, self.a.shape[2])[:, :self.in_features] for v in views]
+            b_rows.append(b.reshape(-1, self.rank)[:n])
+        return torch.cat(a_rows), torch.cat(b_rows)
 
     @torch.no_grad()
     def clear(self, index: int) -> None:
