@@ -18,7 +18,6 @@ them); values, tokens and parameters from the seed handed to prepare().
 """
 from __future__ import annotations
 
-import functools
 import math
 import os
 import sys
@@ -33,7 +32,6 @@ DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 ESIZE = {"fp32": 4, "bf16": 2, "fp16": 2}
 
 
-@functools.lru_cache(maxsize=None)  # a user's program imports once, not at every call
 def _serving():
     # the package folder's name is no Python identifier, so its path is added;
     # the working folder is the repository's root
