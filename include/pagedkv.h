@@ -717,6 +717,8 @@ int pkv_adapter_apply(void* out, int64_t out_stride, const void* base, int64_t b
  *     more than once gets the sum, added up in the list's order.
  *   mask_rows[r] >= 0: -infinity where bit id % 32 of word id / 32 of masks[mask_rows[r]]
  *     ([n_masks, ceil(vocab / 32)] int32) is 0; -1: no mask.
+ * Finite operands give finite results: a step that passes fp32's largest value gives that
+ * value, and so does the rounding for the type's. An infinite or NaN operand shows as usual.
  * Null tokens, bias_starts, mask_rows: none of the kind. out may be logits itself (same
  * address and stride), else it shares no memory with an operand. An id outside the
  * vocabulary is skipped (PKV_STATUS_BAD_TOKEN); a length or offset outside its bounds is

@@ -78,6 +78,37 @@ __device__ __forceinline__ int place_of(int id) {
   return (int)((unsigned)id * 2654435761u >> (32 - kPlaceBits));
 }
 
+// Finite values stay finite: a step whose operands are finite ends at fp32's largest value,
+// and the rounding to T at T's. An infinite logit would make the row undrawable, whatever
+// else its request asks for.
+constexpr float kMost = 3.402823466e38f;
+template <typename T>
+constexpr float kLargest = sizeof(T) == 4 ? kMost : __is_same(T, f16) ? 65504.f : 3.389531390e38f;
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+__device__ __forceinline__ float within(float x, float most) {
+  return x > most ? most : x < -most ? -most : x;  // a NaN stays one
+}
+// x + y
+__device__ __forceinline__ float sum_within(float x, float y) {
+  float z = x + y;
+  if (!finite(z) && finite(x) && finite(y)) z = within(z, kMost);
+  return z;
+}
+// A logit with its penalties: its token is there, `made` times behind the prompt.
+__device__ __forceinline__ float penalised(float x, float rep, float pres, float freq,
+                                           unsigned made) {
+  const float y = x > 0.f ? x / rep : x * rep;
+  const float off = made ? freq * (float)made + pres : 0.f;
+  const float z = y - off;
+  if (finite(z)) return z;  // and so were y and off
+  x = finite(x) && finite(rep) ? within(y, kMost) : y;
+  if (finite(off) || !finite(freq) || !finite(pres)) return sum_within(x, -off);
+  // off by its halves: cut where they pass fp32, as then x less them does
+  const float half = within(0.5f * freq * (float)made + 0.5f * pres, kMost);
+  return sum_within(sum_within(x, -half), -half);
+}
+
 // TH threads, S pieces each: a range of TH S pieces.
 template <typename T, int TH, int S>
 __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
@@ -224,9 +255,7 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
       float x = (float)v[0][0];
 #pragma unroll
       for (int i = 1; i < S * E; ++i) x = k == i ? (float)v[i / E][i % E] : x;
-      x = x > 0.f ? x / rep : x * rep;
-      const unsigned made = c & ~kInPrompt;
-      if (made) x -= freq * (float)made + pres;
+      x = penalised(x, rep, pres, freq, c & ~kInPrompt);
       vals[at] = x;
     }
     stage();
@@ -243,7 +272,7 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
       if (!staged) stage();
       __syncthreads();
       if (todo && alike[place_of(bid)] == 1) {
-        vals[bid - lo] += badd;
+        vals[bid - lo] = sum_within(vals[bid - lo], badd);
         todo = false;
       }
     }
@@ -260,7 +289,7 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
       if (todo) atomicMin(&claim, (unsigned)tid);
       __syncthreads();
       if (todo && claim == (unsigned)tid) {
-        vals[bid - lo] += badd;
+        vals[bid - lo] = sum_within(vals[bid - lo], badd);
         claim = ~0u;
         todo = false;
       }
@@ -275,12 +304,21 @@ __global__ __launch_bounds__(TH) void control_kernel(ControlArgs a) {
     const int id0 = lo + p;
     if (id0 >= hi) break;
     if (staged) {
+      float x[E], most = 0.f;
 #pragma unroll
-      for (int j = 0; j < E; j += 4) {
-        const floatx4 x = *reinterpret_cast<const floatx4*>(&vals[p + j]);
+      for (int j = 0; j < E; j += 4)
+        *reinterpret_cast<floatx4*>(&x[j]) = *reinterpret_cast<const floatx4*>(&vals[p + j]);
+      if constexpr (sizeof(T) < 4) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[s][j + k] = (T)x[k];
+        for (int j = 0; j < E; ++j) most = fmaxf(most, fabsf(x[j]));
+        if (most > kLargest<T>) {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (finite(x[j])) x[j] = within(x[j], kLargest<T>);
+        }
       }
+#pragma unroll
+      for (int j = 0; j < E; ++j) v[s][j] = (T)x[j];
     }
     if (mask) {
 #pragma unroll

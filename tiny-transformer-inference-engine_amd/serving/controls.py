@@ -115,7 +115,8 @@ def control_logits(logits: torch.Tensor, controls: LogitControls,
                    status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """logits [rows, vocab] (float32, float16, bfloat16) with every row's penalties, then
     biases, then its mask (-infinity where an id is not allowed), in fp32 and rounded
-    once. out: where to write, logits itself or memory of no operand. `status` as in
+    once; what finite operands carry past the range of fp32, or of the type at the end, is
+    its largest value. out: where to write, logits itself or memory of no operand. `status` as in
     build_adapter_plan: ids outside the vocabulary, which are skipped, and lengths, offsets
     and mask rows outside their bounds. A mask may leave a row nothing: all -infinity."""
     what = "control_logits"
