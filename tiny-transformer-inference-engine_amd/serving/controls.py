@@ -22,7 +22,7 @@ from .adapters import _overlap, _rows
 from .paged_meta import _status_ptr, raise_step_status
 
 __all__ = ["LogitControls", "RequestParams", "Grammar", "TokenHistory", "control_logits",
-           "sample_each", "pack_mask", "draw_tokens"]
+           "sample_each", "pack_mask", "draw_tokens", "draw_rows"]
 
 MAX_SAMPLE_VOCAB = 1 << 20
 
@@ -360,6 +360,30 @@ def draw_tokens(logits: torch.Tensor, params, history: TokenHistory, keys):
     """One token a row of logits [rows, vocab] on a ROCm device: row i by params[i]
     (RequestParams) with the tokens of request keys[i] in `history`. Returns (ids,
     log-probabilities) as lists; raises where a row has no token left to draw."""
+    ids, logprobs, _, status = _draw(logits, params, history, keys)
+    if status is not None:
+        raise_step_status(status, "draw_tokens")
+    return ids, logprobs
+
+
+def draw_rows(logits: torch.Tensor, params, history: TokenHistory, keys):
+    """draw_tokens for rows that have nothing to do with each other: (ids,
+    log-probabilities, {row: why}), a row that cannot be drawn having id -1 and its reason
+    while the others have their tokens."""
+    ids, logprobs, changed, status = _draw(logits, params, history, keys)
+    failed = {}
+    for i in [i for i, tok in enumerate(ids) if tok < 0]:
+        row = changed[i].float()
+        failed[i] = ("the logits contain NaN or infinity" if not bool((row < math.inf).all())
+                     else "there is no token left to draw" if bool((row == -math.inf).all())
+                     else "a sampling parameter is outside its range")
+    if status is not None and not failed:
+        raise_step_status(status, "draw_rows")
+    return ids, logprobs, failed
+
+
+def _draw(logits, params, history, keys):
+    """(ids, log-probabilities, the logits drawn from, the status word or None where it is 0)"""
     n, dev, f32 = len(params), logits.device, torch.float32
     status = torch.zeros(1, dtype=torch.int32, device=dev)
     # one upload of what is a number a row
@@ -392,6 +416,4 @@ def draw_tokens(logits: torch.Tensor, params, history: TokenHistory, keys):
     ids, logprobs = sample_each(logits, temperature, nums[6].to(torch.int32), top_p, min_p,
                                 status=status)
     got = torch.cat([ids.double(), logprobs.double(), status.double()]).tolist()  # one copy
-    if got[-1]:
-        raise_step_status(status, "draw_tokens")
-    return [int(i) for i in got[:n]], got[n:2 * n]
+    return [int(i) for i in got[:n]], got[n:2 * n], logits, status if got[-1] else None

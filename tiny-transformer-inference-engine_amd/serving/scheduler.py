@@ -38,7 +38,7 @@ from dataclasses import dataclass
 import torch
 
 from .batch import BatchStep, build_batch_step
-from .controls import RequestParams, TokenHistory, draw_tokens
+from .controls import RequestParams, TokenHistory, draw_rows
 from .sampling import sample
 from .sequence import Sequence, blocks_for
 
@@ -60,6 +60,15 @@ class _Request:
 class _Running:
     req: _Request
     computed: int = 0  # tokens of the sequence whose K/V are in the pool
+
+
+class RequestsFailed(ValueError):
+    """Requests that cannot go on (Scheduler.step): failed maps each one's seq_id to the
+    reason. They are out of the scheduler; the others took no token in this step."""
+
+    def __init__(self, failed: dict):
+        self.failed = dict(failed)
+        super().__init__("; ".join(f"request {i}: {why}" for i, why in self.failed.items()))
 
 
 class Scheduler:
@@ -178,17 +187,29 @@ class Scheduler:
     def _draws(self, seqs, logits, rows):
         """The next token of every sequence in seqs, whose tokens are all computed, from
         row rows[i] of logits: those with parameters of their own by one draw together,
-        the others each by the scheduler's."""
+        the others each by the scheduler's. Those that cannot be drawn are taken out and
+        raised, before any token is taken."""
         own = [i for i, seq in enumerate(seqs) if self._state[seq.seq_id].req.params is not None]
         toks = [None] * len(seqs)
         if own:
             at = [rows[i] for i in own]
-            picked, _ = draw_tokens(logits if at == list(range(len(logits))) else logits[at],
-                                    [self._state[seqs[i].seq_id].req.params for i in own],
-                                    self._history, [seqs[i].seq_id for i in own])
+            picked, _, failed = draw_rows(
+                logits if at == list(range(len(logits))) else logits[at],
+                [self._state[seqs[i].seq_id].req.params for i in own], self._history,
+                [seqs[i].seq_id for i in own])
+            if failed:
+                self._fail({seqs[own[i]].seq_id: why for i, why in failed.items()})
             for i, tok in zip(own, picked):
                 toks[i] = tok
         return [self._pick(logits[r]) if t is None else t for r, t in zip(rows, toks)]
+
+    def _fail(self, failed):
+        """Takes the running requests of these seq_ids out and raises their reasons."""
+        for seq in self.running:
+            if seq.seq_id in failed:
+                self._finish(seq)
+        self.running = [seq for seq in self.running if seq.seq_id not in failed]
+        raise RequestsFailed(failed)
 
     def _sampled(self, seq: Sequence, tok):
         """The sequence takes tok; returns whether it is done."""
@@ -207,7 +228,9 @@ class Scheduler:
     def step(self):
         """Returns [(seq_id, token, done)] for every sequence that sampled a
         token (with a SchedulerConfig, a prefill chunk that does not finish
-        its prompt samples nothing)."""
+        its prompt samples nothing). Raises RequestsFailed, before any token is taken,
+        where requests with params cannot go on (a grammar that leaves nothing, say):
+        those are taken out, and the next step goes on with the others."""
         if self.sched_cfg is not None:
             return self._step_budgeted()
         while self.waiting and self._fits(self.waiting[0]):
