@@ -77,3 +77,53 @@ def test_a_dead_end_ends_its_request_alone(plain, budget):
     assert list(errors[0].failed) == [2]
     assert sched.alloc.num_free == sched.alloc.num_usable
     assert not sched._state and not sched._history._row
+
+
+@pytest.mark.parametrize("budget", [None, 16])
+@pytest.mark.parametrize("where", ["advance", "mask", "shape"])
+def test_a_grammar_that_raises_ends_its_request_alone(plain, budget, where):
+    model, cfg = plain
+    prompts = prompts_of([9, 20, 5])
+    want = [alone(model, cfg, prompts[0], 8), None, alone(model, cfg, prompts[2], 8)]
+
+    class Breaks(Words):
+        def mask(self):
+            if len(self.took) == 2 and where == "mask":
+                raise KeyError("no state")
+            if len(self.took) == 2 and where == "shape":
+                return torch.zeros(3, dtype=torch.int32)
+            return super().mask()
+
+        def advance(self, token):
+            if len(self.took) == 2 and where == "advance":
+                raise KeyError("no state")
+            super().advance(token)
+
+    sched = scheduler(model, cfg, budget)
+    for p, r in zip(prompts, (None, RequestParams(temperature=0, grammar=Breaks([[3, 5], [4]])),
+                              None)):
+        sched.add_request(p, 8, params=r)
+    got, errors = run(sched)
+    assert [got[0], got[2]] == [want[0], want[2]]
+    # the token that the grammar choked on was drawn and is handed out
+    assert len(got[1]) == (3 if where == "advance" else 2)
+    assert len(errors) == 1 and list(errors[0].failed) == [1]
+    assert ("words" if where == "shape" else "no state") in str(errors[0])
+    assert sched.alloc.num_free == sched.alloc.num_usable
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_penalties_past_the_types_range_stop_nobody(dtype):
+    model, cfg = make_model(dtype)
+    prompts = prompts_of([9, 20, 5, 12, 7])
+    want = alone(model, cfg, prompts[0], 10)
+    sched = scheduler(model, cfg)
+    for p, r in zip(prompts, (None, RequestParams(repetition_penalty=1e-30),
+                              RequestParams(temperature=0, frequency_penalty=-3e38),
+                              RequestParams(presence_penalty=-1e5, top_p=0.9),
+                              RequestParams(presence_penalty=3e38, frequency_penalty=3e38,
+                                            grammar=Words([[5]])))):
+        sched.add_request(p, 10, params=r)
+    got, errors = run(sched)
+    assert not errors and got[0] == want and all(len(got[i]) == 10 for i in range(5))
+    assert got[4] == [5] * 10  # the only token it may take, whatever it costs

@@ -241,6 +241,15 @@ class Grammar(Protocol):
         """The request took `token`."""
 
 
+def grammar_mask(grammar: Grammar, vocab: int) -> torch.Tensor:
+    """The grammar's mask, refused where it is not one of `vocab` tokens."""
+    mask, words = grammar.mask(), -(-vocab // 32)
+    if not isinstance(mask, torch.Tensor) or tuple(mask.shape) != (words,):
+        raise ValueError(f"the grammar's mask must be [{words}] words "
+                         f"(got {list(getattr(mask, 'shape', ()))})")
+    return mask
+
+
 def _f32(x) -> float:
     return float(torch.tensor(float(x), dtype=torch.float32))
 
@@ -360,7 +369,9 @@ def draw_tokens(logits: torch.Tensor, params, history: TokenHistory, keys):
     """One token a row of logits [rows, vocab] on a ROCm device: row i by params[i]
     (RequestParams) with the tokens of request keys[i] in `history`. Returns (ids,
     log-probabilities) as lists; raises where a row has no token left to draw."""
-    ids, logprobs, _, status = _draw(logits, params, history, keys)
+    masks = {i: grammar_mask(p.grammar, logits.shape[1])
+             for i, p in enumerate(params) if p.grammar is not None}
+    ids, logprobs, _, status = _draw(logits, params, masks, history, keys)
     if status is not None:
         raise_step_status(status, "draw_tokens")
     return ids, logprobs
@@ -369,8 +380,15 @@ def draw_tokens(logits: torch.Tensor, params, history: TokenHistory, keys):
 def draw_rows(logits: torch.Tensor, params, history: TokenHistory, keys):
     """draw_tokens for rows that have nothing to do with each other: (ids,
     log-probabilities, {row: why}), a row that cannot be drawn having id -1 and its reason
-    while the others have their tokens."""
-    ids, logprobs, changed, status = _draw(logits, params, history, keys)
+    (a text, or what its grammar's mask() raised) while the others have their tokens."""
+    masks, broken = {}, {}
+    for i, p in enumerate(params):
+        if p.grammar is not None:
+            try:
+                masks[i] = grammar_mask(p.grammar, logits.shape[1])
+            except Exception as e:
+                broken[i] = e
+    ids, logprobs, changed, status = _draw(logits, params, masks, history, keys)
     failed = {}
     for i in [i for i, tok in enumerate(ids) if tok < 0]:
         row = changed[i].float()
@@ -379,11 +397,14 @@ def draw_rows(logits: torch.Tensor, params, history: TokenHistory, keys):
                      else "a sampling parameter is outside its range")
     if status is not None and not failed:
         raise_step_status(status, "draw_rows")
-    return ids, logprobs, failed
+    for i in broken:
+        ids[i], logprobs[i] = -1, math.nan
+    return ids, logprobs, {**failed, **broken}
 
 
-def _draw(logits, params, history, keys):
-    """(ids, log-probabilities, the logits drawn from, the status word or None where it is 0)"""
+def _draw(logits, params, masks, history, keys):
+    """(ids, log-probabilities, the logits drawn from, the status word or None where it is
+    0); masks {row: mask}"""
     n, dev, f32 = len(params), logits.device, torch.float32
     status = torch.zeros(1, dtype=torch.int32, device=dev)
     # one upload of what is a number a row
@@ -404,12 +425,11 @@ def _draw(logits, params, history, keys):
         kw.update(bias_ids=torch.tensor([t for t, _ in flat], dtype=torch.int32, device=dev),
                   bias_values=torch.tensor([v for _, v in flat], dtype=f32, device=dev),
                   bias_starts=torch.tensor(starts, dtype=torch.int32, device=dev))
-    masks = [(i, p.grammar.mask()) for i, p in enumerate(params) if p.grammar is not None]
     if masks:
         rows = [-1] * n
-        for m, (i, _) in enumerate(masks):
+        for m, i in enumerate(masks):
             rows[i] = m
-        kw.update(masks=torch.stack([m.to(dev, torch.int32) for _, m in masks]),
+        kw.update(masks=torch.stack([m.to(dev, torch.int32) for m in masks.values()]),
                   mask_rows=torch.tensor(rows, dtype=torch.int32, device=dev))
     if kw:
         logits = control_logits(logits, LogitControls(**kw), status=status)

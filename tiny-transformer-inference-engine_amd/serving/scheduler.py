@@ -38,7 +38,7 @@ from dataclasses import dataclass
 import torch
 
 from .batch import BatchStep, build_batch_step
-from .controls import RequestParams, TokenHistory, draw_rows
+from .controls import RequestParams, TokenHistory, draw_rows, grammar_mask
 from .sampling import sample
 from .sequence import Sequence, blocks_for
 
@@ -64,11 +64,15 @@ class _Running:
 
 class RequestsFailed(ValueError):
     """Requests that cannot go on (Scheduler.step): failed maps each one's seq_id to the
-    reason. They are out of the scheduler; the others took no token in this step."""
+    reason, a text. They are out of the scheduler; the others took no token in this step.
+    __cause__ is what the first of their grammars raised, if one did."""
 
     def __init__(self, failed: dict):
-        self.failed = dict(failed)
+        raised = [why for why in failed.values() if isinstance(why, Exception)]
+        self.failed = {i: f"its grammar raised {type(why).__name__}: {why}"
+                       if isinstance(why, Exception) else why for i, why in failed.items()}
         super().__init__("; ".join(f"request {i}: {why}" for i, why in self.failed.items()))
+        self.__cause__ = raised[0] if raised else None
 
 
 class Scheduler:
@@ -89,6 +93,7 @@ class Scheduler:
         self.waiting: list[_Request] = []
         self.running: list[Sequence] = []
         self._state: dict[int, _Running] = {}  # seq_id -> state of a running sequence
+        self._broken: dict[int, Exception] = {}  # seq_id -> what its grammar's advance() raised
         self.next_seq_id = 0
         self.num_preemptions = 0
         self.last_batch_tokens = 0
@@ -137,10 +142,7 @@ class Scheduler:
                    for p in [r.params for r in self.waiting]
                    + [st.req.params for st in self._state.values()]):
                 raise ValueError("the grammar follows the tokens of another request")
-            words = tuple(params.grammar.mask().shape)
-            if words != (-(-vocab // 32),):
-                raise ValueError(f"the grammar's mask must be [{-(-vocab // 32)}] words "
-                                 f"(got {list(words)})")
+            grammar_mask(params.grammar, vocab)
 
     def computed_tokens(self, seq: Sequence) -> int:
         """Tokens of a running sequence whose K/V are in the pool."""
@@ -216,12 +218,20 @@ class Scheduler:
         req = self._state[seq.seq_id].req
         req.generated += 1
         done = tok == self.cfg.eos_token_id or req.generated >= req.max_new_tokens
-        if req.params is not None and not done:
-            if req.params.has_penalties:
-                self._history.append(seq.seq_id, tok)
-            if req.params.grammar is not None:
-                req.params.grammar.advance(tok)
+        if req.params is not None and not done and req.params.has_penalties:
+            self._history.append(seq.seq_id, tok)
         return done
+
+    def _advance(self, results):
+        """The grammars of the requests that go on take a step's tokens, after all else is
+        done: one that raises ends its own request, at the next step."""
+        for seq_id, tok, done in results:
+            params = None if done else self._state[seq_id].req.params
+            if params is not None and params.grammar is not None:
+                try:
+                    params.grammar.advance(tok)
+                except Exception as e:
+                    self._broken[seq_id] = e
 
     # ---- a step -----------------------------------------------------------
 
@@ -229,8 +239,11 @@ class Scheduler:
         """Returns [(seq_id, token, done)] for every sequence that sampled a
         token (with a SchedulerConfig, a prefill chunk that does not finish
         its prompt samples nothing). Raises RequestsFailed, before any token is taken,
-        where requests with params cannot go on (a grammar that leaves nothing, say):
-        those are taken out, and the next step goes on with the others."""
+        where requests with params cannot go on (a grammar that leaves nothing or raises,
+        say): those are taken out, and the next step goes on with the others."""
+        if self._broken:
+            broken, self._broken = self._broken, {}
+            self._fail(broken)
         if self.sched_cfg is not None:
             return self._step_budgeted()
         while self.waiting and self._fits(self.waiting[0]):
@@ -253,6 +266,7 @@ class Scheduler:
                 seq.ensure_blocks(self.alloc)
                 kept.append(seq)
         self.running = kept
+        self._advance(results)
         return results
 
     # ---- SchedulerConfig-driven steps ------------------------------------
@@ -332,4 +346,5 @@ class Scheduler:
                 self.running.remove(seq)
             else:
                 seq.append_token(tok)
+        self._advance(results)
         return results
