@@ -432,11 +432,17 @@ constexpr int kUpThreads = 64 * kUpWaves;
 constexpr int kUpCols = 64 * kUpWaves;  // features of a workgroup
 enum { kEpiAdd = 0, kEpiSwiglu = 1 };
 
-// silu(g) u by the exponential and reciprocal instructions, each within a step of fp32: a
-// third of swiglu_gate's operations, which bind a prompt's gate. Rows without an adapter
-// keep swiglu_gate, and with it the bits of the gate by itself.
+// silu(g) u of sums in fp32. For 16-bit types by the exponential and reciprocal
+// instructions, a third of swiglu_gate's operations, which bind a prompt's gate. The
+// exponential's argument and its constant are rounded, by 2^-24 each, so the result is off by
+// some (3 + |g|) 2^-23: 2^-16 at most, where bf16 then rounds by 2^-9, and 2^-18 for fp16's
+// 2^-12 (whose results end at g = -17); gates below -87.3 give 0 (swiglu_gate: below -88.7).
+// fp32, and rows without an adapter, keep swiglu_gate, and with it the bits of the gate by
+// itself.
+template <typename T>
 __device__ __forceinline__ float gate(float g, float u) {
-  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
+  if constexpr (sizeof(T) == 4) return swiglu_gate(g, u);
+  else return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
 }
 
 // The products with B of 16 rows of a tile and, a wavefront, 64 features of a part (swiglu: of
@@ -627,7 +633,7 @@ __global__ __launch_bounds__(kUpThreads) void adapter_up_kernel(ApplyArgs a) {
     }
   };
   if constexpr (EPI == kEpiAdd) finish([](float y, float) { return y; });
-  else if (t.x >= 0) finish([](float y, float u) { return gate(y, u); });
+  else if (t.x >= 0) finish([](float y, float u) { return gate<T>(y, u); });
   else finish([](float y, float u) { return swiglu_gate(y, u); });
 }
 
