@@ -300,13 +300,16 @@ def _x_stride(x2):
     return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
 
 
-def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None):
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+           fused: bool = False):
     """x W^T + b. Few-row bf16/fp16/fp32 problems run on the split-K MFMA
-    kernel (pkv_linear); others on the library GEMM (F.linear)."""
+    kernel (pkv_linear); others on the tile kernel or the library GEMM (F.linear).
+    fused: by the kernel that the calls with an element-wise op take for this
+    problem, whose sums are then theirs bit for bit."""
     x2 = _as_rows(x)
     n = weight.shape[0]
     if not _linear_ok(x2, weight, bias, n):
-        if _tiles_ok(x2, weight, bias):
+        if _tiles_ok(x2, weight, bias, fused):
             out = x.new_empty((x2.shape[0], n))
             _tiles(out, x2, weight, bias, n, _native.EPILOGUE_NONE, "linear")
             return out.view(*x.shape[:-1], n)

@@ -140,7 +140,8 @@ class SwiGLU(nn.Module):
         attr = fused_ops.module_attr
         h = fused_ops.rms_norm(x, attr(norm, "weight"), norm.eps)
         if "gate_up" in weights:
-            h = adapters.adapter_swiglu(fused_ops.linear(h, w, b), h, weights["gate_up"], plan)
+            h = adapters.adapter_swiglu(fused_ops.linear(h, w, b, fused=True), h,
+                                        weights["gate_up"], plan)
         else:
             h = fused_ops.linear_swiglu(h, w, b)
         down = attr(self, "down_proj")

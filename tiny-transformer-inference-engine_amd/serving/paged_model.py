@@ -89,8 +89,8 @@ class PagedTransformer(nn.Module):
         rounded to the model dtype before it is normalised or carried on.
 
         adapters: the rows' low-rank adapters (StepAdapters, on a ROCm device). The
-        norms, RoPE and the gate then run beside the projections, with the same
-        rounded values for rows without an adapter."""
+        norms, RoPE and the gate then run beside the projections, which are those of a
+        step without adapters: rows without an adapter keep their bits."""
         x = self.embedding(input_ids)
         if not x.is_cuda:
             if adapters is not None:

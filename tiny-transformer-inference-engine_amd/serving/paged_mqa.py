@@ -131,7 +131,7 @@ class MQA_Paged(nn.Module):
         attr = fused_ops.module_attr
         cos, sin = attr(self, "rope")._tables_fp32()
         h = fused_ops.rms_norm(x, attr(norm, "weight"), norm.eps)
-        qkv = fused_ops.linear(h, w, b)
+        qkv = fused_ops.linear(h, w, b, fused=True)
         if "qkv" in weights:
             adapter_add(qkv, h, weights["qkv"], plan, out=qkv)
         nq, nk = self.num_heads * self.headdim, self.num_kv_heads * self.headdim
