@@ -96,3 +96,19 @@ def test_what_is_not_finite_still_shows(dtype):
                       bias_starts=i32([0, 5]))
     out = control_logits(x, c)[0].tolist()
     assert out[:4] == [-INF, INF, INF, -INF] and np.isnan(out[4]) and out[5] == 2.0
+
+
+@pytest.mark.parametrize("temperature", [1e37, 1e38, 3e38])
+def test_top_k_of_logits_further_apart_than_fp32_reaches(temperature):
+    """3e38 and -3e38 are 6e38 apart, which at such temperatures still weighs."""
+    rows = 40
+    u = (np.arange(rows) + 0.5) / rows
+    x = torch.tensor([-3.3e38, 3e38, -3e38, 1.0, -3.2e38], dtype=torch.float32).repeat(rows, 1)
+    for k in (1, 2, 3, 4):
+        ids, _ = sample_each(x.to(DEV), f32([temperature] * rows), i32([k] * rows),
+                             uniforms=f32(u))
+        for r in range(rows):
+            want, _, gap = ref.draw(x[r].double().numpy(), float(np.float32(temperature)), k, 1.0,
+                                    0.0, float(np.float32(u[r])))
+            if gap > 5 * 2.0 ** -43:
+                assert int(ids[r]) == want, (k, r)

@@ -678,9 +678,13 @@ struct Sampler {
     return e;
   }
   __device__ __forceinline__ u64 mass(float x, int& bin) const { return mass_bits(x, bin) - kUnit; }
-  // Bins of counts (weights have their steps).
+  // Bins of counts (weights have their steps). Where steps are wide the distance is taken by
+  // halves, for the whole of it may pass fp32; where they are not it is in the last bin by then,
+  // and halves would lose the last bit of the smallest.
   __device__ __forceinline__ int count_bin(float x) const {
-    return (int)fminf(((float)top - x) * (float)steps, (float)((kBins << kBinShift) - 1)) >> kBinShift;
+    const float half = steps < 1. ? 0.5f : 1.f;
+    const float d = fmaf(-half, x, half * (float)top) * (float)(steps / half);
+    return (int)fminf(d, (float)((kBins << kBinShift) - 1)) >> kBinShift;
   }
 
   // Keys around bin b: its ends as values (a step more), and some for their rounding.
