@@ -127,3 +127,12 @@ def test_penalties_past_the_types_range_stop_nobody(dtype):
     got, errors = run(sched)
     assert not errors and got[0] == want and all(len(got[i]) == 10 for i in range(5))
     assert got[4] == [5] * 10  # the only token it may take, whatever it costs
+
+
+def test_a_vocabulary_past_the_draws_is_refused_when_a_request_is_added(plain):
+    model = torch.nn.Module()
+    model.lm_head = torch.nn.Linear(1, (1 << 20) + 1, device=DEV)
+    sched = Scheduler(model, None, None, None)
+    with pytest.raises(ValueError, match="logits"):
+        sched.add_request([1], 2, params=RequestParams())
+    sched.add_request([1], 2)

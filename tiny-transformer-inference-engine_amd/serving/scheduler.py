@@ -38,7 +38,7 @@ from dataclasses import dataclass
 import torch
 
 from .batch import BatchStep, build_batch_step
-from .controls import RequestParams, TokenHistory, draw_rows, grammar_mask
+from .controls import MAX_SAMPLE_VOCAB, RequestParams, TokenHistory, draw_rows, grammar_mask
 from .sampling import sample
 from .sequence import Sequence, blocks_for
 
@@ -132,6 +132,9 @@ class Scheduler:
                 and 0 <= params.adapter < self.adapters.num_adapters):
             raise ValueError(f"the scheduler has no adapter {params.adapter}")
         vocab = self.model.lm_head.out_features
+        if vocab > MAX_SAMPLE_VOCAB:
+            raise ValueError(f"a request's own draw takes at most {MAX_SAMPLE_VOCAB} logits "
+                             f"(the model has {vocab})")
         if any(i >= vocab for i in params.logit_bias):
             raise ValueError(f"logit_bias names an id outside the vocabulary of {vocab}")
         most = torch.finfo(self.model.lm_head.weight.dtype).max / 2
