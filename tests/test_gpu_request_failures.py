@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from serving.allocator import BlockAllocator
-from serving.controls import RequestParams
+from serving.controls import RequestParams, sample_each
 from serving.layers import SchedulerConfig
 from serving.scheduler import Scheduler
 from test_gpu_requests import VOCAB, Words, make_model, pool_of, prompts_of
@@ -136,3 +136,8 @@ def test_a_vocabulary_past_the_draws_is_refused_when_a_request_is_added(plain):
     with pytest.raises(ValueError, match="logits"):
         sched.add_request([1], 2, params=RequestParams())
     sched.add_request([1], 2)
+
+
+def test_a_draw_without_temperatures_is_refused():
+    with pytest.raises(ValueError, match="temperature"):
+        sample_each(torch.zeros(2, 8, device=DEV), None)

@@ -193,6 +193,8 @@ def sample_each(logits: torch.Tensor, temperature: torch.Tensor,
     if logits.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(
             f"{what} is forward-only (inference); run it under torch.no_grad()")
+    if temperature is None:
+        raise ValueError(f"{what}: temperature must be given, float32 [{logits.shape[0]}]")
     rows, vocab = logits.shape
     dev = logits.device
     for t, dtype, name in ((temperature, torch.float32, "temperature"),
