@@ -240,7 +240,7 @@ def _apply(base, x, weights, plan, out, written, epilogue, what):
     if plan.num_adapters != weights.num_adapters:
         raise ValueError(f"{what}: a plan of {plan.num_adapters} adapters, weights of "
                          f"{weights.num_adapters}")
-    in_place = out is base
+    in_place, given = out is base, out is not None
     (base, base_stride), (x, x_stride) = _rows(base), _rows(x)
     calls, max_tiles = _native.calls(), tiles.shape[0]
     previous = _native.make_current(dev)
@@ -276,7 +276,7 @@ def _apply(base, x, weights, plan, out, written, epilogue, what):
             _native.DTYPE_CODES[dtype], ws.data_ptr(), nbytes, _native.stream_ptr(dev))
         if rc:
             _native.check(rc, what)
-        if in_place:
+        if given:  # a graph that saved out finds it changed
             torch.autograd.graph.increment_version(out)
     finally:
         _native.restore(previous)

@@ -138,7 +138,7 @@ def control_logits(logits: torch.Tensor, controls: LogitControls,
     previous = _native.make_current(dev)
     try:
         src, stride = _rows(logits)
-        in_place = out is logits
+        in_place, given = out is logits, out is not None
         if out is None:
             out, out_stride = src.new_empty((rows, vocab)), vocab
         elif in_place and src is logits:
@@ -164,7 +164,7 @@ def control_logits(logits: torch.Tensor, controls: LogitControls,
             None if status is None else _status_ptr(status, dev, what), _native.stream_ptr(dev))
         if rc:
             _native.check(rc, what)
-        if in_place:
+        if given:  # a graph that saved out finds it changed
             torch.autograd.graph.increment_version(out)
     finally:
         _native.restore(previous)
