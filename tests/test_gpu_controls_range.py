@@ -112,3 +112,41 @@ def test_top_k_of_logits_further_apart_than_fp32_reaches(temperature):
                                     0.0, float(np.float32(u[r])))
             if gap > 5 * 2.0 ** -43:
                 assert int(ids[r]) == want, (k, r)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,vocab,lens", [
+    (3, 50257, (4096, 4097, 8192)), (2, 3000, (5000, 20000)), (5, 40, (4095, 9000, 0, 12289, 1)),
+    (33, 131072, (8192, 6000, 4500))])
+def test_histories_of_several_rounds(rows, vocab, lens, dtype):
+    print(f"[history] {rows} {vocab} {lens} {dtype}", flush=True)
+    rng = np.random.default_rng([rows, vocab])
+    lens = [lens[r % len(lens)] for r in range(rows)]
+    cap = max(lens) + 3
+    x = torch.from_numpy(rng.normal(0, 3, (rows, vocab))).to(dtype)
+    tokens = np.where(rng.random((rows, cap)) < 0.5, rng.integers(0, max(1, vocab // 50), (rows, cap)),
+                      rng.integers(0, vocab, (rows, cap)))
+    prompt = [int(n * f) for n, f in zip(lens, rng.random(rows))]
+    rep, pres, freq = 1.25, 0.5, 2.0 ** -7
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    c = LogitControls(tokens=i32(tokens), lens=i32(lens), prompt_lens=i32(prompt),
+                      repetition=f32([rep] * rows), presence=f32([pres] * rows),
+                      frequency=f32([freq] * rows))
+    got = control_logits(x.to(DEV), c, status=st).cpu().double().numpy()
+    assert int(st) == 0
+    for r in range(rows):
+        row, n, p = x[r].double().numpy(), lens[r], prompt[r]
+        made = np.bincount(tokens[r, p:n], minlength=vocab)
+        there = np.bincount(tokens[r, :n], minlength=vocab) > 0
+        want = np.where(there, np.where(row > 0, row / rep, row * rep), row)
+        want = want - np.where(made > 0, freq * made + pres, 0)
+        size = np.abs(row) * rep + pres + freq * made
+        tol = torch.finfo(dtype).eps / 2 * np.abs(want) + 4 * 2.0 ** -24 * size
+        assert (np.abs(got[r] - want) <= tol * (1 + 2.0 ** -7)).all(), r
+    # an id outside the vocabulary behind the first round is reported, too
+    if max(lens) > 4200:
+        r = lens.index(max(lens))
+        tokens[r, 4150] = vocab
+        c = LogitControls(tokens=i32(tokens), lens=i32(lens))
+        control_logits(x.to(DEV), c, status=st)
+        assert int(st) != 0
