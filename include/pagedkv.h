@@ -689,7 +689,9 @@ size_t pkv_adapter_workspace_bytes(int n_tokens, int max_tiles, int tile_rows, i
  * the block, element; b [n_adapters][features of each part rounded up to 64, zeros there][rank],
  * of each 64 features: 8s of ranks, feature in the order 32 h + 8 q + 4 l + e of h < 2, l < 2,
  * q < 4, e < 4, rank of the 8. Rows without an adapter get y = base. All sums
- * are fp32, also a[i] x[t], and y is rounded once. PKV_EPILOGUE_NONE: out [n_tokens, n] =
+ * are fp32, also a[i] x[t], which for 16-bit types the second product takes as the sum of two
+ * values of the type (to 2^-18 of each for bf16, 2^-24 of the largest of 32 ranks for f16), and
+ * y is rounded once. PKV_EPILOGUE_NONE: out [n_tokens, n] =
  * y; out may be base itself (same address and stride). PKV_EPILOGUE_SWIGLU: two parts,
  * out [n_tokens, n0] = silu(y of part 0) * y of part 1, rounded once. Except for that
  * one case out shares no memory with an operand. rank is a multiple of 8 up to 128

@@ -313,7 +313,7 @@ constexpr int kDownThreads = 64 * kDownWaves;
 // are added up, in order, by whoever needs t: no workgroup waits for another and the
 // results have one order. D[rank][token]: lane l has token l % 16 and four consecutive
 // ranks. XV: x's rows are read in 16-byte pieces, all but the last step's without a
-// condition. 7400 rows of 4096 (bf16, 64 ranks, 64 MB) take 19.8 us, 3.2 TB/s of the copy's
+// condition. 7400 rows of 4096 (bf16, 64 ranks, 64 MB) take 19.6 us, 3.2 TB/s of the copy's
 // 5.2, and the same with eight wavefronts, four steps in flight or four pieces: a CU takes x's
 // rows, 64 bytes of each at a time, no faster. 64 rows over 24 adapters of rank 16 (8 MB) 5.1 us,
 // 256 over 4 of rank 64 (fp16) 5.2, in round trips.
@@ -455,7 +455,7 @@ __device__ __forceinline__ float gate(float g, float u) {
 // requested before t. 16 rows and 64 features a wavefront leave many wavefronts in flight,
 // which a prompt's rows need: 32 rows, or several times 64 features with the next one's rows
 // requested ahead, were slower (7400 rows, gate of 4096, rank 32: 50 us against 55 and 67-84).
-// Now 46.7 us for 182 MB of base and out, 3.9 TB/s, with the VALU's issue slots two thirds full;
+// Now 47.4 us for 182 MB of base and out, 3.8 TB/s, with the VALU's issue slots two thirds full;
 // B shared by 32 or 64 rows of a workgroup took 48 and 59 us when this took 47.5. 64 rows of
 // q/k/v 5.0 us, 256 of rank 64 6.1.
 template <typename T, int P, int EPI>

@@ -41,8 +41,9 @@ __device__ __forceinline__ void load_piece(const T* row, int id0, int vocab, T f
 // the range's logits, counts the row's history over the range in LDS, adds up the biases
 // there, and changes what it holds. Bytes bind at least (logits in and out, once: 5 us for 128
 // rows of 50257 in bf16); the history is read once per range, from L2 after the first. What
-// is in the way is a chain of round trips and barriers: of those rows' 14.9 us, 7 remain without
-// any control, a history of some 1150 tokens adds 4.5, 40 biases 2.5, a mask 1.
+// is in the way is a chain of round trips and barriers: of 13.9 us for the same rows again and
+// again (16.0 where others come in between), 6.8 remain without any control, a history of some
+// 1150 tokens adds 4.6, 40 biases 1.7 behind it (2.9 alone), a mask 0.6 to 0.9.
 // ---------------------------------------------------------------------------
 struct ControlArgs {
   void* out;
@@ -344,10 +345,10 @@ int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
 }
 
 // 8 ids a thread, 4096 a workgroup, where the chip's 1024 places for workgroups of 512 threads
-// hold all of them (4 rows of 50257, fp32: 4.2 us against 5.1); else 16, half the workgroups,
-// which read and count a row's history half as often (64 rows of 131072, histories to 8192: 20.6
-// us against 23.5; 128 rows of 50257, to 2048: 15.9 and 15.8). 256 threads: 15.5 and 29.8 for the
-// last two, 1024: 19.8 and 26.4.
+// hold all of them (4 rows of 50257, fp32: 3.7 us against 4.7); else 16, half the workgroups,
+// which read and count a row's history half as often (64 rows of 131072, histories to 8192: 21.0
+// us against 23.9; 128 rows of 50257, to 2048: 16.0 and 16.2). 256 threads with 16 ids: 25.3 and
+// 15.0 for the last two, 1024: 21.4 and 17.9.
 template <typename T>
 int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
   constexpr int S = 8 / kPiece<T>;
@@ -376,7 +377,7 @@ int launch_control(const ControlArgs& a, int64_t rows, hipStream_t st) {
 // arithmetic: 22 instructions each, half of them of 64 bits at the rate of 32-bit ones here, 9
 // to 13 us a pass over 50257 on one CU, whose issue slots are two thirds full. 128 such rows
 // (bf16): greedy 12 us, without a filter 24, top_k of 50 22, with top_p as well 30, a nucleus
-// of 5600 39, of 22000 46; rows of every kind 42 to 46, the slowest of them. Splitting a row over
+// of 5600 40, of 22000 46; rows of every kind 46, the slowest of them. Splitting a row over
 // workgroups takes a launch a pass, each with its own tables, dispatch and round trips: 83 us
 // for the 128 rows when this took 49, the same for 4 rows, so it is not done.
 // ---------------------------------------------------------------------------

@@ -33,7 +33,15 @@ MAX_ADAPTERS = 1000
 MAX_RANK = 128
 _I32 = torch.int32
 # Rows a tile: 16 leaves no empty matrix rows where most adapters have a few rows;
-# 64 reads an adapter's weights a quarter as often where a step holds prompts.
+# 64 reads an adapter's weights a quarter as often where a step holds prompts. us of both
+# products by tiles of 16 / 64 rows (q/k/v of 4096 + 256 features, k 4096, rank 16, bf16):
+#   rows                  256        768        1024       1536       2048       4096
+#   one adapter         9.2/16.6  14.0/18.9  17.8/20.3  20.6/23.2  24.5/25.2  39.6/32.8
+#   24, rows mixed     10.8/13.0  16.7/19.5  19.1/22.1  23.5/25.0  27.3/27.5  41.6/37.0
+#   256, rows mixed    30.0/37.0  38.6/40.6  40.4/42.5  47.4/44.5  51.8/47.4  70.7/58.5
+# and alike for rank 64 and for the gate (512 rows of one adapter 13.3/19.3, 1024 20.3/23.2, 4096
+# 51.6/42.4). The border is early for few adapters: from 1024 to some 2000 rows tiles of 16
+# would take up to 3 us less.
 TILE_ROWS_FEW, TILE_ROWS_MANY, TILE_MANY_FROM = 16, 64, 1024
 
 
@@ -286,7 +294,8 @@ def _apply(base, x, weights, plan, out, written, epilogue, what):
 def adapter_add(base: torch.Tensor, x: torch.Tensor, weights: AdapterWeights, plan: AdapterPlan,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """base [T, sum(out_features)] plus each row's adapter's product with x [T,
-    in_features]; float32, float16 or bfloat16, sums in fp32, rounded once. Rows without
+    in_features]; float32, float16 or bfloat16, sums in fp32, rounded once (between its
+    two products a 16-bit type's A x is the sum of two values of the type). Rows without
     an adapter are base's. out: where to write, base itself (in place) or memory of no
     operand."""
     return _apply(base, x, weights, plan, out, weights._features, _native.EPILOGUE_NONE,

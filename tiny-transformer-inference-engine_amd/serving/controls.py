@@ -260,7 +260,7 @@ def _f32(x) -> float:
 class RequestParams:
     """What one request of a batch asks for beyond its prompt (Scheduler.add_request);
     the defaults ask for nothing but a draw at temperature 1. Numbers are checked as the
-    float32 that the kernels get: a step that fails would fail for the whole batch."""
+    float32 that the kernels get, when a request is added: what a step finds ends the request."""
     temperature: float = 1.0         # 0: the most likely token
     top_k: int = 0                   # 0: off
     top_p: float = 1.0

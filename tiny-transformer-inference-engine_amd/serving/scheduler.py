@@ -139,7 +139,7 @@ class Scheduler:
             raise ValueError(f"logit_bias names an id outside the vocabulary of {vocab}")
         most = torch.finfo(self.model.lm_head.weight.dtype).max / 2
         if any(v > most for v in params.logit_bias.values()):
-            raise ValueError(f"a logit_bias above {most} would leave an infinite logit")
+            raise ValueError(f"a logit_bias above {most} asks for an infinite logit")
         if params.grammar is not None:
             if any(p is not None and p.grammar is params.grammar
                    for p in [r.params for r in self.waiting]
